@@ -138,6 +138,39 @@ class DecodePlan(C.Structure):
     _fields_ = [("opaque", C.c_uint64 * 8)]
 
 
+G4_KV_F16, G4_KV_E4M3 = 0, 1
+G4_LOGITS_F32, G4_LOGITS_F16, G4_LOGITS_BF16 = 0, 1, 2
+G4_LOGPROBS_MAX_TOP = 64
+G4_COMMIT_MAX_CACHES = 64
+
+
+class PagedCache(C.Structure):
+    _fields_ = [("k_pool", C.c_void_p), ("v_pool", C.c_void_p), ("num_pages", C.c_uint32), ("page_size", C.c_uint32),
+                ("num_kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("dtype", C.c_uint32), ("reserved", C.c_uint32)]
+
+
+class PagedBatch(C.Structure):
+    _fields_ = [("block_table", C.c_void_p), ("token_start", C.c_void_p), ("ctx_lens", C.c_void_p),
+                ("positions", C.c_void_p), ("tree_mask", C.c_void_p), ("n_seqs", C.c_uint32),
+                ("table_stride", C.c_uint32), ("n_tokens", C.c_uint32), ("max_tokens", C.c_uint32),
+                ("mask_words", C.c_uint32), ("reserved", C.c_uint32)]
+
+
+class PagedAppendParams(C.Structure):
+    _fields_ = [("num_q_heads", C.c_uint32), ("eps", C.c_float), ("q_stride", C.c_uint64), ("k_stride", C.c_uint64),
+                ("v_stride", C.c_uint64)]
+
+
+class PagedAttnParams(C.Structure):
+    _fields_ = [("num_q_heads", C.c_uint32), ("sliding_window", C.c_uint32), ("scale", C.c_float),
+                ("softcap", C.c_float)]
+
+
+class TokenLogprobsParams(C.Structure):
+    _fields_ = [("rows", C.c_uint32), ("vocab", C.c_uint32), ("row_stride", C.c_uint64), ("dtype", C.c_uint32),
+                ("top_k", C.c_uint32), ("cap", C.c_float), ("temperature", C.c_float)]
+
+
 _P = C.c_void_p
 _U32 = C.c_uint32
 _SZ = C.c_size_t
@@ -220,6 +253,13 @@ SIGNATURES: dict[str, list] = {
     "g4_lm_head_workspace_size": [LmHeadParams, C.POINTER(C.c_size_t)],
     "g4_lm_head_argmax": [_P, _P, _P, _P, _P, _SZ, LmHeadParams, _P],
     "g4_lm_head_argmax_timed": [_P, _P, _P, _P, _P, _SZ, LmHeadParams, _P, _P, _P],
+    "g4_paged_append": [C.POINTER(PagedCache), C.POINTER(PagedBatch), _P, _P, _P, _P, _P, _P, _P,
+                        C.POINTER(PagedAppendParams), _P],
+    "g4_paged_attn_workspace_size": [C.POINTER(PagedCache), C.POINTER(PagedBatch), _U32, C.POINTER(C.c_size_t)],
+    "g4_paged_attn": [C.POINTER(PagedCache), C.POINTER(PagedBatch), _P, _P, C.POINTER(PagedAttnParams), _P, _SZ, _P],
+    "g4_paged_commit": [C.POINTER(PagedCache), _U32, C.POINTER(PagedBatch), _P, _U32, _P, _P, _P],
+    "g4_token_logprobs_workspace_size": [C.POINTER(TokenLogprobsParams), C.POINTER(C.c_size_t)],
+    "g4_token_logprobs": [_P, _P, _P, _P, _P, _P, C.POINTER(TokenLogprobsParams), _P, _SZ, _P],
 }
 STRING_FUNCS = ("g4_last_error", "g4_version")
 

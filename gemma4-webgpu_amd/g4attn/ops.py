@@ -684,3 +684,212 @@ def lm_head_argmax_timed(hidden, weight, logits, result, workspace, vocab, hidde
     abi.call("g4_lm_head_argmax_timed", *_lm_head_args(hidden, weight, logits, result, workspace, vocab,
                                                       hidden_size, cap),
              _stream(stream), C.c_void_p(start.cuda_event), C.c_void_p(stop.cuda_event))
+
+
+# ---- drafted tokens over a paged cache ---------------------------------------------
+
+def _on_device(device, **tensors):
+    """Every given tensor lies on `device`, which is the current one (the stream's)."""
+    if device.index != _current_device():
+        raise ValueError(f"tensors on {device}, but the current device is cuda:{_current_device()}")
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name}: on {t.device}, expected {device}")
+
+
+def _shaped(t, name, shape):
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
+
+
+class PagedCache:
+    """One layer's K and V pools, [num_pages, page_size, num_kv_heads, head_dim] each: float16 (or its bits) or
+    float8_e4m3fn. Keeps the tensors alive; describe a layer's pools once and pass it to every call."""
+
+    def __init__(self, k_pool, v_pool):
+        for name, t in (("k_pool", k_pool), ("v_pool", v_pool)):
+            _dev(t, name, F16_TYPES + (torch.float8_e4m3fn,), 1)
+            if t.dim() != 4:
+                raise ValueError(f"{name}: expected [num_pages, page_size, num_kv_heads, head_dim]")
+        if k_pool.shape != v_pool.shape or k_pool.dtype != v_pool.dtype:
+            raise ValueError("k_pool and v_pool differ in shape or dtype")
+        self.k_pool, self.v_pool = k_pool, v_pool
+        self.device = k_pool.device
+        if v_pool.device != self.device:
+            raise ValueError(f"v_pool: on {v_pool.device}, expected {self.device}")
+        self.num_pages, self.page_size, self.num_kv_heads, self.head_dim = (int(n) for n in k_pool.shape)
+        f8 = k_pool.dtype == torch.float8_e4m3fn
+        self.c = abi.PagedCache(k_pool.data_ptr(), v_pool.data_ptr(), self.num_pages, self.page_size,
+                                self.num_kv_heads, self.head_dim, abi.G4_KV_E4M3 if f8 else abi.G4_KV_F16, 0)
+
+
+class PagedBatch:
+    """A step's sequences and their new tokens: block_table int32 [n_seqs, pages], token_start int32 [n_seqs + 1],
+    ctx_lens int32 [n_seqs], all on the GPU and read there when a kernel runs (update them in place between
+    replays of a captured step). n_tokens: rows of the token buffers, padding included; max_tokens: at least the
+    longest sequence's new tokens (n_tokens when not given). positions: int32 [n_tokens], for trees (ctx + depth);
+    tree_mask: int64 bits [n_tokens, words] of the new tokens each token attends, itself included."""
+
+    def __init__(self, block_table, token_start, ctx_lens, n_tokens, max_tokens=None, positions=None, tree_mask=None):
+        _dev(block_table, "block_table", torch.int32, 1)
+        if block_table.dim() != 2:
+            raise ValueError("block_table: expected [n_seqs, pages]")
+        self.n_seqs, stride = (int(n) for n in block_table.shape)
+        self.n_tokens = int(n_tokens)
+        self.max_tokens = self.n_tokens if max_tokens is None else int(max_tokens)
+        if not 0 <= self.n_tokens < 1 << 32 or not 0 <= self.max_tokens < 1 << 32:
+            raise ValueError(f"n_tokens {n_tokens}, max_tokens {max_tokens}")
+        words = 0
+        if tree_mask is not None:
+            if tree_mask.dim() != 2:
+                raise ValueError("tree_mask: expected [n_tokens, words]")
+            words = int(tree_mask.shape[1])
+        self.device = block_table.device
+        for name, t in (("token_start", token_start), ("ctx_lens", ctx_lens), ("positions", positions),
+                        ("tree_mask", tree_mask)):
+            if t is not None and t.device != self.device:
+                raise ValueError(f"{name}: on {t.device}, expected {self.device}")
+        self.tensors = (block_table, token_start, ctx_lens, positions, tree_mask)
+        self.c = abi.PagedBatch(
+            block_table.data_ptr(), _dev(token_start, "token_start", torch.int32, self.n_seqs + 1),
+            _dev(ctx_lens, "ctx_lens", torch.int32, self.n_seqs),
+            None if positions is None else _dev(positions, "positions", torch.int32, self.n_tokens),
+            None if tree_mask is None else _dev(tree_mask, "tree_mask", (torch.int64, torch.uint64), self.n_tokens * words),
+            self.n_seqs, stride, self.n_tokens, self.max_tokens, words, 0)
+
+
+def _token_rows(t, name, heads, head_dim, tokens, dtype):
+    """A [tokens, heads, head_dim] tensor whose tokens may lie apart: (pointer, elements from token to token)."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name}: must be on the GPU, got {t.device}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name}: dtype {t.dtype}, expected {dtype}")
+    _shaped(t, name, (tokens, heads, head_dim))
+    if t.stride(2) != 1 or (heads > 1 and t.stride(1) != head_dim):
+        raise ValueError(f"{name}: a token's heads must be contiguous")
+    if tokens <= 1:
+        return t.data_ptr(), 0
+    if t.stride(0) < heads * head_dim:
+        raise ValueError(f"{name}: tokens overlap")
+    return t.data_ptr(), t.stride(0)
+
+
+def paged_append(cache, batch, q, k, v, q_weight, k_weight, rope_inv_freq, q_out, eps=1e-6, stream=None):
+    """Norms and rotation of a batch's tokens and their rows' store (g4_paged_append). q: f32 [n_tokens, NQH, HD];
+    k, v: f32 [n_tokens, NKH, HD]; tokens may lie apart (slices of one projection's output). q_out: f16
+    [n_tokens, NQH, HD]. k, v, k_weight None: a KV-consumer layer; q, q_weight, q_out None: only the store.
+    rope_inv_freq: the f32 [HD / 2] table of rope_inv_freq()."""
+    if q is None and k is None:
+        raise ValueError("paged_append: neither q nor k and v")
+    hd, nt = cache.head_dim, batch.n_tokens
+    _on_device(cache.device, batch=batch, q=q, k=k, v=v, q_weight=q_weight, k_weight=k_weight,
+               rope_inv_freq=rope_inv_freq, q_out=q_out)
+    nqh, qp, qw, qo, ks, kp, vs, vp, kw, qs = 0, None, None, None, 0, None, 0, None, None, 0
+    if q is not None:
+        if q.dim() != 3:
+            raise ValueError("q: expected [n_tokens, heads, head_dim]")
+        nqh = int(q.shape[1])
+        qp, qs = _token_rows(q, "q", nqh, hd, nt, torch.float32)
+        qw = _f16(q_weight, "q_weight", hd)
+        qo = _f16(q_out, "q_out", nt * nqh * hd)
+    elif q_weight is not None or q_out is not None:
+        raise ValueError("paged_append: q, q_weight and q_out go together")
+    if k is not None:
+        kp, ks = _token_rows(k, "k", cache.num_kv_heads, hd, nt, torch.float32)
+        vp, vs = _token_rows(v, "v", cache.num_kv_heads, hd, nt, torch.float32)
+        kw = _f16(k_weight, "k_weight", hd)
+    elif v is not None or k_weight is not None:
+        raise ValueError("paged_append: k, v and k_weight go together")
+    if nt == 0:
+        return
+    p = abi.PagedAppendParams(nqh, eps, qs, ks, vs)
+    abi.call("g4_paged_append", cache.c, batch.c, qp, kp, vp, qw, kw, _f32(rope_inv_freq, "rope_inv_freq", hd // 2), qo, p,
+             _stream(stream))
+
+
+def paged_attn_workspace_bytes(cache, batch, num_q_heads) -> int:
+    n = C.c_size_t(0)
+    abi.call("g4_paged_attn_workspace_size", cache.c, batch.c, num_q_heads, C.byref(n))
+    return n.value
+
+
+def paged_attn(cache, batch, q, out, workspace, scale=1.0, sliding_window=0, softcap=0.0, stream=None):
+    """Attention of a batch's new tokens over their sequences' rows (g4_paged_attn). q: f16 [n_tokens, NQH, HD] as
+    paged_append leaves it; out: f32, the same shape; the new tokens' own rows are already stored. workspace: uint8,
+    paged_attn_workspace_bytes."""
+    _on_device(cache.device, batch=batch, q=q, out=out, workspace=workspace)
+    if q.dim() != 3:
+        raise ValueError("q: expected [n_tokens, heads, head_dim]")
+    nqh = int(q.shape[1])
+    shape = (batch.n_tokens, nqh, cache.head_dim)
+    _shaped(q, "q", shape)
+    _shaped(out, "out", shape)
+    if batch.n_tokens == 0:
+        return
+    p = abi.PagedAttnParams(nqh, int(sliding_window), float(scale), float(softcap))
+    abi.call("g4_paged_attn", cache.c, batch.c, _f16(q, "q", 0), _f32(out, "out", 0), p,
+             _dev(workspace, "workspace", torch.uint8, 0), workspace.numel(), _stream(stream))
+
+
+def paged_commit(caches, batch, path, n_accepted, new_ctx_lens, stream=None):
+    """The accepted drafted rows moved together in every cache of `caches` (g4_paged_commit). path: int32
+    [n_seqs, steps], ascending new-token indices; n_accepted, new_ctx_lens: int32 [n_seqs]."""
+    caches = list(caches)
+    _on_device(batch.device, path=path, n_accepted=n_accepted, new_ctx_lens=new_ctx_lens,
+               **{f"caches[{i}]": c for i, c in enumerate(caches)})
+    if path.dim() != 2 or path.shape[0] != batch.n_seqs:
+        raise ValueError(f"path: shape {tuple(path.shape)}, expected [{batch.n_seqs}, steps]")
+    arr = (abi.PagedCache * max(1, len(caches)))(*[c.c for c in caches])
+    abi.call("g4_paged_commit", arr, len(caches), batch.c, _dev(path, "path", torch.int32, 1), int(path.shape[1]),
+             _dev(n_accepted, "n_accepted", torch.int32, batch.n_seqs),
+             _dev(new_ctx_lens, "new_ctx_lens", torch.int32, batch.n_seqs), _stream(stream))
+
+
+# ---- log probabilities ---------------------------------------------------------------
+
+LOGIT_TYPES = {torch.float32: abi.G4_LOGITS_F32, torch.float16: abi.G4_LOGITS_F16, torch.bfloat16: abi.G4_LOGITS_BF16}
+
+
+def token_logprobs_workspace_bytes(rows, vocab, top_k) -> int:
+    n = C.c_size_t(0)
+    p = abi.TokenLogprobsParams(rows, vocab, 0, abi.G4_LOGITS_F32, top_k, 0.0, 1.0)
+    abi.call("g4_token_logprobs_workspace_size", p, C.byref(n))
+    return n.value
+
+
+def token_logprobs(logits, tokens, logprobs, entropy, workspace, top_ids=None, top_logprobs=None, cap=0.0,
+                   temperature=1.0, stream=None):
+    """Log probabilities of given tokens, entropy and the best alternatives (g4_token_logprobs). logits: f32, f16 or
+    bf16 [rows, vocab], rows may lie apart (a slice of a padded vocabulary); tokens: int32 [rows], with logprobs f32
+    [rows] (or both None); entropy: f32 [rows] or None; top_ids int32 and top_logprobs f32 [rows, k], or both None.
+    workspace: uint8, token_logprobs_workspace_bytes."""
+    if not isinstance(logits, torch.Tensor) or logits.dim() != 2:
+        raise ValueError("logits: expected a [rows, vocab] tensor")
+    if not logits.is_cuda:
+        raise ValueError(f"logits: must be on the GPU, got {logits.device}")
+    if logits.dtype not in LOGIT_TYPES:
+        raise TypeError(f"logits: dtype {logits.dtype} not in {tuple(LOGIT_TYPES)}")
+    rows, vocab = (int(n) for n in logits.shape)
+    if vocab > 1 and logits.stride(1) != 1 or rows > 1 and logits.stride(0) < vocab:
+        raise ValueError("logits: a row's logits must be contiguous, and rows apart")
+    _on_device(logits.device, tokens=tokens, logprobs=logprobs, entropy=entropy, workspace=workspace, top_ids=top_ids,
+               top_logprobs=top_logprobs)
+    k = 0
+    if top_ids is not None:
+        if top_ids.dim() != 2 or top_ids.shape[0] != rows:
+            raise ValueError(f"top_ids: shape {tuple(top_ids.shape)}, expected [{rows}, k]")
+        k = int(top_ids.shape[1])
+    if rows == 0:
+        return
+    p = abi.TokenLogprobsParams(rows, vocab, logits.stride(0) if rows > 1 else 0, LOGIT_TYPES[logits.dtype], k, cap,
+                                temperature)
+
+    def opt(t, name, dtype, n):
+        return None if t is None else _dev(t, name, dtype, n)
+
+    abi.call("g4_token_logprobs", logits.data_ptr(), opt(tokens, "tokens", torch.int32, rows),
+             opt(logprobs, "logprobs", torch.float32, rows), opt(entropy, "entropy", torch.float32, rows),
+             opt(top_ids, "top_ids", torch.int32, rows * k), opt(top_logprobs, "top_logprobs", torch.float32, rows * k), p,
+             _dev(workspace, "workspace", torch.uint8, 0), workspace.numel(), _stream(stream))

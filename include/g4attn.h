@@ -715,6 +715,150 @@ int g4_lm_head_argmax_timed(const float* hidden, const uint16_t* weight, float* 
                             void* workspace, size_t workspace_bytes, g4_lm_head_params p, void* stream,
                             void* start_event, void* stop_event);
 
+/* ---- serving drafted tokens over a paged cache -----------------------------
+ * A decode step of a batch of sequences, each with any number of new tokens:
+ * one (plain decoding), a chain (a prompt's chunk, or tokens drafted one after
+ * the other) or a tree of drafted tokens. Rows live in pages of a pool;
+ * sequences name their pages in a block table on the device. No counterpart in
+ * the reference (one sequence, one token a forward: src/engine.ts:116,
+ * 2469-2475); g4_paged_append does its vNorm, fusedNormRope and kvCacheStore
+ * (:2056-2091) and g4_paged_attn its attnScore, softmax and attnOutput
+ * (:2092-2094) for every token of the batch.
+ *
+ * A step: g4_paged_append (norms, rotation, the rows' store), g4_paged_attn,
+ * both per layer; then g4_token_logprobs over the logits, and, once the caller
+ * has decided which drafted tokens stand, g4_paged_commit for all layers.
+ *
+ * Lengths, pages, positions and masks are device arrays, read by the kernels
+ * when they run: a captured step replays with what they then hold. The host
+ * sees only the bounds in g4_paged_batch. Values out of range are defined:
+ * token ranges are cut to [0, n_tokens) and to max_tokens tokens a sequence,
+ * ctx_lens to [0, table_stride * page_size]; a row whose page id is not in
+ * [0, num_pages), or that lies past the block table, is not stored and not
+ * attended. Sequences whose token ranges overlap, or pages that two sequences
+ * write, are the caller's to avoid. Tokens outside every sequence's range
+ * (padding) are left alone: their rows of q_out and out keep what they held. */
+#define G4_KV_F16 0
+#define G4_KV_E4M3 1 /* OCP e4m3, round to nearest even, saturating at 448; NaN stays NaN */
+typedef struct g4_paged_cache {
+    void* k_pool;          /* [num_pages][page_size][num_kv_heads][head_dim], 16-byte aligned */
+    void* v_pool;
+    uint32_t num_pages;
+    uint32_t page_size;    /* rows: a power of two in [16, 1024] */
+    uint32_t num_kv_heads;
+    uint32_t head_dim;     /* 256 or 512 */
+    uint32_t dtype;        /* G4_KV_F16 or G4_KV_E4M3 */
+    uint32_t reserved;     /* 0 */
+} g4_paged_cache;
+
+/* Row r of sequence s is row r % page_size of page block_table[s * table_stride
+ * + r / page_size]. Rows [0, ctx_lens[s]) are committed; new token j of the
+ * sequence (token_start[s] + j of the batch) has row ctx_lens[s] + j. */
+typedef struct g4_paged_batch {
+    const int32_t* block_table; /* DEVICE [n_seqs][table_stride] */
+    const int32_t* token_start; /* DEVICE [n_seqs + 1], ascending */
+    const int32_t* ctx_lens;    /* DEVICE [n_seqs]: rows before the batch's tokens */
+    const int32_t* positions;   /* DEVICE [n_tokens] or NULL: a token's position is its row. For trees: ctx + depth.
+                                   At least ctx_lens of the token's sequence */
+    const uint64_t* tree_mask;  /* DEVICE [n_tokens][mask_words] or NULL (a chain: a token attends the new tokens up to
+                                   itself). Bit j: the token attends new token j of its sequence; its own bit is not
+                                   implied. Committed rows are always attended (up to the window) */
+    uint32_t n_seqs;            /* 1 .. 65535 */
+    uint32_t table_stride;      /* pages a sequence can name; table_stride * page_size <= 2^30 */
+    uint32_t n_tokens;          /* tokens of the batch's buffers (padding included), at most 2^22 */
+    uint32_t max_tokens;        /* at least the longest sequence's new tokens */
+    uint32_t mask_words;        /* with tree_mask: at least ceil(max_tokens / 64) */
+    uint32_t reserved;          /* 0 */
+} g4_paged_batch;
+
+/* Every new token's q and k normed and rotated, v normed, and the rows stored:
+ * the values of g4_attn_prompt_prep (bit for bit before the rounding to the
+ * cache's type), at positions[t]. q, k, v: f32, token t at t * q_stride (k_stride,
+ * v_stride) elements, heads and elements contiguous, so that they may be parts of
+ * one projection's output; a stride of 0 stands for contiguous tokens. q_out: f16
+ * [n_tokens][num_q_heads][head_dim], what g4_paged_attn takes. k, v and k_weight
+ * NULL: a KV-consumer layer, only q; q, q_weight and q_out NULL: only the store.
+ * rope_inv_freq: device [head_dim / 2] from g4_rope_inv_freq. Rows 16-byte
+ * aligned (pointers and strides). */
+typedef struct g4_paged_append_params {
+    uint32_t num_q_heads;
+    float eps;
+    uint64_t q_stride;
+    uint64_t k_stride;
+    uint64_t v_stride;
+} g4_paged_append_params;
+int g4_paged_append(const g4_paged_cache* cache, const g4_paged_batch* batch, const float* q, const float* k,
+                    const float* v, const uint16_t* q_weight, const uint16_t* k_weight, const float* rope_inv_freq,
+                    uint16_t* q_out, const g4_paged_append_params* p, void* stream);
+
+/* Attention of every new token over its sequence's rows: committed rows and the
+ * new tokens' rows its mask names (stored before, by g4_paged_append), all
+ * limited to positions above its own minus sliding_window (0: no limit).
+ * score = scale * q . k, then softcap * tanh(score / softcap) where softcap > 0;
+ * softmax and products in f32 (the probabilities enter the matrix products as the
+ * sum of two f16). A token that attends nothing gets 0; rows that a token does
+ * not attend do not reach it, whatever they hold. q: f16 [n_tokens][num_q_heads]
+ * [head_dim]; out: f32, the same shape, 16-byte aligned; num_q_heads up to 8 times
+ * num_kv_heads. The workspace (g4_paged_attn_workspace_size: it depends on the
+ * head layout, head_dim, n_seqs and max_tokens alone) holds partial results within
+ * a call; calls that overlap need one each. Results do not depend on scheduling:
+ * the same call gives the same bits. */
+typedef struct g4_paged_attn_params {
+    uint32_t num_q_heads;
+    uint32_t sliding_window;
+    float scale;
+    float softcap;
+} g4_paged_attn_params;
+int g4_paged_attn_workspace_size(const g4_paged_cache* cache, const g4_paged_batch* batch, uint32_t num_q_heads,
+                                 size_t* bytes);
+int g4_paged_attn(const g4_paged_cache* cache, const g4_paged_batch* batch, const uint16_t* q, float* out,
+                  const g4_paged_attn_params* p, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The accepted drafted tokens' rows moved together, in every pool of up to 64
+ * caches (layers; of one page size and page count) in one launch: row
+ * ctx_lens[s] + path[s][d] goes to row ctx_lens[s] + d for d < n_accepted[s].
+ * path: DEVICE [n_seqs][path_stride], strictly ascending new-token indices of each
+ * sequence (a tree's ancestors come before their descendants); n_accepted: DEVICE
+ * [n_seqs], cut to [0, path_stride]. An index that is negative, not above the one before it, or
+ * not below the sequence's new tokens ends its sequence's path there.
+ * new_ctx_lens (DEVICE [n_seqs], not ctx_lens itself) receives ctx_lens + the
+ * length of the path. Of the batch, positions and tree_mask are not read. */
+#define G4_COMMIT_MAX_CACHES 64
+int g4_paged_commit(const g4_paged_cache* caches, uint32_t n_caches, const g4_paged_batch* batch, const int32_t* path,
+                    uint32_t path_stride, const int32_t* n_accepted, int32_t* new_ctx_lens, void* stream);
+
+/* ---- log probabilities ------------------------------------------------------
+ * For each row of logits: z = logit, or cap * tanh(logit / cap) where cap > 0
+ * (the final softcap, logit_softcap.wgsl:9-16), divided by temperature;
+ * lse = log(sum exp(z)); logprob = z[token] - lse of the given token; entropy =
+ * lse - sum p z; and the top_k logits' indices with their log probabilities,
+ * by descending logit, equal logits (cap and temperature aside) by ascending
+ * index. A token outside [0, vocab) gets logprob 0 (padding). Logits of -inf
+ * have probability 0 and are never among the top; where fewer than top_k logits
+ * are above -inf, the rest have id -1 and logprob -inf. A row with a NaN or
+ * +inf logit, or with -inf alone, has NaN as logprob, entropy and top_logprobs
+ * (its top ids as said, NaN never among them). logits: f32, f16 or bf16, row r
+ * at r * row_stride elements. logprobs and tokens may be NULL together, and so
+ * entropy, and top_ids and top_logprobs (with top_k 0). The workspace holds
+ * partial results within a call; calls that overlap need one each. */
+#define G4_LOGITS_F32 0
+#define G4_LOGITS_F16 1
+#define G4_LOGITS_BF16 2
+#define G4_LOGPROBS_MAX_TOP 64
+typedef struct g4_token_logprobs_params {
+    uint32_t rows;
+    uint32_t vocab;       /* 1 .. 2^24 */
+    uint64_t row_stride;  /* elements from row to row, at least vocab; 0: vocab */
+    uint32_t dtype;
+    uint32_t top_k;       /* 0 .. min(vocab, 64) */
+    float cap;            /* 0: none */
+    float temperature;    /* above 0 */
+} g4_token_logprobs_params;
+int g4_token_logprobs_workspace_size(const g4_token_logprobs_params* p, size_t* bytes);
+int g4_token_logprobs(const void* logits, const int32_t* tokens, float* logprobs, float* entropy, int32_t* top_ids,
+                      float* top_logprobs, const g4_token_logprobs_params* p, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
 #ifdef __cplusplus
 }
 #endif
