@@ -16,18 +16,22 @@
 //     an f32 result keeps f32 accuracy (one f16 P alone leaves 2e-4).
 // e4m3 pools are widened to f16 in registers, which is exact.
 //
-// Work split: a (sequence, kv head, tile of query rows) is an item of ceil(rows / 32)
+// Two forms: at most 16 query rows a kv head (k_paged_few: the workgroup's waves take
+// different cache rows, K and V go from memory to registers) and more (k_paged_tile:
+// the waves take different query rows of one tile, K and V rows shared through LDS).
+//
+// Work split: a (sequence, tile of query rows, kv head) is an item of ceil(rows / 32)
 // row tiles; all items' tiles in order are cut into equal shares, one a workgroup,
 // whatever the lengths, so a ragged batch fills the chip and one long sequence does
 // too. Lengths are read on the device (a captured launch serves the next step's),
-// every workgroup finds its share by a scan over the sequences. An item cut between
+// every workgroup finds its share by a scan over the items. An item cut between
 // workgroups leaves (m, l, o) records that a second launch joins in a fixed order.
 #include "decode_core.h"
 #include "paged.h"
 
 namespace g4 {
 
-constexpr int kPagedWaves = 4;
+constexpr int kPagedWaves = 4;  // of k_paged_few
 constexpr int kPagedThreads = 64 * kPagedWaves;
 
 struct PagedAttnArgs {
@@ -35,50 +39,40 @@ struct PagedAttnArgs {
     float* __restrict__ out;
     const char* __restrict__ k;
     const char* __restrict__ v;
-    float* __restrict__ part_o;   // [2 * workgroups][16 C][HD]
-    float* __restrict__ part_ml;  // [2 * workgroups][16 C][2]
+    float* __restrict__ part_o;   // [2 * workgroups][tile rows][HD]
+    float* __restrict__ part_ml;  // [2 * workgroups][tile rows][2]
     uint32_t nkh, group;
+    uint32_t q_tiles;             // query tiles a sequence and kv head has at most
     int32_t window;               // 0: none
-    float scale, cap, inv_cap;
+    float qscale;                 // scale * log2(e)
+    float cap_scale, cap_log2;    // scale / cap and cap * log2(e); 0: no cap
     uint32_t wgs, min_share;      // workgroups of the attention launch; least tiles a workgroup takes
     PagedBatchDev b;
 };
 
 // ---- the items ----------------------------------------------------------------
 
-// Row tiles of query tile qt (16 C rows) of a sequence: [first, first + n), n >= 1.
-// hi: one past the last row that any of its tokens attends.
+// Row tiles of query tile qt (MQ query rows) of a sequence: [first, first + n), n >= 1
+// where it has such a tile, 0 otherwise. hi: one past the last row that any of its
+// tokens attends.
 struct PagedSpan {
     unsigned first, n, hi;
 };
-template <int C>
+template <int MQ>
 __device__ __forceinline__ PagedSpan paged_span(const PagedAttnArgs& a, const PagedSeq& sq, unsigned qt) {
-    const unsigned j0 = qt * (16 * C) / a.group;
-    const unsigned j1 = min((qt * (16 * C) + 16 * C - 1) / a.group, sq.n - 1);
-    const unsigned hi = min(sq.ctx + (a.b.mask ? sq.n : j1 + 1), paged_rows(a.b));
+    PagedSpan s{};
+    if (qt * MQ >= sq.n * a.group) return s;
+    const unsigned j0 = qt * MQ / a.group;
+    const unsigned j1 = min((qt * MQ + MQ - 1) / a.group, sq.n - 1);
+    s.hi = min(sq.ctx + (a.b.mask ? sq.n : j1 + 1), paged_rows(a.b));
     unsigned lo = 0;
     if (a.window) {  // positions are at least ctx (a chain's: ctx + j)
         const int at = (int)(sq.ctx + (a.b.positions || a.b.mask ? 0u : j0)) - a.window + 1;
         lo = min((unsigned)max(at, 0), sq.ctx);
     }
-    lo = min(lo, hi - 1);
-    PagedSpan s;
-    s.first = lo / 32;
-    s.n = (hi + 31) / 32 - s.first;
-    s.hi = hi;
+    s.first = min(lo, s.hi - 1) / 32;
+    s.n = (s.hi + 31) / 32 - s.first;
     return s;
-}
-template <int C>
-__device__ __forceinline__ unsigned paged_q_tiles(const PagedAttnArgs& a, const PagedSeq& sq) {
-    return (sq.n * a.group + 16 * C - 1) / (16 * C);
-}
-// Row tiles of all query tiles of one kv head of a sequence.
-template <int C>
-__device__ __forceinline__ unsigned paged_tiles(const PagedAttnArgs& a, const PagedSeq& sq) {
-    unsigned u = 0;
-    const unsigned nq = paged_q_tiles<C>(a, sq);
-    for (unsigned qt = 0; qt < nq; qt++) u += paged_span<C>(a, sq, qt).n;
-    return u;
 }
 
 __device__ __forceinline__ unsigned wave_scan(unsigned x, unsigned lane) {  // inclusive
@@ -93,21 +87,23 @@ __device__ __forceinline__ unsigned lane_value(unsigned x, unsigned lane) {
     return __builtin_amdgcn_readlane(x, lane);
 }
 
-// The batch's row tiles, as a wave sees them: lane l holds sequence l of a group of 64.
-template <int C>
+// The batch's row tiles, as a wave sees them: lane l holds query tile i0 + l of all
+// sequences' (q_tiles each, in order) and its row tiles for all kv heads.
+template <int MQ>
 struct PagedScan {
-    unsigned total = 0;           // row tiles of the whole batch
-    unsigned tiles = 0, incl = 0;  // of the group held: a sequence's (all kv heads), and up to it
+    unsigned total = 0;
+    unsigned tiles = 0, incl = 0;
 
-    __device__ __forceinline__ void group(const PagedAttnArgs& a, unsigned s0, unsigned lane) {
-        const unsigned s = s0 + lane;
+    __device__ __forceinline__ static unsigned items(const PagedAttnArgs& a) { return a.b.n_seqs * a.q_tiles; }
+    __device__ __forceinline__ void group(const PagedAttnArgs& a, unsigned i0, unsigned lane) {
+        const unsigned i = i0 + lane;
         tiles = 0;
-        if (s < a.b.n_seqs) tiles = paged_tiles<C>(a, paged_seq(a.b, s)) * a.nkh;
+        if (i < items(a)) tiles = paged_span<MQ>(a, paged_seq(a.b, i / a.q_tiles), i % a.q_tiles).n * a.nkh;
         incl = wave_scan(tiles, lane);
     }
     __device__ __forceinline__ void run(const PagedAttnArgs& a, unsigned lane) {
-        for (unsigned s0 = 0; s0 < a.b.n_seqs; s0 += 64) {
-            group(a, s0, lane);
+        for (unsigned i0 = 0; i0 < items(a); i0 += 64) {
+            group(a, i0, lane);
             total += lane_value(incl, 63);
         }
     }
@@ -119,39 +115,39 @@ struct PagedScan {
 
 // An item and where a tile number lies in it.
 struct PagedPlace {
-    unsigned s, kvh, qt;
-    unsigned off;   // tiles of the item before it
-    unsigned base;  // the item's first tile number
+    unsigned i;    // sequence * q_tiles + query tile
+    unsigned kvh;
+    unsigned off;  // tiles of the item before it
 };
-template <int C>
-__device__ __forceinline__ PagedPlace paged_place(const PagedAttnArgs& a, PagedScan<C>& scan, unsigned u, unsigned lane) {
+template <int MQ>
+__device__ __forceinline__ PagedPlace paged_place(const PagedAttnArgs& a, PagedScan<MQ>& scan, unsigned u, unsigned lane) {
     PagedPlace p{};
     unsigned before = 0;
-    for (unsigned s0 = 0;; s0 += 64) {
-        if (a.b.n_seqs > 64) scan.group(a, s0, lane);
+    for (unsigned i0 = 0;; i0 += 64) {
+        if (scan.items(a) > 64) scan.group(a, i0, lane);
         const unsigned all = lane_value(scan.incl, 63);
-        if (u < before + all || s0 + 64 >= a.b.n_seqs) {
+        if (u < before + all || i0 + 64 >= scan.items(a)) {
             const unsigned l = __builtin_ctzll(__ballot(scan.incl > u - before) | (1ull << 63));
-            p.s = s0 + l;
-            before += lane_value(scan.incl, l) - lane_value(scan.tiles, l);
-            const unsigned per_head = lane_value(scan.tiles, l) / a.nkh;
-            const unsigned rem = u - before;
+            const unsigned mine = lane_value(scan.tiles, l);
+            const unsigned per_head = mine / a.nkh;
+            const unsigned rem = u - (before + lane_value(scan.incl, l) - mine);
+            p.i = i0 + l;
             p.kvh = rem / per_head;
             p.off = rem % per_head;
-            p.base = before + p.kvh * per_head;
-            break;
+            return p;
         }
         before += all;
     }
-    const PagedSeq sq = paged_seq(a.b, p.s);
-    for (;;) {
-        const unsigned n = paged_span<C>(a, sq, p.qt).n;
-        if (p.off < n) break;
-        p.off -= n;
-        p.base += n;
-        p.qt++;
-    }
-    return p;
+}
+// The item after p's: the next kv head, or the next query tile that there is.
+template <int MQ>
+__device__ __forceinline__ void paged_next(const PagedAttnArgs& a, PagedPlace& p) {
+    p.off = 0;
+    if (++p.kvh < a.nkh) return;
+    p.kvh = 0;
+    const unsigned items = a.b.n_seqs * a.q_tiles;
+    do p.i++;
+    while (p.i < items && paged_span<MQ>(a, paged_seq(a.b, p.i / a.q_tiles), p.i % a.q_tiles).n == 0);
 }
 
 // ---- cache tiles ----------------------------------------------------------------
@@ -222,43 +218,40 @@ __device__ __forceinline__ float paged_tanh(float x) {
     return copysignf(__builtin_fmaf(__builtin_fmaf(-q, den, num), y, q), x);
 }
 
-// O^T += V^T P^T for one piece block, all query groups. Word w of a row's piece holds
+// O^T += V^T P^T for piece block b of V, all query groups. Word w of a row's piece holds
 // elements (2w, 2w + 1) (f16) or 4w .. 4w + 3 (e4m3): acc tile b E + e takes element e of
 // every lane's piece, so its rows are d = 16 E b + E (row) + e.
 template <int HD, int C, bool F8>
-__device__ __forceinline__ void paged_pv(const PagedV<HD, F8>& vr, const f16x8 (&hi)[C],
-                                         const f16x8 (&lo)[C], f32x4 (&acc)[C][PagedDims<HD, F8>::NO]) {
+__device__ __forceinline__ void paged_pv(int b, const u32x4 (&vr)[8], const f16x8 (&hi)[C], const f16x8 (&lo)[C],
+                                         f32x4 (&acc)[C][PagedDims<HD, F8>::NO]) {
     using D = PagedDims<HD, F8>;
 #pragma unroll
-    for (int b = 0; b < D::VP; b++)
+    for (int w = 0; w < 4; w++)
 #pragma unroll
-        for (int w = 0; w < 4; w++)
+        for (int h = 0; h < (F8 ? 2 : 1); h++) {
+            uint32_t x[8];
 #pragma unroll
-            for (int h = 0; h < (F8 ? 2 : 1); h++) {
-                uint32_t x[8];
+            for (int t = 0; t < 8; t++) x[t] = F8 ? fp8x2_f16(vr[t][w], h) : vr[t][w];
+            u32x4 e0, e1;
 #pragma unroll
-                for (int t = 0; t < 8; t++) x[t] = F8 ? fp8x2_f16(vr[b][t][w], h) : vr[b][t][w];
-                u32x4 e0, e1;
-#pragma unroll
-                for (int p = 0; p < 4; p++) {
-                    e0[p] = perm_lo(x[2 * p], x[2 * p + 1]);
-                    e1[p] = perm_hi(x[2 * p], x[2 * p + 1]);
-                }
-                const int i = b * D::E + (F8 ? 4 * w + 2 * h : 2 * w);
-#pragma unroll
-                for (int c = 0; c < C; c++) {
-                    acc[c][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, e0), hi[c], acc[c][i], 0, 0, 0);
-                    acc[c][i + 1] =
-                        __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, e1), hi[c], acc[c][i + 1], 0, 0, 0);
-                }
-#pragma unroll
-                for (int c = 0; c < C; c++) {
-                    acc[c][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, e0), lo[c], acc[c][i], 0, 0, 0);
-                    acc[c][i + 1] =
-                        __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, e1), lo[c], acc[c][i + 1], 0, 0, 0);
-                }
-                if constexpr (HD == 512) __builtin_amdgcn_sched_barrier(0);
+            for (int p = 0; p < 4; p++) {
+                e0[p] = perm_lo(x[2 * p], x[2 * p + 1]);
+                e1[p] = perm_hi(x[2 * p], x[2 * p + 1]);
             }
+            const int i = b * D::E + (F8 ? 4 * w + 2 * h : 2 * w);
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                acc[c][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, e0), hi[c], acc[c][i], 0, 0, 0);
+                acc[c][i + 1] =
+                    __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, e1), hi[c], acc[c][i + 1], 0, 0, 0);
+            }
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                acc[c][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, e0), lo[c], acc[c][i], 0, 0, 0);
+                acc[c][i + 1] =
+                    __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, e1), lo[c], acc[c][i + 1], 0, 0, 0);
+            }
+        }
 }
 
 // Words of V pieces whose elements are Inf or NaN (exponent all ones; e4m3: NaN alone): their places, as
@@ -268,23 +261,29 @@ __device__ __forceinline__ uint32_t odd_elements(uint32_t w) {
     return F8 ? ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u : ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
 }
 
-// Takes Inf and NaN out of a lane's V pieces; returns the rows (bit t) that had some.
-template <int HD, bool F8>
-__device__ __forceinline__ unsigned paged_take_odd(PagedV<HD, F8>& vr) {
-    unsigned rows = 0;
+// Takes Inf and NaN out of a lane's V pieces; returns the rows that had some, as bits 4 t + g
+// over the wave's lane groups.
+template <bool F8>
+__device__ __forceinline__ uint32_t paged_take_odd(u32x4 (&vr)[8]) {
+    uint32_t odd = 0;
+#pragma unroll
+    for (int t = 0; t < 8; t++)
+#pragma unroll
+        for (int w = 0; w < 4; w++) odd |= odd_elements<F8>(vr[t][w]);
+    if (!__any(odd != 0)) return 0;  // uniform
+    uint32_t rows = 0;
 #pragma unroll
     for (int t = 0; t < 8; t++) {
         uint32_t any = 0;
 #pragma unroll
-        for (int b = 0; b < PagedDims<HD, F8>::VP; b++)
+        for (int w = 0; w < 4; w++) {
+            const uint32_t o = odd_elements<F8>(vr[t][w]);
+            any |= o;
+            vr[t][w] &= ~((o >> (F8 ? 7 : 15)) * (F8 ? 0xffu : 0xffffu));  // each odd element's bit 0, times all ones
+        }
+        const uint64_t lanes = __ballot(any != 0);
 #pragma unroll
-            for (int w = 0; w < 4; w++) {
-                const uint32_t odd = odd_elements<F8>(vr[b][t][w]);
-                any |= odd;
-                const uint32_t low = odd >> (F8 ? 7 : 15);  // each odd element's bit 0, times all ones
-                vr[b][t][w] &= ~(low * (F8 ? 0xffu : 0xffffu));
-            }
-        rows |= (any ? 1u : 0u) << t;
+        for (int g = 0; g < 4; g++) rows |= ((lanes >> (16 * g) & 0xffff) ? 1u : 0u) << (4 * t + g);
     }
     return rows;
 }
@@ -307,158 +306,223 @@ __device__ __forceinline__ void paged_add_odd(const char* row, int g, bool atten
     }
 }
 
-// ---- attention --------------------------------------------------------------------
+// ---- a row tile against a lane's query columns ------------------------------------
 
-template <int HD, int C>
-struct PagedSmem {
-    f16x8 q[C][HD / 32][64];                           // score operand, lane-major
-    float o[kPagedWaves][HD / 16 * 4][64];             // one query group's outputs, per wave
-    float m[kPagedWaves][16 * C], l[kPagedWaves][16 * C];
+// Column n of the lane's query groups (group c: 16 query rows).
+template <int C>
+struct PagedCols {
+    unsigned j[C];     // new-token index; ~0: no row
+    int pos[C];
+    uint64_t bits[C];  // the mask's first word
+
+    __device__ __forceinline__ void load(const PagedAttnArgs& a, const PagedSeq& sq, unsigned r0) {
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            const unsigned r = r0 + 16 * c;
+            const bool live = r < sq.n * a.group;
+            const unsigned jj = live ? r / a.group : 0u, tok = sq.start + jj;
+            j[c] = live ? jj : ~0u;
+            pos[c] = a.b.positions ? max(a.b.positions[tok], 0) : (int)(sq.ctx + jj);
+            bits[c] = a.b.mask ? a.b.mask[(uint64_t)tok * a.b.mask_words] : 0;
+        }
+    }
+    // seen[c] bit t: the column attends the lane's row t of the tile at kt0 (rows 4g + t, and
+    // 16 + 4g + t - 4 from t = 4 on). dead: the rows nobody may read (past the last, or without a page).
+    __device__ __forceinline__ void look(const PagedAttnArgs& a, const PagedSeq& sq, unsigned hi, unsigned kt0, int g, bool ok0,
+                                         bool ok1, unsigned (&seen)[C], unsigned& dead) const {
+#pragma unroll
+        for (int c = 0; c < C; c++) seen[c] = 0;
+        dead = 0;
+#pragma unroll 1
+        for (int t = 0; t < 8; t++) {
+            const unsigned row = kt0 + (t < 4 ? 0 : 16) + 4 * g + (t & 3);
+            if (row >= hi || !(t < 4 ? ok0 : ok1)) {
+                dead |= 1u << t;
+                continue;
+            }
+            const unsigned dj = row - sq.ctx;  // the new-token index, for rows from ctx on
+            int rpos = (int)row;
+            if (row >= sq.ctx && a.window && a.b.positions) rpos = max(a.b.positions[sq.start + dj], 0);
+#pragma unroll
+            for (int c = 0; c < C; c++) {
+                bool ok = j[c] != ~0u;
+                if (row >= sq.ctx) {
+                    if (a.b.mask) {
+                        uint64_t word = bits[c];
+                        if (a.b.mask_words > 1 && ok) word = a.b.mask[(uint64_t)(sq.start + j[c]) * a.b.mask_words + (dj >> 6)];
+                        ok = ok && ((word >> (dj & 63)) & 1);
+                    } else {
+                        ok = ok && dj <= j[c];
+                    }
+                }
+                if (a.window) ok = ok && rpos > pos[c] - a.window;
+                seen[c] |= (ok ? 1u : 0u) << t;
+            }
+        }
+    }
 };
 
+// The online softmax of a tile's scores (log2 units): the running maximum moves once a score
+// is 8 above it (P stays within f16), P leaves as f16 and its residual.
 template <int HD, int C, bool F8>
-__global__ __launch_bounds__(kPagedThreads, C == 1 && HD == 256 ? 2 : 1) void k_paged_attn(const PagedAttnArgs a) {
+__device__ __forceinline__ void paged_softmax(const PagedAttnArgs& a, const f32x4 (&sc)[C][2], const unsigned (&seen)[C],
+                                              bool clear, float (&m_run)[C], float (&l_run)[C],
+                                              f32x4 (&acc)[C][PagedDims<HD, F8>::NO], f16x8 (&hi)[C], f16x8 (&lo)[C]) {
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+        float sv[8];
+        float tmax = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float x = sc[c][i >> 2][i & 3];
+            sv[i] = a.cap_log2 > 0.0f ? a.cap_log2 * paged_tanh(x * a.cap_scale) : x * a.qscale;
+        }
+        if (!clear) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) sv[i] = seen[c] >> i & 1 ? sv[i] : -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) tmax = fmaxf(tmax, sv[i]);
+        tmax = max_xor16(tmax);  // the column's rows lie in four lane groups
+        tmax = max_xor32(tmax);
+        const bool move = tmax > m_run[c] + 8.0f;
+        if (__any(move)) {
+            const float m_new = move ? tmax : m_run[c];
+            const float alpha = move ? __builtin_amdgcn_exp2f(m_run[c] - m_new) : 1.0f;
+            m_run[c] = m_new;
+            l_run[c] *= alpha;
+#pragma unroll
+            for (int i = 0; i < PagedDims<HD, F8>::NO; i++) acc[c][i] *= alpha;
+        }
+        const float base = m_run[c] == -INFINITY ? 0.0f : m_run[c];
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            const float p0 = __builtin_amdgcn_exp2f(sv[i] - base), p1 = __builtin_amdgcn_exp2f(sv[i + 1] - base);
+            l_run[c] += p0 + p1;
+            const f16x2 h = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(p0, p1));
+            const f16x2 r = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(p0 - (float)h[0], p1 - (float)h[1]));
+            hi[c][i] = h[0];
+            hi[c][i + 1] = h[1];
+            lo[c][i] = r[0];
+            lo[c][i + 1] = r[1];
+        }
+    }
+}
+
+// Page ids of the two 16-row halves of 64 row tiles, lane i the i-th (stride tiles apart from tile0 on).
+struct PagedPages {
+    unsigned half0, half1;
+    __device__ __forceinline__ void load(const PagedAttnArgs& a, const int32_t* table, unsigned tile0, unsigned stride,
+                                         unsigned hi, unsigned lane) {
+        const unsigned r = (tile0 + stride * lane) * 32;
+        half0 = (unsigned)table[min(r, hi - 1) >> a.b.page_shift];
+        half1 = (unsigned)table[min(r + 16, hi - 1) >> a.b.page_shift];
+    }
+};
+// Byte offsets of a tile's halves in the pools (page 0 where there is none, ok false).
+struct PagedAt {
+    uint64_t half0, half1;
+    bool ok0, ok1;
+};
+__device__ __forceinline__ PagedAt paged_at(const PagedAttnArgs& a, const PagedPages& p, unsigned i, unsigned kt0,
+                                            uint32_t row_bytes, uint32_t head_off) {
+    const unsigned pg0 = lane_value(p.half0, i), pg1 = lane_value(p.half1, i), in = (1u << a.b.page_shift) - 1;
+    PagedAt t;
+    t.ok0 = pg0 < a.b.num_pages;
+    t.ok1 = pg1 < a.b.num_pages;
+    t.half0 = (((uint64_t)(t.ok0 ? pg0 : 0u) << a.b.page_shift) + (kt0 & in)) * row_bytes + head_off;
+    t.half1 = (((uint64_t)(t.ok1 ? pg1 : 0u) << a.b.page_shift) + ((kt0 + 16) & in)) * row_bytes + head_off;
+    return t;
+}
+
+__device__ __forceinline__ float paged_inverse(float L) { return L > 0.0f ? 1.0f / L : (L == 0.0f ? 0.0f : L); }
+
+// ---- at most 16 query rows --------------------------------------------------------
+
+// Bound by the cache's bytes: the waves of a workgroup take every fourth row tile of its share, each
+// with a tile's K and V in registers (32 KB in flight a wave, two workgroups a CU at head_dim 256).
+template <int HD>
+struct PagedFewSmem {
+    f16x8 q[HD / 32][64];                   // score operand, lane-major
+    float o[kPagedWaves][HD / 16 * 4][64];  // the waves' outputs
+    float m[kPagedWaves][16], l[kPagedWaves][16];
+};
+
+template <int HD, bool F8>
+__global__ __launch_bounds__(kPagedThreads, HD == 256 ? 2 : 1) void k_paged_few(const PagedAttnArgs a) {
     using D = PagedDims<HD, F8>;
-    __shared__ PagedSmem<HD, C> sm;
+    constexpr int MQ = 16;
+    __shared__ PagedFewSmem<HD> sm;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, g = lane >> 4;
     const unsigned G = a.group;
 
-    PagedScan<C> scan;
+    PagedScan<MQ> scan;
     scan.run(a, lane);
     const unsigned share = scan.share(a);
     const uint64_t first = (uint64_t)blockIdx.x * share;
     if (first >= scan.total) return;  // uniform
     unsigned u = (unsigned)first;
     const unsigned u_end = min(u + share, scan.total);
-    PagedPlace at = paged_place<C>(a, scan, u, lane);
+    PagedPlace at = paged_place<MQ>(a, scan, u, lane);
     const uint32_t row_bytes = a.nkh * HD * D::ES;
-    const unsigned page_rows = 1u << a.b.page_shift;
 
     while (u < u_end) {  // one item or a part of one
-        const unsigned s = __builtin_amdgcn_readfirstlane(at.s);
+        const unsigned i = __builtin_amdgcn_readfirstlane(at.i);
+        const unsigned s = i / a.q_tiles, qt = i % a.q_tiles;
+        const unsigned kvh = __builtin_amdgcn_readfirstlane(at.kvh), off = __builtin_amdgcn_readfirstlane(at.off);
         const PagedSeq sq = paged_seq(a.b, s);
-        const unsigned kvh = __builtin_amdgcn_readfirstlane(at.kvh), qt = __builtin_amdgcn_readfirstlane(at.qt);
-        const PagedSpan sp = paged_span<C>(a, sq, qt);
-        const unsigned off = __builtin_amdgcn_readfirstlane(at.off);
+        const PagedSpan sp = paged_span<MQ>(a, sq, qt);
         const unsigned seg = min(sp.n - off, u_end - u);
-        const unsigned rows = sq.n * G;               // query rows of this (sequence, kv head)
-        const uint64_t head_off = (uint64_t)kvh * HD * D::ES;
+        const unsigned rows = sq.n * G, r0 = qt * MQ + n;
+        const uint32_t head_off = kvh * HD * D::ES;
         const int32_t* table = a.b.table + (uint64_t)s * a.b.table_stride;
 
-        // The query tile into LDS: column n of group c is query row 16 (C qt + c) + n.
         __syncthreads();  // the last segment's combine has read sm
-        for (int i = threadIdx.x; i < C * D::NC * 64; i += kPagedThreads) {
-            const int l = i & 63, c = i / 64 % D::NC, cg = i / 64 / D::NC;
-            const unsigned r = (qt * C + cg) * 16 + (l & 15);
-            f16x8 x = {};
-            if (r < rows) {
-                const unsigned tok = sq.start + r / G;
-                x = ldg<f16x8>(a.q + ((uint64_t)tok * (a.nkh * G) + kvh * G + r % G) * HD + paged_q_elem<F8>(c, l >> 4));
-            }
-            sm.q[cg][c][l] = x;
+        for (int x = threadIdx.x; x < D::NC * 64; x += kPagedThreads) {
+            const int l = x & 63, c = x >> 6;
+            const unsigned r = qt * MQ + (l & 15);
+            f16x8 v = {};
+            if (r < rows)
+                v = ldg<f16x8>(a.q + ((uint64_t)(sq.start + r / G) * (a.nkh * G) + kvh * G + r % G) * HD +
+                               paged_q_elem<F8>(c, l >> 4));
+            sm.q[c][l] = v;
         }
-        // The lane's columns.
-        unsigned jq[C];  // new-token index, or ~0 past the rows
-        int pos[C];
-        uint64_t bits[C];
-#pragma unroll
-        for (int c = 0; c < C; c++) {
-            const unsigned r = (qt * C + c) * 16 + n;
-            jq[c] = r < rows ? r / G : ~0u;
-            const unsigned tok = sq.start + (r < rows ? r / G : 0u);
-            pos[c] = a.b.positions ? max(a.b.positions[tok], 0) : (int)(sq.ctx + (r < rows ? r / G : 0u));
-            bits[c] = a.b.mask ? a.b.mask[(uint64_t)tok * a.b.mask_words] : 0;
-        }
+        PagedCols<1> cols;
+        cols.load(a, sq, r0);
         __syncthreads();
 
-        float m_run[C], l_run[C];
-        f32x4 acc[C][D::NO];
+        float m_run[1] = {-INFINITY}, l_run[1] = {0.0f};
+        f32x4 acc[1][D::NO];
 #pragma unroll
-        for (int c = 0; c < C; c++) {
-            m_run[c] = -INFINITY;
-            l_run[c] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < D::NO; i++) acc[c][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-        }
+        for (int x = 0; x < D::NO; x++) acc[0][x] = f32x4{0.f, 0.f, 0.f, 0.f};
         // Rows that every column attends: committed, and above every window's start.
-        const unsigned clear_hi = sq.ctx;
-        unsigned clear_lo = 0;
-        if (a.window)
-            clear_lo = a.b.positions ? sq.ctx : (unsigned)max((int)(sq.ctx + sq.n) - a.window, 0);
+        const unsigned clear_lo = !a.window ? 0u : a.b.positions ? sq.ctx : (unsigned)max((int)(sq.ctx + sq.n) - a.window, 0);
 
-        unsigned pages0 = 0, pages1 = 0;  // lane i: page of the two 16-row halves of the wave's tile i (of 64)
-        unsigned have = 0;
+        PagedPages pages;
         for (unsigned it = 0, t = wave; t < seg; it++, t += kPagedWaves) {
-            if (it == have) {  // uniform
-                const unsigned r0 = (sp.first + off + wave + kPagedWaves * (it + lane)) * 32;
-                const unsigned p0 = min(r0, sp.hi - 1) >> a.b.page_shift, p1 = min(r0 + 16, sp.hi - 1) >> a.b.page_shift;
-                pages0 = (unsigned)table[p0];
-                pages1 = (unsigned)table[p1];
-                have += 64;
-            }
+            if ((it & 63) == 0) pages.load(a, table, sp.first + off + t, kPagedWaves, sp.hi, lane);
             const unsigned kt0 = (sp.first + off + t) * 32;
-            const unsigned pg0 = lane_value(pages0, it & 63), pg1 = lane_value(pages1, it & 63);
-            const bool ok0 = pg0 < a.b.num_pages, ok1 = pg1 < a.b.num_pages;
-            const unsigned in0 = kt0 & (page_rows - 1), in1 = (kt0 + 16) & (page_rows - 1);
-            const uint64_t at0 = (((uint64_t)(ok0 ? pg0 : 0u) << a.b.page_shift) + in0) * row_bytes + head_off;
-            const uint64_t at1 = (((uint64_t)(ok1 ? pg1 : 0u) << a.b.page_shift) + in1) * row_bytes + head_off;
+            const PagedAt pa = paged_at(a, pages, it & 63, kt0, row_bytes, head_off);
             u32x4 kr[2][D::KP];
-            u32x4 vr[D::VP][8];
-            paged_load_k<HD, F8>(a.k + at0, row_bytes, n, g, kr[0]);
-            paged_load_k<HD, F8>(a.k + at1, row_bytes, n, g, kr[1]);
-            paged_load_v<HD, F8>(a.v + at0, a.v + at1, row_bytes, n, g, vr);
+            PagedV<HD, F8> vr;
+            paged_load_k<HD, F8>(a.k + pa.half0, row_bytes, n, g, kr[0]);
+            paged_load_k<HD, F8>(a.k + pa.half1, row_bytes, n, g, kr[1]);
+            paged_load_v<HD, F8>(a.v + pa.half0, a.v + pa.half1, row_bytes, n, g, vr);
 
-            f32x4 sc[C][2];
-#pragma unroll
-            for (int c = 0; c < C; c++)
-#pragma unroll
-                for (int h = 0; h < 2; h++) sc[c][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+            f32x4 sc[1][2] = {{f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}}};
 #pragma unroll
             for (int ch = 0; ch < D::NC; ch++) {
-                const f16x8 k0 = paged_k_chunk<HD, F8>(kr[0], ch), k1 = paged_k_chunk<HD, F8>(kr[1], ch);
+                const f16x8 qv = sm.q[ch][lane];
 #pragma unroll
-                for (int c = 0; c < C; c++) {
-                    const f16x8 qv = sm.q[c][ch][lane];
-                    sc[c][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qv, sc[c][0], 0, 0, 0);
-                    sc[c][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qv, sc[c][1], 0, 0, 0);
-                }
+                for (int h = 0; h < 2; h++)
+                    sc[0][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(paged_k_chunk<HD, F8>(kr[h], ch), qv, sc[0][h], 0, 0, 0);
             }
-            const bool clear = kt0 >= clear_lo && kt0 + 32 <= clear_hi && ok0 && ok1;
-            unsigned seen[C];  // bit t: column c of this lane attends the lane's row t
-#pragma unroll
-            for (int c = 0; c < C; c++) seen[c] = 0xffu;
+            const bool clear = kt0 >= clear_lo && kt0 + 32 <= sq.ctx && pa.ok0 && pa.ok1;
+            unsigned seen[1], dead = 0;
             if (!clear) {
-#pragma unroll
-                for (int c = 0; c < C; c++) seen[c] = 0;
-                unsigned dead = 0;
-                for (int t8 = 0; t8 < 8; t8++) {
-                    const unsigned row = kt0 + (t8 < 4 ? 0 : 16) + 4 * g + (t8 & 3);
-                    if (row >= sp.hi || !(t8 < 4 ? ok0 : ok1)) {
-                        dead |= 1u << t8;
-                        continue;
-                    }
-                    const unsigned dj = row - sq.ctx;  // new-token index (row >= ctx)
-                    int rpos = (int)row;
-                    if (row >= sq.ctx && a.window && a.b.positions) rpos = max(a.b.positions[sq.start + dj], 0);
-#pragma unroll
-                    for (int c = 0; c < C; c++) {
-                        bool ok = jq[c] != ~0u;
-                        if (row >= sq.ctx) {
-                            if (a.b.mask) {
-                                uint64_t word = bits[c];
-                                if (a.b.mask_words > 1 && ok)
-                                    word = a.b.mask[(uint64_t)(sq.start + jq[c]) * a.b.mask_words + (dj >> 6)];
-                                ok = ok && ((word >> (dj & 63)) & 1);
-                            } else {
-                                ok = ok && dj <= jq[c];
-                            }
-                        }
-                        if (a.window) ok = ok && rpos > pos[c] - a.window;
-                        seen[c] |= (ok ? 1u : 0u) << t8;
-                    }
-                }
+                cols.look(a, sq, sp.hi, kt0, g, pa.ok0, pa.ok1, seen, dead);
 #pragma unroll
                 for (int t8 = 0; t8 < 8; t8++)
                     if (dead >> t8 & 1) {
@@ -466,217 +530,382 @@ __global__ __launch_bounds__(kPagedThreads, C == 1 && HD == 256 ? 2 : 1) void k_
                         for (int b = 0; b < D::VP; b++) vr[b][t8] = u32x4{0u, 0u, 0u, 0u};
                     }
             }
-            f16x8 hi[C], lo[C];
-#pragma unroll
-            for (int c = 0; c < C; c++) {
-                float sv[8];
-                float tmax = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    float x = sc[c][i >> 2][i & 3] * a.scale;
-                    if (a.cap > 0.0f) x = a.cap * paged_tanh(x * a.inv_cap);
-                    sv[i] = seen[c] >> i & 1 ? x : -INFINITY;
-                    tmax = fmaxf(tmax, sv[i]);
-                }
-                tmax = max_xor16(tmax);  // the column's rows lie in four lane groups
-                tmax = max_xor32(tmax);
-                const float m_new = fmaxf(m_run[c], tmax);
-                if (__any(m_new > m_run[c])) {
-                    const float alpha = m_new == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m_run[c] - m_new) * kLog2e);
-                    l_run[c] *= alpha;
-#pragma unroll
-                    for (int i = 0; i < D::NO; i++) acc[c][i] *= alpha;
-                }
-                m_run[c] = m_new;
-                const float base = m_new == -INFINITY ? 0.0f : m_new;
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float p = __builtin_amdgcn_exp2f((sv[i] - base) * kLog2e);
-                    l_run[c] += p;
-                    const f16 h = (f16)p;
-                    hi[c][i] = h;
-                    lo[c][i] = (f16)(p - (float)h);
-                }
-            }
+            f16x8 hi[1], lo[1];
+            paged_softmax<HD, 1, F8>(a, sc, seen, clear, m_run, l_run, acc, hi, lo);
             // Rows that only some columns attend may hold Inf or NaN, and 0 times those is no 0: they are
             // left out of the products and added to the columns that attend them.
-            uint32_t odd_rows = 0;  // bit 4 t + g: the row t of lane group g; uniform
+            uint32_t odd_rows = 0;
             if (!clear) {
-                unsigned odd = 0;
 #pragma unroll
-                for (int b = 0; b < D::VP; b++)
-#pragma unroll
-                    for (int t8 = 0; t8 < 8; t8++)
-#pragma unroll
-                        for (int w = 0; w < 4; w++) odd |= odd_elements<F8>(vr[b][t8][w]);
-                if (__any(odd != 0)) {
-                    const unsigned mine = paged_take_odd<HD, F8>(vr);
-                    for (int t8 = 0; t8 < 8; t8++) {
-                        const uint64_t b = __ballot(mine >> t8 & 1);
-                        for (int gg = 0; gg < 4; gg++) odd_rows |= (b >> (16 * gg) & 0xffff ? 1u : 0u) << (4 * t8 + gg);
-                    }
-                }
+                for (int b = 0; b < D::VP; b++) odd_rows |= paged_take_odd<F8>(vr[b]);
             }
-            paged_pv<HD, C, F8>(vr, hi, lo, acc);
+#pragma unroll
+            for (int b = 0; b < D::VP; b++) {
+                paged_pv<HD, 1, F8>(b, vr[b], hi, lo, acc);
+                if constexpr (HD == 512) __builtin_amdgcn_sched_barrier(0);
+            }
             while (odd_rows) {
                 const int bit = __builtin_ctz(odd_rows), t8 = bit >> 2, gg = bit & 3;
                 odd_rows &= odd_rows - 1;
-                const char* row = a.v + (t8 < 4 ? at0 : at1) + (uint32_t)(4 * gg + (t8 & 3)) * row_bytes;
-#pragma unroll
-                for (int c = 0; c < C; c++)
-                    paged_add_odd<HD, F8>(row, g, __shfl(seen[c], 16 * gg + n) >> t8 & 1, acc[c]);
+                paged_add_odd<HD, F8>(a.v + (t8 < 4 ? pa.half0 : pa.half1) + (uint32_t)(4 * gg + (t8 & 3)) * row_bytes, g,
+                                      __shfl(seen[0], 16 * gg + n) >> t8 & 1, acc[0]);
             }
         }
 
-        // The four waves' states joined: maxima first, then a query group's outputs at a time.
+        // The four waves' states joined.
         const bool whole = seg == sp.n;
-        const unsigned slot = 2 * blockIdx.x + (off ? 0u : 1u);  // a part that begins its item, or continues one
-#pragma unroll
-        for (int c = 0; c < C; c++) {
-            float l = add_xor16(l_run[c]);
+        const unsigned slot = 2 * blockIdx.x + (off ? 0u : 1u);  // a part that continues its item, or begins it
+        {
+            float l = add_xor16(l_run[0]);
             l = add_xor32(l);
             if (g == 0) {
-                sm.m[wave][16 * c + n] = m_run[c];
-                sm.l[wave][16 * c + n] = l;
+                sm.m[wave][n] = m_run[0];
+                sm.l[wave][n] = l;
             }
         }
         __syncthreads();
+        float M = -INFINITY, L = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kPagedWaves; w++) M = fmaxf(M, sm.m[w][n]);
+        const float base = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+        for (int w = 0; w < kPagedWaves; w++) L += sm.l[w][n] * __builtin_amdgcn_exp2f(sm.m[w][n] - base);
+        const float f = __builtin_amdgcn_exp2f(m_run[0] - base);
+#pragma unroll
+        for (int x = 0; x < D::NO; x++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) sm.o[wave][x * 4 + j][lane] = acc[0][x][j] * f;
+        __syncthreads();
+        if (r0 < rows) {
+            const float inv = whole ? paged_inverse(L) : 1.0f;
+            float* dst = whole ? a.out + ((uint64_t)(sq.start + r0 / G) * (a.nkh * G) + kvh * G + r0 % G) * HD
+                               : a.part_o + ((uint64_t)slot * MQ + n) * HD;
+            if (!whole && wave == 0 && g == 0) stg<f32x2>(a.part_ml + ((uint64_t)slot * MQ + n) * 2, f32x2{M, L});
+            const int j = wave;  // of the 4 rows 4g + j of every output tile
+#pragma unroll
+            for (int b = 0; b < D::VP; b++)
+#pragma unroll
+                for (int e = 0; e < D::E; e += 4) {
+                    f32x4 x;
+#pragma unroll
+                    for (int y = 0; y < 4; y++) {
+                        const int k = (b * D::E + e + y) * 4 + j;
+                        x[y] = ((sm.o[0][k][lane] + sm.o[1][k][lane]) + (sm.o[2][k][lane] + sm.o[3][k][lane])) * inv;
+                    }
+                    stg<f32x4>(dst + 16 * D::E * b + D::E * (4 * g + j) + e, x);
+                }
+        }
+        u += seg;
+        if (u < u_end) paged_next<MQ>(a, at);
+    }
+}
+
+// ---- more query rows -----------------------------------------------------------------
+
+// W waves, each with 16 C of the tile's 16 C W query rows (its query in registers, its own maxima and
+// sums), over the same row tiles: K and V rows come to LDS by DMA, NB tiles in a ring, the next
+// ones requested while one is worked on; one barrier a tile. A row's 16-byte pieces are stored at
+// piece ^ (row % 16), which spreads both operands' reads over all banks (sixteen lanes read sixteen
+// rows of K, or sixteen pieces of one row of V).
+template <int HD, bool F8, int NB>
+struct PagedTileSmem {
+    unsigned char t[NB][2][32][HD * (F8 ? 1 : 2)];  // [ring][K, V][row]
+};
+
+// Waits until at most `n` of the wave's DMA requests are outstanding, and for the other waves.
+template <int N>
+__device__ __forceinline__ void dma_barrier() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+template <int HD, int C, int W, int NB, bool F8, int WPS>
+__global__ __launch_bounds__(64 * W, WPS) void k_paged_tile(const PagedAttnArgs a) {
+    using D = PagedDims<HD, F8>;
+    constexpr int MQ = 16 * C * W;
+    constexpr uint32_t RB = HD * D::ES;        // a row's bytes
+    constexpr uint32_t PPR = RB / 16;          // pieces a row
+    constexpr uint32_t RPI = 1024 / RB;        // rows a DMA instruction moves
+    constexpr int IH = 16 / RPI;               // instructions a 16-row half
+    constexpr int PER = 4 * IH / W;            // of a tile's instructions, a wave's
+    static_assert(4 * IH % W == 0 && (PER % IH == 0 || IH % PER == 0), "whole instructions a wave");
+    __shared__ __align__(1024) PagedTileSmem<HD, F8, NB> sm;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = lane & 15, g = lane >> 4;
+    const unsigned G = a.group;
+
+    PagedScan<MQ> scan;
+    scan.run(a, lane);
+    const unsigned share = scan.share(a);
+    const uint64_t first = (uint64_t)blockIdx.x * share;
+    if (first >= scan.total) return;  // uniform
+    unsigned u = (unsigned)first;
+    const unsigned u_end = min(u + share, scan.total);
+    PagedPlace at = paged_place<MQ>(a, scan, u, lane);
+    const uint32_t row_bytes = a.nkh * RB;
+
+    // The lane's places in a tile: K row n (+ 16), pieces 4 c + g; V rows 4 g + t (+ 16), pieces n (+ 16).
+    uint32_t k_at[4], v_at[4];
+#pragma unroll
+    for (int x = 0; x < 4; x++) {
+        k_at[x] = n * RB + (((4 * x + g) ^ n) << 4);
+        v_at[x] = (4 * g + x) * RB + ((n ^ (4 * g + x)) << 4);
+    }
+
+    while (u < u_end) {  // one item or a part of one
+        const unsigned i = __builtin_amdgcn_readfirstlane(at.i);
+        const unsigned s = i / a.q_tiles, qt = i % a.q_tiles;
+        const unsigned kvh = __builtin_amdgcn_readfirstlane(at.kvh), off = __builtin_amdgcn_readfirstlane(at.off);
+        const PagedSeq sq = paged_seq(a.b, s);
+        const PagedSpan sp = paged_span<MQ>(a, sq, qt);
+        const unsigned seg = min(sp.n - off, u_end - u);
+        const unsigned rows = sq.n * G;
+        const unsigned w0 = qt * MQ + wave * (16 * C);  // the wave's first query row
+        const uint32_t head_off = kvh * RB;
+        const int32_t* table = a.b.table + (uint64_t)s * a.b.table_stride;
+        // Rows past the wave's own last token are not its business; rows every one of its columns attends
+        // need no mask.
+        const bool work = w0 < rows;
+        const unsigned j0 = w0 / G, j1 = min((w0 + 16 * C - 1) / G, sq.n - 1);
+        const unsigned wave_hi = !work ? 0u : a.b.mask ? sp.hi : min(sq.ctx + j1 + 1, sp.hi);
+        const unsigned clear_lo = !a.window ? 0u : a.b.positions ? ~0u : (unsigned)max((int)(sq.ctx + j1 + 1) - a.window, 0);
+        const unsigned clear_hi = a.b.mask ? sq.ctx : sq.ctx + min(j0 + 1, sq.n);
+
+        // Page ids of 64 tiles each: the even and the odd groups of 64.
+        PagedPages even, odd;
+        even.load(a, table, sp.first + off, 1, sp.hi, lane);
+        odd = even;
+        auto place = [&](unsigned t) __attribute__((always_inline)) {
+            PagedPages p;
+            p.half0 = t & 64 ? odd.half0 : even.half0;
+            p.half1 = t & 64 ? odd.half1 : even.half1;
+            return paged_at(a, p, t & 63, (sp.first + off + t) * 32, row_bytes, head_off);
+        };
+        auto request = [&](unsigned t) __attribute__((always_inline)) {
+            const PagedAt pa = place(t);
+            const uint32_t ring = (uint32_t)(uintptr_t)&sm.t[t % NB][0][0][0];
+#pragma unroll
+            for (int x = 0; x < PER; x++) {
+                const int idx = wave * PER + x, part = idx / IH, inst = idx % IH;  // K halves, V halves
+                const uint64_t src = (part & 1 ? pa.half1 : pa.half0);
+                const unsigned r = inst * RPI + lane / PPR;  // of the half's 16
+                const uint32_t voff = r * row_bytes + ((lane % PPR ^ r) << 4);
+                lds_dma16_s(voff, uniform_ptr((part < 2 ? a.k : a.v) + src),
+                            __builtin_amdgcn_readfirstlane(ring + part * 16 * RB + inst * 1024));
+            }
+        };
+        __syncthreads();  // the last segment's tiles are read
+#pragma unroll
+        for (int t = 0; t < NB - 1; t++)
+            if ((unsigned)t < seg) request(t);
+
+        f16x8 qr[C][D::NC];
 #pragma unroll
         for (int c = 0; c < C; c++) {
-            float M = -INFINITY, L = 0.0f;
+            const unsigned r = w0 + 16 * c + n;
+            const bool live = r < rows;
+            const uint16_t* src = a.q + ((uint64_t)(sq.start + (live ? r / G : 0u)) * (a.nkh * G) + kvh * G + (live ? r % G : 0u)) * HD;
 #pragma unroll
-            for (int w = 0; w < kPagedWaves; w++) M = fmaxf(M, sm.m[w][16 * c + n]);
-            const float base = M == -INFINITY ? 0.0f : M;
+            for (int ch = 0; ch < D::NC; ch++) {
+                qr[c][ch] = ldg<f16x8>(src + paged_q_elem<F8>(ch, g));
+                if (!live) qr[c][ch] = f16x8{};
+            }
+        }
+        PagedCols<C> cols;
+        cols.load(a, sq, w0 + n);
+        float m_run[C], l_run[C];
+        f32x4 acc[C][D::NO];
 #pragma unroll
-            for (int w = 0; w < kPagedWaves; w++)
-                L += sm.l[w][16 * c + n] * __builtin_amdgcn_exp2f((sm.m[w][16 * c + n] - base) * kLog2e);
-            const float f = __builtin_amdgcn_exp2f((m_run[c] - base) * kLog2e);
+        for (int c = 0; c < C; c++) {
+            m_run[c] = -INFINITY;
+            l_run[c] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < D::NO; i++)
+            for (int x = 0; x < D::NO; x++) acc[c][x] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+
+        for (unsigned t = 0; t < seg; t++) {
+            // Tile t is in LDS once the requests behind it alone are outstanding; then every wave has also
+            // left tile t - 1, whose place takes tile t + NB - 1.
+            const unsigned behind = min(seg - 1 - t, (unsigned)(NB - 2));
+            if (NB > 3 && behind == 2) dma_barrier<(NB > 3 ? 2 * PER : 0)>();
+            else if (NB > 2 && behind == 1) dma_barrier<(NB > 2 ? PER : 0)>();
+            else dma_barrier<0>();
+            const unsigned kt0 = (sp.first + off + t) * 32;
+            const PagedAt pa = place(t);
+            const unsigned ahead = t + NB - 1;
+            if (ahead < seg) {
+                if ((ahead & 63) == 0) {  // the group before last is done with
+                    if (ahead & 64) odd.load(a, table, sp.first + off + ahead, 1, sp.hi, lane);
+                    else even.load(a, table, sp.first + off + ahead, 1, sp.hi, lane);
+                }
+                request(ahead);
+            }
+            if (kt0 >= wave_hi) continue;  // uniform: nothing in it for this wave's rows
+            const unsigned char* kt = &sm.t[t % NB][0][0][0];
+            const unsigned char* vt = &sm.t[t % NB][1][0][0];
+
+            f32x4 sc[C][2];
 #pragma unroll
-                for (int j = 0; j < 4; j++) sm.o[wave][i * 4 + j][lane] = acc[c][i][j] * f;
-            __syncthreads();
-            const unsigned r = (qt * C + c) * 16 + n;
-            if (r < rows) {
-                const float inv = whole ? (L > 0.0f ? 1.0f / L : (L == 0.0f ? 0.0f : L)) : 1.0f;
-                float* dst = whole ? a.out + ((uint64_t)(sq.start + r / G) * (a.nkh * G) + kvh * G + r % G) * HD
-                                   : a.part_o + ((uint64_t)slot * (16 * C) + 16 * c + n) * HD;
-                if (!whole && wave == 0 && g == 0)
-                    stg<f32x2>(a.part_ml + ((uint64_t)slot * (16 * C) + 16 * c + n) * 2, f32x2{M, L});
-                const int j = wave;  // of the 4 rows 4g + j of every output tile
+            for (int c = 0; c < C; c++)
 #pragma unroll
-                for (int b = 0; b < D::VP; b++) {
-                    const int d0 = 16 * D::E * b + D::E * (4 * g + j);
+                for (int h = 0; h < 2; h++) sc[c][h] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int e = 0; e < D::E; e += 4) {
-                        f32x4 x;
+            for (int p = 0; p < D::KP; p++) {
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const int k = (b * D::E + e + i) * 4 + j;
-                            x[i] = ((sm.o[0][k][lane] + sm.o[1][k][lane]) + (sm.o[2][k][lane] + sm.o[3][k][lane])) * inv;
-                        }
-                        stg<f32x4>(dst + d0 + e, x);
+                for (int h = 0; h < 2; h++) {
+                    const u32x4 k1[1] = {*reinterpret_cast<const u32x4*>(kt + k_at[p & 3] + (p >> 2) * 256 + h * 16 * RB)};
+#pragma unroll
+                    for (int y = 0; y < (F8 ? 2 : 1); y++) {
+                        const int ch = F8 ? 2 * p + y : p;
+                        f16x8 kv;
+                        if constexpr (F8)
+                            kv = __builtin_bit_cast(f16x8, u32x4{fp8x2_f16(k1[0][2 * y], false), fp8x2_f16(k1[0][2 * y], true),
+                                                                 fp8x2_f16(k1[0][2 * y + 1], false),
+                                                                 fp8x2_f16(k1[0][2 * y + 1], true)});
+                        else
+                            kv = __builtin_bit_cast(f16x8, k1[0]);
+#pragma unroll
+                        for (int c = 0; c < C; c++)
+                            sc[c][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv, qr[c][ch], sc[c][h], 0, 0, 0);
                     }
                 }
             }
-            __syncthreads();
-        }
-
-        u += seg;
-        at.off = 0;
-        if (u < u_end) {  // the next item: this head's next query tile, the next head, the next sequence with tokens
-            at.qt = qt + 1;
-            at.kvh = kvh;
-            at.s = s;
-            if (at.qt >= paged_q_tiles<C>(a, sq)) {
-                at.qt = 0;
-                at.kvh++;
-                if (at.kvh >= a.nkh) {
-                    at.kvh = 0;
-                    do at.s++;
-                    while (at.s < a.b.n_seqs && paged_seq(a.b, at.s).n == 0);
+            const bool clear = kt0 >= clear_lo && kt0 + 32 <= clear_hi && pa.ok0 && pa.ok1;
+            unsigned seen[C], dead = 0;
+            if (!clear) cols.look(a, sq, sp.hi, kt0, g, pa.ok0, pa.ok1, seen, dead);
+            f16x8 hi[C], lo[C];
+            paged_softmax<HD, C, F8>(a, sc, seen, clear, m_run, l_run, acc, hi, lo);
+            uint32_t odd_rows = 0;  // as in k_paged_few
+#pragma unroll
+            for (int b = 0; b < D::VP; b++) {
+                u32x4 vr[8];
+#pragma unroll
+                for (int x = 0; x < 8; x++)
+                    vr[x] = *reinterpret_cast<const u32x4*>(vt + v_at[x & 3] + (x >> 2) * 16 * RB + b * 256);
+                if (!clear) {
+#pragma unroll
+                    for (int x = 0; x < 8; x++)
+                        if (dead >> x & 1) vr[x] = u32x4{0u, 0u, 0u, 0u};
+                    odd_rows |= paged_take_odd<F8>(vr);
                 }
+                paged_pv<HD, C, F8>(b, vr, hi, lo, acc);
+            }
+            while (odd_rows) {
+                const int bit = __builtin_ctz(odd_rows), t8 = bit >> 2, gg = bit & 3;
+                odd_rows &= odd_rows - 1;
+#pragma unroll
+                for (int c = 0; c < C; c++)
+                    paged_add_odd<HD, F8>(a.v + (t8 < 4 ? pa.half0 : pa.half1) + (uint32_t)(4 * gg + (t8 & 3)) * row_bytes, g,
+                                          __shfl(seen[c], 16 * gg + n) >> t8 & 1, acc[c]);
             }
         }
+
+        const bool whole = seg == sp.n;
+        const unsigned slot = 2 * blockIdx.x + (off ? 0u : 1u);  // a part that continues its item, or begins it
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            float L = add_xor16(l_run[c]);
+            L = add_xor32(L);
+            const unsigned r = w0 + 16 * c + n, rec = wave * (16 * C) + 16 * c + n;
+            if (r < rows) {
+                const float inv = whole ? paged_inverse(L) : 1.0f;
+                float* dst = whole ? a.out + ((uint64_t)(sq.start + r / G) * (a.nkh * G) + kvh * G + r % G) * HD
+                                   : a.part_o + ((uint64_t)slot * MQ + rec) * HD;
+                if (!whole && g == 0) stg<f32x2>(a.part_ml + ((uint64_t)slot * MQ + rec) * 2, f32x2{m_run[c], L});
+#pragma unroll
+                for (int b = 0; b < D::VP; b++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+#pragma unroll
+                        for (int e = 0; e < D::E; e += 4) {
+                            const int x = b * D::E + e;
+                            stg<f32x4>(dst + 16 * D::E * b + D::E * (4 * g + j) + e,
+                                       f32x4{acc[c][x][j], acc[c][x + 1][j], acc[c][x + 2][j], acc[c][x + 3][j]} * inv);
+                        }
+            }
+        }
+        u += seg;
+        if (u < u_end) paged_next<MQ>(a, at);
     }
 }
 
 // ---- the join ------------------------------------------------------------------------
 
 // Workgroup (item, rows): the records of an item that was cut, in the order of its
-// rows. HD / 4 threads a query row. Items beyond the batch's and items that one
-// workgroup had leave at once.
-template <int HD, int C>
-__global__ __launch_bounds__(256) void k_paged_join(const PagedAttnArgs a, uint32_t per_seq) {
+// rows. HD / 4 threads a query row. Items that are none and items that one workgroup
+// had leave at once.
+template <int HD, int MQ>
+__global__ __launch_bounds__(256) void k_paged_join(const PagedAttnArgs a) {
     constexpr unsigned TPR = HD / 4, R = 256 / TPR;
     const unsigned lane = threadIdx.x & 63;
-    const unsigned per_head = per_seq / a.nkh;  // query tiles of a kv head at most
-    const unsigned s = blockIdx.x / per_seq, kvh = blockIdx.x % per_seq / per_head, qt = blockIdx.x % per_head;
+    const unsigned i = blockIdx.x / a.nkh, kvh = blockIdx.x % a.nkh;
+    const unsigned s = i / a.q_tiles, qt = i % a.q_tiles;
     const PagedSeq sq = paged_seq(a.b, s);
-    if (sq.n == 0 || qt >= paged_q_tiles<C>(a, sq)) return;  // uniform
-    // The item's first tile number, and the share.
-    PagedScan<C> scan;
-    unsigned base = 0;
-    for (unsigned s0 = 0; s0 < a.b.n_seqs; s0 += 64) {
-        scan.group(a, s0, lane);
-        if (s >= s0 && s < s0 + 64) base = scan.total + lane_value(scan.incl, s - s0) - lane_value(scan.tiles, s - s0);
+    const unsigned mine = paged_span<MQ>(a, sq, qt).n;
+    const unsigned r16 = blockIdx.y * R + threadIdx.x / TPR, r = qt * MQ + r16;
+    if (mine == 0 || qt * MQ + blockIdx.y * R >= sq.n * a.group) return;  // uniform
+    PagedScan<MQ> scan;
+    unsigned base = 0;  // the item's first tile number
+    for (unsigned i0 = 0; i0 < scan.items(a); i0 += 64) {
+        scan.group(a, i0, lane);
+        if (i >= i0 && i < i0 + 64) base = scan.total + lane_value(scan.incl, i - i0) - lane_value(scan.tiles, i - i0);
         scan.total += lane_value(scan.incl, 63);
     }
+    base += kvh * mine;
     const unsigned share = scan.share(a);
-    unsigned head = 0, mine = 0;
-    const unsigned nq = paged_q_tiles<C>(a, sq);
-    for (unsigned i = 0; i < nq; i++) {
-        const unsigned t = paged_span<C>(a, sq, i).n;
-        if (i < qt) base += t;
-        if (i == qt) mine = t;
-        head += t;
-    }
-    base += kvh * head;
     const unsigned w0 = base / share, w1 = (base + mine - 1) / share;
     if (w0 == w1) return;  // uniform: one workgroup wrote the result
-    const unsigned r16 = blockIdx.y * R + threadIdx.x / TPR, r = qt * (16 * C) + r16;
     if (r >= sq.n * a.group) return;
     const unsigned d = threadIdx.x % TPR * 4;
     // The first record is its workgroup's slot 1, the others continue the item: slot 0.
-    auto rec = [&](unsigned w) __attribute__((always_inline)) { return ((uint64_t)2 * w + (w == w0 ? 1u : 0u)) * (16 * C) + r16; };
+    auto rec = [&](unsigned w) __attribute__((always_inline)) { return ((uint64_t)2 * w + (w == w0 ? 1u : 0u)) * MQ + r16; };
     float M = -INFINITY;
     for (unsigned w = w0; w <= w1; w++) M = fmaxf(M, ldg<f32x2>(a.part_ml + rec(w) * 2)[0]);
     const float ref = M == -INFINITY ? 0.0f : M;
     float L = 0.0f;
     f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
     for (unsigned w = w0; w <= w1; w++) {
         const f32x2 ml = ldg<f32x2>(a.part_ml + rec(w) * 2);
-        const float f = __builtin_amdgcn_exp2f((ml[0] - ref) * kLog2e);
+        const float f = __builtin_amdgcn_exp2f(ml[0] - ref);
         const f32x4 x = ldg<f32x4>(a.part_o + rec(w) * HD + d);
         L += ml[1] * f;
         o += x * f;
     }
-    const float inv = L > 0.0f ? 1.0f / L : (L == 0.0f ? 0.0f : L);
-    stg<f32x4>(a.out + ((uint64_t)(sq.start + r / a.group) * (a.nkh * a.group) + kvh * a.group + r % a.group) * HD + d, o * inv);
+    stg<f32x4>(a.out + ((uint64_t)(sq.start + r / a.group) * (a.nkh * a.group) + kvh * a.group + r % a.group) * HD + d,
+               o * paged_inverse(L));
 }
 
 // ---- host --------------------------------------------------------------------------
 
 struct PagedPlan {
-    unsigned c, wgs;
-    uint64_t q_tiles;  // of a kv head, at most
+    unsigned mq, wgs;
+    uint64_t q_tiles;  // of a sequence and kv head, at most
     size_t bytes;
 };
 static PagedPlan paged_plan(unsigned head_dim, unsigned num_kv_heads, unsigned num_q_heads, const PagedBatchDev& b) {
     PagedPlan p;
     const uint64_t rows = (uint64_t)b.max_tokens * (num_q_heads / num_kv_heads);
-    p.c = 1;
-    p.q_tiles = (rows + 16 * p.c - 1) / (16 * p.c);
-    p.wgs = device_cus() * (p.c == 1 && head_dim == 256 ? 2 : 1);
-    p.bytes = (size_t)2 * p.wgs * 16 * p.c * (head_dim + 2) * sizeof(float);
+    p.mq = rows <= 16 ? 16 : rows <= 64 || head_dim == 512 ? 64 : 128;
+    p.q_tiles = (rows + p.mq - 1) / p.mq;
+    p.wgs = device_cus() * (head_dim == 256 && p.mq < 128 ? 2 : 1);
+    p.bytes = (size_t)2 * p.wgs * p.mq * (head_dim + 2) * sizeof(float);
     return p;
 }
 
-template <int HD, int C, bool F8>
+template <int HD, bool F8>
 static void launch_paged(const PagedAttnArgs& a, const PagedPlan& p, hipStream_t st) {
-    G4_LAUNCH((k_paged_attn<HD, C, F8>), dim3(p.wgs), dim3(kPagedThreads), 0, st, a);
-    const uint32_t per_seq = (uint32_t)p.q_tiles * a.nkh;
-    G4_LAUNCH((k_paged_join<HD, C>), dim3(a.b.n_seqs * per_seq, 16 * C * HD / 4 / 256), dim3(256), 0, st, a, per_seq);
+    const dim3 grid(p.wgs), items(a.b.n_seqs * a.q_tiles * a.nkh, p.mq * HD / 4 / 256);
+    if (p.mq == 16) {
+        G4_LAUNCH((k_paged_few<HD, F8>), grid, dim3(kPagedThreads), 0, st, a);
+        G4_LAUNCH((k_paged_join<HD, 16>), items, dim3(256), 0, st, a);
+    } else if (p.mq == 64) {
+        G4_LAUNCH((k_paged_tile<HD, 1, 4, F8 ? 4 : 2, F8, HD == 256 ? 2 : 1>), grid, dim3(256), 0, st, a);
+        G4_LAUNCH((k_paged_join<HD, 64>), items, dim3(256), 0, st, a);
+    } else if constexpr (HD == 256) {
+        G4_LAUNCH((k_paged_tile<HD, 1, 8, 4, F8, 2>), grid, dim3(512), 0, st, a);
+        G4_LAUNCH((k_paged_join<HD, 128>), items, dim3(256), 0, st, a);
+    }
 }
 
 }  // namespace g4
@@ -735,23 +964,24 @@ int g4_paged_attn(const g4_paged_cache* cache, const g4_paged_batch* batch, cons
     a.k = static_cast<const char*>(cache->k_pool);
     a.v = static_cast<const char*>(cache->v_pool);
     a.part_o = static_cast<float*>(workspace);
-    a.part_ml = a.part_o + (size_t)2 * plan.wgs * 16 * plan.c * cache->head_dim;
+    a.part_ml = a.part_o + (size_t)2 * plan.wgs * plan.mq * cache->head_dim;
     a.nkh = cache->num_kv_heads;
     a.group = p->num_q_heads / cache->num_kv_heads;
     a.window = p->sliding_window > (1u << 30) ? 0 : (int32_t)p->sliding_window;  // positions are below 2^31 - 2^30
-    a.scale = p->scale;
-    a.cap = p->softcap;
-    a.inv_cap = p->softcap > 0.0f ? 1.0f / p->softcap : 0.0f;
+    a.q_tiles = (uint32_t)plan.q_tiles;
+    a.qscale = p->scale * kLog2e;
+    a.cap_scale = p->softcap > 0.0f ? p->scale / p->softcap : 0.0f;
+    a.cap_log2 = p->softcap * kLog2e;
     a.wgs = plan.wgs;
     a.min_share = 8;
     hipStream_t st = as_stream(stream);
     const bool f8 = cache->dtype == G4_KV_E4M3;
     if (cache->head_dim == 512) {
-        if (f8) launch_paged<512, 1, true>(a, plan, st);
-        else launch_paged<512, 1, false>(a, plan, st);
+        if (f8) launch_paged<512, true>(a, plan, st);
+        else launch_paged<512, false>(a, plan, st);
     } else {
-        if (f8) launch_paged<256, 1, true>(a, plan, st);
-        else launch_paged<256, 1, false>(a, plan, st);
+        if (f8) launch_paged<256, true>(a, plan, st);
+        else launch_paged<256, false>(a, plan, st);
     }
     G4_CHECK_LAUNCH("pagedAttn");
     return G4_OK;
