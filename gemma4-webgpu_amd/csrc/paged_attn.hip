@@ -52,13 +52,13 @@ struct PagedAttnArgs {
 
 // ---- the items ----------------------------------------------------------------
 
-// Row tiles of query tile qt (MQ query rows) of a sequence: [first, first + n), n >= 1
+// Row tiles (UR rows) of query tile qt (MQ query rows) of a sequence: [first, first + n), n >= 1
 // where it has such a tile, 0 otherwise. hi: one past the last row that any of its
 // tokens attends.
 struct PagedSpan {
     unsigned first, n, hi;
 };
-template <int MQ>
+template <int MQ, int UR>
 __device__ __forceinline__ PagedSpan paged_span(const PagedAttnArgs& a, const PagedSeq& sq, unsigned qt) {
     PagedSpan s{};
     if (qt * MQ >= sq.n * a.group) return s;
@@ -70,8 +70,8 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedAttnArgs& a, const Pa
         const int at = (int)(sq.ctx + (a.b.positions || a.b.mask ? 0u : j0)) - a.window + 1;
         lo = min((unsigned)max(at, 0), sq.ctx);
     }
-    s.first = min(lo, s.hi - 1) / 32;
-    s.n = (s.hi + 31) / 32 - s.first;
+    s.first = min(lo, s.hi - 1) / UR;
+    s.n = (s.hi + UR - 1) / UR - s.first;
     return s;
 }
 
@@ -87,18 +87,30 @@ __device__ __forceinline__ unsigned lane_value(unsigned x, unsigned lane) {
     return __builtin_amdgcn_readlane(x, lane);
 }
 
+// x, with whatever is computed from it computed where it stands: lane addresses of a loop's ends would
+// otherwise be computed ahead of the loop and held through it.
+__device__ __forceinline__ int not_hoisted(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+__device__ __forceinline__ unsigned uniform(unsigned x) { return __builtin_amdgcn_readfirstlane(x); }
+
 // The batch's row tiles, as a wave sees them: lane l holds query tile i0 + l of all
 // sequences' (q_tiles each, in order) and its row tiles for all kv heads.
-template <int MQ>
+template <int MQ, int UR>
 struct PagedScan {
     unsigned total = 0;
     unsigned tiles = 0, incl = 0;
+    PagedSeq sq{};
 
     __device__ __forceinline__ static unsigned items(const PagedAttnArgs& a) { return a.b.n_seqs * a.q_tiles; }
     __device__ __forceinline__ void group(const PagedAttnArgs& a, unsigned i0, unsigned lane) {
         const unsigned i = i0 + lane;
         tiles = 0;
-        if (i < items(a)) tiles = paged_span<MQ>(a, paged_seq(a.b, i / a.q_tiles), i % a.q_tiles).n * a.nkh;
+        if (i < items(a)) {
+            sq = paged_seq(a.b, i / a.q_tiles);
+            tiles = paged_span<MQ, UR>(a, sq, i % a.q_tiles).n * a.nkh;
+        }
         incl = wave_scan(tiles, lane);
     }
     __device__ __forceinline__ void run(const PagedAttnArgs& a, unsigned lane) {
@@ -118,9 +130,10 @@ struct PagedPlace {
     unsigned i;    // sequence * q_tiles + query tile
     unsigned kvh;
     unsigned off;  // tiles of the item before it
+    PagedSeq sq;
 };
-template <int MQ>
-__device__ __forceinline__ PagedPlace paged_place(const PagedAttnArgs& a, PagedScan<MQ>& scan, unsigned u, unsigned lane) {
+template <int MQ, int UR>
+__device__ __forceinline__ PagedPlace paged_place(const PagedAttnArgs& a, PagedScan<MQ, UR>& scan, unsigned u, unsigned lane) {
     PagedPlace p{};
     unsigned before = 0;
     for (unsigned i0 = 0;; i0 += 64) {
@@ -134,20 +147,24 @@ __device__ __forceinline__ PagedPlace paged_place(const PagedAttnArgs& a, PagedS
             p.i = i0 + l;
             p.kvh = rem / per_head;
             p.off = rem % per_head;
+            p.sq = PagedSeq{lane_value(scan.sq.start, l), lane_value(scan.sq.n, l), lane_value(scan.sq.ctx, l)};
             return p;
         }
         before += all;
     }
 }
 // The item after p's: the next kv head, or the next query tile that there is.
-template <int MQ>
+template <int MQ, int UR>
 __device__ __forceinline__ void paged_next(const PagedAttnArgs& a, PagedPlace& p) {
     p.off = 0;
     if (++p.kvh < a.nkh) return;
     p.kvh = 0;
     const unsigned items = a.b.n_seqs * a.q_tiles;
-    do p.i++;
-    while (p.i < items && paged_span<MQ>(a, paged_seq(a.b, p.i / a.q_tiles), p.i % a.q_tiles).n == 0);
+    do {
+        p.i++;
+        if (p.i >= items) return;
+        p.sq = paged_seq(a.b, p.i / a.q_tiles);
+    } while (paged_span<MQ, UR>(a, p.sq, p.i % a.q_tiles).n == 0);
 }
 
 // ---- cache tiles ----------------------------------------------------------------
@@ -193,7 +210,7 @@ __device__ __forceinline__ void paged_load_k(const char* base, uint32_t row_byte
                                              u32x4 (&kr)[PagedDims<HD, F8>::KP]) {
     const uint32_t off = (uint32_t)n * row_bytes + (uint32_t)g * 16u;
 #pragma unroll
-    for (int c = 0; c < PagedDims<HD, F8>::KP; c++) kr[c] = ldg<u32x4>(base + (off + c * 64u));
+    for (int c = 0; c < PagedDims<HD, F8>::KP; c++) kr[c] = ldg_stream<u32x4>(base + (off + c * 64u));
 }
 // The two 16-row halves of V: lane (n, g) piece n of rows 4g + t of either half (t < 4: the first).
 template <int HD, bool F8>
@@ -204,7 +221,7 @@ __device__ __forceinline__ void paged_load_v(const char* base0, const char* base
     for (int t = 0; t < 8; t++)
 #pragma unroll
         for (int b = 0; b < PagedDims<HD, F8>::VP; b++)
-            vr[b][t] = ldg<u32x4>((t < 4 ? base0 : base1) + (off + (uint32_t)(t & 3) * row_bytes + b * 256u));
+            vr[b][t] = ldg_stream<u32x4>((t < 4 ? base0 : base1) + (off + (uint32_t)(t & 3) * row_bytes + b * 256u));
 }
 
 // tanh(x) to f32 accuracy (logprobs.hip has the derivation).
@@ -292,6 +309,7 @@ __device__ __forceinline__ uint32_t paged_take_odd(u32x4 (&vr)[8]) {
 template <int HD, bool F8>
 __device__ __forceinline__ void paged_add_odd(const char* row, int g, bool attends, f32x4 (&acc)[PagedDims<HD, F8>::NO]) {
     using D = PagedDims<HD, F8>;
+    g = not_hoisted(g);
 #pragma unroll
     for (int i = 0; i < D::NO; i++) {
 #pragma unroll
@@ -306,33 +324,37 @@ __device__ __forceinline__ void paged_add_odd(const char* row, int g, bool atten
     }
 }
 
+// Waits for the wave's loads (vmcnt 0, the other counters as they are). Stands at the end of code that
+// runs now and then and loads: left to the compiler, the wait would be put where that code's paths meet
+// the common one, and there wait for every request of the pipeline, tile after tile.
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0F70); }
+
 // ---- a row tile against a lane's query columns ------------------------------------
 
-// Column n of the lane's query groups (group c: 16 query rows).
+// Column n of the lane's query groups (group c: 16 query rows from r0 on).
 template <int C>
 struct PagedCols {
-    unsigned j[C];     // new-token index; ~0: no row
-    int pos[C];
-    uint64_t bits[C];  // the mask's first word
+    unsigned j[C];  // new-token index; ~0: no row
 
     __device__ __forceinline__ void load(const PagedAttnArgs& a, const PagedSeq& sq, unsigned r0) {
 #pragma unroll
-        for (int c = 0; c < C; c++) {
-            const unsigned r = r0 + 16 * c;
-            const bool live = r < sq.n * a.group;
-            const unsigned jj = live ? r / a.group : 0u, tok = sq.start + jj;
-            j[c] = live ? jj : ~0u;
-            pos[c] = a.b.positions ? max(a.b.positions[tok], 0) : (int)(sq.ctx + jj);
-            bits[c] = a.b.mask ? a.b.mask[(uint64_t)tok * a.b.mask_words] : 0;
-        }
+        for (int c = 0; c < C; c++) j[c] = r0 + 16 * c < sq.n * a.group ? (r0 + 16 * c) / a.group : ~0u;
     }
     // seen[c] bit t: the column attends the lane's row t of the tile at kt0 (rows 4g + t, and
     // 16 + 4g + t - 4 from t = 4 on). dead: the rows nobody may read (past the last, or without a page).
     __device__ __forceinline__ void look(const PagedAttnArgs& a, const PagedSeq& sq, unsigned hi, unsigned kt0, int g, bool ok0,
                                          bool ok1, unsigned (&seen)[C], unsigned& dead) const {
+        int pos[C];
+        uint64_t bits[C];  // the mask's first word
 #pragma unroll
-        for (int c = 0; c < C; c++) seen[c] = 0;
+        for (int c = 0; c < C; c++) {
+            seen[c] = 0;
+            const unsigned jj = j[c] != ~0u ? j[c] : 0u, tok = sq.start + jj;
+            pos[c] = a.window && a.b.positions ? max(a.b.positions[tok], 0) : (int)(sq.ctx + jj);
+            bits[c] = a.b.mask ? a.b.mask[(uint64_t)tok * a.b.mask_words] : 0;
+        }
         dead = 0;
+        g = not_hoisted(g);
 #pragma unroll 1
         for (int t = 0; t < 8; t++) {
             const unsigned row = kt0 + (t < 4 ? 0 : 16) + 4 * g + (t & 3);
@@ -359,30 +381,40 @@ struct PagedCols {
                 seen[c] |= (ok ? 1u : 0u) << t;
             }
         }
+        wait_loads();
     }
 };
 
-// The online softmax of a tile's scores (log2 units): the running maximum moves once a score
-// is 8 above it (P stays within f16), P leaves as f16 and its residual.
-template <int HD, int C, bool F8>
-__device__ __forceinline__ void paged_softmax(const PagedAttnArgs& a, const f32x4 (&sc)[C][2], const unsigned (&seen)[C],
-                                              bool clear, float (&m_run)[C], float (&l_run)[C],
-                                              f32x4 (&acc)[C][PagedDims<HD, F8>::NO], f16x8 (&hi)[C], f16x8 (&lo)[C]) {
+// How a wave takes a 32-row tile: not at all, as it is, or masked.
+enum PagedTake { kSkip, kClear, kMasked };
+
+// The online softmax of NX tiles' scores (log2 units), together: the running maximum moves once a
+// score is 8 above it (P stays within f16), P leaves as f16 and its residual.
+template <int HD, int C, bool F8, int NX>
+__device__ __forceinline__ void paged_softmax(const PagedAttnArgs& a, const f32x4 (&sc)[NX][C][2], const unsigned (&seen)[NX][C],
+                                              const PagedTake (&how)[NX], float (&m_run)[C], float (&l_run)[C],
+                                              f32x4 (&acc)[C][PagedDims<HD, F8>::NO], f16x8 (&hi)[NX][C], f16x8 (&lo)[NX][C]) {
 #pragma unroll
     for (int c = 0; c < C; c++) {
-        float sv[8];
+        float sv[NX][8];
         float tmax = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float x = sc[c][i >> 2][i & 3];
-            sv[i] = a.cap_log2 > 0.0f ? a.cap_log2 * paged_tanh(x * a.cap_scale) : x * a.qscale;
-        }
-        if (!clear) {
+        for (int x = 0; x < NX; x++) {
+            if (a.cap_log2 > 0.0f) {  // uniform, once a tile
 #pragma unroll
-            for (int i = 0; i < 8; i++) sv[i] = seen[c] >> i & 1 ? sv[i] : -INFINITY;
-        }
+                for (int i = 0; i < 8; i++) sv[x][i] = a.cap_log2 * paged_tanh(sc[x][c][i >> 2][i & 3] * a.cap_scale);
+            } else {
 #pragma unroll
-        for (int i = 0; i < 8; i++) tmax = fmaxf(tmax, sv[i]);
+                for (int i = 0; i < 8; i++) sv[x][i] = sc[x][c][i >> 2][i & 3] * a.qscale;
+            }
+            if (how[x] != kClear) {
+                const unsigned keep = how[x] == kSkip ? 0u : seen[x][c];
+#pragma unroll
+                for (int i = 0; i < 8; i++) sv[x][i] = keep >> i & 1 ? sv[x][i] : -INFINITY;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) tmax = fmaxf(tmax, sv[x][i]);
+        }
         tmax = max_xor16(tmax);  // the column's rows lie in four lane groups
         tmax = max_xor32(tmax);
         const bool move = tmax > m_run[c] + 8.0f;
@@ -396,16 +428,18 @@ __device__ __forceinline__ void paged_softmax(const PagedAttnArgs& a, const f32x
         }
         const float base = m_run[c] == -INFINITY ? 0.0f : m_run[c];
 #pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-            const float p0 = __builtin_amdgcn_exp2f(sv[i] - base), p1 = __builtin_amdgcn_exp2f(sv[i + 1] - base);
-            l_run[c] += p0 + p1;
-            const f16x2 h = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(p0, p1));
-            const f16x2 r = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(p0 - (float)h[0], p1 - (float)h[1]));
-            hi[c][i] = h[0];
-            hi[c][i + 1] = h[1];
-            lo[c][i] = r[0];
-            lo[c][i + 1] = r[1];
-        }
+        for (int x = 0; x < NX; x++)
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                const float p0 = __builtin_amdgcn_exp2f(sv[x][i] - base), p1 = __builtin_amdgcn_exp2f(sv[x][i + 1] - base);
+                l_run[c] += p0 + p1;
+                const f16x2 h = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(p0, p1));
+                const f16x2 r = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(p0 - (float)h[0], p1 - (float)h[1]));
+                hi[x][c][i] = h[0];
+                hi[x][c][i + 1] = h[1];
+                lo[x][c][i] = r[0];
+                lo[x][c][i + 1] = r[1];
+            }
     }
 }
 
@@ -437,282 +471,75 @@ __device__ __forceinline__ PagedAt paged_at(const PagedAttnArgs& a, const PagedP
 
 __device__ __forceinline__ float paged_inverse(float L) { return L > 0.0f ? 1.0f / L : (L == 0.0f ? 0.0f : L); }
 
-// ---- at most 16 query rows --------------------------------------------------------
+// ---- at most 32 query rows --------------------------------------------------------
 
 // Bound by the cache's bytes: the waves of a workgroup take every fourth row tile of its share, each
-// with a tile's K and V in registers (32 KB in flight a wave, two workgroups a CU at head_dim 256).
-template <int HD>
+// with a tile's K and V in registers: the next tile's K is requested when the scores have used this
+// one's, its V when the products have.
+template <int HD, int C>
 struct PagedFewSmem {
-    f16x8 q[HD / 32][64];                   // score operand, lane-major
-    float o[kPagedWaves][HD / 16 * 4][64];  // the waves' outputs
-    float m[kPagedWaves][16], l[kPagedWaves][16];
+    f16x8 q[C][HD / 32][64];                // score operand, lane-major
+    float o[kPagedWaves][HD / 16 * 4][64];  // one query group's outputs, per wave
+    float m[kPagedWaves][16 * C], l[kPagedWaves][16 * C];
 };
 
-template <int HD, bool F8>
-__global__ __launch_bounds__(kPagedThreads, HD == 256 ? 2 : 1) void k_paged_few(const PagedAttnArgs a) {
+template <int HD, int C, bool F8>
+__global__ __launch_bounds__(kPagedThreads, 1) void k_paged_few(const PagedAttnArgs a) {
     using D = PagedDims<HD, F8>;
-    constexpr int MQ = 16;
-    __shared__ PagedFewSmem<HD> sm;
+    constexpr int MQ = 16 * C, UR = 32;
+    __shared__ PagedFewSmem<HD, C> sm;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, g = lane >> 4;
     const unsigned G = a.group;
 
-    PagedScan<MQ> scan;
+    PagedScan<MQ, UR> scan;
     scan.run(a, lane);
     const unsigned share = scan.share(a);
     const uint64_t first = (uint64_t)blockIdx.x * share;
     if (first >= scan.total) return;  // uniform
     unsigned u = (unsigned)first;
     const unsigned u_end = min(u + share, scan.total);
-    PagedPlace at = paged_place<MQ>(a, scan, u, lane);
+    PagedPlace at = paged_place<MQ, UR>(a, scan, u, lane);
     const uint32_t row_bytes = a.nkh * HD * D::ES;
 
     while (u < u_end) {  // one item or a part of one
-        const unsigned i = __builtin_amdgcn_readfirstlane(at.i);
+        const unsigned i = uniform(at.i);
         const unsigned s = i / a.q_tiles, qt = i % a.q_tiles;
-        const unsigned kvh = __builtin_amdgcn_readfirstlane(at.kvh), off = __builtin_amdgcn_readfirstlane(at.off);
-        const PagedSeq sq = paged_seq(a.b, s);
-        const PagedSpan sp = paged_span<MQ>(a, sq, qt);
+        const unsigned kvh = uniform(at.kvh), off = uniform(at.off);
+        const PagedSeq sq{uniform(at.sq.start), uniform(at.sq.n), uniform(at.sq.ctx)};
+        const PagedSpan sp = paged_span<MQ, UR>(a, sq, qt);
         const unsigned seg = min(sp.n - off, u_end - u);
-        const unsigned rows = sq.n * G, r0 = qt * MQ + n;
+        const unsigned rows = sq.n * G;
         const uint32_t head_off = kvh * HD * D::ES;
         const int32_t* table = a.b.table + (uint64_t)s * a.b.table_stride;
 
-        __syncthreads();  // the last segment's combine has read sm
-        for (int x = threadIdx.x; x < D::NC * 64; x += kPagedThreads) {
-            const int l = x & 63, c = x >> 6;
-            const unsigned r = qt * MQ + (l & 15);
-            f16x8 v = {};
-            if (r < rows)
-                v = ldg<f16x8>(a.q + ((uint64_t)(sq.start + r / G) * (a.nkh * G) + kvh * G + r % G) * HD +
-                               paged_q_elem<F8>(c, l >> 4));
-            sm.q[c][l] = v;
-        }
-        PagedCols<1> cols;
-        cols.load(a, sq, r0);
-        __syncthreads();
-
-        float m_run[1] = {-INFINITY}, l_run[1] = {0.0f};
-        f32x4 acc[1][D::NO];
-#pragma unroll
-        for (int x = 0; x < D::NO; x++) acc[0][x] = f32x4{0.f, 0.f, 0.f, 0.f};
-        // Rows that every column attends: committed, and above every window's start.
-        const unsigned clear_lo = !a.window ? 0u : a.b.positions ? sq.ctx : (unsigned)max((int)(sq.ctx + sq.n) - a.window, 0);
-
+        // The wave's first tile is requested before the query is read.
         PagedPages pages;
-        for (unsigned it = 0, t = wave; t < seg; it++, t += kPagedWaves) {
-            if ((it & 63) == 0) pages.load(a, table, sp.first + off + t, kPagedWaves, sp.hi, lane);
-            const unsigned kt0 = (sp.first + off + t) * 32;
-            const PagedAt pa = paged_at(a, pages, it & 63, kt0, row_bytes, head_off);
-            u32x4 kr[2][D::KP];
-            PagedV<HD, F8> vr;
+        u32x4 kr[2][D::KP];
+        PagedV<HD, F8> vr;
+        PagedAt pa{};
+        if ((unsigned)wave < seg) {
+            pages.load(a, table, sp.first + off + wave, kPagedWaves, sp.hi, lane);
+            pa = paged_at(a, pages, 0, (sp.first + off + wave) * 32, row_bytes, head_off);
             paged_load_k<HD, F8>(a.k + pa.half0, row_bytes, n, g, kr[0]);
             paged_load_k<HD, F8>(a.k + pa.half1, row_bytes, n, g, kr[1]);
             paged_load_v<HD, F8>(a.v + pa.half0, a.v + pa.half1, row_bytes, n, g, vr);
-
-            f32x4 sc[1][2] = {{f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}}};
-#pragma unroll
-            for (int ch = 0; ch < D::NC; ch++) {
-                const f16x8 qv = sm.q[ch][lane];
-#pragma unroll
-                for (int h = 0; h < 2; h++)
-                    sc[0][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(paged_k_chunk<HD, F8>(kr[h], ch), qv, sc[0][h], 0, 0, 0);
-            }
-            const bool clear = kt0 >= clear_lo && kt0 + 32 <= sq.ctx && pa.ok0 && pa.ok1;
-            unsigned seen[1], dead = 0;
-            if (!clear) {
-                cols.look(a, sq, sp.hi, kt0, g, pa.ok0, pa.ok1, seen, dead);
-#pragma unroll
-                for (int t8 = 0; t8 < 8; t8++)
-                    if (dead >> t8 & 1) {
-#pragma unroll
-                        for (int b = 0; b < D::VP; b++) vr[b][t8] = u32x4{0u, 0u, 0u, 0u};
-                    }
-            }
-            f16x8 hi[1], lo[1];
-            paged_softmax<HD, 1, F8>(a, sc, seen, clear, m_run, l_run, acc, hi, lo);
-            // Rows that only some columns attend may hold Inf or NaN, and 0 times those is no 0: they are
-            // left out of the products and added to the columns that attend them.
-            uint32_t odd_rows = 0;
-            if (!clear) {
-#pragma unroll
-                for (int b = 0; b < D::VP; b++) odd_rows |= paged_take_odd<F8>(vr[b]);
-            }
-#pragma unroll
-            for (int b = 0; b < D::VP; b++) {
-                paged_pv<HD, 1, F8>(b, vr[b], hi, lo, acc);
-                if constexpr (HD == 512) __builtin_amdgcn_sched_barrier(0);
-            }
-            while (odd_rows) {
-                const int bit = __builtin_ctz(odd_rows), t8 = bit >> 2, gg = bit & 3;
-                odd_rows &= odd_rows - 1;
-                paged_add_odd<HD, F8>(a.v + (t8 < 4 ? pa.half0 : pa.half1) + (uint32_t)(4 * gg + (t8 & 3)) * row_bytes, g,
-                                      __shfl(seen[0], 16 * gg + n) >> t8 & 1, acc[0]);
-            }
         }
-
-        // The four waves' states joined.
-        const bool whole = seg == sp.n;
-        const unsigned slot = 2 * blockIdx.x + (off ? 0u : 1u);  // a part that continues its item, or begins it
-        {
-            float l = add_xor16(l_run[0]);
-            l = add_xor32(l);
-            if (g == 0) {
-                sm.m[wave][n] = m_run[0];
-                sm.l[wave][n] = l;
-            }
-        }
-        __syncthreads();
-        float M = -INFINITY, L = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kPagedWaves; w++) M = fmaxf(M, sm.m[w][n]);
-        const float base = M == -INFINITY ? 0.0f : M;
-#pragma unroll
-        for (int w = 0; w < kPagedWaves; w++) L += sm.l[w][n] * __builtin_amdgcn_exp2f(sm.m[w][n] - base);
-        const float f = __builtin_amdgcn_exp2f(m_run[0] - base);
-#pragma unroll
-        for (int x = 0; x < D::NO; x++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) sm.o[wave][x * 4 + j][lane] = acc[0][x][j] * f;
-        __syncthreads();
-        if (r0 < rows) {
-            const float inv = whole ? paged_inverse(L) : 1.0f;
-            float* dst = whole ? a.out + ((uint64_t)(sq.start + r0 / G) * (a.nkh * G) + kvh * G + r0 % G) * HD
-                               : a.part_o + ((uint64_t)slot * MQ + n) * HD;
-            if (!whole && wave == 0 && g == 0) stg<f32x2>(a.part_ml + ((uint64_t)slot * MQ + n) * 2, f32x2{M, L});
-            const int j = wave;  // of the 4 rows 4g + j of every output tile
-#pragma unroll
-            for (int b = 0; b < D::VP; b++)
-#pragma unroll
-                for (int e = 0; e < D::E; e += 4) {
-                    f32x4 x;
-#pragma unroll
-                    for (int y = 0; y < 4; y++) {
-                        const int k = (b * D::E + e + y) * 4 + j;
-                        x[y] = ((sm.o[0][k][lane] + sm.o[1][k][lane]) + (sm.o[2][k][lane] + sm.o[3][k][lane])) * inv;
-                    }
-                    stg<f32x4>(dst + 16 * D::E * b + D::E * (4 * g + j) + e, x);
-                }
-        }
-        u += seg;
-        if (u < u_end) paged_next<MQ>(a, at);
-    }
-}
-
-// ---- more query rows -----------------------------------------------------------------
-
-// W waves, each with 16 C of the tile's 16 C W query rows (its query in registers, its own maxima and
-// sums), over the same row tiles: K and V rows come to LDS by DMA, NB tiles in a ring, the next
-// ones requested while one is worked on; one barrier a tile. A row's 16-byte pieces are stored at
-// piece ^ (row % 16), which spreads both operands' reads over all banks (sixteen lanes read sixteen
-// rows of K, or sixteen pieces of one row of V).
-template <int HD, bool F8, int NB>
-struct PagedTileSmem {
-    unsigned char t[NB][2][32][HD * (F8 ? 1 : 2)];  // [ring][K, V][row]
-};
-
-// Waits until at most `n` of the wave's DMA requests are outstanding, and for the other waves.
-template <int N>
-__device__ __forceinline__ void dma_barrier() {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
-}
-
-template <int HD, int C, int W, int NB, bool F8, int WPS>
-__global__ __launch_bounds__(64 * W, WPS) void k_paged_tile(const PagedAttnArgs a) {
-    using D = PagedDims<HD, F8>;
-    constexpr int MQ = 16 * C * W;
-    constexpr uint32_t RB = HD * D::ES;        // a row's bytes
-    constexpr uint32_t PPR = RB / 16;          // pieces a row
-    constexpr uint32_t RPI = 1024 / RB;        // rows a DMA instruction moves
-    constexpr int IH = 16 / RPI;               // instructions a 16-row half
-    constexpr int PER = 4 * IH / W;            // of a tile's instructions, a wave's
-    static_assert(4 * IH % W == 0 && (PER % IH == 0 || IH % PER == 0), "whole instructions a wave");
-    __shared__ __align__(1024) PagedTileSmem<HD, F8, NB> sm;
-    const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int n = lane & 15, g = lane >> 4;
-    const unsigned G = a.group;
-
-    PagedScan<MQ> scan;
-    scan.run(a, lane);
-    const unsigned share = scan.share(a);
-    const uint64_t first = (uint64_t)blockIdx.x * share;
-    if (first >= scan.total) return;  // uniform
-    unsigned u = (unsigned)first;
-    const unsigned u_end = min(u + share, scan.total);
-    PagedPlace at = paged_place<MQ>(a, scan, u, lane);
-    const uint32_t row_bytes = a.nkh * RB;
-
-    // The lane's places in a tile: K row n (+ 16), pieces 4 c + g; V rows 4 g + t (+ 16), pieces n (+ 16).
-    uint32_t k_at[4], v_at[4];
-#pragma unroll
-    for (int x = 0; x < 4; x++) {
-        k_at[x] = n * RB + (((4 * x + g) ^ n) << 4);
-        v_at[x] = (4 * g + x) * RB + ((n ^ (4 * g + x)) << 4);
-    }
-
-    while (u < u_end) {  // one item or a part of one
-        const unsigned i = __builtin_amdgcn_readfirstlane(at.i);
-        const unsigned s = i / a.q_tiles, qt = i % a.q_tiles;
-        const unsigned kvh = __builtin_amdgcn_readfirstlane(at.kvh), off = __builtin_amdgcn_readfirstlane(at.off);
-        const PagedSeq sq = paged_seq(a.b, s);
-        const PagedSpan sp = paged_span<MQ>(a, sq, qt);
-        const unsigned seg = min(sp.n - off, u_end - u);
-        const unsigned rows = sq.n * G;
-        const unsigned w0 = qt * MQ + wave * (16 * C);  // the wave's first query row
-        const uint32_t head_off = kvh * RB;
-        const int32_t* table = a.b.table + (uint64_t)s * a.b.table_stride;
-        // Rows past the wave's own last token are not its business; rows every one of its columns attends
-        // need no mask.
-        const bool work = w0 < rows;
-        const unsigned j0 = w0 / G, j1 = min((w0 + 16 * C - 1) / G, sq.n - 1);
-        const unsigned wave_hi = !work ? 0u : a.b.mask ? sp.hi : min(sq.ctx + j1 + 1, sp.hi);
-        const unsigned clear_lo = !a.window ? 0u : a.b.positions ? ~0u : (unsigned)max((int)(sq.ctx + j1 + 1) - a.window, 0);
-        const unsigned clear_hi = a.b.mask ? sq.ctx : sq.ctx + min(j0 + 1, sq.n);
-
-        // Page ids of 64 tiles each: the even and the odd groups of 64.
-        PagedPages even, odd;
-        even.load(a, table, sp.first + off, 1, sp.hi, lane);
-        odd = even;
-        auto place = [&](unsigned t) __attribute__((always_inline)) {
-            PagedPages p;
-            p.half0 = t & 64 ? odd.half0 : even.half0;
-            p.half1 = t & 64 ? odd.half1 : even.half1;
-            return paged_at(a, p, t & 63, (sp.first + off + t) * 32, row_bytes, head_off);
-        };
-        auto request = [&](unsigned t) __attribute__((always_inline)) {
-            const PagedAt pa = place(t);
-            const uint32_t ring = (uint32_t)(uintptr_t)&sm.t[t % NB][0][0][0];
-#pragma unroll
-            for (int x = 0; x < PER; x++) {
-                const int idx = wave * PER + x, part = idx / IH, inst = idx % IH;  // K halves, V halves
-                const uint64_t src = (part & 1 ? pa.half1 : pa.half0);
-                const unsigned r = inst * RPI + lane / PPR;  // of the half's 16
-                const uint32_t voff = r * row_bytes + ((lane % PPR ^ r) << 4);
-                lds_dma16_s(voff, uniform_ptr((part < 2 ? a.k : a.v) + src),
-                            __builtin_amdgcn_readfirstlane(ring + part * 16 * RB + inst * 1024));
-            }
-        };
-        __syncthreads();  // the last segment's tiles are read
-#pragma unroll
-        for (int t = 0; t < NB - 1; t++)
-            if ((unsigned)t < seg) request(t);
-
-        f16x8 qr[C][D::NC];
-#pragma unroll
-        for (int c = 0; c < C; c++) {
-            const unsigned r = w0 + 16 * c + n;
-            const bool live = r < rows;
-            const uint16_t* src = a.q + ((uint64_t)(sq.start + (live ? r / G : 0u)) * (a.nkh * G) + kvh * G + (live ? r % G : 0u)) * HD;
-#pragma unroll
-            for (int ch = 0; ch < D::NC; ch++) {
-                qr[c][ch] = ldg<f16x8>(src + paged_q_elem<F8>(ch, g));
-                if (!live) qr[c][ch] = f16x8{};
-            }
+        if (u != (unsigned)first) __syncthreads();  // the last segment's combine has read sm
+        for (int x = not_hoisted(threadIdx.x); x < C * D::NC * 64; x += kPagedThreads) {
+            const int l = x & 63, ch = (x >> 6) % D::NC, c = (x >> 6) / D::NC;
+            const unsigned r = qt * MQ + 16 * c + (l & 15);
+            f16x8 v = {};
+            if (r < rows)
+                v = ldg<f16x8>(a.q + ((uint64_t)(sq.start + r / G) * (a.nkh * G) + kvh * G + r % G) * HD +
+                               paged_q_elem<F8>(ch, l >> 4));
+            sm.q[c][ch][l] = v;
         }
         PagedCols<C> cols;
-        cols.load(a, sq, w0 + n);
+        cols.load(a, sq, qt * MQ + (not_hoisted(lane) & 15));
+        __syncthreads();
+
         float m_run[C], l_run[C];
         f32x4 acc[C][D::NO];
 #pragma unroll
@@ -722,73 +549,63 @@ __global__ __launch_bounds__(64 * W, WPS) void k_paged_tile(const PagedAttnArgs 
 #pragma unroll
             for (int x = 0; x < D::NO; x++) acc[c][x] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
+        // Rows that every column attends: committed, and above every window's start.
+        const unsigned clear_lo = !a.window ? 0u : a.b.positions ? sq.ctx : (unsigned)max((int)(sq.ctx + sq.n) - a.window, 0);
 
-        for (unsigned t = 0; t < seg; t++) {
-            // Tile t is in LDS once the requests behind it alone are outstanding; then every wave has also
-            // left tile t - 1, whose place takes tile t + NB - 1.
-            const unsigned behind = min(seg - 1 - t, (unsigned)(NB - 2));
-            if (NB > 3 && behind == 2) dma_barrier<(NB > 3 ? 2 * PER : 0)>();
-            else if (NB > 2 && behind == 1) dma_barrier<(NB > 2 ? PER : 0)>();
-            else dma_barrier<0>();
+        for (unsigned it = 0, t = wave; t < seg; it++, t += kPagedWaves) {
             const unsigned kt0 = (sp.first + off + t) * 32;
-            const PagedAt pa = place(t);
-            const unsigned ahead = t + NB - 1;
-            if (ahead < seg) {
-                if ((ahead & 63) == 0) {  // the group before last is done with
-                    if (ahead & 64) odd.load(a, table, sp.first + off + ahead, 1, sp.hi, lane);
-                    else even.load(a, table, sp.first + off + ahead, 1, sp.hi, lane);
-                }
-                request(ahead);
-            }
-            if (kt0 >= wave_hi) continue;  // uniform: nothing in it for this wave's rows
-            const unsigned char* kt = &sm.t[t % NB][0][0][0];
-            const unsigned char* vt = &sm.t[t % NB][1][0][0];
-
-            f32x4 sc[C][2];
+            f32x4 sc[1][C][2];
 #pragma unroll
             for (int c = 0; c < C; c++)
 #pragma unroll
-                for (int h = 0; h < 2; h++) sc[c][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int h = 0; h < 2; h++) sc[0][c][h] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int p = 0; p < D::KP; p++) {
+            for (int ch = 0; ch < D::NC; ch++) {
+                const f16x8 k0 = paged_k_chunk<HD, F8>(kr[0], ch), k1 = paged_k_chunk<HD, F8>(kr[1], ch);
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const u32x4 k1[1] = {*reinterpret_cast<const u32x4*>(kt + k_at[p & 3] + (p >> 2) * 256 + h * 16 * RB)};
-#pragma unroll
-                    for (int y = 0; y < (F8 ? 2 : 1); y++) {
-                        const int ch = F8 ? 2 * p + y : p;
-                        f16x8 kv;
-                        if constexpr (F8)
-                            kv = __builtin_bit_cast(f16x8, u32x4{fp8x2_f16(k1[0][2 * y], false), fp8x2_f16(k1[0][2 * y], true),
-                                                                 fp8x2_f16(k1[0][2 * y + 1], false),
-                                                                 fp8x2_f16(k1[0][2 * y + 1], true)});
-                        else
-                            kv = __builtin_bit_cast(f16x8, k1[0]);
-#pragma unroll
-                        for (int c = 0; c < C; c++)
-                            sc[c][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv, qr[c][ch], sc[c][h], 0, 0, 0);
-                    }
+                for (int c = 0; c < C; c++) {
+                    const f16x8 qv = sm.q[c][ch][lane];
+                    sc[0][c][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qv, sc[0][c][0], 0, 0, 0);
+                    sc[0][c][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qv, sc[0][c][1], 0, 0, 0);
                 }
             }
-            const bool clear = kt0 >= clear_lo && kt0 + 32 <= clear_hi && pa.ok0 && pa.ok1;
-            unsigned seen[C], dead = 0;
-            if (!clear) cols.look(a, sq, sp.hi, kt0, g, pa.ok0, pa.ok1, seen, dead);
-            f16x8 hi[C], lo[C];
-            paged_softmax<HD, C, F8>(a, sc, seen, clear, m_run, l_run, acc, hi, lo);
-            uint32_t odd_rows = 0;  // as in k_paged_few
+            // The next tile's K into the registers just used (behind a masked tile's work: that needs some).
+            const bool more = t + kPagedWaves < seg;
+            PagedAt pn{};
+            auto next_k = [&]() __attribute__((always_inline)) {
+                paged_load_k<HD, F8>(a.k + pn.half0, row_bytes, n, g, kr[0]);
+                paged_load_k<HD, F8>(a.k + pn.half1, row_bytes, n, g, kr[1]);
+            };
+            if (more) {
+                if (((it + 1) & 63) == 0) pages.load(a, table, sp.first + off + t + kPagedWaves, kPagedWaves, sp.hi, lane);
+                pn = paged_at(a, pages, (it + 1) & 63, kt0 + kPagedWaves * 32, row_bytes, head_off);
+            }
+            const bool clear = kt0 >= clear_lo && kt0 + 32 <= sq.ctx && pa.ok0 && pa.ok1;
+            unsigned seen[1][C], dead = 0;
+            if (!clear) {
+                cols.look(a, sq, sp.hi, kt0, g, pa.ok0, pa.ok1, seen[0], dead);
+#pragma unroll
+                for (int t8 = 0; t8 < 8; t8++)
+                    if (dead >> t8 & 1) {
+#pragma unroll
+                        for (int b = 0; b < D::VP; b++) vr[b][t8] = u32x4{0u, 0u, 0u, 0u};
+                    }
+            }
+            if (clear && more) next_k();
+            f16x8 hi[1][C], lo[1][C];
+            const PagedTake how[1] = {clear ? kClear : kMasked};
+            paged_softmax<HD, C, F8, 1>(a, sc, seen, how, m_run, l_run, acc, hi, lo);
+            // Rows that only some columns attend may hold Inf or NaN, and 0 times those is no 0: they are
+            // left out of the products and added to the columns that attend them.
+            uint32_t odd_rows = 0;
+            if (!clear) {
+#pragma unroll
+                for (int b = 0; b < D::VP; b++) odd_rows |= paged_take_odd<F8>(vr[b]);
+            }
 #pragma unroll
             for (int b = 0; b < D::VP; b++) {
-                u32x4 vr[8];
-#pragma unroll
-                for (int x = 0; x < 8; x++)
-                    vr[x] = *reinterpret_cast<const u32x4*>(vt + v_at[x & 3] + (x >> 2) * 16 * RB + b * 256);
-                if (!clear) {
-#pragma unroll
-                    for (int x = 0; x < 8; x++)
-                        if (dead >> x & 1) vr[x] = u32x4{0u, 0u, 0u, 0u};
-                    odd_rows |= paged_take_odd<F8>(vr);
-                }
-                paged_pv<HD, C, F8>(b, vr, hi, lo, acc);
+                paged_pv<HD, C, F8>(b, vr[b], hi[0], lo[0], acc);
+                if constexpr (HD == 512) __builtin_amdgcn_sched_barrier(0);  // block by block: registers
             }
             while (odd_rows) {
                 const int bit = __builtin_ctz(odd_rows), t8 = bit >> 2, gg = bit & 3;
@@ -796,55 +613,402 @@ __global__ __launch_bounds__(64 * W, WPS) void k_paged_tile(const PagedAttnArgs 
 #pragma unroll
                 for (int c = 0; c < C; c++)
                     paged_add_odd<HD, F8>(a.v + (t8 < 4 ? pa.half0 : pa.half1) + (uint32_t)(4 * gg + (t8 & 3)) * row_bytes, g,
-                                          __shfl(seen[c], 16 * gg + n) >> t8 & 1, acc[c]);
+                                          __shfl(seen[0][c], 16 * gg + n) >> t8 & 1, acc[c]);
+            }
+            if (more) {
+                if (!clear) next_k();
+                paged_load_v<HD, F8>(a.v + pn.half0, a.v + pn.half1, row_bytes, n, g, vr);
+            }
+            pa = pn;
+        }
+
+        // The four waves' states joined: maxima first, then a query group's outputs at a time.
+        const bool whole = seg == sp.n;
+        const unsigned slot = 2 * blockIdx.x + (off ? 0u : 1u);  // a part that continues its item, or begins it
+        const int el = not_hoisted(lane), en = el & 15, eg = el >> 4;
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            float l = add_xor16(l_run[c]);
+            l = add_xor32(l);
+            if (eg == 0) {
+                sm.m[wave][16 * c + en] = m_run[c];
+                sm.l[wave][16 * c + en] = l;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            if (qt * MQ + 16 * c >= rows) break;  // uniform
+            float M = -INFINITY, L = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kPagedWaves; w++) M = fmaxf(M, sm.m[w][16 * c + en]);
+            const float base = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+            for (int w = 0; w < kPagedWaves; w++) L += sm.l[w][16 * c + en] * __builtin_amdgcn_exp2f(sm.m[w][16 * c + en] - base);
+            const float f = __builtin_amdgcn_exp2f(m_run[c] - base);
+            if (c) __syncthreads();
+#pragma unroll
+            for (int x = 0; x < D::NO; x++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) sm.o[wave][x * 4 + j][el] = acc[c][x][j] * f;
+            __syncthreads();
+            const unsigned r = qt * MQ + 16 * c + en, rec = 16 * c + en;
+            if (r < rows) {
+                const float inv = whole ? paged_inverse(L) : 1.0f;
+                float* dst = whole ? a.out + ((uint64_t)(sq.start + r / G) * (a.nkh * G) + kvh * G + r % G) * HD
+                                   : a.part_o + ((uint64_t)slot * MQ + rec) * HD;
+                if (!whole && wave == 0 && eg == 0) stg<f32x2>(a.part_ml + ((uint64_t)slot * MQ + rec) * 2, f32x2{M, L});
+                const int j = wave;  // of the 4 rows 4g + j of every output tile
+#pragma unroll
+                for (int b = 0; b < D::VP; b++)
+#pragma unroll
+                    for (int e = 0; e < D::E; e += 4) {
+                        f32x4 x;
+#pragma unroll
+                        for (int y = 0; y < 4; y++) {
+                            const int k = (b * D::E + e + y) * 4 + j;
+                            x[y] = ((sm.o[0][k][el] + sm.o[1][k][el]) + (sm.o[2][k][el] + sm.o[3][k][el])) * inv;
+                        }
+                        stg<f32x4>(dst + 16 * D::E * b + D::E * (4 * eg + j) + e, x);
+                    }
+            }
+        }
+        u += seg;
+        if (u < u_end) paged_next<MQ, UR>(a, at);
+    }
+}
+
+// ---- more query rows -----------------------------------------------------------------
+
+// WQ x WK waves: 16 of the tile's 16 WQ query rows each (the query in registers), and every WK-th part
+// of a row tile of 32 TS rows, with maxima and sums of their own. K and V come to LDS by DMA, a row
+// tile's K or its V a slot, NS slots in a ring: K, V, K of the next tile and so on, NS - 1 requested
+// ahead; one barrier a slot. A row's 16-byte pieces are stored at piece ^ (row % 16), which spreads
+// both operands' reads over all banks (sixteen lanes read sixteen rows of K, or sixteen pieces of one
+// row of V). NT: the rows are read by one workgroup alone and bypass the caches.
+template <int HD, bool F8, int TS, int NS>
+struct PagedTileSmem {
+    unsigned char t[NS][32 * TS][HD * (F8 ? 1 : 2)];
+};
+
+// Waits until at most behind * PER of the wave's DMA requests are outstanding (behind <= MOST, uniform),
+// and for the other waves.
+template <int MOST, int PER>
+__device__ __forceinline__ void dma_barrier(unsigned behind) {
+    if constexpr (MOST > 0) {
+        if (behind < (unsigned)MOST) {
+            dma_barrier<MOST - 1, PER>(behind);
+            return;
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(MOST * PER) : "memory");
+}
+
+// One LDS-DMA instruction (decode_core.h: lds_dma16_s), for a kernel in which the compiler itself never
+// uses M0 (checked in the assembly: its only writes of it are these).
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // M0 is a reserved register: clobbering it is what is meant
+template <bool NT>
+__device__ __forceinline__ void paged_dma(uint32_t voff, const void* sbase, uint32_t lds) {
+    if constexpr (NT)
+        asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(voff), "s"(sbase), "s"(lds) : "memory", "m0");
+    else
+        asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "s"(lds) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+template <int HD, int WQ, int WK, int TS, int NS, bool F8, bool NT, int WPS>
+__global__ __launch_bounds__(64 * WQ * WK, WPS) void k_paged_tile(const PagedAttnArgs a) {
+    using D = PagedDims<HD, F8>;
+    constexpr int W = WQ * WK, MQ = 16 * WQ, UR = 32 * TS;
+    constexpr int NX = TS / WK;                // 32-row tiles of a slot that a wave works on
+    constexpr uint32_t RB = HD * D::ES;        // a row's bytes
+    constexpr uint32_t PPR = RB / 16;          // pieces a row
+    constexpr uint32_t RPI = 1024 / RB;        // rows a DMA instruction moves
+    constexpr int IH = 16 / RPI;               // instructions 16 rows take
+    constexpr int PER = 2 * TS * IH / W;       // of a slot's instructions, a wave's
+    static_assert(2 * TS * IH % W == 0 && IH % PER == 0 && TS % WK == 0, "whole instructions, of one half, a wave");
+    static_assert((NS - 2) * PER < 64, "outstanding requests are counted in six bits");
+    static_assert(WK == 1 || WQ * HD * 16 * 4 + 2 * MQ * 4 <= NS * UR * (int)RB, "the waves' states are joined in the ring");
+    __shared__ __align__(1024) PagedTileSmem<HD, F8, TS, NS> sm;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wq = wave % WQ, wk = wave / WQ;
+    const int n = lane & 15, g = lane >> 4;
+    const unsigned G = a.group;
+
+    PagedScan<MQ, UR> scan;
+    scan.run(a, lane);
+    const unsigned share = scan.share(a);
+    const uint64_t first = (uint64_t)blockIdx.x * share;
+    if (first >= scan.total) return;  // uniform
+    unsigned u = (unsigned)first;
+    const unsigned u_end = min(u + share, scan.total);
+    PagedPlace at = paged_place<MQ, UR>(a, scan, u, lane);
+    const uint32_t row_bytes = a.nkh * RB;
+
+    // The lane's places in 32 rows: K row n (+ 16), pieces 4 c + g; V rows 4 g + t (+ 16), pieces n (+ 16).
+    uint32_t k_at[4], v_at[4];
+#pragma unroll
+    for (int x = 0; x < 4; x++) {
+        k_at[x] = n * RB + (((4 * x + g) ^ n) << 4);
+        v_at[x] = (4 * g + x) * RB + ((n ^ (4 * g + x)) << 4);
+    }
+    // The wave's DMA instructions: its half of a slot, and the lane's bytes in it.
+    const unsigned dma_half = wave * PER / IH, inst0 = wave * PER % IH;
+    uint32_t dma_off[PER];
+#pragma unroll
+    for (int x = 0; x < PER; x++) {
+        const unsigned r = (inst0 + x) * RPI + lane / PPR;  // of the half's 16 rows
+        dma_off[x] = r * row_bytes + ((lane % PPR ^ r) << 4);
+    }
+
+    while (u < u_end) {  // one item or a part of one
+        const unsigned i = uniform(at.i);
+        const unsigned s = i / a.q_tiles, qt = i % a.q_tiles;
+        const unsigned kvh = uniform(at.kvh), off = uniform(at.off);
+        const PagedSeq sq{uniform(at.sq.start), uniform(at.sq.n), uniform(at.sq.ctx)};
+        const PagedSpan sp = paged_span<MQ, UR>(a, sq, qt);
+        const unsigned seg = min(sp.n - off, u_end - u);
+        const unsigned rows = sq.n * G;
+        const unsigned w0 = qt * MQ + wq * 16;  // the wave's first query row
+        const uint32_t head_off = kvh * RB;
+        const int32_t* table = a.b.table + (uint64_t)s * a.b.table_stride;
+        // Rows past the wave's own last token are not its business; rows every one of its columns attends
+        // need no mask.
+        const bool work = w0 < rows;
+        const unsigned j0 = w0 / G, j1 = min((w0 + 15) / G, sq.n - 1);
+        const unsigned wave_hi = !work ? 0u : a.b.mask ? sp.hi : min(sq.ctx + j1 + 1, sp.hi);
+        const unsigned clear_lo = !a.window ? 0u : a.b.positions ? ~0u : (unsigned)max((int)(sq.ctx + j1 + 1) - a.window, 0);
+        const unsigned clear_hi = a.b.mask ? sq.ctx : sq.ctx + min(j0 + 1, sq.n);
+
+        // The query first: its wait, before the page ids', would otherwise be one for the requests below too.
+        f16x8 qr[D::NC];
+        {
+            const unsigned r = w0 + (not_hoisted(lane) & 15);
+            const bool live = r < rows;
+            const uint16_t* src = a.q + ((uint64_t)(sq.start + (live ? r / G : 0u)) * (a.nkh * G) + kvh * G + (live ? r % G : 0u)) * HD;
+#pragma unroll
+            for (int ch = 0; ch < D::NC; ch++) {
+                qr[ch] = ldg<f16x8>(src + paged_q_elem<F8>(ch, g));
+                if (!live) qr[ch] = f16x8{};
+            }
+        }
+        // Page ids: lane l has those of row tile l of 64, for each 16-row half of it; the even and the odd
+        // groups of 64.
+        unsigned even[2 * TS], odd[2 * TS];
+        auto load_pages = [&](unsigned t, unsigned (&p)[2 * TS]) __attribute__((always_inline)) {
+            const unsigned r = (sp.first + off + t + (unsigned)lane) * UR;
+#pragma unroll
+            for (int h = 0; h < 2 * TS; h++) p[h] = (unsigned)table[min(r + 16 * h, sp.hi - 1) >> a.b.page_shift];
+            wait_loads();
+        };
+        load_pages(0, even);
+#pragma unroll
+        for (int h = 0; h < 2 * TS; h++) odd[h] = 0;
+        auto page_of = [&](unsigned t, int h) __attribute__((always_inline)) -> unsigned {  // h: a constant
+            const unsigned m = t & 64 ? ~0u : 0u;
+            return lane_value((odd[h] & m) | (even[h] & ~m), t & 63);
+        };
+        // Byte offset in a pool of the half's first row (page 0 where there is none).
+        auto half_at = [&](unsigned t, unsigned h, unsigned page) __attribute__((always_inline)) -> uint64_t {
+            const unsigned r = (sp.first + off + t) * UR + 16 * h;
+            return (((uint64_t)(page < a.b.num_pages ? page : 0u) << a.b.page_shift) + (r & ((1u << a.b.page_shift) - 1))) *
+                       row_bytes + head_off;
+        };
+        // Requests slot j (K of row tile j / 2, or its V) into its place of the ring.
+        unsigned ring_in = 0, ring_out = 0;
+        auto request = [&](unsigned j) __attribute__((always_inline)) {
+            const unsigned t = j >> 1;
+            unsigned page = page_of(t, 0);
+#pragma unroll
+            for (int h = 1; h < 2 * TS; h++) {
+                const unsigned p = page_of(t, h);
+                page = dma_half == (unsigned)h ? p : page;
+            }
+            const char* src = uniform_ptr((j & 1 ? a.v : a.k) + half_at(t, dma_half, page));
+            const uint32_t dst = (uint32_t)(uintptr_t)&sm.t[ring_in][0][0] + dma_half * 16 * RB + inst0 * 1024;
+#pragma unroll
+            for (int x = 0; x < PER; x++) paged_dma<NT>(dma_off[x], src, uniform(dst + x * 1024));
+            ring_in = ring_in + 1 == NS ? 0 : ring_in + 1;
+        };
+        // Waits for slot j; every wave has left the one before it then, whose place slot j + NS - 1 takes.
+        const unsigned slots = 2 * seg;
+        auto take = [&](unsigned j) __attribute__((always_inline)) -> const unsigned char* {
+            dma_barrier<NS - 2, PER>(min(slots - 1 - j, (unsigned)(NS - 2)));
+            const unsigned ahead = j + NS - 1;
+            if (ahead < slots) {
+                if ((ahead & 127) == 0) {  // the next 64 tiles' pages; the group before last is done with
+                    if (ahead & 128) load_pages(ahead >> 1, odd);
+                    else load_pages(ahead >> 1, even);
+                }
+                request(ahead);
+            }
+            const unsigned char* p = &sm.t[ring_out][0][0];
+            ring_out = ring_out + 1 == NS ? 0 : ring_out + 1;
+            return p;
+        };
+        __syncthreads();  // the last segment's ring is free
+#pragma unroll
+        for (int j = 0; j < NS - 1; j++)
+            if ((unsigned)j < slots) request(j);
+
+        PagedCols<1> cols;
+        cols.load(a, sq, w0 + n);
+        float m_run[1] = {-INFINITY}, l_run[1] = {0.0f};
+        f32x4 acc[1][D::NO];
+#pragma unroll
+        for (int x = 0; x < D::NO; x++) acc[0][x] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+        for (unsigned t = 0; t < seg; t++) {
+            f16x8 hi[NX][1], lo[NX][1];
+            f32x4 sc[NX][1][2];
+            unsigned seen[NX][1], dead[NX];
+            PagedTake how[NX];
+            bool some = false;
+            const unsigned char* kt = take(2 * t) + wk * NX * 32 * RB;
+#pragma unroll
+            for (int x = 0; x < NX; x++) {
+                const unsigned kt0 = (sp.first + off + t) * UR + (wk * NX + x) * 32;
+                how[x] = kSkip;  // uniform
+                sc[x][0][0] = sc[x][0][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (kt0 >= wave_hi) continue;  // nothing in it for this wave's rows
+                some = true;
+#pragma unroll
+                for (int p = 0; p < D::KP; p++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const u32x4 kv = *reinterpret_cast<const u32x4*>(kt + k_at[p & 3] + (p >> 2) * 256 + (2 * x + h) * 16 * RB);
+                        if constexpr (F8) {
+#pragma unroll
+                            for (int y = 0; y < 2; y++)
+                                sc[x][0][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                    __builtin_bit_cast(f16x8, u32x4{fp8x2_f16(kv[2 * y], false), fp8x2_f16(kv[2 * y], true),
+                                                                    fp8x2_f16(kv[2 * y + 1], false), fp8x2_f16(kv[2 * y + 1], true)}),
+                                    qr[2 * p + y], sc[x][0][h], 0, 0, 0);
+                        } else {
+                            sc[x][0][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, kv), qr[p], sc[x][0][h], 0, 0, 0);
+                        }
+                    }
+                bool ok0 = true, ok1 = true;
+#pragma unroll
+                for (int h = 0; h < 2 * TS; h += 2)
+                    if (h == 2 * (int)(wk * NX + x)) {
+                        ok0 = page_of(t, h) < a.b.num_pages;
+                        ok1 = page_of(t, h + 1) < a.b.num_pages;
+                    }
+                how[x] = kt0 >= clear_lo && kt0 + 32 <= clear_hi && ok0 && ok1 ? kClear : kMasked;
+                if (how[x] == kMasked) cols.look(a, sq, sp.hi, kt0, g, ok0, ok1, seen[x], dead[x]);
+            }
+            if (some) paged_softmax<HD, 1, F8, NX>(a, sc, seen, how, m_run, l_run, acc, hi, lo);
+            const unsigned char* vt = take(2 * t + 1) + wk * NX * 32 * RB;
+#pragma unroll
+            for (int x = 0; x < NX; x++) {
+                const unsigned part = wk * NX + x;
+                if (how[x] == kSkip) continue;
+                uint32_t odd_rows = 0;  // as in k_paged_few
+#pragma unroll
+                for (int b = 0; b < D::VP; b++) {
+                    u32x4 vr[8];
+#pragma unroll
+                    for (int y = 0; y < 8; y++)
+                        vr[y] = *reinterpret_cast<const u32x4*>(vt + v_at[y & 3] + (2 * x + (y >> 2)) * 16 * RB + b * 256);
+                    if (how[x] == kMasked) {
+#pragma unroll
+                        for (int y = 0; y < 8; y++)
+                            if (dead[x] >> y & 1) vr[y] = u32x4{0u, 0u, 0u, 0u};
+                        odd_rows |= paged_take_odd<F8>(vr);
+                    }
+                    paged_pv<HD, 1, F8>(b, vr, hi[x], lo[x], acc);
+                }
+                while (odd_rows) {
+                    const int bit = __builtin_ctz(odd_rows), t8 = bit >> 2, gg = bit & 3;
+                    odd_rows &= odd_rows - 1;
+                    const unsigned half = 2 * part + (t8 >> 2);
+                    unsigned page = page_of(t, 0);
+#pragma unroll
+                    for (int h = 1; h < 2 * TS; h++) {
+                        const unsigned p = page_of(t, h);
+                        page = half == (unsigned)h ? p : page;
+                    }
+                    paged_add_odd<HD, F8>(a.v + half_at(t, half, page) + (uint32_t)(4 * gg + (t8 & 3)) * row_bytes, g,
+                                          __shfl(seen[x][0], 16 * gg + n) >> t8 & 1, acc[0]);
+                }
             }
         }
 
         const bool whole = seg == sp.n;
         const unsigned slot = 2 * blockIdx.x + (off ? 0u : 1u);  // a part that continues its item, or begins it
+        float L = add_xor16(l_run[0]);
+        L = add_xor32(L);
+        float M = m_run[0];
+        if constexpr (WK > 1) {  // the waves of the same query rows joined, in the ring's place
+            static_assert(WK == 2, "two parts");
+            float* so = reinterpret_cast<float*>(&sm.t[0][0][0]);
+            float* sml = so + WQ * HD * 16;
+            __syncthreads();
+            if (wk == 1) {
 #pragma unroll
-        for (int c = 0; c < C; c++) {
-            float L = add_xor16(l_run[c]);
-            L = add_xor32(L);
-            const unsigned r = w0 + 16 * c + n, rec = wave * (16 * C) + 16 * c + n;
-            if (r < rows) {
-                const float inv = whole ? paged_inverse(L) : 1.0f;
-                float* dst = whole ? a.out + ((uint64_t)(sq.start + r / G) * (a.nkh * G) + kvh * G + r % G) * HD
-                                   : a.part_o + ((uint64_t)slot * MQ + rec) * HD;
-                if (!whole && g == 0) stg<f32x2>(a.part_ml + ((uint64_t)slot * MQ + rec) * 2, f32x2{m_run[c], L});
+                for (int x = 0; x < D::NO; x++)
+                    *reinterpret_cast<f32x4*>(so + ((wq * D::NO + x) * 64 + lane) * 4) = acc[0][x];
+                if (g == 0) {
+                    sml[2 * (wq * 16 + n)] = M;
+                    sml[2 * (wq * 16 + n) + 1] = L;
+                }
+            }
+            __syncthreads();
+            if (wk == 0) {
+                const float m2 = sml[2 * (wq * 16 + n)], l2 = sml[2 * (wq * 16 + n) + 1];
+                const float m1 = M;
+                M = fmaxf(m1, m2);
+                const float base = M == -INFINITY ? 0.0f : M;
+                const float f1 = __builtin_amdgcn_exp2f(m1 - base), f2 = __builtin_amdgcn_exp2f(m2 - base);
+                L = L * f1 + l2 * f2;
 #pragma unroll
-                for (int b = 0; b < D::VP; b++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-#pragma unroll
-                        for (int e = 0; e < D::E; e += 4) {
-                            const int x = b * D::E + e;
-                            stg<f32x4>(dst + 16 * D::E * b + D::E * (4 * g + j) + e,
-                                       f32x4{acc[c][x][j], acc[c][x + 1][j], acc[c][x + 2][j], acc[c][x + 3][j]} * inv);
-                        }
+                for (int x = 0; x < D::NO; x++)
+                    acc[0][x] = acc[0][x] * f1 + *reinterpret_cast<const f32x4*>(so + ((wq * D::NO + x) * 64 + lane) * 4) * f2;
             }
         }
+        const unsigned r = w0 + (not_hoisted(lane) & 15);
+        if (wk == 0 && r < rows) {
+            const unsigned rec = r - qt * MQ;
+            const float inv = whole ? paged_inverse(L) : 1.0f;
+            float* dst = whole ? a.out + ((uint64_t)(sq.start + r / G) * (a.nkh * G) + kvh * G + r % G) * HD
+                               : a.part_o + ((uint64_t)slot * MQ + rec) * HD;
+            if (!whole && g == 0) stg<f32x2>(a.part_ml + ((uint64_t)slot * MQ + rec) * 2, f32x2{M, L});
+#pragma unroll
+            for (int b = 0; b < D::VP; b++)
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+#pragma unroll
+                    for (int e = 0; e < D::E; e += 4) {
+                        const int x = b * D::E + e;
+                        stg<f32x4>(dst + 16 * D::E * b + D::E * (4 * g + j) + e,
+                                   f32x4{acc[0][x][j], acc[0][x + 1][j], acc[0][x + 2][j], acc[0][x + 3][j]} * inv);
+                    }
+        }
         u += seg;
-        if (u < u_end) paged_next<MQ>(a, at);
+        if (u < u_end) paged_next<MQ, UR>(a, at);
     }
 }
 
 // ---- the join ------------------------------------------------------------------------
 
-// Workgroup (item, rows): the records of an item that was cut, in the order of its
-// rows. HD / 4 threads a query row. Items that are none and items that one workgroup
-// had leave at once.
-template <int HD, int MQ>
+// The records of an item that was cut, in P groups of consecutive ones, added in order: the records of
+// a group in turn, then the groups. A workgroup takes COLS columns (COLS / 4 threads a group) of
+// R = 256 / (P COLS / 4) query rows. Items that are none and items that one workgroup had leave at once.
+template <int HD, int MQ, int UR, int P, int COLS>
 __global__ __launch_bounds__(256) void k_paged_join(const PagedAttnArgs a) {
-    constexpr unsigned TPR = HD / 4, R = 256 / TPR;
+    constexpr unsigned TPG = COLS / 4, R = 256 / (P * TPG);
+    __shared__ f32x4 so[P > 1 ? 256 : 1];
+    __shared__ f32x2 sml[P > 1 ? 256 : 1];
     const unsigned lane = threadIdx.x & 63;
     const unsigned i = blockIdx.x / a.nkh, kvh = blockIdx.x % a.nkh;
     const unsigned s = i / a.q_tiles, qt = i % a.q_tiles;
     const PagedSeq sq = paged_seq(a.b, s);
-    const unsigned mine = paged_span<MQ>(a, sq, qt).n;
-    const unsigned r16 = blockIdx.y * R + threadIdx.x / TPR, r = qt * MQ + r16;
+    const unsigned mine = paged_span<MQ, UR>(a, sq, qt).n;
     if (mine == 0 || qt * MQ + blockIdx.y * R >= sq.n * a.group) return;  // uniform
-    PagedScan<MQ> scan;
+    PagedScan<MQ, UR> scan;
     unsigned base = 0;  // the item's first tile number
     for (unsigned i0 = 0; i0 < scan.items(a); i0 += 64) {
         scan.group(a, i0, lane);
@@ -855,25 +1019,60 @@ __global__ __launch_bounds__(256) void k_paged_join(const PagedAttnArgs a) {
     const unsigned share = scan.share(a);
     const unsigned w0 = base / share, w1 = (base + mine - 1) / share;
     if (w0 == w1) return;  // uniform: one workgroup wrote the result
-    if (r >= sq.n * a.group) return;
-    const unsigned d = threadIdx.x % TPR * 4;
+    const unsigned grp = threadIdx.x / TPG % P;
+    const unsigned rq = blockIdx.y * R + threadIdx.x / (TPG * P), r = qt * MQ + rq;  // R divides MQ
+    const unsigned d = blockIdx.z * COLS + threadIdx.x % TPG * 4;
     // The first record is its workgroup's slot 1, the others continue the item: slot 0.
-    auto rec = [&](unsigned w) __attribute__((always_inline)) { return ((uint64_t)2 * w + (w == w0 ? 1u : 0u)) * MQ + r16; };
-    float M = -INFINITY;
-    for (unsigned w = w0; w <= w1; w++) M = fmaxf(M, ldg<f32x2>(a.part_ml + rec(w) * 2)[0]);
-    const float ref = M == -INFINITY ? 0.0f : M;
-    float L = 0.0f;
+    auto rec = [&](unsigned w) __attribute__((always_inline)) { return ((uint64_t)2 * w + (w == w0 ? 1u : 0u)) * MQ + rq; };
+    const unsigned per = (w1 - w0 + P) / P;  // records a group
+    const unsigned first = w0 + grp * per, end = min(first + per, w1 + 1);
+    float M = -INFINITY, L = 0.0f;
     f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (unsigned w = w0; w <= w1; w++) {
-        const f32x2 ml = ldg<f32x2>(a.part_ml + rec(w) * 2);
-        const float f = __builtin_amdgcn_exp2f(ml[0] - ref);
-        const f32x4 x = ldg<f32x4>(a.part_o + rec(w) * HD + d);
-        L += ml[1] * f;
-        o += x * f;
+    if (r < sq.n * a.group) {  // rows that are none have no records
+        constexpr int B = 8;  // records requested at once
+        for (unsigned w = first; w < end; w += B) {
+            f32x2 ml[B];
+            f32x4 x[B];
+#pragma unroll
+            for (int k = 0; k < B; k++) {
+                const uint64_t at = rec(min(w + k, end - 1));
+                ml[k] = ldg<f32x2>(a.part_ml + at * 2);
+                x[k] = ldg<f32x4>(a.part_o + at * HD + d);
+            }
+            float m = M;
+#pragma unroll
+            for (int k = 0; k < B; k++) m = fmaxf(m, ml[k][0]);
+            const float ref = m == -INFINITY ? 0.0f : m, f0 = __builtin_amdgcn_exp2f(M - ref);
+            L *= f0;
+            o *= f0;
+#pragma unroll
+            for (int k = 0; k < B; k++) {
+                const float f = w + k < end ? __builtin_amdgcn_exp2f(ml[k][0] - ref) : 0.0f;
+                L += ml[k][1] * f;
+                o += x[k] * f;
+            }
+            M = m;
+        }
     }
-    stg<f32x4>(a.out + ((uint64_t)(sq.start + r / a.group) * (a.nkh * a.group) + kvh * a.group + r % a.group) * HD + d,
-               o * paged_inverse(L));
+    if constexpr (P > 1) {
+        so[threadIdx.x] = o;
+        sml[threadIdx.x] = f32x2{M, L};
+        __syncthreads();
+        if (grp) return;
+        for (unsigned k = 1; k < P; k++) M = fmaxf(M, sml[threadIdx.x + k * TPG][0]);
+        const float ref = M == -INFINITY ? 0.0f : M;
+        L = 0.0f;
+        o = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (unsigned k = 0; k < P; k++) {
+            const f32x2 ml = sml[threadIdx.x + k * TPG];
+            const float f = __builtin_amdgcn_exp2f(ml[0] - ref);
+            L += ml[1] * f;
+            o += so[threadIdx.x + k * TPG] * f;
+        }
+    }
+    if (r < sq.n * a.group)
+        stg<f32x4>(a.out + ((uint64_t)(sq.start + r / a.group) * (a.nkh * a.group) + kvh * a.group + r % a.group) * HD + d,
+                   o * paged_inverse(L));
 }
 
 // ---- host --------------------------------------------------------------------------
@@ -886,25 +1085,45 @@ struct PagedPlan {
 static PagedPlan paged_plan(unsigned head_dim, unsigned num_kv_heads, unsigned num_q_heads, const PagedBatchDev& b) {
     PagedPlan p;
     const uint64_t rows = (uint64_t)b.max_tokens * (num_q_heads / num_kv_heads);
-    p.mq = rows <= 16 ? 16 : rows <= 64 || head_dim == 512 ? 64 : 128;
+    p.mq = rows <= 16 ? 16 : rows <= 32 && head_dim == 256 ? 32 : rows <= 64 || head_dim == 512 ? 64 : 128;
     p.q_tiles = (rows + p.mq - 1) / p.mq;
-    p.wgs = device_cus() * (head_dim == 256 && p.mq < 128 ? 2 : 1);
+    p.wgs = device_cus();
     p.bytes = (size_t)2 * p.wgs * p.mq * (head_dim + 2) * sizeof(float);
     return p;
 }
 
+template <int HD, int MQ, int UR>
+static void launch_join(const PagedAttnArgs& a, hipStream_t st) {
+    const unsigned items = a.b.n_seqs * a.q_tiles * a.nkh;
+    if (items * 16 >= a.wgs) {  // few records an item
+        G4_LAUNCH((k_paged_join<HD, MQ, UR, 1, HD>), dim3(items, MQ * HD / 4 / 256), dim3(256), 0, st, a);
+    } else {
+        G4_LAUNCH((k_paged_join<HD, MQ, UR, 16, 64>), dim3(items, MQ, HD / 64), dim3(256), 0, st, a);
+    }
+}
+
 template <int HD, bool F8>
 static void launch_paged(const PagedAttnArgs& a, const PagedPlan& p, hipStream_t st) {
-    const dim3 grid(p.wgs), items(a.b.n_seqs * a.q_tiles * a.nkh, p.mq * HD / 4 / 256);
+    const dim3 grid(p.wgs);
     if (p.mq == 16) {
-        G4_LAUNCH((k_paged_few<HD, F8>), grid, dim3(kPagedThreads), 0, st, a);
-        G4_LAUNCH((k_paged_join<HD, 16>), items, dim3(256), 0, st, a);
+        G4_LAUNCH((k_paged_few<HD, 1, F8>), grid, dim3(kPagedThreads), 0, st, a);
+        launch_join<HD, 16, 32>(a, st);
+    } else if constexpr (HD == 512) {
+        constexpr int TS = F8 ? 2 : 1;
+        if (p.q_tiles == 1)
+            G4_LAUNCH((k_paged_tile<512, 4, 1, TS, 5, F8, true, 1>), grid, dim3(256), 0, st, a);
+        else
+            G4_LAUNCH((k_paged_tile<512, 4, 1, TS, 5, F8, false, 1>), grid, dim3(256), 0, st, a);
+        launch_join<HD, 64, 32 * TS>(a, st);
+    } else if (p.mq == 32) {
+        G4_LAUNCH((k_paged_few<256, 2, F8>), grid, dim3(kPagedThreads), 0, st, a);
+        launch_join<HD, 32, 32>(a, st);
     } else if (p.mq == 64) {
-        G4_LAUNCH((k_paged_tile<HD, 1, 4, F8 ? 4 : 2, F8, HD == 256 ? 2 : 1>), grid, dim3(256), 0, st, a);
-        G4_LAUNCH((k_paged_join<HD, 64>), items, dim3(256), 0, st, a);
-    } else if constexpr (HD == 256) {
-        G4_LAUNCH((k_paged_tile<HD, 1, 8, 4, F8, 2>), grid, dim3(512), 0, st, a);
-        G4_LAUNCH((k_paged_join<HD, 128>), items, dim3(256), 0, st, a);
+        G4_LAUNCH((k_paged_tile<256, 4, 2, 2, F8 ? 10 : 5, F8, true, 2>), grid, dim3(512), 0, st, a);
+        launch_join<HD, 64, 64>(a, st);
+    } else {
+        G4_LAUNCH((k_paged_tile<256, 8, 1, 2, F8 ? 10 : 5, F8, false, 2>), grid, dim3(512), 0, st, a);
+        launch_join<HD, 128, 64>(a, st);
     }
 }
 
@@ -973,7 +1192,7 @@ int g4_paged_attn(const g4_paged_cache* cache, const g4_paged_batch* batch, cons
     a.cap_scale = p->softcap > 0.0f ? p->scale / p->softcap : 0.0f;
     a.cap_log2 = p->softcap * kLog2e;
     a.wgs = plan.wgs;
-    a.min_share = 8;
+    a.min_share = plan.mq <= 32 ? kPagedWaves : 1;
     hipStream_t st = as_stream(stream);
     const bool f8 = cache->dtype == G4_KV_E4M3;
     if (cache->head_dim == 512) {
