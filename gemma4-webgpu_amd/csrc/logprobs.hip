@@ -2,29 +2,32 @@
 // of logits (g4_token_logprobs): what a step that verifies drafted tokens needs
 // of them, next to the greedy head's argmax (lmhead.hip).
 //
-// z = cap tanh(x / cap) / T (or x / T), m = max z, S = sum e^(z - m),
-// U = sum (z - m) e^(z - m):  log p(i) = z_i - m - log S,  entropy = log S - U / S.
-// Bound by the logits' bytes, read once: a workgroup takes kLpChunk consecutive
+// z = cap tanh(x / cap) (or x), m = max z, t = (z - m) log2(e) / T, S = sum 2^t,
+// U = sum t 2^t:  log p(i) = (t_i - log2 S) ln 2,  entropy = (log2 S - U / S) ln 2.
+// Bound by the logits' bytes, read once: a workgroup takes a chunk of consecutive
 // logits of a row into registers, so the maximum, the sums and the selection all
 // work on what one pass has loaded. z is monotone in x, so maxima and ranks are
-// taken on x itself and each element's z is evaluated once.
+// taken on x itself and each element's z is evaluated once: 2 transcendental
+// operations less one with a cap of 3 an element, and 6 plain ones (9 with a cap),
+// which the loads of the other workgroups on a CU cover.
 //
 // Selection: candidates are 64-bit keys (order-preserving logit in the high half,
 // inverted index in the low half), all different, so equal logits rank by index.
-// The k-th largest of 64 groups' maxima bounds the k-th largest key from below;
-// the few keys at or above it are collected in LDS and ranked by counting. Where
-// that bound lets too many through (logits in ascending order, or most of them
-// -inf), k rounds of a maximum below the last one take their place.
+// The k-th largest of 64 groups' maxima bounds the k-th largest logit from below;
+// the few logits at or above it are collected in LDS and ranked by counting. Where
+// that bound lets too many through (logits in ascending order, or many equal
+// ones), k rounds of a maximum below the last one take their place.
 //
-// Rows longer than a chunk leave (m, S, U) and k keys per chunk in the workspace;
+// Rows longer than a chunk leave (max x, S, U) and k keys per chunk in the workspace;
 // a second launch, a workgroup a row, joins them in a fixed order.
+#include "decode_core.h"
 #include "paged.h"
 
 namespace g4 {
 
 constexpr unsigned kLpThreads = 256;
-constexpr unsigned kLpElems = 32;  // logits a thread holds
-constexpr unsigned kLpChunk = kLpThreads * kLpElems;
+constexpr unsigned kLpShort = 2048;  // logits of a chunk where rows are few: more workgroups, shorter chains
+constexpr unsigned kLpLong = 8192;   // and where they are many (twice as many logits of 16 bits)
 constexpr unsigned kLpMaxK = G4_LOGPROBS_MAX_TOP;
 constexpr unsigned kLpGroups = 64;  // at least kLpMaxK
 constexpr unsigned kLpCandidates = 1024;
@@ -37,11 +40,12 @@ struct LogprobsArgs {
     float* __restrict__ entropy;
     int32_t* __restrict__ top_ids;
     float* __restrict__ top_logprobs;
-    float* __restrict__ part;      // [rows][chunks][4]: m (in z), S, U
+    float* __restrict__ part;      // [rows][chunks][4]: max x, S, U
     uint64_t* __restrict__ cand;   // [rows][chunks][k]
     uint64_t row_stride;
     uint32_t vocab, chunks, k;
-    float cap, inv_cap, temperature, inv_temperature;
+    float cap, cap_exp;  // and 2 log2(e) / cap
+    float slope;         // log2(e) / temperature
 };
 
 template <int DT>
@@ -60,39 +64,14 @@ __device__ __forceinline__ float logit_f32(typename LogitType<DT>::T v) {
     else return __uint_as_float((uint32_t)v << 16);
 }
 
-// tanh(x) to f32 accuracy: below 1/2 the convergent of Lambert's continued
-// fraction x / (1 + x^2 / (3 + x^2 / (5 + ...))) (its relative error there is under
-// 2^-26), above it (1 - t) / (1 + t), t = e^(-2|x|), which loses no more than a bit.
-__device__ __forceinline__ float tanh_f32(float x) {
-    const float ax = fabsf(x), z = x * x;
-    const float t = __builtin_amdgcn_exp2f(-2.0f * kLog2e * ax);
-    const bool small = ax < 0.5f;
-    const float num = small ? ax * (945.0f + z * (105.0f + z)) : 1.0f - t;
-    const float den = small ? 945.0f + z * (420.0f + 15.0f * z) : 1.0f + t;
-    const float y = __builtin_amdgcn_rcpf(den), q = num * y;
-    return copysignf(__builtin_fmaf(__builtin_fmaf(-q, den, num), y, q), x);
+// cap tanh(x / cap) = cap - 2 cap / (e^(2 x / cap) + 1), to a few half-steps of cap. A mask of -inf stays
+// one, and +inf too (it makes the row's sums NaN).
+__device__ __forceinline__ float logit_capped(float x, const LogprobsArgs& a) {
+    const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * a.cap_exp) + 1.0f);
+    const float z = __builtin_fmaf(-2.0f * a.cap, r, a.cap);
+    return fabsf(x) == INFINITY ? x : z;
 }
-
-// e^t for t <= 0 (0 from -200 on): the product's rounding error goes into the result.
-__device__ __forceinline__ float exp_f32(float t) {
-    constexpr float kLo = 1.92596299e-8f;  // log2(e) - kLog2e
-    t = t < -200.0f ? -200.0f : t;         // -inf has no residual; a NaN stays one
-    const float h = t * kLog2e;
-    const float l = __builtin_fmaf(t, kLog2e, -h) + t * kLo;
-    const float e = __builtin_amdgcn_exp2f(h);
-    return __builtin_fmaf(e, l * 0.6931471805599453f, e);
-}
-
-__device__ __forceinline__ float logit_z(float x, const LogprobsArgs& a) {
-    float z = x;
-    if (a.cap > 0.0f && fabsf(x) != INFINITY) z = a.cap * tanh_f32(x * a.inv_cap);  // a mask of -inf stays one
-    if (a.temperature != 1.0f) {
-        const float q = z * a.inv_temperature;  // z / T with the quotient's residual
-        const float r = __builtin_fmaf(-q, a.temperature, z);
-        z = fabsf(z) == INFINITY ? z : __builtin_fmaf(r, a.inv_temperature, q);
-    }
-    return z;
-}
+__device__ __forceinline__ float logit_z(float x, const LogprobsArgs& a) { return a.cap > 0.0f ? logit_capped(x, a) : x; }
 
 // Key of logit x at index i: larger first, equal ones by lower index; 0 for none.
 __device__ __forceinline__ uint32_t logit_order(float x) {
@@ -104,10 +83,9 @@ __device__ __forceinline__ uint64_t logit_key(float x, uint32_t i) {
     const uint32_t o = logit_order(x);
     return o ? ((uint64_t)o << 32) | (uint64_t)(0xFFFFFFFFu - i) : 0;
 }
-__device__ __forceinline__ float key_logit(uint64_t key) {
-    const uint32_t o = (uint32_t)(key >> 32);
-    return __uint_as_float((o & 0x80000000u) ? (o & 0x7FFFFFFFu) : ~o);
-}
+constexpr uint32_t kLpLeast = 0x00800000u;  // the lowest finite logit's order
+__device__ __forceinline__ float order_logit(uint32_t o) { return __uint_as_float((o & 0x80000000u) ? (o & 0x7FFFFFFFu) : ~o); }
+__device__ __forceinline__ float key_logit(uint64_t key) { return order_logit((uint32_t)(key >> 32)); }
 
 __device__ __forceinline__ uint64_t lp_shfl_xor(uint64_t v, int m) {
     const unsigned lo = __shfl_xor((unsigned)v, m), hi = __shfl_xor((unsigned)(v >> 32), m);
@@ -115,50 +93,68 @@ __device__ __forceinline__ uint64_t lp_shfl_xor(uint64_t v, int m) {
 }
 __device__ __forceinline__ uint64_t lp_max(uint64_t x, uint64_t y) { return x > y ? x : y; }
 
+// Sum and maximum over the wave, in every lane: rotations of 16-lane rows, then rows and halves swapped.
+template <int CTRL>
+__device__ __forceinline__ float lp_dpp(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), CTRL, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float lp_wave_sum(float x) {
+    x += lp_dpp<0x128>(x);  // row_ror:8
+    x += lp_dpp<0x124>(x);
+    x += lp_dpp<0x122>(x);
+    x += lp_dpp<0x121>(x);
+    return add_xor32(add_xor16(x));
+}
+__device__ __forceinline__ float lp_wave_max(float x) {
+    x = fmaxf(x, lp_dpp<0x128>(x));
+    x = fmaxf(x, lp_dpp<0x124>(x));
+    x = fmaxf(x, lp_dpp<0x122>(x));
+    x = fmaxf(x, lp_dpp<0x121>(x));
+    return max_xor32(max_xor16(x));
+}
+
 struct LpShared {
-    uint64_t group[kLpGroups];
-    uint32_t rank[kLpGroups];
+    uint32_t group[kLpGroups];
+    uint32_t at_least[kLpGroups];
     uint64_t cand[kLpCandidates];
     uint64_t top[kLpMaxK];
-    uint64_t bound;
+    uint32_t bound;
     uint64_t wave[kLpThreads / 64];
     uint32_t count;
     float red[3][kLpThreads / 64];
 };
 
 // The k largest of the workgroup's keys into sh.top, descending (0 where there
-// are fewer). best: the thread's largest key; each(f) calls f on every key of the
-// thread that may be among them.
+// are fewer). best: the thread's largest logit, as its order; each(bound, f) calls f(key) on every
+// logit of the thread whose order is at least bound (at least kLpLeast).
 template <typename EACH>
-__device__ __forceinline__ void lp_select(LpShared& sh, unsigned k, uint64_t best, EACH&& each) {
+__device__ __forceinline__ void lp_select(LpShared& sh, unsigned k, uint32_t best, EACH&& each) {
     const unsigned t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    uint64_t g = lp_max(best, lp_shfl_xor(best, 1));  // groups of four threads
-    g = lp_max(g, lp_shfl_xor(g, 2));
+    uint32_t g = max(best, (uint32_t)__builtin_amdgcn_mov_dpp((int)best, 0xB1, 0xf, 0xf, false));  // groups of four threads:
+    g = max(g, (uint32_t)__builtin_amdgcn_mov_dpp((int)g, 0x4E, 0xf, 0xf, false));                 // quad_perm 1,0,3,2; 2,3,0,1
     if ((t & 3) == 0) sh.group[t >> 2] = g;
-    if (t < kLpGroups) sh.rank[t] = 0;
+    if (t < kLpGroups) sh.at_least[t] = 0;
     if (t < kLpMaxK) sh.top[t] = 0;
     if (t == 0) {
-        sh.bound = 1;
+        sh.bound = kLpLeast;
         sh.count = 0;
     }
     __syncthreads();
     {
-        const uint64_t mine = sh.group[lane];
-        unsigned above = 0;
+        const uint32_t mine = sh.group[lane];
+        unsigned n = 0;
 #pragma unroll
-        for (unsigned i = 0; i < kLpGroups / 4; i++) above += sh.group[wave * (kLpGroups / 4) + i] > mine;
-        atomicAdd(&sh.rank[lane], above);
+        for (unsigned i = 0; i < kLpGroups / 4; i++) n += sh.group[wave * (kLpGroups / 4) + i] >= mine;
+        atomicAdd(&sh.at_least[lane], n);
     }
     __syncthreads();
-    if (t < kLpGroups && sh.rank[t] == k - 1 && sh.group[t]) sh.bound = sh.group[t];
+    if (t < kLpGroups && sh.at_least[t] >= k) atomicMax(&sh.bound, sh.group[t]);
     __syncthreads();
-    const uint64_t bound = sh.bound;
+    const uint32_t bound = sh.bound;
     if (best >= bound)
-        each([&](uint64_t key) {
-            if (key >= bound) {
-                const unsigned at = atomicAdd(&sh.count, 1u);
-                if (at < kLpCandidates) sh.cand[at] = key;
-            }
+        each(bound, [&](uint64_t key) {
+            const unsigned at = atomicAdd(&sh.count, 1u);
+            if (at < kLpCandidates) sh.cand[at] = key;
         });
     __syncthreads();
     const unsigned n = sh.count;
@@ -166,14 +162,20 @@ __device__ __forceinline__ void lp_select(LpShared& sh, unsigned k, uint64_t bes
         for (unsigned i = t; i < n; i += kLpThreads) {
             const uint64_t key = sh.cand[i];
             unsigned above = 0;
-            for (unsigned j = 0; j < n; j++) above += sh.cand[j] > key;
+            for (unsigned j = 0; j < n; j += 8) {  // eight reads at once
+                uint64_t c[8];
+#pragma unroll
+                for (unsigned e = 0; e < 8; e++) c[e] = sh.cand[min(j + e, n - 1)];
+#pragma unroll
+                for (unsigned e = 0; e < 8; e++) above += j + e < n && c[e] > key;
+            }
             if (above < k) sh.top[above] = key;
         }
     } else {
         uint64_t last = ~0ull;
         for (unsigned r = 0; r < k; r++) {  // uniform
             uint64_t b = 0;
-            each([&](uint64_t key) { b = key < last ? lp_max(b, key) : b; });
+            each(kLpLeast, [&](uint64_t key) { b = key < last ? lp_max(b, key) : b; });
 #pragma unroll
             for (int m = 32; m >= 1; m >>= 1) b = lp_max(b, lp_shfl_xor(b, m));
             if (lane == 0) sh.wave[wave] = b;
@@ -187,33 +189,23 @@ __device__ __forceinline__ void lp_select(LpShared& sh, unsigned k, uint64_t bes
     __syncthreads();
 }
 
-__device__ __forceinline__ float lp_wave_sum(float x) {
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) x += __shfl_xor(x, m);
-    return x;
-}
-__device__ __forceinline__ float lp_wave_max(float x) {
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) x = fmaxf(x, __shfl_xor(x, m));
-    return x;
-}
-
-// A row's results from its (m, S, U) and sh.top.
+// A row's results from its (max x, S, U) and sh.top.
 template <int DT>
-__device__ __forceinline__ void lp_finish(const LogprobsArgs& a, const LpShared& sh, unsigned row, float m, float S, float U) {
+__device__ __forceinline__ void lp_finish(const LogprobsArgs& a, const LpShared& sh, unsigned row, float mx, float S, float U) {
     const unsigned t = threadIdx.x;
+    constexpr float kLn2 = 0.69314718055994531f;
     const float none = __uint_as_float(0x7FC00000u);  // NaN
     const bool ok = S > 0.0f;                         // neither NaN nor empty
-    const float logS = logf(S);
+    const float m = logit_z(mx, a), logS = log2f(S);
     if (t == 0) {
-        if (a.entropy) a.entropy[row] = ok ? logS - U / S : none;
+        if (a.entropy) a.entropy[row] = ok ? (logS - U / S) * kLn2 : none;
         if (a.logprobs) {
             const int32_t tok = a.tokens[row];
             float lp = 0.0f;
             if (tok >= 0 && (uint32_t)tok < a.vocab) {
                 typedef typename LogitType<DT>::T T;
                 const float x = logit_f32<DT>(static_cast<const T*>(a.logits)[row * a.row_stride + (uint32_t)tok]);
-                lp = ok ? (logit_z(x, a) - m) - logS : none;
+                lp = ok ? ((logit_z(x, a) - m) * a.slope - logS) * kLn2 : none;
             }
             a.logprobs[row] = lp;
         }
@@ -222,72 +214,82 @@ __device__ __forceinline__ void lp_finish(const LogprobsArgs& a, const LpShared&
         const uint64_t key = sh.top[t];
         a.top_ids[(uint64_t)row * a.k + t] = key ? (int32_t)(0xFFFFFFFFu - (uint32_t)key) : -1;
         a.top_logprobs[(uint64_t)row * a.k + t] =
-            !ok ? none : key ? (logit_z(key_logit(key), a) - m) - logS : -INFINITY;
+            !ok ? none : key ? ((logit_z(key_logit(key), a) - m) * a.slope - logS) * kLn2 : -INFINITY;
     }
 }
 
-// One chunk of one row. VEC: 16-byte loads (rows aligned), otherwise one element a load.
-template <int DT, bool VEC>
+// One chunk of one row, E logits a thread. VEC: 16-byte loads (rows aligned), otherwise one element a load.
+template <int DT, bool VEC, int E>
 __global__ __launch_bounds__(kLpThreads) void k_logprobs(const LogprobsArgs a) {
     typedef typename LogitType<DT>::T T;
-    constexpr unsigned V = VEC ? 16 / sizeof(T) : 1;  // elements a load
-    constexpr unsigned N = kLpElems / V;
+    constexpr int V = VEC ? 16 / sizeof(T) : 1;  // elements a load
+    constexpr int N = E / V, P = sizeof(T) == 2 ? 2 : 1;  // logits a register
+    static_assert(E % V == 0 && E % P == 0, "whole loads and registers");
     __shared__ LpShared sh;
     const unsigned t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const unsigned chunk = blockIdx.x, row = blockIdx.y;
-    const unsigned i0 = chunk * kLpChunk;
+    const unsigned i0 = chunk * (kLpThreads * E);
     const T* src = static_cast<const T*>(a.logits) + row * a.row_stride;
-    float x[kLpElems];
-    if (i0 + kLpChunk <= a.vocab) {
+    uint32_t raw[E / P];
+    auto index_of = [&](int i) __attribute__((always_inline)) { return i0 + (i / V * kLpThreads + t) * V + i % V; };
+    auto logit = [&](int i) __attribute__((always_inline)) -> float {  // i: a constant
+        if constexpr (P == 1) return __uint_as_float(raw[i]);
+        else return logit_f32<DT>((T)(raw[i / 2] >> (16 * (i & 1))));
+    };
+    if (i0 + kLpThreads * E <= a.vocab) {
         if constexpr (VEC) {
-            u32x4 v[N];
 #pragma unroll
-            for (unsigned i = 0; i < N; i++)
-                v[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(src + i0 + (i * kLpThreads + t) * V));
+            for (int i = 0; i < N; i++) {
+                const u32x4 v = ldg_stream<u32x4>(src + i0 + (i * kLpThreads + t) * V);
 #pragma unroll
-            for (unsigned i = 0; i < N; i++)
-#pragma unroll
-                for (unsigned e = 0; e < V; e++) {
-                    if constexpr (sizeof(T) == 4) x[i * V + e] = __uint_as_float(v[i][e]);
-                    else x[i * V + e] = logit_f32<DT>((uint16_t)(v[i][e / 2] >> (16 * (e & 1))));
-                }
+                for (int e = 0; e < 4; e++) raw[4 * i + e] = v[e];
+            }
         } else {
+            T v[E];
 #pragma unroll
-            for (unsigned i = 0; i < kLpElems; i++) x[i] = logit_f32<DT>(src[i0 + i * kLpThreads + t]);
+            for (int i = 0; i < E; i++) v[i] = src[index_of(i)];
+#pragma unroll
+            for (int i = 0; i < E; i += P) {
+                if constexpr (P == 1) raw[i] = __builtin_bit_cast(uint32_t, v[i]);
+                else raw[i / 2] = (uint32_t)v[i] | (uint32_t)v[i + 1] << 16;
+            }
         }
     } else {
+        const T none = P == 1 ? (T)-INFINITY : DT == G4_LOGITS_F16 ? (T)0xFC00 : (T)0xFF80;  // -inf
+        T v[E];
 #pragma unroll
-        for (unsigned i = 0; i < N; i++)
+        for (int i = 0; i < E; i++) v[i] = index_of(i) < a.vocab ? src[index_of(i)] : none;
 #pragma unroll
-            for (unsigned e = 0; e < V; e++) {
-                const unsigned at = i0 + (i * kLpThreads + t) * V + e;
-                x[i * V + e] = at < a.vocab ? logit_f32<DT>(src[at]) : -INFINITY;
-            }
+        for (int i = 0; i < E; i += P) {
+            if constexpr (P == 1) raw[i] = __builtin_bit_cast(uint32_t, v[i]);
+            else raw[i / 2] = (uint32_t)v[i] | (uint32_t)v[i + 1] << 16;
+        }
     }
 
     float mx = -INFINITY;
-    uint32_t mi = 0;  // the first place of the thread's maximum
 #pragma unroll
-    for (unsigned i = 0; i < kLpElems; i++) {
-        if (x[i] > mx) {
-            mx = x[i];
-            mi = i;
-        }
-    }
-    auto index_of = [&](unsigned i) __attribute__((always_inline)) { return i0 + (i / V * kLpThreads + t) * V + i % V; };
+    for (int i = 0; i < E; i++) mx = fmaxf(mx, logit(i));  // leaves NaN aside
     const float wmax = lp_wave_max(mx);
     if (lane == 0) sh.red[0][wave] = wmax;
     __syncthreads();
     const float xmax = fmaxf(fmaxf(sh.red[0][0], sh.red[0][1]), fmaxf(sh.red[0][2], sh.red[0][3]));
-    const float m = xmax == -INFINITY ? -INFINITY : logit_z(xmax, a);
-    const float base = m == -INFINITY ? 0.0f : m;
+    const float m = xmax == -INFINITY ? 0.0f : logit_z(xmax, a);
     float S = 0.0f, U = 0.0f;
+    // 2^t is 0 from -200 on, where t 2^t must not become -inf times 0; a NaN goes on in S.
+    if (a.cap > 0.0f) {
 #pragma unroll
-    for (unsigned i = 0; i < kLpElems; i++) {
-        const float d = logit_z(x[i], a) - base;
-        const float e = exp_f32(d);
-        S += e;
-        U += e == 0.0f ? 0.0f : d * e;
+        for (int i = 0; i < E; i++) {
+            const float d = (logit_capped(logit(i), a) - m) * a.slope, e = __builtin_amdgcn_exp2f(d);
+            S += e;
+            U = __builtin_fmaf(e, fmaxf(d, -200.0f), U);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; i++) {
+            const float d = (logit(i) - m) * a.slope, e = __builtin_amdgcn_exp2f(d);
+            S += e;
+            U = __builtin_fmaf(e, fmaxf(d, -200.0f), U);
+        }
     }
     S = lp_wave_sum(S);
     U = lp_wave_sum(U);
@@ -295,20 +297,24 @@ __global__ __launch_bounds__(kLpThreads) void k_logprobs(const LogprobsArgs a) {
         sh.red[1][wave] = S;
         sh.red[2][wave] = U;
     }
-    __syncthreads();
+    if (a.k) {
+        lp_select(sh, a.k, logit_order(mx), [&](uint32_t bound, auto&& f) __attribute__((always_inline)) {
+            const float least = order_logit(bound);
+#pragma unroll
+            for (int i = 0; i < E; i++)
+                if (logit(i) >= least && logit(i) > -INFINITY) f(logit_key(logit(i), index_of(i)));  // no NaN
+        });
+    } else {
+        __syncthreads();
+    }
     S = (sh.red[1][0] + sh.red[1][1]) + (sh.red[1][2] + sh.red[1][3]);
     U = (sh.red[2][0] + sh.red[2][1]) + (sh.red[2][2] + sh.red[2][3]);
-    if (a.k)
-        lp_select(sh, a.k, logit_key(mx, index_of(mi)), [&](auto&& f) __attribute__((always_inline)) {
-#pragma unroll
-            for (unsigned i = 0; i < kLpElems; i++) f(logit_key(x[i], index_of(i)));
-        });
     if (a.chunks == 1) {
-        lp_finish<DT>(a, sh, row, m, S, U);
+        lp_finish<DT>(a, sh, row, xmax, S, U);
         return;
     }
     const uint64_t at = (uint64_t)row * a.chunks + chunk;
-    if (t == 0) stg<f32x4>(a.part + at * 4, f32x4{m, S, U, 0.0f});
+    if (t == 0) stg<f32x4>(a.part + at * 4, f32x4{xmax, S, U, 0.0f});
     if (t < a.k) a.cand[at * a.k + t] = sh.top[t];
 }
 
@@ -318,46 +324,78 @@ __global__ __launch_bounds__(kLpThreads) void k_logprobs_join(const LogprobsArgs
     __shared__ LpShared sh;
     const unsigned t = threadIdx.x, lane = t & 63, wave = t >> 6, row = blockIdx.x;
     const f32x4* part = reinterpret_cast<const f32x4*>(a.part) + (uint64_t)row * a.chunks;
-    float m = -INFINITY;
-    for (unsigned i = t; i < a.chunks; i += kLpThreads) m = fmaxf(m, part[i][0]);
-    m = lp_wave_max(m);
-    if (lane == 0) sh.red[0][wave] = m;
+    const uint64_t* cand = a.cand + (uint64_t)row * a.chunks * a.k;
+    const unsigned n = a.chunks * a.k;
+    constexpr unsigned H = 4;  // keys a thread holds; more are read again
+    uint64_t held[H];
+    uint64_t best = 0;
+#pragma unroll
+    for (unsigned i = 0; i < H; i++) held[i] = t + i * kLpThreads < n ? cand[t + i * kLpThreads] : 0;
+    const f32x4 p0 = t < a.chunks ? part[t] : f32x4{-INFINITY, 0.0f, 0.0f, 0.0f};
+    float mx = p0[0];
+    for (unsigned i = t + kLpThreads; i < a.chunks; i += kLpThreads) mx = fmaxf(mx, part[i][0]);
+    mx = lp_wave_max(mx);
+    if (lane == 0) sh.red[0][wave] = mx;
     __syncthreads();
-    m = fmaxf(fmaxf(sh.red[0][0], sh.red[0][1]), fmaxf(sh.red[0][2], sh.red[0][3]));
+    mx = fmaxf(fmaxf(sh.red[0][0], sh.red[0][1]), fmaxf(sh.red[0][2], sh.red[0][3]));
+    const float m = mx == -INFINITY ? 0.0f : logit_z(mx, a);
     float S = 0.0f, U = 0.0f;
-    for (unsigned i = t; i < a.chunks; i += kLpThreads) {
-        const f32x4 p = part[i];
-        if (p[0] == -INFINITY && !(p[1] != p[1])) continue;  // nothing in it (a NaN sum stays one)
-        const float d = p[0] - m, f = exp_f32(d);
+    auto add = [&](const f32x4& p) __attribute__((always_inline)) {
+        const float d = (p[0] == -INFINITY ? 0.0f : logit_z(p[0], a) - m) * a.slope;  // of an empty chunk: S is 0 or NaN
+        const float f = __builtin_amdgcn_exp2f(d);
         S += p[1] * f;
         U += f == 0.0f ? 0.0f : (p[2] + d * p[1]) * f;
-    }
+    };
+    add(p0);
+    for (unsigned i = t + kLpThreads; i < a.chunks; i += kLpThreads) add(part[i]);
     S = lp_wave_sum(S);
     U = lp_wave_sum(U);
     if (lane == 0) {
         sh.red[1][wave] = S;
         sh.red[2][wave] = U;
     }
-    __syncthreads();
+    if (a.k) {
+#pragma unroll
+        for (unsigned i = 0; i < H; i++) best = lp_max(best, held[i]);
+        for (unsigned i = t + H * kLpThreads; i < n; i += kLpThreads) best = lp_max(best, cand[i]);
+        lp_select(sh, a.k, (uint32_t)(best >> 32), [&](uint32_t bound, auto&& f) __attribute__((always_inline)) {
+#pragma unroll
+            for (unsigned i = 0; i < H; i++)
+                if ((uint32_t)(held[i] >> 32) >= bound) f(held[i]);
+            for (unsigned i = t + H * kLpThreads; i < n; i += kLpThreads) {
+                const uint64_t key = cand[i];
+                if ((uint32_t)(key >> 32) >= bound) f(key);
+            }
+        });
+    } else {
+        __syncthreads();
+    }
     S = (sh.red[1][0] + sh.red[1][1]) + (sh.red[1][2] + sh.red[1][3]);
     U = (sh.red[2][0] + sh.red[2][1]) + (sh.red[2][2] + sh.red[2][3]);
-    if (a.k) {
-        const uint64_t* cand = a.cand + (uint64_t)row * a.chunks * a.k;
-        const unsigned n = a.chunks * a.k;
-        uint64_t best = 0;
-        for (unsigned i = t; i < n; i += kLpThreads) best = lp_max(best, cand[i]);
-        lp_select(sh, a.k, best, [&](auto&& f) __attribute__((always_inline)) {
-            for (unsigned i = t; i < n; i += kLpThreads) f(cand[i]);
-        });
-    }
-    lp_finish<DT>(a, sh, row, m, S, U);
+    lp_finish<DT>(a, sh, row, mx, S, U);
+}
+
+// Short chunks while the long ones leave CUs idle.
+static bool lp_short(uint32_t rows, uint32_t vocab) {
+    return (uint64_t)rows * ((vocab + kLpLong - 1) / kLpLong) < device_cus();
 }
 
 template <int DT>
-void launch_logprobs(const LogprobsArgs& a, uint32_t rows, bool vec, hipStream_t st) {
+void launch_logprobs(LogprobsArgs& a, uint32_t rows, bool vec, hipStream_t st) {
+    constexpr int P = DT == G4_LOGITS_F32 ? 1 : 2;
+    constexpr int LONG = (int)(kLpLong * P / kLpThreads), SHORT = (int)(kLpShort / kLpThreads);
+    const bool brief = lp_short(rows, a.vocab);
+    const uint32_t chunk = brief ? kLpShort : kLpLong * P;
+    a.chunks = (a.vocab + chunk - 1) / chunk;
+    a.cand = reinterpret_cast<uint64_t*>(a.part + (uint64_t)rows * a.chunks * 4);
     const dim3 grid(a.chunks, rows), block(kLpThreads);
-    if (vec) G4_LAUNCH((k_logprobs<DT, true>), grid, block, 0, st, a);
-    else G4_LAUNCH((k_logprobs<DT, false>), grid, block, 0, st, a);
+    if (brief) {
+        if (vec) G4_LAUNCH((k_logprobs<DT, true, SHORT>), grid, block, 0, st, a);
+        else G4_LAUNCH((k_logprobs<DT, false, SHORT>), grid, block, 0, st, a);
+    } else {
+        if (vec) G4_LAUNCH((k_logprobs<DT, true, LONG>), grid, block, 0, st, a);
+        else G4_LAUNCH((k_logprobs<DT, false, LONG>), grid, block, 0, st, a);
+    }
     if (a.chunks > 1) G4_LAUNCH((k_logprobs_join<DT>), dim3(rows), block, 0, st, a);
 }
 
@@ -367,7 +405,7 @@ using namespace g4;
 
 namespace {
 
-int logprobs_check(const g4_token_logprobs_params* p, uint64_t* chunks) {
+int logprobs_check(const g4_token_logprobs_params* p) {
     if (!p) return fail(G4_EINVAL, "tokenLogprobs: NULL params");
     if (p->vocab == 0 || p->vocab > (1u << 24)) return fail(G4_EINVAL, "tokenLogprobs: vocab %u (1 to 2^24)", p->vocab);
     if (p->rows > 65535) return fail(G4_EINVAL, "tokenLogprobs: %u rows (at most 65535)", p->rows);
@@ -381,12 +419,13 @@ int logprobs_check(const g4_token_logprobs_params* p, uint64_t* chunks) {
     if (!(p->temperature >= 1e-6f) || p->temperature > 1e6f)
         return fail(G4_EINVAL, "tokenLogprobs: temperature %g (1e-6 to 1e6)", (double)p->temperature);
     if (p->cap > 0.0f && p->cap < 1e-6f) return fail(G4_EINVAL, "tokenLogprobs: cap %g (0, or 1e-6 to 1e30)", (double)p->cap);
-    *chunks = ((uint64_t)p->vocab + kLpChunk - 1) / kLpChunk;
     return G4_OK;
 }
 
-size_t logprobs_bytes(const g4_token_logprobs_params* p, uint64_t chunks) {
-    return chunks == 1 ? 16 : (size_t)p->rows * chunks * (16 + 8ull * p->top_k) + 16;
+// Room for the chunks of any type and alignment.
+size_t logprobs_bytes(const g4_token_logprobs_params* p) {
+    const uint64_t chunk = lp_short(p->rows, p->vocab) ? kLpShort : kLpLong, chunks = (p->vocab + chunk - 1) / chunk;
+    return (size_t)p->rows * chunks * (16 + 8ull * p->top_k) + 16;
 }
 
 }  // namespace
@@ -395,18 +434,16 @@ extern "C" {
 
 int g4_token_logprobs_workspace_size(const g4_token_logprobs_params* p, size_t* bytes) {
     if (!bytes) return fail(G4_EINVAL, "g4_token_logprobs_workspace_size: bytes is NULL");
-    uint64_t chunks = 0;
-    const int rc = logprobs_check(p, &chunks);
+    const int rc = logprobs_check(p);
     if (rc) return rc;
-    *bytes = logprobs_bytes(p, chunks);
+    *bytes = logprobs_bytes(p);
     return G4_OK;
 }
 
 int g4_token_logprobs(const void* logits, const int32_t* tokens, float* logprobs, float* entropy, int32_t* top_ids,
                       float* top_logprobs, const g4_token_logprobs_params* p, void* workspace, size_t workspace_bytes,
                       void* stream) {
-    uint64_t chunks = 0;
-    const int rc = logprobs_check(p, &chunks);
+    const int rc = logprobs_check(p);
     if (rc) return rc;
     if (!logits || !workspace) return fail(G4_EINVAL, "tokenLogprobs: NULL logits or workspace");
     if (!tokens != !logprobs) return fail(G4_EINVAL, "tokenLogprobs: tokens and logprobs go together");
@@ -417,8 +454,8 @@ int g4_token_logprobs(const void* logits, const int32_t* tokens, float* logprobs
     if (reinterpret_cast<uintptr_t>(logits) & (elem - 1)) return fail(G4_EINVAL, "tokenLogprobs: misaligned logits");
     if (reinterpret_cast<uintptr_t>(workspace) & 15)
         return fail(G4_EINVAL, "tokenLogprobs: workspace must be 16-byte aligned");
-    if (workspace_bytes < logprobs_bytes(p, chunks))
-        return fail(G4_ENOSPC, "tokenLogprobs: workspace %zu bytes < %zu needed", workspace_bytes, logprobs_bytes(p, chunks));
+    if (workspace_bytes < logprobs_bytes(p))
+        return fail(G4_ENOSPC, "tokenLogprobs: workspace %zu bytes < %zu needed", workspace_bytes, logprobs_bytes(p));
     if (p->rows == 0) return G4_OK;
     LogprobsArgs a = {};
     a.logits = logits;
@@ -428,15 +465,12 @@ int g4_token_logprobs(const void* logits, const int32_t* tokens, float* logprobs
     a.top_ids = top_ids;
     a.top_logprobs = top_logprobs;
     a.part = static_cast<float*>(workspace);
-    a.cand = reinterpret_cast<uint64_t*>(a.part + (uint64_t)p->rows * chunks * 4);
     a.row_stride = p->row_stride ? p->row_stride : p->vocab;
     a.vocab = p->vocab;
-    a.chunks = (uint32_t)chunks;
     a.k = p->top_k;
     a.cap = p->cap;
-    a.inv_cap = p->cap > 0.0f ? 1.0f / p->cap : 0.0f;
-    a.temperature = p->temperature;
-    a.inv_temperature = 1.0f / p->temperature;
+    a.cap_exp = p->cap > 0.0f ? 2.0f * kLog2e / p->cap : 0.0f;
+    a.slope = kLog2e / p->temperature;
     const bool vec = !((reinterpret_cast<uintptr_t>(logits) | (a.row_stride * elem)) & 15);
     hipStream_t st = as_stream(stream);
     if (p->dtype == G4_LOGITS_F32) launch_logprobs<G4_LOGITS_F32>(a, p->rows, vec, st);

@@ -688,18 +688,26 @@ def lm_head_argmax_timed(hidden, weight, logits, result, workspace, vocab, hidde
 
 # ---- drafted tokens over a paged cache ---------------------------------------------
 
-def _on_device(device, **tensors):
-    """Every given tensor lies on `device`, which is the current one (the stream's)."""
-    if device.index != _current_device():
-        raise ValueError(f"tensors on {device}, but the current device is cuda:{_current_device()}")
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name}: on {t.device}, expected {device}")
+def _at(t, name, dtype, n, device):
+    """The checked pointer of a contiguous tensor of at least n elements on GPU `device` (an index)."""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == device and t.is_contiguous() and t.numel() >= n:
+        return t.data_ptr()
+    p = _dev(t, name, F16_TYPES if dtype is torch.float16 else dtype, n)
+    if t.get_device() != device:
+        raise ValueError(f"{name}: on {t.device}, expected cuda:{device}")
+    return p
+
+
+def _call_device(device):
+    """GPU `device` (an index) is the current one, whose stream a call takes."""
+    if device != _current_device():
+        raise ValueError(f"tensors on cuda:{device}, but the current device is cuda:{_current_device()}")
+    return device
 
 
 def _shaped(t, name, shape):
-    if tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {shape}")
 
 
 class PagedCache:
@@ -714,9 +722,9 @@ class PagedCache:
         if k_pool.shape != v_pool.shape or k_pool.dtype != v_pool.dtype:
             raise ValueError("k_pool and v_pool differ in shape or dtype")
         self.k_pool, self.v_pool = k_pool, v_pool
-        self.device = k_pool.device
-        if v_pool.device != self.device:
-            raise ValueError(f"v_pool: on {v_pool.device}, expected {self.device}")
+        self.device = k_pool.get_device()
+        if v_pool.get_device() != self.device:
+            raise ValueError(f"v_pool: on {v_pool.device}, expected cuda:{self.device}")
         self.num_pages, self.page_size, self.num_kv_heads, self.head_dim = (int(n) for n in k_pool.shape)
         f8 = k_pool.dtype == torch.float8_e4m3fn
         self.c = abi.PagedCache(k_pool.data_ptr(), v_pool.data_ptr(), self.num_pages, self.page_size,
@@ -744,29 +752,30 @@ class PagedBatch:
             if tree_mask.dim() != 2:
                 raise ValueError("tree_mask: expected [n_tokens, words]")
             words = int(tree_mask.shape[1])
-        self.device = block_table.device
-        for name, t in (("token_start", token_start), ("ctx_lens", ctx_lens), ("positions", positions),
-                        ("tree_mask", tree_mask)):
-            if t is not None and t.device != self.device:
-                raise ValueError(f"{name}: on {t.device}, expected {self.device}")
+        self.device = dev = block_table.get_device()
         self.tensors = (block_table, token_start, ctx_lens, positions, tree_mask)
+        if tree_mask is not None and tree_mask.dtype == torch.uint64:
+            tree_mask = tree_mask.view(torch.int64)
         self.c = abi.PagedBatch(
-            block_table.data_ptr(), _dev(token_start, "token_start", torch.int32, self.n_seqs + 1),
-            _dev(ctx_lens, "ctx_lens", torch.int32, self.n_seqs),
-            None if positions is None else _dev(positions, "positions", torch.int32, self.n_tokens),
-            None if tree_mask is None else _dev(tree_mask, "tree_mask", (torch.int64, torch.uint64), self.n_tokens * words),
+            block_table.data_ptr(), _at(token_start, "token_start", torch.int32, self.n_seqs + 1, dev),
+            _at(ctx_lens, "ctx_lens", torch.int32, self.n_seqs, dev),
+            None if positions is None else _at(positions, "positions", torch.int32, self.n_tokens, dev),
+            None if tree_mask is None else _at(tree_mask, "tree_mask", torch.int64, self.n_tokens * words, dev),
             self.n_seqs, stride, self.n_tokens, self.max_tokens, words, 0)
 
 
-def _token_rows(t, name, heads, head_dim, tokens, dtype):
-    """A [tokens, heads, head_dim] tensor whose tokens may lie apart: (pointer, elements from token to token)."""
+def _token_rows(t, name, heads, head_dim, tokens, device):
+    """A f32 [tokens, heads, head_dim] tensor whose tokens may lie apart: (pointer, elements from token to token)."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a tensor")
-    if not t.is_cuda:
-        raise ValueError(f"{name}: must be on the GPU, got {t.device}")
-    if t.dtype != dtype:
-        raise TypeError(f"{name}: dtype {t.dtype}, expected {dtype}")
-    _shaped(t, name, (tokens, heads, head_dim))
+    if t.get_device() != device:
+        raise ValueError(f"{name}: must be on the GPU cuda:{device}, got {t.device}")
+    if t.dtype is not torch.float32:
+        raise TypeError(f"{name}: dtype {t.dtype}, expected float32")
+    if t.shape != (tokens, heads, head_dim):
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {(tokens, heads, head_dim)}")
+    if t.is_contiguous():
+        return t.data_ptr(), 0
     if t.stride(2) != 1 or (heads > 1 and t.stride(1) != head_dim):
         raise ValueError(f"{name}: a token's heads must be contiguous")
     if tokens <= 1:
@@ -781,32 +790,32 @@ def paged_append(cache, batch, q, k, v, q_weight, k_weight, rope_inv_freq, q_out
     k, v: f32 [n_tokens, NKH, HD]; tokens may lie apart (slices of one projection's output). q_out: f16
     [n_tokens, NQH, HD]. k, v, k_weight None: a KV-consumer layer; q, q_weight, q_out None: only the store.
     rope_inv_freq: the f32 [HD / 2] table of rope_inv_freq()."""
-    if q is None and k is None:
-        raise ValueError("paged_append: neither q nor k and v")
-    hd, nt = cache.head_dim, batch.n_tokens
-    _on_device(cache.device, batch=batch, q=q, k=k, v=v, q_weight=q_weight, k_weight=k_weight,
-               rope_inv_freq=rope_inv_freq, q_out=q_out)
+    hd, nt, dev = cache.head_dim, batch.n_tokens, _call_device(cache.device)
+    if batch.device != dev:
+        raise ValueError(f"batch: on cuda:{batch.device}, expected cuda:{dev}")
     nqh, qp, qw, qo, ks, kp, vs, vp, kw, qs = 0, None, None, None, 0, None, 0, None, None, 0
     if q is not None:
         if q.dim() != 3:
             raise ValueError("q: expected [n_tokens, heads, head_dim]")
-        nqh = int(q.shape[1])
-        qp, qs = _token_rows(q, "q", nqh, hd, nt, torch.float32)
-        qw = _f16(q_weight, "q_weight", hd)
-        qo = _f16(q_out, "q_out", nt * nqh * hd)
+        nqh = q.shape[1]
+        qp, qs = _token_rows(q, "q", nqh, hd, nt, dev)
+        qw = _at(q_weight, "q_weight", torch.float16, hd, dev)
+        qo = _at(q_out, "q_out", torch.float16, nt * nqh * hd, dev)
     elif q_weight is not None or q_out is not None:
         raise ValueError("paged_append: q, q_weight and q_out go together")
     if k is not None:
-        kp, ks = _token_rows(k, "k", cache.num_kv_heads, hd, nt, torch.float32)
-        vp, vs = _token_rows(v, "v", cache.num_kv_heads, hd, nt, torch.float32)
-        kw = _f16(k_weight, "k_weight", hd)
+        kp, ks = _token_rows(k, "k", cache.num_kv_heads, hd, nt, dev)
+        vp, vs = _token_rows(v, "v", cache.num_kv_heads, hd, nt, dev)
+        kw = _at(k_weight, "k_weight", torch.float16, hd, dev)
     elif v is not None or k_weight is not None:
         raise ValueError("paged_append: k, v and k_weight go together")
+    elif q is None:
+        raise ValueError("paged_append: neither q nor k and v")
     if nt == 0:
         return
-    p = abi.PagedAppendParams(nqh, eps, qs, ks, vs)
-    abi.call("g4_paged_append", cache.c, batch.c, qp, kp, vp, qw, kw, _f32(rope_inv_freq, "rope_inv_freq", hd // 2), qo, p,
-             _stream(stream))
+    abi.call("g4_paged_append", cache.c, batch.c, qp, kp, vp, qw, kw, _at(rope_inv_freq, "rope_inv_freq", torch.float32,
+                                                                         hd // 2, dev), qo,
+             abi.PagedAppendParams(nqh, eps, qs, ks, vs), _stream(stream))
 
 
 def paged_attn_workspace_bytes(cache, batch, num_q_heads) -> int:
@@ -819,32 +828,50 @@ def paged_attn(cache, batch, q, out, workspace, scale=1.0, sliding_window=0, sof
     """Attention of a batch's new tokens over their sequences' rows (g4_paged_attn). q: f16 [n_tokens, NQH, HD] as
     paged_append leaves it; out: f32, the same shape; the new tokens' own rows are already stored. workspace: uint8,
     paged_attn_workspace_bytes."""
-    _on_device(cache.device, batch=batch, q=q, out=out, workspace=workspace)
+    dev = _call_device(cache.device)
+    if batch.device != dev:
+        raise ValueError(f"batch: on cuda:{batch.device}, expected cuda:{dev}")
     if q.dim() != 3:
         raise ValueError("q: expected [n_tokens, heads, head_dim]")
-    nqh = int(q.shape[1])
+    nqh = q.shape[1]
     shape = (batch.n_tokens, nqh, cache.head_dim)
     _shaped(q, "q", shape)
     _shaped(out, "out", shape)
     if batch.n_tokens == 0:
         return
-    p = abi.PagedAttnParams(nqh, int(sliding_window), float(scale), float(softcap))
-    abi.call("g4_paged_attn", cache.c, batch.c, _f16(q, "q", 0), _f32(out, "out", 0), p,
-             _dev(workspace, "workspace", torch.uint8, 0), workspace.numel(), _stream(stream))
+    abi.call("g4_paged_attn", cache.c, batch.c, _at(q, "q", torch.float16, 0, dev), _at(out, "out", torch.float32, 0, dev),
+             abi.PagedAttnParams(nqh, sliding_window, scale, softcap), _at(workspace, "workspace", torch.uint8, 0, dev),
+             workspace.numel(), _stream(stream))
+
+
+class PagedCaches:
+    """The caches of several layers, described once for paged_commit."""
+
+    def __init__(self, caches):
+        self.caches = tuple(caches)
+        if not self.caches:
+            raise ValueError("no caches")
+        self.device = self.caches[0].device
+        for i, c in enumerate(self.caches):
+            if c.device != self.device:
+                raise ValueError(f"caches[{i}]: on cuda:{c.device}, expected cuda:{self.device}")
+        self.c = (abi.PagedCache * len(self.caches))(*[c.c for c in self.caches])
 
 
 def paged_commit(caches, batch, path, n_accepted, new_ctx_lens, stream=None):
-    """The accepted drafted rows moved together in every cache of `caches` (g4_paged_commit). path: int32
-    [n_seqs, steps], ascending new-token indices; n_accepted, new_ctx_lens: int32 [n_seqs]."""
-    caches = list(caches)
-    _on_device(batch.device, path=path, n_accepted=n_accepted, new_ctx_lens=new_ctx_lens,
-               **{f"caches[{i}]": c for i, c in enumerate(caches)})
-    if path.dim() != 2 or path.shape[0] != batch.n_seqs:
-        raise ValueError(f"path: shape {tuple(path.shape)}, expected [{batch.n_seqs}, steps]")
-    arr = (abi.PagedCache * max(1, len(caches)))(*[c.c for c in caches])
-    abi.call("g4_paged_commit", arr, len(caches), batch.c, _dev(path, "path", torch.int32, 1), int(path.shape[1]),
-             _dev(n_accepted, "n_accepted", torch.int32, batch.n_seqs),
-             _dev(new_ctx_lens, "new_ctx_lens", torch.int32, batch.n_seqs), _stream(stream))
+    """The accepted drafted rows moved together in every cache of `caches` (a PagedCaches, or a sequence of PagedCache)
+    (g4_paged_commit). path: int32 [n_seqs, steps], ascending new-token indices; n_accepted, new_ctx_lens: int32
+    [n_seqs]."""
+    if not isinstance(caches, PagedCaches):
+        caches = PagedCaches(caches)
+    dev, n = _call_device(batch.device), batch.n_seqs
+    if caches.device != dev:
+        raise ValueError(f"caches: on cuda:{caches.device}, expected cuda:{dev}")
+    if path.dim() != 2 or path.shape[0] != n:
+        raise ValueError(f"path: shape {tuple(path.shape)}, expected [{n}, steps]")
+    abi.call("g4_paged_commit", caches.c, len(caches.c), batch.c, _at(path, "path", torch.int32, 1, dev), path.shape[1],
+             _at(n_accepted, "n_accepted", torch.int32, n, dev), _at(new_ctx_lens, "new_ctx_lens", torch.int32, n, dev),
+             _stream(stream))
 
 
 # ---- log probabilities ---------------------------------------------------------------
@@ -871,25 +898,23 @@ def token_logprobs(logits, tokens, logprobs, entropy, workspace, top_ids=None, t
         raise ValueError(f"logits: must be on the GPU, got {logits.device}")
     if logits.dtype not in LOGIT_TYPES:
         raise TypeError(f"logits: dtype {logits.dtype} not in {tuple(LOGIT_TYPES)}")
-    rows, vocab = (int(n) for n in logits.shape)
+    rows, vocab = logits.shape
     if vocab > 1 and logits.stride(1) != 1 or rows > 1 and logits.stride(0) < vocab:
         raise ValueError("logits: a row's logits must be contiguous, and rows apart")
-    _on_device(logits.device, tokens=tokens, logprobs=logprobs, entropy=entropy, workspace=workspace, top_ids=top_ids,
-               top_logprobs=top_logprobs)
+    dev = _call_device(logits.get_device())
     k = 0
     if top_ids is not None:
         if top_ids.dim() != 2 or top_ids.shape[0] != rows:
             raise ValueError(f"top_ids: shape {tuple(top_ids.shape)}, expected [{rows}, k]")
-        k = int(top_ids.shape[1])
+        k = top_ids.shape[1]
     if rows == 0:
         return
-    p = abi.TokenLogprobsParams(rows, vocab, logits.stride(0) if rows > 1 else 0, LOGIT_TYPES[logits.dtype], k, cap,
-                                temperature)
-
-    def opt(t, name, dtype, n):
-        return None if t is None else _dev(t, name, dtype, n)
-
-    abi.call("g4_token_logprobs", logits.data_ptr(), opt(tokens, "tokens", torch.int32, rows),
-             opt(logprobs, "logprobs", torch.float32, rows), opt(entropy, "entropy", torch.float32, rows),
-             opt(top_ids, "top_ids", torch.int32, rows * k), opt(top_logprobs, "top_logprobs", torch.float32, rows * k), p,
-             _dev(workspace, "workspace", torch.uint8, 0), workspace.numel(), _stream(stream))
+    i32, f32 = torch.int32, torch.float32
+    abi.call("g4_token_logprobs", logits.data_ptr(), None if tokens is None else _at(tokens, "tokens", i32, rows, dev),
+             None if logprobs is None else _at(logprobs, "logprobs", f32, rows, dev),
+             None if entropy is None else _at(entropy, "entropy", f32, rows, dev),
+             None if top_ids is None else _at(top_ids, "top_ids", i32, rows * k, dev),
+             None if top_logprobs is None else _at(top_logprobs, "top_logprobs", f32, rows * k, dev),
+             abi.TokenLogprobsParams(rows, vocab, logits.stride(0) if rows > 1 else 0, LOGIT_TYPES[logits.dtype], k, cap,
+                                     temperature),
+             _at(workspace, "workspace", torch.uint8, 0, dev), workspace.numel(), _stream(stream))
