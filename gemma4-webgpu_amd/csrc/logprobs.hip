@@ -115,50 +115,54 @@ __device__ __forceinline__ float lp_wave_max(float x) {
 
 struct LpShared {
     uint32_t group[kLpGroups];
-    uint32_t at_least[kLpGroups];
     uint64_t cand[kLpCandidates];
     uint64_t top[kLpMaxK];
-    uint32_t bound;
     uint64_t wave[kLpThreads / 64];
     uint32_t count;
     float red[3][kLpThreads / 64];
 };
 
-// The k largest of the workgroup's keys into sh.top, descending (0 where there
-// are fewer). best: the thread's largest logit, as its order; each(bound, f) calls f(key) on every
-// logit of the thread whose order is at least bound (at least kLpLeast).
-template <typename EACH>
-__device__ __forceinline__ void lp_select(LpShared& sh, unsigned k, uint32_t best, EACH&& each) {
-    const unsigned t = threadIdx.x, lane = t & 63, wave = t >> 6;
+// The selection of the k largest keys, in three steps with a barrier after each of the first two.
+//
+// Before the first barrier: best is the thread's largest logit, as its order.
+__device__ __forceinline__ void lp_groups(LpShared& sh, uint32_t best) {
+    const unsigned t = threadIdx.x;
     uint32_t g = max(best, (uint32_t)__builtin_amdgcn_mov_dpp((int)best, 0xB1, 0xf, 0xf, false));  // groups of four threads:
     g = max(g, (uint32_t)__builtin_amdgcn_mov_dpp((int)g, 0x4E, 0xf, 0xf, false));                 // quad_perm 1,0,3,2; 2,3,0,1
     if ((t & 3) == 0) sh.group[t >> 2] = g;
-    if (t < kLpGroups) sh.at_least[t] = 0;
     if (t < kLpMaxK) sh.top[t] = 0;
-    if (t == 0) {
-        sh.bound = kLpLeast;
-        sh.count = 0;
-    }
-    __syncthreads();
-    {
-        const uint32_t mine = sh.group[lane];
-        unsigned n = 0;
+    if (t == 0) sh.count = 0;
+}
+// After it: an order that at least k logits reach (kLpLeast where fewer are above -inf). The k-th largest of
+// the 64 groups' maxima, bit by bit over the top 18 (sign, exponent, 9 of the fraction): each wave counts
+// for itself.
+__device__ __forceinline__ uint32_t lp_bound(const LpShared& sh, unsigned k) {
+    const uint32_t mine = sh.group[threadIdx.x & 63];
+    uint32_t bound = 0;
 #pragma unroll
-        for (unsigned i = 0; i < kLpGroups / 4; i++) n += sh.group[wave * (kLpGroups / 4) + i] >= mine;
-        atomicAdd(&sh.at_least[lane], n);
+    for (int bit = 31; bit >= 14; bit--) {
+        const uint32_t with = bound | 1u << bit;
+        if ((unsigned)__popcll(__ballot(mine >= with)) >= k) bound = with;
     }
-    __syncthreads();
-    if (t < kLpGroups && sh.at_least[t] >= k) atomicMax(&sh.bound, sh.group[t]);
-    __syncthreads();
-    const uint32_t bound = sh.bound;
-    if (best >= bound)
-        each(bound, [&](uint64_t key) {
-            const unsigned at = atomicAdd(&sh.count, 1u);
-            if (at < kLpCandidates) sh.cand[at] = key;
-        });
-    __syncthreads();
+    return max(bound, kLpLeast);
+}
+// A thread's n keys into the candidates: put(f) calls f(key) for each.
+template <typename PUT>
+__device__ __forceinline__ void lp_push(LpShared& sh, unsigned n, PUT&& put) {
+    if (n == 0) return;
+    unsigned at = atomicAdd(&sh.count, n);
+    put([&](uint64_t key) __attribute__((always_inline)) {
+        if (at < kLpCandidates) sh.cand[at] = key;
+        at++;
+    });
+}
+// After the second barrier: store(rank, key) for the k largest, by the threads that have them; ranks there
+// is no key for are left out. each(f) calls f on every key of the thread, should the candidates be too many.
+template <typename STORE, typename EACH>
+__device__ __forceinline__ void lp_rank(LpShared& sh, unsigned k, STORE&& store, EACH&& each) {
+    const unsigned t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const unsigned n = sh.count;
-    if (n <= kLpCandidates) {
+    if (n <= kLpCandidates) {  // uniform
         for (unsigned i = t; i < n; i += kLpThreads) {
             const uint64_t key = sh.cand[i];
             unsigned above = 0;
@@ -169,24 +173,23 @@ __device__ __forceinline__ void lp_select(LpShared& sh, unsigned k, uint32_t bes
 #pragma unroll
                 for (unsigned e = 0; e < 8; e++) above += j + e < n && c[e] > key;
             }
-            if (above < k) sh.top[above] = key;
+            if (above < k) store(above, key);
         }
-    } else {
-        uint64_t last = ~0ull;
-        for (unsigned r = 0; r < k; r++) {  // uniform
-            uint64_t b = 0;
-            each(kLpLeast, [&](uint64_t key) { b = key < last ? lp_max(b, key) : b; });
-#pragma unroll
-            for (int m = 32; m >= 1; m >>= 1) b = lp_max(b, lp_shfl_xor(b, m));
-            if (lane == 0) sh.wave[wave] = b;
-            __syncthreads();
-            last = lp_max(lp_max(sh.wave[0], sh.wave[1]), lp_max(sh.wave[2], sh.wave[3]));
-            if (t == 0) sh.top[r] = last;
-            __syncthreads();
-            if (!last) break;
-        }
+        return;
     }
-    __syncthreads();
+    uint64_t last = ~0ull;
+    for (unsigned r = 0; r < k; r++) {  // uniform
+        uint64_t b = 0;
+        each([&](uint64_t key) __attribute__((always_inline)) { b = key < last ? lp_max(b, key) : b; });
+#pragma unroll
+        for (int m = 32; m >= 1; m >>= 1) b = lp_max(b, lp_shfl_xor(b, m));
+        if (lane == 0) sh.wave[wave] = b;
+        __syncthreads();
+        last = lp_max(lp_max(sh.wave[0], sh.wave[1]), lp_max(sh.wave[2], sh.wave[3]));
+        if (t == 0) store(r, last);
+        __syncthreads();
+        if (!last) break;
+    }
 }
 
 // A row's results from its (max x, S, U) and sh.top.
@@ -220,7 +223,7 @@ __device__ __forceinline__ void lp_finish(const LogprobsArgs& a, const LpShared&
 
 // One chunk of one row, E logits a thread. VEC: 16-byte loads (rows aligned), otherwise one element a load.
 template <int DT, bool VEC, int E>
-__global__ __launch_bounds__(kLpThreads) void k_logprobs(const LogprobsArgs a) {
+__global__ __launch_bounds__(kLpThreads, E <= 32 ? 4 : 3) void k_logprobs(const LogprobsArgs a) {
     typedef typename LogitType<DT>::T T;
     constexpr int V = VEC ? 16 / sizeof(T) : 1;  // elements a load
     constexpr int N = E / V, P = sizeof(T) == 2 ? 2 : 1;  // logits a register
@@ -271,6 +274,7 @@ __global__ __launch_bounds__(kLpThreads) void k_logprobs(const LogprobsArgs a) {
     for (int i = 0; i < E; i++) mx = fmaxf(mx, logit(i));  // leaves NaN aside
     const float wmax = lp_wave_max(mx);
     if (lane == 0) sh.red[0][wave] = wmax;
+    if (a.k) lp_groups(sh, logit_order(mx));
     __syncthreads();
     const float xmax = fmaxf(fmaxf(sh.red[0][0], sh.red[0][1]), fmaxf(sh.red[0][2], sh.red[0][3]));
     const float m = xmax == -INFINITY ? 0.0f : logit_z(xmax, a);
@@ -298,24 +302,44 @@ __global__ __launch_bounds__(kLpThreads) void k_logprobs(const LogprobsArgs a) {
         sh.red[2][wave] = U;
     }
     if (a.k) {
-        lp_select(sh, a.k, logit_order(mx), [&](uint32_t bound, auto&& f) __attribute__((always_inline)) {
-            const float least = order_logit(bound);
+        const float least = order_logit(lp_bound(sh, a.k));
+        unsigned n = 0;
+        if (mx >= least) {
+#pragma unroll
+            for (int i = 0; i < E; i++) n += logit(i) >= least;  // neither NaN nor -inf
+        }
+        lp_push(sh, n, [&](auto&& f) __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < E; i++)
-                if (logit(i) >= least && logit(i) > -INFINITY) f(logit_key(logit(i), index_of(i)));  // no NaN
+                if (logit(i) >= least) f(logit_key(logit(i), index_of(i)));
         });
-    } else {
-        __syncthreads();
     }
+    __syncthreads();
     S = (sh.red[1][0] + sh.red[1][1]) + (sh.red[1][2] + sh.red[1][3]);
     U = (sh.red[2][0] + sh.red[2][1]) + (sh.red[2][2] + sh.red[2][3]);
+    auto each = [&](auto&& f) __attribute__((always_inline)) {
+        // Computed where it stands: kept for the next round, the keys would take the registers of the common path.
+        float zero = 0.0f;
+        asm volatile("" : "+v"(zero));
+#pragma unroll
+        for (int i = 0; i < E; i++) f(logit_key(logit(i) + zero, index_of(i)));
+    };
     if (a.chunks == 1) {
+        if (a.k) {
+            lp_rank(sh, a.k, [&](unsigned r, uint64_t key) __attribute__((always_inline)) { sh.top[r] = key; }, each);
+            __syncthreads();
+        }
         lp_finish<DT>(a, sh, row, xmax, S, U);
         return;
     }
     const uint64_t at = (uint64_t)row * a.chunks + chunk;
     if (t == 0) stg<f32x4>(a.part + at * 4, f32x4{xmax, S, U, 0.0f});
-    if (t < a.k) a.cand[at * a.k + t] = sh.top[t];
+    if (a.k) {
+        uint64_t* dst = a.cand + at * a.k;
+        const unsigned n = sh.count;
+        if (n < a.k && t >= n && t < a.k) dst[t] = 0;  // fewer above -inf
+        lp_rank(sh, a.k, [&](unsigned r, uint64_t key) __attribute__((always_inline)) { dst[r] = key; }, each);
+    }
 }
 
 // One row's chunks joined.
@@ -336,6 +360,12 @@ __global__ __launch_bounds__(kLpThreads) void k_logprobs_join(const LogprobsArgs
     for (unsigned i = t + kLpThreads; i < a.chunks; i += kLpThreads) mx = fmaxf(mx, part[i][0]);
     mx = lp_wave_max(mx);
     if (lane == 0) sh.red[0][wave] = mx;
+    if (a.k) {
+#pragma unroll
+        for (unsigned i = 0; i < H; i++) best = lp_max(best, held[i]);
+        for (unsigned i = t + H * kLpThreads; i < n; i += kLpThreads) best = lp_max(best, cand[i]);
+        lp_groups(sh, (uint32_t)(best >> 32));
+    }
     __syncthreads();
     mx = fmaxf(fmaxf(sh.red[0][0], sh.red[0][1]), fmaxf(sh.red[0][2], sh.red[0][3]));
     const float m = mx == -INFINITY ? 0.0f : logit_z(mx, a);
@@ -354,24 +384,29 @@ __global__ __launch_bounds__(kLpThreads) void k_logprobs_join(const LogprobsArgs
         sh.red[1][wave] = S;
         sh.red[2][wave] = U;
     }
+    auto each = [&](auto&& f) __attribute__((always_inline)) {
+#pragma unroll
+        for (unsigned i = 0; i < H; i++) f(held[i]);
+        for (unsigned i = t + H * kLpThreads; i < n; i += kLpThreads) f(cand[i]);
+    };
     if (a.k) {
-#pragma unroll
-        for (unsigned i = 0; i < H; i++) best = lp_max(best, held[i]);
-        for (unsigned i = t + H * kLpThreads; i < n; i += kLpThreads) best = lp_max(best, cand[i]);
-        lp_select(sh, a.k, (uint32_t)(best >> 32), [&](uint32_t bound, auto&& f) __attribute__((always_inline)) {
-#pragma unroll
-            for (unsigned i = 0; i < H; i++)
-                if ((uint32_t)(held[i] >> 32) >= bound) f(held[i]);
-            for (unsigned i = t + H * kLpThreads; i < n; i += kLpThreads) {
-                const uint64_t key = cand[i];
+        const uint32_t bound = lp_bound(sh, a.k);
+        unsigned many = 0;
+        if ((uint32_t)(best >> 32) >= bound)
+            each([&](uint64_t key) __attribute__((always_inline)) { many += (uint32_t)(key >> 32) >= bound; });
+        lp_push(sh, many, [&](auto&& f) __attribute__((always_inline)) {
+            each([&](uint64_t key) __attribute__((always_inline)) {
                 if ((uint32_t)(key >> 32) >= bound) f(key);
-            }
+            });
         });
-    } else {
-        __syncthreads();
     }
+    __syncthreads();
     S = (sh.red[1][0] + sh.red[1][1]) + (sh.red[1][2] + sh.red[1][3]);
     U = (sh.red[2][0] + sh.red[2][1]) + (sh.red[2][2] + sh.red[2][3]);
+    if (a.k) {
+        lp_rank(sh, a.k, [&](unsigned r, uint64_t key) __attribute__((always_inline)) { sh.top[r] = key; }, each);
+        __syncthreads();
+    }
     lp_finish<DT>(a, sh, row, mx, S, U);
 }
 

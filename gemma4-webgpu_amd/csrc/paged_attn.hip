@@ -31,8 +31,7 @@
 
 namespace g4 {
 
-constexpr int kPagedWaves = 4;  // of k_paged_few
-constexpr int kPagedThreads = 64 * kPagedWaves;
+constexpr int kPagedWaves = 4;  // of k_paged_few where items are cut
 
 struct PagedAttnArgs {
     const uint16_t* __restrict__ q;
@@ -47,6 +46,7 @@ struct PagedAttnArgs {
     float qscale;                 // scale * log2(e)
     float cap_scale, cap_log2;    // scale / cap and cap * log2(e); 0: no cap
     uint32_t wgs, min_share;      // workgroups of the attention launch; least tiles a workgroup takes
+    uint32_t whole;               // 1: a workgroup an item, nothing is cut
     PagedBatchDev b;
 };
 
@@ -108,8 +108,9 @@ struct PagedScan {
         const unsigned i = i0 + lane;
         tiles = 0;
         if (i < items(a)) {
-            sq = paged_seq(a.b, i / a.q_tiles);
-            tiles = paged_span<MQ, UR>(a, sq, i % a.q_tiles).n * a.nkh;
+            const bool one = a.q_tiles == 1;
+            sq = paged_seq(a.b, one ? i : i / a.q_tiles);
+            tiles = paged_span<MQ, UR>(a, sq, one ? 0u : i % a.q_tiles).n * a.nkh;
         }
         incl = wave_scan(tiles, lane);
     }
@@ -152,6 +153,31 @@ __device__ __forceinline__ PagedPlace paged_place(const PagedAttnArgs& a, PagedS
         }
         before += all;
     }
+}
+// A workgroup's share [u, end) of the batch's tiles and where it begins; false: none is left for it.
+template <int MQ, int UR>
+__device__ __forceinline__ bool paged_begin(const PagedAttnArgs& a, unsigned lane, PagedPlace& p, unsigned& u, unsigned& end) {
+    if (a.whole) {  // one item, counted from its own first tile
+        p.i = blockIdx.x;
+        p.kvh = p.off = 0;
+        if (a.nkh > 1) {
+            p.i = blockIdx.x / a.nkh;
+            p.kvh = blockIdx.x % a.nkh;
+        }
+        p.sq = paged_seq(a.b, a.q_tiles > 1 ? p.i / a.q_tiles : p.i);
+        u = 0;
+        end = paged_span<MQ, UR>(a, p.sq, a.q_tiles > 1 ? p.i % a.q_tiles : 0u).n;
+        return end > 0;
+    }
+    PagedScan<MQ, UR> scan;
+    scan.run(a, lane);
+    const unsigned share = scan.share(a);
+    const uint64_t first = (uint64_t)blockIdx.x * share;
+    if (first >= scan.total) return false;
+    u = (unsigned)first;
+    end = min(u + share, scan.total);
+    p = paged_place<MQ, UR>(a, scan, u, lane);
+    return true;
 }
 // The item after p's: the next kv head, or the next query tile that there is.
 template <int MQ, int UR>
@@ -473,39 +499,38 @@ __device__ __forceinline__ float paged_inverse(float L) { return L > 0.0f ? 1.0f
 
 // ---- at most 32 query rows --------------------------------------------------------
 
-// Bound by the cache's bytes: the waves of a workgroup take every fourth row tile of its share, each
-// with a tile's K and V in registers: the next tile's K is requested when the scores have used this
-// one's, its V when the products have.
-template <int HD, int C>
+// Bound by the cache's bytes: the W waves of a workgroup take every W-th row tile of its share, each
+// with a tile's K and V in registers. With four waves (512 registers each) the next tile's K is
+// requested when the scores have used this one's, its V when the products have; with eight (256
+// registers) a wave requests a tile at a time, and a short item, which one workgroup has whole, takes
+// half as many in turn.
+template <int HD, int C, int W>
 struct PagedFewSmem {
-    f16x8 q[C][HD / 32][64];                // score operand, lane-major
-    float o[kPagedWaves][HD / 16 * 4][64];  // one query group's outputs, per wave
-    float m[kPagedWaves][16 * C], l[kPagedWaves][16 * C];
+    f16x8 q[C][HD / 32][64];      // score operand, lane-major
+    float o[W][HD / 16 * 4][64];  // one query group's outputs, per wave
+    float m[W][16 * C], l[W][16 * C];
 };
 
-template <int HD, int C, bool F8>
-__global__ __launch_bounds__(kPagedThreads, 1) void k_paged_few(const PagedAttnArgs a) {
+template <int HD, int C, bool F8, int W>
+__global__ __launch_bounds__(64 * W, W / 4) void k_paged_few(const PagedAttnArgs a) {
+    constexpr bool AHEAD = W == 4;
     using D = PagedDims<HD, F8>;
     constexpr int MQ = 16 * C, UR = 32;
-    __shared__ PagedFewSmem<HD, C> sm;
+    __shared__ PagedFewSmem<HD, C, W> sm;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, g = lane >> 4;
     const unsigned G = a.group;
 
-    PagedScan<MQ, UR> scan;
-    scan.run(a, lane);
-    const unsigned share = scan.share(a);
-    const uint64_t first = (uint64_t)blockIdx.x * share;
-    if (first >= scan.total) return;  // uniform
-    unsigned u = (unsigned)first;
-    const unsigned u_end = min(u + share, scan.total);
-    PagedPlace at = paged_place<MQ, UR>(a, scan, u, lane);
+    PagedPlace at;
+    unsigned u, u_end;
+    if (!paged_begin<MQ, UR>(a, lane, at, u, u_end)) return;  // uniform
     const uint32_t row_bytes = a.nkh * HD * D::ES;
 
+    bool again = false;
     while (u < u_end) {  // one item or a part of one
         const unsigned i = uniform(at.i);
-        const unsigned s = i / a.q_tiles, qt = i % a.q_tiles;
+        const unsigned s = a.q_tiles > 1 ? i / a.q_tiles : i, qt = a.q_tiles > 1 ? i % a.q_tiles : 0u;
         const unsigned kvh = uniform(at.kvh), off = uniform(at.off);
         const PagedSeq sq{uniform(at.sq.start), uniform(at.sq.n), uniform(at.sq.ctx)};
         const PagedSpan sp = paged_span<MQ, UR>(a, sq, qt);
@@ -519,15 +544,19 @@ __global__ __launch_bounds__(kPagedThreads, 1) void k_paged_few(const PagedAttnA
         u32x4 kr[2][D::KP];
         PagedV<HD, F8> vr;
         PagedAt pa{};
-        if ((unsigned)wave < seg) {
-            pages.load(a, table, sp.first + off + wave, kPagedWaves, sp.hi, lane);
-            pa = paged_at(a, pages, 0, (sp.first + off + wave) * 32, row_bytes, head_off);
+        auto load_tile = [&]() __attribute__((always_inline)) {
             paged_load_k<HD, F8>(a.k + pa.half0, row_bytes, n, g, kr[0]);
             paged_load_k<HD, F8>(a.k + pa.half1, row_bytes, n, g, kr[1]);
             paged_load_v<HD, F8>(a.v + pa.half0, a.v + pa.half1, row_bytes, n, g, vr);
+        };
+        if ((unsigned)wave < seg) {
+            pages.load(a, table, sp.first + off + wave, W, sp.hi, lane);
+            pa = paged_at(a, pages, 0, (sp.first + off + wave) * 32, row_bytes, head_off);
+            if constexpr (AHEAD) load_tile();
         }
-        if (u != (unsigned)first) __syncthreads();  // the last segment's combine has read sm
-        for (int x = not_hoisted(threadIdx.x); x < C * D::NC * 64; x += kPagedThreads) {
+        if (again) __syncthreads();  // the last segment's combine has read sm
+        again = true;
+        for (int x = not_hoisted(threadIdx.x); x < C * D::NC * 64; x += 64 * W) {
             const int l = x & 63, ch = (x >> 6) % D::NC, c = (x >> 6) / D::NC;
             const unsigned r = qt * MQ + 16 * c + (l & 15);
             f16x8 v = {};
@@ -552,8 +581,9 @@ __global__ __launch_bounds__(kPagedThreads, 1) void k_paged_few(const PagedAttnA
         // Rows that every column attends: committed, and above every window's start.
         const unsigned clear_lo = !a.window ? 0u : a.b.positions ? sq.ctx : (unsigned)max((int)(sq.ctx + sq.n) - a.window, 0);
 
-        for (unsigned it = 0, t = wave; t < seg; it++, t += kPagedWaves) {
+        for (unsigned it = 0, t = wave; t < seg; it++, t += W) {
             const unsigned kt0 = (sp.first + off + t) * 32;
+            if constexpr (!AHEAD) load_tile();
             f32x4 sc[1][C][2];
 #pragma unroll
             for (int c = 0; c < C; c++)
@@ -570,15 +600,15 @@ __global__ __launch_bounds__(kPagedThreads, 1) void k_paged_few(const PagedAttnA
                 }
             }
             // The next tile's K into the registers just used (behind a masked tile's work: that needs some).
-            const bool more = t + kPagedWaves < seg;
+            const bool more = t + W < seg;
             PagedAt pn{};
             auto next_k = [&]() __attribute__((always_inline)) {
                 paged_load_k<HD, F8>(a.k + pn.half0, row_bytes, n, g, kr[0]);
                 paged_load_k<HD, F8>(a.k + pn.half1, row_bytes, n, g, kr[1]);
             };
             if (more) {
-                if (((it + 1) & 63) == 0) pages.load(a, table, sp.first + off + t + kPagedWaves, kPagedWaves, sp.hi, lane);
-                pn = paged_at(a, pages, (it + 1) & 63, kt0 + kPagedWaves * 32, row_bytes, head_off);
+                if (((it + 1) & 63) == 0) pages.load(a, table, sp.first + off + t + W, W, sp.hi, lane);
+                pn = paged_at(a, pages, (it + 1) & 63, kt0 + W * 32, row_bytes, head_off);
             }
             const bool clear = kt0 >= clear_lo && kt0 + 32 <= sq.ctx && pa.ok0 && pa.ok1;
             unsigned seen[1][C], dead = 0;
@@ -591,7 +621,7 @@ __global__ __launch_bounds__(kPagedThreads, 1) void k_paged_few(const PagedAttnA
                         for (int b = 0; b < D::VP; b++) vr[b][t8] = u32x4{0u, 0u, 0u, 0u};
                     }
             }
-            if (clear && more) next_k();
+            if (AHEAD && clear && more) next_k();
             f16x8 hi[1][C], lo[1][C];
             const PagedTake how[1] = {clear ? kClear : kMasked};
             paged_softmax<HD, C, F8, 1>(a, sc, seen, how, m_run, l_run, acc, hi, lo);
@@ -615,7 +645,7 @@ __global__ __launch_bounds__(kPagedThreads, 1) void k_paged_few(const PagedAttnA
                     paged_add_odd<HD, F8>(a.v + (t8 < 4 ? pa.half0 : pa.half1) + (uint32_t)(4 * gg + (t8 & 3)) * row_bytes, g,
                                           __shfl(seen[0][c], 16 * gg + n) >> t8 & 1, acc[c]);
             }
-            if (more) {
+            if (AHEAD && more) {
                 if (!clear) next_k();
                 paged_load_v<HD, F8>(a.v + pn.half0, a.v + pn.half1, row_bytes, n, g, vr);
             }
@@ -641,10 +671,10 @@ __global__ __launch_bounds__(kPagedThreads, 1) void k_paged_few(const PagedAttnA
             if (qt * MQ + 16 * c >= rows) break;  // uniform
             float M = -INFINITY, L = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kPagedWaves; w++) M = fmaxf(M, sm.m[w][16 * c + en]);
+            for (int w = 0; w < W; w++) M = fmaxf(M, sm.m[w][16 * c + en]);
             const float base = M == -INFINITY ? 0.0f : M;
 #pragma unroll
-            for (int w = 0; w < kPagedWaves; w++) L += sm.l[w][16 * c + en] * __builtin_amdgcn_exp2f(sm.m[w][16 * c + en] - base);
+            for (int w = 0; w < W; w++) L += sm.l[w][16 * c + en] * __builtin_amdgcn_exp2f(sm.m[w][16 * c + en] - base);
             const float f = __builtin_amdgcn_exp2f(m_run[c] - base);
             if (c) __syncthreads();
 #pragma unroll
@@ -658,16 +688,23 @@ __global__ __launch_bounds__(kPagedThreads, 1) void k_paged_few(const PagedAttnA
                 float* dst = whole ? a.out + ((uint64_t)(sq.start + r / G) * (a.nkh * G) + kvh * G + r % G) * HD
                                    : a.part_o + ((uint64_t)slot * MQ + rec) * HD;
                 if (!whole && wave == 0 && eg == 0) stg<f32x2>(a.part_ml + ((uint64_t)slot * MQ + rec) * 2, f32x2{M, L});
-                const int j = wave;  // of the 4 rows 4g + j of every output tile
+                // Of the 4 rows 4g + j of every output tile, j = wave % 4; eight waves share its elements too.
+                const int j = wave & 3;
+                constexpr int PART = D::E * 4 / W;
+                const int e0 = (wave >> 2) * PART;
 #pragma unroll
                 for (int b = 0; b < D::VP; b++)
 #pragma unroll
-                    for (int e = 0; e < D::E; e += 4) {
+                    for (int e1 = 0; e1 < PART; e1 += 4) {
+                        const int e = e0 + e1;
                         f32x4 x;
 #pragma unroll
                         for (int y = 0; y < 4; y++) {
                             const int k = (b * D::E + e + y) * 4 + j;
-                            x[y] = ((sm.o[0][k][el] + sm.o[1][k][el]) + (sm.o[2][k][el] + sm.o[3][k][el])) * inv;
+                            float sum = (sm.o[0][k][el] + sm.o[1][k][el]) + (sm.o[2][k][el] + sm.o[3][k][el]);
+                            if constexpr (W == 8)
+                                sum += (sm.o[4][k][el] + sm.o[5][k][el]) + (sm.o[6][k][el] + sm.o[7][k][el]);
+                            x[y] = sum * inv;
                         }
                         stg<f32x4>(dst + 16 * D::E * b + D::E * (4 * eg + j) + e, x);
                     }
@@ -737,14 +774,9 @@ __global__ __launch_bounds__(64 * WQ * WK, WPS) void k_paged_tile(const PagedAtt
     const int n = lane & 15, g = lane >> 4;
     const unsigned G = a.group;
 
-    PagedScan<MQ, UR> scan;
-    scan.run(a, lane);
-    const unsigned share = scan.share(a);
-    const uint64_t first = (uint64_t)blockIdx.x * share;
-    if (first >= scan.total) return;  // uniform
-    unsigned u = (unsigned)first;
-    const unsigned u_end = min(u + share, scan.total);
-    PagedPlace at = paged_place<MQ, UR>(a, scan, u, lane);
+    PagedPlace at;
+    unsigned u, u_end;
+    if (!paged_begin<MQ, UR>(a, lane, at, u, u_end)) return;  // uniform
     const uint32_t row_bytes = a.nkh * RB;
 
     // The lane's places in 32 rows: K row n (+ 16), pieces 4 c + g; V rows 4 g + t (+ 16), pieces n (+ 16).
@@ -765,7 +797,7 @@ __global__ __launch_bounds__(64 * WQ * WK, WPS) void k_paged_tile(const PagedAtt
 
     while (u < u_end) {  // one item or a part of one
         const unsigned i = uniform(at.i);
-        const unsigned s = i / a.q_tiles, qt = i % a.q_tiles;
+        const unsigned s = a.q_tiles > 1 ? i / a.q_tiles : i, qt = a.q_tiles > 1 ? i % a.q_tiles : 0u;
         const unsigned kvh = uniform(at.kvh), off = uniform(at.off);
         const PagedSeq sq{uniform(at.sq.start), uniform(at.sq.n), uniform(at.sq.ctx)};
         const PagedSpan sp = paged_span<MQ, UR>(a, sq, qt);
@@ -1092,8 +1124,15 @@ static PagedPlan paged_plan(unsigned head_dim, unsigned num_kv_heads, unsigned n
     return p;
 }
 
+// Whether every item goes to one workgroup: its rows are few for certain (by the window, or the block
+// table's size), so that cutting it and joining the parts in a second launch would cost more.
+static bool paged_whole(uint64_t rows, uint64_t items, unsigned cus) {
+    return rows <= 800 || (rows <= 2048 && items >= cus);
+}
+
 template <int HD, int MQ, int UR>
 static void launch_join(const PagedAttnArgs& a, hipStream_t st) {
+    if (a.whole) return;
     const unsigned items = a.b.n_seqs * a.q_tiles * a.nkh;
     if (items * 16 >= a.wgs) {  // few records an item
         G4_LAUNCH((k_paged_join<HD, MQ, UR, 1, HD>), dim3(items, MQ * HD / 4 / 256), dim3(256), 0, st, a);
@@ -1104,9 +1143,13 @@ static void launch_join(const PagedAttnArgs& a, hipStream_t st) {
 
 template <int HD, bool F8>
 static void launch_paged(const PagedAttnArgs& a, const PagedPlan& p, hipStream_t st) {
-    const dim3 grid(p.wgs);
+    const dim3 grid(a.whole ? a.b.n_seqs * a.q_tiles * a.nkh : p.wgs);
     if (p.mq == 16) {
-        G4_LAUNCH((k_paged_few<HD, 1, F8>), grid, dim3(kPagedThreads), 0, st, a);
+        if (HD == 256 && a.whole) {
+            if constexpr (HD == 256) G4_LAUNCH((k_paged_few<256, 1, F8, 8>), grid, dim3(512), 0, st, a);
+        } else {
+            G4_LAUNCH((k_paged_few<HD, 1, F8, kPagedWaves>), grid, dim3(64 * kPagedWaves), 0, st, a);
+        }
         launch_join<HD, 16, 32>(a, st);
     } else if constexpr (HD == 512) {
         constexpr int TS = F8 ? 2 : 1;
@@ -1116,7 +1159,7 @@ static void launch_paged(const PagedAttnArgs& a, const PagedPlan& p, hipStream_t
             G4_LAUNCH((k_paged_tile<512, 4, 1, TS, 5, F8, false, 1>), grid, dim3(256), 0, st, a);
         launch_join<HD, 64, 32 * TS>(a, st);
     } else if (p.mq == 32) {
-        G4_LAUNCH((k_paged_few<256, 2, F8>), grid, dim3(kPagedThreads), 0, st, a);
+        G4_LAUNCH((k_paged_few<256, 2, F8, kPagedWaves>), grid, dim3(64 * kPagedWaves), 0, st, a);
         launch_join<HD, 32, 32>(a, st);
     } else if (p.mq == 64) {
         G4_LAUNCH((k_paged_tile<256, 4, 2, 2, F8 ? 10 : 5, F8, true, 2>), grid, dim3(512), 0, st, a);
@@ -1193,6 +1236,9 @@ int g4_paged_attn(const g4_paged_cache* cache, const g4_paged_batch* batch, cons
     a.cap_log2 = p->softcap * kLog2e;
     a.wgs = plan.wgs;
     a.min_share = plan.mq <= 32 ? kPagedWaves : 1;
+    const uint64_t cap = (uint64_t)batch->table_stride * cache->page_size;
+    const uint64_t span = a.window ? (uint64_t)a.window + a.b.max_tokens : cap;
+    a.whole = paged_whole(span < cap ? span : cap, (uint64_t)a.b.n_seqs * a.q_tiles * a.nkh, device_cus());
     hipStream_t st = as_stream(stream);
     const bool f8 = cache->dtype == G4_KV_E4M3;
     if (cache->head_dim == 512) {

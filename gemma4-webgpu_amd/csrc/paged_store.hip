@@ -143,8 +143,9 @@ struct CommitPool {
     uint32_t row_bytes;
     uint32_t pieces;  // row_bytes / 16
 };
+template <int N>
 struct CommitArgs {
-    CommitPool pool[2 * G4_COMMIT_MAX_CACHES];
+    CommitPool pool[2 * N];
     const int32_t* __restrict__ path;
     const int32_t* __restrict__ accepted;
     int32_t* __restrict__ new_ctx;
@@ -154,7 +155,8 @@ struct CommitArgs {
 
 constexpr int kCommitBatch = 8;
 
-__global__ __launch_bounds__(kWG) void k_paged_commit(const CommitArgs a) {
+template <int N>
+__global__ __launch_bounds__(kWG) void k_paged_commit(const CommitArgs<N> a) {
     const CommitPool pool = a.pool[blockIdx.y];
     const unsigned i = blockIdx.x * kWG + threadIdx.x;  // below 2^31 (checked on the host)
     const unsigned s = i / pool.pieces, piece = i % pool.pieces;
@@ -239,6 +241,44 @@ int paged_check(const char* who, const g4_paged_cache* c, const g4_paged_batch* 
 
 using namespace g4;
 
+namespace {
+
+// The pools go by value in the kernel arguments: a block for up to 16 caches (a launch's cost grows with
+// its size), and one for the most there may be.
+template <int N>
+int commit(const g4_paged_cache* caches, uint32_t n_caches, const g4_paged_batch* batch, const int32_t* path,
+           uint32_t path_stride, const int32_t* n_accepted, int32_t* new_ctx_lens, void* stream) {
+    CommitArgs<N> a;
+    uint32_t most = 0;
+    for (uint32_t i = 0; i < n_caches; i++) {
+        const g4_paged_cache& c = caches[i];
+        g4_paged_batch plain = batch ? *batch : g4_paged_batch{};
+        plain.positions = nullptr;
+        plain.tree_mask = nullptr;
+        const int rc = paged_check("pagedCommit", &c, batch ? &plain : nullptr, &a.b);
+        if (rc) return rc;
+        if (c.page_size != caches[0].page_size || c.num_pages != caches[0].num_pages)
+            return fail(G4_EINVAL, "pagedCommit: cache %u has %u pages of %u rows, cache 0 %u of %u", i, c.num_pages,
+                        c.page_size, caches[0].num_pages, caches[0].page_size);
+        const uint32_t row_bytes = c.num_kv_heads * c.head_dim * (c.dtype == G4_KV_E4M3 ? 1u : 2u);
+        a.pool[2 * i] = {c.k_pool, row_bytes, row_bytes / 16};
+        a.pool[2 * i + 1] = {c.v_pool, row_bytes, row_bytes / 16};
+        if (row_bytes / 16 > most) most = row_bytes / 16;
+    }
+    if (new_ctx_lens == batch->ctx_lens) return fail(G4_EINVAL, "pagedCommit: new_ctx_lens is ctx_lens itself");
+    a.path = path;
+    a.accepted = n_accepted;
+    a.new_ctx = new_ctx_lens;
+    a.path_stride = path_stride;
+    const uint64_t threads = (uint64_t)batch->n_seqs * most;
+    if (threads > 0x7fffff00u) return fail(G4_EINVAL, "pagedCommit: %u sequences of %u-byte rows are too many", batch->n_seqs, most * 16);
+    G4_LAUNCH(k_paged_commit<N>, dim3((uint32_t)((threads + kWG - 1) / kWG), 2 * n_caches), dim3(kWG), 0, as_stream(stream), a);
+    G4_CHECK_LAUNCH("pagedCommit");
+    return G4_OK;
+}
+
+}  // namespace
+
 extern "C" {
 
 int g4_paged_append(const g4_paged_cache* cache, const g4_paged_batch* batch, const float* q, const float* k,
@@ -299,33 +339,9 @@ int g4_paged_commit(const g4_paged_cache* caches, uint32_t n_caches, const g4_pa
         return fail(G4_EINVAL, "pagedCommit: %u caches (1 to %d)", n_caches, G4_COMMIT_MAX_CACHES);
     if (!path || !n_accepted || !new_ctx_lens) return fail(G4_EINVAL, "pagedCommit: NULL path, n_accepted or new_ctx_lens");
     if (path_stride == 0 || path_stride > (1u << 30)) return fail(G4_EINVAL, "pagedCommit: path_stride %u", path_stride);
-    CommitArgs a = {};
-    uint32_t most = 0;
-    for (uint32_t i = 0; i < n_caches; i++) {
-        const g4_paged_cache& c = caches[i];
-        g4_paged_batch plain = batch ? *batch : g4_paged_batch{};
-        plain.positions = nullptr;
-        plain.tree_mask = nullptr;
-        const int rc = paged_check("pagedCommit", &c, batch ? &plain : nullptr, &a.b);
-        if (rc) return rc;
-        if (c.page_size != caches[0].page_size || c.num_pages != caches[0].num_pages)
-            return fail(G4_EINVAL, "pagedCommit: cache %u has %u pages of %u rows, cache 0 %u of %u", i, c.num_pages,
-                        c.page_size, caches[0].num_pages, caches[0].page_size);
-        const uint32_t row_bytes = c.num_kv_heads * c.head_dim * (c.dtype == G4_KV_E4M3 ? 1u : 2u);
-        a.pool[2 * i] = {c.k_pool, row_bytes, row_bytes / 16};
-        a.pool[2 * i + 1] = {c.v_pool, row_bytes, row_bytes / 16};
-        if (row_bytes / 16 > most) most = row_bytes / 16;
-    }
-    if (new_ctx_lens == batch->ctx_lens) return fail(G4_EINVAL, "pagedCommit: new_ctx_lens is ctx_lens itself");
-    a.path = path;
-    a.accepted = n_accepted;
-    a.new_ctx = new_ctx_lens;
-    a.path_stride = path_stride;
-    const uint64_t threads = (uint64_t)batch->n_seqs * most;
-    if (threads > 0x7fffff00u) return fail(G4_EINVAL, "pagedCommit: %u sequences of %u-byte rows are too many", batch->n_seqs, most * 16);
-    G4_LAUNCH(k_paged_commit, dim3((uint32_t)((threads + kWG - 1) / kWG), 2 * n_caches), dim3(kWG), 0, as_stream(stream), a);
-    G4_CHECK_LAUNCH("pagedCommit");
-    return G4_OK;
+    static_assert(G4_COMMIT_MAX_CACHES == 64, "the largest argument block");
+    return n_caches <= 16 ? commit<16>(caches, n_caches, batch, path, path_stride, n_accepted, new_ctx_lens, stream)
+                          : commit<64>(caches, n_caches, batch, path, path_stride, n_accepted, new_ctx_lens, stream);
 }
 
 }  // extern "C"
