@@ -805,9 +805,10 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_paged_few(const PagedAttnArgs
 // ahead; one barrier a slot. A row's 16-byte pieces are stored at piece ^ (row % 16), which spreads
 // both operands' reads over all banks (sixteen lanes read sixteen rows of K, or sixteen pieces of one
 // row of V). NT: the rows are read by one workgroup alone and bypass the caches.
-template <int HD, bool F8, int TS, int NS>
+template <int HD, bool F8, int TS, int NS, int PW>
 struct PagedTileSmem {
     unsigned char t[NS][32 * TS][HD * (F8 ? 1 : 2)];
+    f32x4 parts[PW][TS][2][64];  // parts of the scores
 };
 
 // Waits until at most behind * PER of the wave's DMA requests are outstanding (behind <= MOST, uniform),
@@ -836,23 +837,25 @@ __device__ __forceinline__ void paged_dma(uint32_t voff, const void* sbase, uint
 }
 #pragma clang diagnostic pop
 
-template <int HD, int WQ, int WK, int TS, int NS, bool F8, bool NT, int WPS>
-__global__ __launch_bounds__(64 * WQ * WK, WPS) void k_paged_tile(const PagedAttnArgs a) {
-    using D = PagedDims<HD, F8>;
-    constexpr int W = WQ * WK, MQ = 16 * WQ, UR = 32 * TS;
+template <int HD, int WQ, int WK, int WD, int TS, int NS, bool F8, bool NT>
+__global__ __launch_bounds__(64 * WQ * WK * WD, WQ * WK * WD / 4) void k_paged_tile(const PagedAttnArgs a) {
+    using D = PagedDims<HD / WD, F8>;  // a wave's part of a row
+    constexpr int W = WQ * WK * WD, MQ = 16 * WQ, UR = 32 * TS;
     constexpr int NX = TS / WK;                // 32-row tiles of a slot that a wave works on
     constexpr uint32_t RB = HD * D::ES;        // a row's bytes
+    constexpr uint32_t PB = RB / WD;           // a wave's part's
     constexpr uint32_t PPR = RB / 16;          // pieces a row
     constexpr uint32_t RPI = 1024 / RB;        // rows a DMA instruction moves
     constexpr int IH = 16 / RPI;               // instructions 16 rows take
     constexpr int PER = 2 * TS * IH / W;       // of a slot's instructions, a wave's
     static_assert(2 * TS * IH % W == 0 && IH % PER == 0 && TS % WK == 0, "whole instructions, of one half, a wave");
     static_assert((NS - 2) * PER < 64, "outstanding requests are counted in six bits");
+    static_assert(WK == 1 || WD == 1, "one of them");
     static_assert(WK == 1 || WQ * HD * 16 * 4 + 2 * MQ * 4 <= NS * UR * (int)RB, "the waves' states are joined in the ring");
-    __shared__ __align__(1024) PagedTileSmem<HD, F8, TS, NS> sm;
+    __shared__ __align__(1024) PagedTileSmem<HD, F8, TS, NS, WD == 1 ? 0 : W> sm;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wq = wave % WQ, wk = wave / WQ;
+    const int wq = wave % WQ, wk = WK > 1 ? wave / WQ : 0, wd = WD > 1 ? wave / WQ : 0;
     const int n = lane & 15, g = lane >> 4;
     const unsigned G = a.group;
 
@@ -904,7 +907,7 @@ __global__ __launch_bounds__(64 * WQ * WK, WPS) void k_paged_tile(const PagedAtt
             const uint16_t* src = a.q + ((uint64_t)(sq.start + (live ? r / G : 0u)) * (a.nkh * G) + kvh * G + (live ? r % G : 0u)) * HD;
 #pragma unroll
             for (int ch = 0; ch < D::NC; ch++) {
-                qr[ch] = ldg<f16x8>(src + paged_q_elem<F8>(ch, g));
+                qr[ch] = ldg<f16x8>(src + wd * (HD / WD) + paged_q_elem<F8>(ch, g));
                 if (!live) qr[ch] = f16x8{};
             }
         }
@@ -980,7 +983,7 @@ __global__ __launch_bounds__(64 * WQ * WK, WPS) void k_paged_tile(const PagedAtt
             unsigned seen[NX][1], dead[NX];
             PagedTake how[NX];
             bool some = false;
-            const unsigned char* kt = take(2 * t) + wk * NX * 32 * RB;
+            const unsigned char* kt = take(2 * t) + wk * NX * 32 * RB + wd * PB;
 #pragma unroll
             for (int x = 0; x < NX; x++) {
                 const unsigned kt0 = (sp.first + off + t) * UR + (wk * NX + x) * 32;
@@ -1014,8 +1017,24 @@ __global__ __launch_bounds__(64 * WQ * WK, WPS) void k_paged_tile(const PagedAtt
                 how[x] = kt0 >= clear_lo && kt0 + 32 <= clear_hi && ok0 && ok1 ? kClear : kMasked;
                 if (how[x] == kMasked) cols.look(a, sq, sp.hi, kt0, g, ok0, ok1, seen[x], dead[x]);
             }
-            if (some) paged_softmax<HD, 1, F8, NX>(a, sc, seen, how, m_run, l_run, acc, hi, lo);
-            const unsigned char* vt = take(2 * t + 1) + wk * NX * 32 * RB;
+            if constexpr (WD > 1) {  // the parts' scores, added behind the barrier of V's slot
+#pragma unroll
+                for (int x = 0; x < NX; x++) {
+                    sm.parts[wave][x][0][lane] = sc[x][0][0];
+                    sm.parts[wave][x][1][lane] = sc[x][0][1];
+                }
+            }
+            if constexpr (WD == 1)
+                if (some) paged_softmax<HD, 1, F8, NX>(a, sc, seen, how, m_run, l_run, acc, hi, lo);
+            const unsigned char* vt = take(2 * t + 1) + wk * NX * 32 * RB + wd * PB;
+            if constexpr (WD > 1) {
+#pragma unroll
+                for (int x = 0; x < NX; x++) {
+                    sc[x][0][0] += sm.parts[wave ^ WQ][x][0][lane];
+                    sc[x][0][1] += sm.parts[wave ^ WQ][x][1][lane];
+                }
+                if (some) paged_softmax<HD / WD, 1, F8, NX>(a, sc, seen, how, m_run, l_run, acc, hi, lo);
+            }
 #pragma unroll
             for (int x = 0; x < NX; x++) {
                 const unsigned part = wk * NX + x;
@@ -1033,7 +1052,7 @@ __global__ __launch_bounds__(64 * WQ * WK, WPS) void k_paged_tile(const PagedAtt
                             if (dead[x] >> y & 1) vr[y] = u32x4{0u, 0u, 0u, 0u};
                         odd_rows |= paged_take_odd<F8>(vr);
                     }
-                    paged_pv<HD, 1, F8>(b, vr, hi[x], lo[x], acc);
+                    paged_pv<HD / WD, 1, F8>(b, vr, hi[x], lo[x], acc);
                 }
                 while (odd_rows) {
                     const int bit = __builtin_ctz(odd_rows), t8 = bit >> 2, gg = bit & 3;
@@ -1045,7 +1064,7 @@ __global__ __launch_bounds__(64 * WQ * WK, WPS) void k_paged_tile(const PagedAtt
                         const unsigned p = page_of(t, h);
                         page = half == (unsigned)h ? p : page;
                     }
-                    paged_add_odd<HD, F8>(a.v + half_at(t, half, page) + (uint32_t)(4 * gg + (t8 & 3)) * row_bytes, g,
+                    paged_add_odd<HD / WD, F8>(a.v + half_at(t, half, page) + (uint32_t)(4 * gg + (t8 & 3)) * row_bytes + wd * PB, g,
                                           __shfl(seen[x][0], 16 * gg + n) >> t8 & 1, acc[0]);
                 }
             }
@@ -1089,7 +1108,7 @@ __global__ __launch_bounds__(64 * WQ * WK, WPS) void k_paged_tile(const PagedAtt
             const float inv = whole ? paged_inverse(L) : 1.0f;
             float* dst = whole ? a.out + ((uint64_t)(sq.start + r / G) * (a.nkh * G) + kvh * G + r % G) * HD
                                : a.part_o + ((uint64_t)slot * MQ + rec) * HD;
-            if (!whole && g == 0) stg<f32x2>(a.part_ml + ((uint64_t)slot * MQ + rec) * 2, f32x2{M, L});
+            if (!whole && g == 0 && wd == 0) stg<f32x2>(a.part_ml + ((uint64_t)slot * MQ + rec) * 2, f32x2{M, L});
 #pragma unroll
             for (int b = 0; b < D::VP; b++)
 #pragma unroll
@@ -1097,7 +1116,7 @@ __global__ __launch_bounds__(64 * WQ * WK, WPS) void k_paged_tile(const PagedAtt
 #pragma unroll
                     for (int e = 0; e < D::E; e += 4) {
                         const int x = b * D::E + e;
-                        stg<f32x4>(dst + 16 * D::E * b + D::E * (4 * g + j) + e,
+                        stg<f32x4>(dst + wd * (HD / WD) + 16 * D::E * b + D::E * (4 * g + j) + e,
                                    f32x4{acc[0][x][j], acc[0][x + 1][j], acc[0][x + 2][j], acc[0][x + 3][j]} * inv);
                     }
         }
@@ -1244,18 +1263,18 @@ static void launch_paged(const PagedAttnArgs& a, const PagedPlan& p, hipStream_t
     } else if constexpr (HD == 512) {
         constexpr int TS = F8 ? 2 : 1;
         if (p.q_tiles == 1)
-            G4_LAUNCH((k_paged_tile<512, 4, 1, TS, 5, F8, true, 1>), grid, dim3(256), 0, st, a);
+            G4_LAUNCH((k_paged_tile<512, 4, 1, 2, TS, 4, F8, true>), grid, dim3(512), 0, st, a);
         else
-            G4_LAUNCH((k_paged_tile<512, 4, 1, TS, 5, F8, false, 1>), grid, dim3(256), 0, st, a);
+            G4_LAUNCH((k_paged_tile<512, 4, 1, 2, TS, 4, F8, false>), grid, dim3(512), 0, st, a);
         launch_join<HD, 64, 32 * TS>(a, st);
     } else if (p.mq == 32) {
         G4_LAUNCH((k_paged_few<256, 2, F8, kPagedWaves>), grid, dim3(64 * kPagedWaves), 0, st, a);
         launch_join<HD, 32, 32>(a, st);
     } else if (p.mq == 64) {
-        G4_LAUNCH((k_paged_tile<256, 4, 2, 2, F8 ? 10 : 5, F8, true, 2>), grid, dim3(512), 0, st, a);
+        G4_LAUNCH((k_paged_tile<256, 4, 2, 1, 2, F8 ? 10 : 5, F8, true>), grid, dim3(512), 0, st, a);
         launch_join<HD, 64, 64>(a, st);
     } else {
-        G4_LAUNCH((k_paged_tile<256, 8, 1, 2, F8 ? 10 : 5, F8, false, 2>), grid, dim3(512), 0, st, a);
+        G4_LAUNCH((k_paged_tile<256, 8, 1, 1, 2, F8 ? 10 : 5, F8, false>), grid, dim3(512), 0, st, a);
         launch_join<HD, 128, 64>(a, st);
     }
 }
