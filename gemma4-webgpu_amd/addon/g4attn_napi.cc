@@ -1358,6 +1358,114 @@ napi_value SizeofPromptPrepEntry(napi_env env, napi_callback_info) {
     return number(env, (double)sizeof(g4_prompt_prep_entry));
 }
 
+// ---- drafted tokens over a paged cache ----------------------------------------
+// g4_paged_cache and g4_paged_batch travel as their bytes (pointers as 64-bit words), in one array each.
+
+bool paged_args(Args& a, size_t i, g4_paged_cache* cache, g4_paged_batch* batch) {
+    a.params(i, cache);
+    a.params(i + 1, batch);
+    return a.ok;
+}
+
+// pagedAppend(cache, batch, q, k, v, qWeight, kWeight, ropeInvFreq, qOut, params, stream): q, qWeight, qOut or
+// k, v, kWeight may be null together.
+napi_value PagedAppend(napi_env env, napi_callback_info info) {
+    Args a(env, info, 11);
+    g4_paged_cache cache;
+    g4_paged_batch batch;
+    g4_paged_append_params p;
+    if (!paged_args(a, 0, &cache, &batch)) return nullptr;
+    void* d[7];
+    for (int i = 0; i < 7; i++) d[i] = a.ptr(2 + i);
+    a.params(9, &p);
+    void* s = a.ptr(10);
+    if (!a.ok) return nullptr;
+    CALL(env, g4_paged_append(&cache, &batch, (const float*)d[0], (const float*)d[1], (const float*)d[2],
+                              (const uint16_t*)d[3], (const uint16_t*)d[4], (const float*)d[5], (uint16_t*)d[6], &p, s));
+    return undefined(env);
+}
+
+napi_value PagedAttnWorkspaceSize(napi_env env, napi_callback_info info) {
+    Args a(env, info, 3);  // cache, batch, nqh
+    g4_paged_cache cache;
+    g4_paged_batch batch;
+    if (!paged_args(a, 0, &cache, &batch)) return nullptr;
+    const uint32_t nqh = a.u32(2);
+    if (!a.ok) return nullptr;
+    size_t bytes = 0;
+    CALL(env, g4_paged_attn_workspace_size(&cache, &batch, nqh, &bytes));
+    return number(env, (double)bytes);
+}
+
+napi_value PagedAttn(napi_env env, napi_callback_info info) {
+    Args a(env, info, 8);  // cache, batch, q, out, params, workspace, workspaceBytes, stream
+    g4_paged_cache cache;
+    g4_paged_batch batch;
+    g4_paged_attn_params p;
+    if (!paged_args(a, 0, &cache, &batch)) return nullptr;
+    void* q = a.ptr(2);
+    void* out = a.ptr(3);
+    a.params(4, &p);
+    void* ws = a.ptr(5);
+    const double ws_bytes = a.f64(6);
+    void* s = a.ptr(7);
+    if (!a.ok) return nullptr;
+    CALL(env, g4_paged_attn(&cache, &batch, (const uint16_t*)q, (float*)out, &p, ws, (size_t)ws_bytes, s));
+    return undefined(env);
+}
+
+// pagedCommit(caches, nCaches, batch, path, pathStride, nAccepted, newCtxLens, stream): caches' records one behind
+// the other.
+napi_value PagedCommit(napi_env env, napi_callback_info info) {
+    Args a(env, info, 8);
+    void* d = nullptr;
+    size_t n = 0;
+    a.bytes(0, &d, &n);
+    const uint32_t nc = a.u32(1);
+    g4_paged_batch batch;
+    a.params(2, &batch);
+    void* path = a.ptr(3);
+    const uint32_t stride = a.u32(4);
+    void* acc = a.ptr(5);
+    void* ctx = a.ptr(6);
+    void* s = a.ptr(7);
+    if (!a.ok) return nullptr;
+    if (n < (size_t)nc * sizeof(g4_paged_cache)) {
+        napi_throw_range_error(env, nullptr, "pagedCommit: fewer bytes than the caches' records");
+        return nullptr;
+    }
+    std::vector<g4_paged_cache> caches(nc);
+    if (nc) memcpy(caches.data(), d, nc * sizeof(g4_paged_cache));
+    CALL(env, g4_paged_commit(caches.data(), nc, &batch, (const int32_t*)path, stride, (const int32_t*)acc, (int32_t*)ctx, s));
+    return undefined(env);
+}
+
+napi_value TokenLogprobsWorkspaceSize(napi_env env, napi_callback_info info) {
+    Args a(env, info, 1);  // params
+    g4_token_logprobs_params p;
+    a.params(0, &p);
+    if (!a.ok) return nullptr;
+    size_t bytes = 0;
+    CALL(env, g4_token_logprobs_workspace_size(&p, &bytes));
+    return number(env, (double)bytes);
+}
+
+// tokenLogprobs(logits, tokens, logprobs, entropy, topIds, topLogprobs, params, workspace, workspaceBytes, stream)
+napi_value TokenLogprobs(napi_env env, napi_callback_info info) {
+    Args a(env, info, 10);
+    void* d[6];
+    for (int i = 0; i < 6; i++) d[i] = a.ptr(i);
+    g4_token_logprobs_params p;
+    a.params(6, &p);
+    void* ws = a.ptr(7);
+    const double ws_bytes = a.f64(8);
+    void* s = a.ptr(9);
+    if (!a.ok) return nullptr;
+    CALL(env, g4_token_logprobs(d[0], (const int32_t*)d[1], (float*)d[2], (float*)d[3], (int32_t*)d[4], (float*)d[5], &p, ws,
+                                (size_t)ws_bytes, s));
+    return undefined(env);
+}
+
 napi_value Init(napi_env env, napi_value exports) {
     struct {
         const char* name;
@@ -1417,6 +1525,12 @@ napi_value Init(napi_env env, napi_value exports) {
         {"attnPromptPrepMany", AttnPromptPrepMany},
         {"sizeofPromptPrepEntry", SizeofPromptPrepEntry},
         {"attnPromptPrepVt", AttnPromptPrepVt},
+        {"pagedAppend", PagedAppend},
+        {"pagedAttnWorkspaceSize", PagedAttnWorkspaceSize},
+        {"pagedAttn", PagedAttn},
+        {"pagedCommit", PagedCommit},
+        {"tokenLogprobsWorkspaceSize", TokenLogprobsWorkspaceSize},
+        {"tokenLogprobs", TokenLogprobs},
     };
     for (auto& f : fns) {
         napi_value fn;
@@ -1438,6 +1552,11 @@ napi_value Init(napi_env env, napi_value exports) {
         {"sizeofSoftcapParams", sizeof(g4_softcap_params)},
         {"sizeofArgmaxParams", sizeof(ArgmaxUniform)},
         {"sizeofQkvPrepParams", sizeof(g4_qkv_prep_params)},
+        {"sizeofPagedCache", sizeof(g4_paged_cache)},
+        {"sizeofPagedBatch", sizeof(g4_paged_batch)},
+        {"sizeofPagedAppendParams", sizeof(g4_paged_append_params)},
+        {"sizeofPagedAttnParams", sizeof(g4_paged_attn_params)},
+        {"sizeofTokenLogprobsParams", sizeof(g4_token_logprobs_params)},
     };
     for (auto& s : sizes) NAPI_OK(env, napi_set_named_property(env, exports, s.name, number(env, (double)s.size)));
     return exports;

@@ -32,7 +32,8 @@ export type QuantKernelName = 'matmulQ8' | 'matmulQ4K';
 
 export type KernelName = AttnKernelName | SampleKernelName | QuantKernelName;
 
-export type FusedKernelName = 'attnStep' | 'attnPrefill' | 'attnPromptPrep' | 'lmHeadArgmax' | 'linearQkvPrep';
+export type FusedKernelName = 'attnStep' | 'attnPrefill' | 'attnPromptPrep' | 'lmHeadArgmax' | 'linearQkvPrep'
+  | 'pagedAppend' | 'pagedAttn' | 'pagedCommit' | 'tokenLogprobs';
 
 export type UniformValue = { u: number } | { f: number };
 
@@ -87,6 +88,10 @@ export const PASS_LABELS: Record<string, string> = {
   linearOut: 'attn.linearOut',
   attnStepOut: 'attn.linearOut',
   linearQkvPrep: 'attn.linearQKVPrep',
+  pagedAppend: 'attn.pagedAppend',
+  pagedAttn: 'attn.paged',
+  pagedCommit: 'attn.pagedCommit',
+  tokenLogprobs: 'sample.tokenLogprobs',
 };
 
 // The profiler's report types (src/types.ts:490-515).
@@ -266,6 +271,78 @@ export interface QuantSegment {
   rows: number;
 }
 
+// One layer's paged cache: pages of pageSize rows [numPages][pageSize][numKvHeads][headDim], f16 or e4m3.
+export interface PagedCache {
+  kPool: DeviceBuffer;
+  vPool: DeviceBuffer;
+  numPages: number;
+  pageSize: number;           // a power of two in [16, 1024]
+  numKvHeads: number;
+  headDim: number;            // 256 or 512
+  dtype?: 'f16' | 'e4m3';     // default f16
+}
+
+// A step's sequences and their new tokens. The buffers are read when a kernel runs: row r of sequence s lies in page
+// blockTable[s * tableStride + r / pageSize], rows below ctxLens[s] are committed, new token j of the sequence
+// (token tokenStart[s] + j of the batch) has row ctxLens[s] + j.
+export interface PagedBatch {
+  blockTable: DeviceBuffer;   // i32 [nSeqs][tableStride]
+  tokenStart: DeviceBuffer;   // i32 [nSeqs + 1], ascending
+  ctxLens: DeviceBuffer;      // i32 [nSeqs]
+  positions?: DeviceBuffer;   // i32 [nTokens], for trees: ctx + depth (default: a token's row)
+  treeMask?: DeviceBuffer;    // u64 [nTokens][maskWords]: bit j, the token attends new token j (default: a chain)
+  nSeqs: number;
+  tableStride: number;
+  nTokens: number;            // of the token buffers, padding included
+  maxTokens: number;          // at least the longest sequence's new tokens
+  maskWords?: number;         // with treeMask: at least ceil(maxTokens / 64)
+}
+
+// pagedAppend's operands. q, qWeight, qOut absent: only the rows' store; k, v, kWeight absent: a KV-consumer layer.
+export interface PagedAppend {
+  q?: DeviceBuffer;           // f32 [nTokens][numQHeads][headDim], tokens qStride elements apart (0: contiguous)
+  k?: DeviceBuffer;           // f32 [nTokens][numKvHeads][headDim]
+  v?: DeviceBuffer;
+  qWeight?: DeviceBuffer;     // attn_q_norm f16 [headDim]
+  kWeight?: DeviceBuffer;     // attn_k_norm f16 [headDim]
+  ropeInvFreq: DeviceBuffer;  // f32 [headDim / 2] from ropeInvFreq
+  qOut?: DeviceBuffer;        // f16 [nTokens][numQHeads][headDim]: pagedAttn's query
+  numQHeads?: number;         // with q
+  eps?: number;
+  qStride?: number;
+  kStride?: number;
+  vStride?: number;
+}
+
+export interface PagedAttn {
+  q: DeviceBuffer;            // f16 [nTokens][numQHeads][headDim], as pagedAppend leaves it
+  out: DeviceBuffer;          // f32, the same shape
+  numQHeads: number;
+  slidingWindow?: number;     // 0 = full
+  scale?: number;
+  softcap?: number;           // 0 = none
+}
+
+// Log probabilities of given tokens, entropy and the best alternatives of each row of logits.
+export interface TokenLogprobs {
+  logits: DeviceBuffer;       // [rows][vocab] of dtype, rows rowStride elements apart
+  tokens?: DeviceBuffer;      // i32 [rows] and logprobs f32 [rows], together
+  logprobs?: DeviceBuffer;
+  entropy?: DeviceBuffer;     // f32 [rows]
+  topIds?: DeviceBuffer;      // i32 and f32 [rows][topK], together
+  topLogprobs?: DeviceBuffer;
+  rows: number;
+  vocab: number;
+  rowStride?: number;         // 0: vocab
+  dtype?: 'f32' | 'f16' | 'bf16';
+  topK?: number;
+  cap?: number;               // the final softcap, 0 = none
+  temperature?: number;
+}
+
+const LOGIT_DTYPES: Record<string, number> = { f32: 0, f16: 1, bf16: 2 };
+const LOGIT_BYTES: Record<string, number> = { f32: 4, f16: 2, bf16: 2 };
+
 export interface StepShape {
   numQHeads: number;
   numKvHeads: number;
@@ -336,6 +413,16 @@ export interface Addon {
   attnPromptPrepVt(q: bigint, k: bigint, v: bigint, qw: bigint, kw: bigint, rf: bigint | null,
     inv: bigint | null, qOut: bigint, kc: bigint, vc: bigint, vt: bigint, p: Uint8Array, s: bigint): void;
   attnPromptPrepMany(entries: Uint8Array, n: number, s: bigint): void;
+  pagedAppend(cache: Uint8Array, batch: Uint8Array, q: bigint | null, k: bigint | null, v: bigint | null, qw: bigint | null,
+    kw: bigint | null, inv: bigint, qOut: bigint | null, p: Uint8Array, s: bigint): void;
+  pagedAttnWorkspaceSize(cache: Uint8Array, batch: Uint8Array, nqh: number): number;
+  pagedAttn(cache: Uint8Array, batch: Uint8Array, q: bigint, out: bigint, p: Uint8Array, ws: bigint, wsBytes: number,
+    s: bigint): void;
+  pagedCommit(caches: Uint8Array, n: number, batch: Uint8Array, path: bigint, pathStride: number, accepted: bigint,
+    newCtxLens: bigint, s: bigint): void;
+  tokenLogprobsWorkspaceSize(p: Uint8Array): number;
+  tokenLogprobs(logits: bigint, tokens: bigint | null, logprobs: bigint | null, entropy: bigint | null,
+    topIds: bigint | null, topLogprobs: bigint | null, p: Uint8Array, ws: bigint, wsBytes: number, s: bigint): void;
   [key: string]: any;
 }
 
@@ -739,6 +826,159 @@ export class HipAttention {
     const slot = this.beginPass(PASS_LABELS.attnPromptPrep);
     try {
       this.g4.attnPromptPrepMany(bytes, chunks.length, this.stream);
+    } finally {
+      this.endPass(slot);
+    }
+  }
+
+  // g4_paged_cache: two pointers, then six 4-byte fields; one record a cache.
+  static pagedCacheBytes(caches: PagedCache[]): Uint8Array {
+    const REC = 40;
+    const bytes = new Uint8Array(REC * caches.length);
+    const dv = new DataView(bytes.buffer);
+    caches.forEach(function (c, i) {
+      const need = c.numPages * c.pageSize * c.numKvHeads * c.headDim * (c.dtype === 'e4m3' ? 1 : 2);
+      if (c.kPool.size < need || c.vPool.size < need) throw new RangeError('paged cache ' + i + ': pools too small');
+      const o = i * REC;
+      dv.setBigUint64(o, c.kPool.ptr, true);
+      dv.setBigUint64(o + 8, c.vPool.ptr, true);
+      [c.numPages, c.pageSize, c.numKvHeads, c.headDim, c.dtype === 'e4m3' ? 1 : 0, 0].forEach(function (x, j) {
+        dv.setUint32(o + 16 + 4 * j, x, true);
+      });
+    });
+    return bytes;
+  }
+
+  // g4_paged_batch: five pointers, then six 4-byte fields.
+  static pagedBatchBytes(b: PagedBatch): Uint8Array {
+    const words = b.treeMask ? b.maskWords || 0 : 0;
+    if (b.blockTable.size < b.nSeqs * b.tableStride * 4) throw new RangeError('paged batch: blockTable too small');
+    if (b.tokenStart.size < (b.nSeqs + 1) * 4) throw new RangeError('paged batch: tokenStart too small');
+    if (b.ctxLens.size < b.nSeqs * 4) throw new RangeError('paged batch: ctxLens too small');
+    if (b.positions && b.positions.size < b.nTokens * 4) throw new RangeError('paged batch: positions too small');
+    if (b.treeMask && b.treeMask.size < b.nTokens * words * 8) throw new RangeError('paged batch: treeMask too small');
+    const bytes = new Uint8Array(64);
+    const dv = new DataView(bytes.buffer);
+    [b.blockTable, b.tokenStart, b.ctxLens, b.positions, b.treeMask].forEach(function (x, j) {
+      dv.setBigUint64(8 * j, x ? x.ptr : BigInt(0), true);
+    });
+    [b.nSeqs, b.tableStride, b.nTokens, b.maxTokens, words, 0].forEach(function (x, j) {
+      dv.setUint32(40 + 4 * j, x, true);
+    });
+    return bytes;
+  }
+
+  // A batch's new tokens normed, rotated and stored in one layer's paged cache, its query left for pagedAttn: the
+  // values of attnPromptPrep at each token's position.
+  pagedAppend(cache: PagedCache, batch: PagedBatch, p: PagedAppend): void {
+    if ((p.q === undefined) !== (p.qWeight === undefined) || (p.q === undefined) !== (p.qOut === undefined)) {
+      throw new Error('pagedAppend: q, qWeight and qOut go together');
+    }
+    if ((p.k === undefined) !== (p.v === undefined) || (p.k === undefined) !== (p.kWeight === undefined)) {
+      throw new Error('pagedAppend: k, v and kWeight go together');
+    }
+    const nqh = p.q ? p.numQHeads || 0 : 0;
+    function rows(b: DeviceBuffer | undefined, stride: number | undefined, heads: number, what: string): number {
+      const width = heads * cache.headDim;
+      const step = stride || width;
+      if (b && batch.nTokens > 0 && b.size < ((batch.nTokens - 1) * step + width) * 4) {
+        throw new RangeError('pagedAppend: ' + what + ' too small');
+      }
+      return stride || 0;
+    }
+    const strides = [rows(p.q, p.qStride, nqh, 'q'), rows(p.k, p.kStride, cache.numKvHeads, 'k'),
+      rows(p.v, p.vStride, cache.numKvHeads, 'v')];
+    if (p.qOut && p.qOut.size < batch.nTokens * nqh * cache.headDim * 2) throw new RangeError('pagedAppend: qOut too small');
+    for (const w of [p.qWeight, p.kWeight, p.ropeInvFreq]) {
+      if (w && w.size < cache.headDim * 2) throw new RangeError('pagedAppend: weights or ropeInvFreq too small');
+    }
+    const params = new Uint8Array(32);
+    const dv = new DataView(params.buffer);
+    dv.setUint32(0, nqh, true);
+    dv.setFloat32(4, p.eps === undefined ? 1e-6 : p.eps, true);
+    strides.forEach(function (x, j) { dv.setBigUint64(8 + 8 * j, BigInt(x), true); });
+    function ptr(b: DeviceBuffer | undefined): bigint | null { return b ? b.ptr : null; }
+    const cb = HipAttention.pagedCacheBytes([cache]);
+    const bb = HipAttention.pagedBatchBytes(batch);
+    const slot = this.beginPass(PASS_LABELS.pagedAppend);
+    try {
+      this.g4.pagedAppend(cb, bb, ptr(p.q), ptr(p.k), ptr(p.v), ptr(p.qWeight), ptr(p.kWeight), p.ropeInvFreq.ptr,
+        ptr(p.qOut), params, this.stream);
+    } finally {
+      this.endPass(slot);
+    }
+  }
+
+  pagedAttnWorkspaceSize(cache: PagedCache, batch: PagedBatch, numQHeads: number): number {
+    return this.g4.pagedAttnWorkspaceSize(HipAttention.pagedCacheBytes([cache]), HipAttention.pagedBatchBytes(batch), numQHeads);
+  }
+
+  // Attention of a batch's new tokens over their sequences' committed rows and the new rows their mask names (stored
+  // before, by pagedAppend).
+  pagedAttn(cache: PagedCache, batch: PagedBatch, p: PagedAttn, workspace: DeviceBuffer): void {
+    const n = batch.nTokens * p.numQHeads * cache.headDim;
+    if (p.q.size < n * 2) throw new RangeError('pagedAttn: q too small');
+    if (p.out.size < n * 4) throw new RangeError('pagedAttn: out too small');
+    const params = new Uniform([{ u: p.numQHeads }, { u: p.slidingWindow || 0 }, { f: p.scale === undefined ? 1.0 : p.scale },
+      { f: p.softcap || 0 }]);
+    const cb = HipAttention.pagedCacheBytes([cache]);
+    const bb = HipAttention.pagedBatchBytes(batch);
+    const slot = this.beginPass(PASS_LABELS.pagedAttn);
+    try {
+      this.g4.pagedAttn(cb, bb, p.q.ptr, p.out.ptr, params.bytes, workspace.ptr, workspace.size, this.stream);
+    } finally {
+      this.endPass(slot);
+    }
+  }
+
+  // The accepted drafted tokens' rows moved together, in every layer's cache: path i32 [nSeqs][pathStride] new-token
+  // indices, ascending, nAccepted i32 [nSeqs] of them; newCtxLens i32 [nSeqs] receives the lengths after.
+  pagedCommit(caches: PagedCache[], batch: PagedBatch, path: DeviceBuffer, pathStride: number, nAccepted: DeviceBuffer,
+    newCtxLens: DeviceBuffer): void {
+    if (path.size < batch.nSeqs * pathStride * 4) throw new RangeError('pagedCommit: path too small');
+    if (nAccepted.size < batch.nSeqs * 4) throw new RangeError('pagedCommit: nAccepted too small');
+    if (newCtxLens.size < batch.nSeqs * 4) throw new RangeError('pagedCommit: newCtxLens too small');
+    const cb = HipAttention.pagedCacheBytes(caches);
+    const bb = HipAttention.pagedBatchBytes(batch);
+    const slot = this.beginPass(PASS_LABELS.pagedCommit);
+    try {
+      this.g4.pagedCommit(cb, caches.length, bb, path.ptr, pathStride, nAccepted.ptr, newCtxLens.ptr, this.stream);
+    } finally {
+      this.endPass(slot);
+    }
+  }
+
+  // g4_token_logprobs_params: rows, vocab, a 64-bit stride, dtype, topK, cap, temperature.
+  static tokenLogprobsParams(p: TokenLogprobs): Uint8Array {
+    const params = new Uint8Array(32);
+    const dv = new DataView(params.buffer);
+    dv.setUint32(0, p.rows, true);
+    dv.setUint32(4, p.vocab, true);
+    dv.setBigUint64(8, BigInt(p.rowStride || 0), true);
+    dv.setUint32(16, LOGIT_DTYPES[p.dtype || 'f32'], true);
+    dv.setUint32(20, p.topK || 0, true);
+    dv.setFloat32(24, p.cap || 0, true);
+    dv.setFloat32(28, p.temperature === undefined ? 1.0 : p.temperature, true);
+    return params;
+  }
+
+  tokenLogprobsWorkspaceSize(p: TokenLogprobs): number {
+    return this.g4.tokenLogprobsWorkspaceSize(HipAttention.tokenLogprobsParams(p));
+  }
+
+  tokenLogprobs(p: TokenLogprobs, workspace: DeviceBuffer): void {
+    const k = p.topK || 0;
+    const need: [DeviceBuffer | undefined, number, string][] = [
+      [p.logits, p.rows ? ((p.rows - 1) * (p.rowStride || p.vocab) + p.vocab) * LOGIT_BYTES[p.dtype || 'f32'] : 0, 'logits'],
+      [p.tokens, p.rows * 4, 'tokens'], [p.logprobs, p.rows * 4, 'logprobs'], [p.entropy, p.rows * 4, 'entropy'],
+      [p.topIds, p.rows * k * 4, 'topIds'], [p.topLogprobs, p.rows * k * 4, 'topLogprobs']];
+    for (const n of need) if (n[0] && n[0].size < n[1]) throw new RangeError('tokenLogprobs: ' + n[2] + ' too small');
+    function ptr(b: DeviceBuffer | undefined): bigint | null { return b ? b.ptr : null; }
+    const params = HipAttention.tokenLogprobsParams(p);
+    const slot = this.beginPass(PASS_LABELS.tokenLogprobs);
+    try {
+      this.g4.tokenLogprobs(p.logits.ptr, ptr(p.tokens), ptr(p.logprobs), ptr(p.entropy), ptr(p.topIds), ptr(p.topLogprobs),
+        params, workspace.ptr, workspace.size, this.stream);
     } finally {
       this.endPass(slot);
     }

@@ -90,6 +90,38 @@ function slotTableChecks(): void {
   throws(function () { return new SlotTable(0, 4); }, 'zero capacity');
 }
 
+// The paged cache's records and the refusals that need no GPU.
+function pagedChecks(g4: any): void {
+  const sizes: [string, number][] = [['sizeofPagedCache', 40], ['sizeofPagedBatch', 64], ['sizeofPagedAppendParams', 32],
+    ['sizeofPagedAttnParams', 16], ['sizeofTokenLogprobsParams', 32]];
+  for (const s of sizes) if (g4[s[0]] !== s[1]) fail(`${s[0]}: ${g4[s[0]]} B, the host writes ${s[1]}`);
+  function buf(ptr: number, size: number): DeviceBuffer { return { ptr: BigInt(ptr), size: size }; }
+  const pool = 4 * 32 * 256 * 2;
+  const cache = { kPool: buf(0x1000, pool), vPool: buf(0x100000, pool), numPages: 4, pageSize: 32, numKvHeads: 1, headDim: 256 };
+  const batch = { blockTable: buf(0x2000, 16), tokenStart: buf(0x3000, 12), ctxLens: buf(0x4000, 8), nSeqs: 2, tableStride: 2,
+    nTokens: 5, maxTokens: 3 };
+  const bytes = HipAttention.pagedCacheBytes([cache, cache]);
+  const dv = new DataView(bytes.buffer);
+  if (bytes.length !== 80 || dv.getBigUint64(48, true) !== BigInt(0x100000) || dv.getUint32(68, true) !== 256) fail('paged cache record');
+  const bb = new DataView(HipAttention.pagedBatchBytes(batch).buffer);
+  if (bb.getBigUint64(16, true) !== BigInt(0x4000) || bb.getBigUint64(24, true) !== BigInt(0) || bb.getUint32(48, true) !== 5) {
+    fail('paged batch record');
+  }
+  throws(() => HipAttention.pagedCacheBytes([Object.assign({}, cache, { numPages: 5 })]), 'pools too small');
+  throws(() => HipAttention.pagedBatchBytes(Object.assign({}, batch, { tokenStart: buf(0x3000, 8) })), 'tokenStart too small');
+  const c1 = HipAttention.pagedCacheBytes([cache]);
+  const b1 = HipAttention.pagedBatchBytes(batch);
+  if (!(g4.pagedAttnWorkspaceSize(c1, b1, 8) > 0)) fail('pagedAttnWorkspaceSize');
+  throws(() => g4.pagedAttnWorkspaceSize(c1.subarray(0, 16), b1, 8), 'short cache record');
+  throws(() => g4.pagedAttnWorkspaceSize(c1, b1, 9), 'nine query heads on one');
+  throws(() => g4.pagedCommit(c1, 2, b1, BigInt(16), 1, BigInt(16), BigInt(32), BigInt(0)), 'two caches, one record');
+  const lp = { logits: buf(0x1000, 4000), rows: 1, vocab: 1000, topK: 20 };
+  if (!(g4.tokenLogprobsWorkspaceSize(HipAttention.tokenLogprobsParams(lp)) > 0)) fail('tokenLogprobsWorkspaceSize');
+  throws(() => g4.tokenLogprobsWorkspaceSize(HipAttention.tokenLogprobsParams(Object.assign({}, lp, { topK: 65 }))), 'top 65');
+  throws(() => g4.tokenLogprobsWorkspaceSize(HipAttention.tokenLogprobsParams(Object.assign({}, lp, { temperature: 0 }))),
+    'temperature 0');
+}
+
 export function cpuChecks(): string[] {
   const done: string[] = [];
   const g4 = loadAddon();
@@ -130,6 +162,8 @@ export function cpuChecks(): string[] {
   if (g4.sizeofPromptPrepEntry() !== 128) fail(`g4_prompt_prep_entry is ${g4.sizeofPromptPrepEntry()} B, the host writes 128`);
   throws(() => g4.attnPromptPrepMany(new Uint8Array(100), 1, BigInt(0)), 'attnPromptPrepMany: short record');
   done.push('prompt prep records');
+  pagedChecks(g4);
+  done.push('paged records');
   return done;
 }
 
@@ -299,6 +333,75 @@ function prefill(dir: string): string[] {
   for (const b of bufs) att.destroyBuffer(b);
   att.dispose();
   return ['attnPrefill: ' + entries.length + ' entries', 'results written'];
+}
+
+interface PagedSpec {
+  nqh: number; nkh: number; hd: number; pages: number; pageSize: number; nSeqs: number; tableStride: number; nTokens: number;
+  maxTokens: number; pathStride: number; window: number; vocab: number; topK: number; f8: boolean;
+  arrays: Record<string, number[]>;
+}
+
+// A step of drafted trees through the paged operators, in the order a server calls them: append, attention, the
+// tokens' log probabilities, commit. out.bin = out, logprobs, entropy, topIds, topLogprobs, newCtxLens, K pool, V pool.
+function paged(dir: string): string[] {
+  const spec = JSON.parse(fs.readFileSync(path.join(dir, 'case.json'), 'utf8')) as PagedSpec;
+  const bin: Uint8Array = fs.readFileSync(path.join(dir, 'case.bin'));
+  const att = new HipAttention(loadAddon(), 0);
+  const bufs: DeviceBuffer[] = [];
+  function alloc(bytes: number): DeviceBuffer {
+    const b = att.createBuffer(bytes);
+    bufs.push(b);
+    return b;
+  }
+  function upload(name: string): DeviceBuffer {
+    const r = spec.arrays[name];
+    const b = alloc(r[1]);
+    att.writeBuffer(b, 0, bin.subarray(r[0], r[0] + r[1]));
+    return b;
+  }
+  const cache = { kPool: upload('kPool'), vPool: upload('vPool'), numPages: spec.pages, pageSize: spec.pageSize,
+    numKvHeads: spec.nkh, headDim: spec.hd, dtype: (spec.f8 ? 'e4m3' : 'f16') as 'f16' | 'e4m3' };
+  const batch = { blockTable: upload('table'), tokenStart: upload('start'), ctxLens: upload('ctx'), positions: upload('positions'),
+    treeMask: upload('mask'), nSeqs: spec.nSeqs, tableStride: spec.tableStride, nTokens: spec.nTokens,
+    maxTokens: spec.maxTokens, maskWords: 1 };
+  const qOut = alloc(spec.nTokens * spec.nqh * spec.hd * 2);
+  const out = alloc(spec.nTokens * spec.nqh * spec.hd * 4);
+  // q, k and v are parts of one projection's output: a token's row holds all three.
+  const qkv = upload('qkv');
+  const width = (spec.nqh + 2 * spec.nkh) * spec.hd;
+  function part(first: number): DeviceBuffer {
+    return { ptr: qkv.ptr + BigInt(first * spec.hd * 4), size: qkv.size - first * spec.hd * 4 };
+  }
+  att.pagedAppend(cache, batch, { q: part(0), k: part(spec.nqh), v: part(spec.nqh + spec.nkh), qWeight: upload('qw'),
+    kWeight: upload('kw'), ropeInvFreq: upload('inv'), qOut: qOut, numQHeads: spec.nqh, qStride: width, kStride: width,
+    vStride: width });
+  const ws = alloc(att.pagedAttnWorkspaceSize(cache, batch, spec.nqh));
+  att.pagedAttn(cache, batch, { q: qOut, out: out, numQHeads: spec.nqh, slidingWindow: spec.window }, ws);
+  const n = spec.nTokens;
+  const lp = { logits: upload('logits'), tokens: upload('tokens'), logprobs: alloc(n * 4), entropy: alloc(n * 4),
+    topIds: alloc(n * spec.topK * 4), topLogprobs: alloc(n * spec.topK * 4), rows: n, vocab: spec.vocab, topK: spec.topK,
+    cap: 30.0, temperature: 0.7 };
+  const lws = alloc(att.tokenLogprobsWorkspaceSize(lp));
+  att.tokenLogprobs(lp, lws);
+  const newCtx = alloc(spec.nSeqs * 4);
+  att.pagedCommit([cache], batch, upload('path'), spec.pathStride, upload('accepted'), newCtx);
+  throws(function () {
+    att.pagedAttn(cache, batch, { q: qOut, out: qOut, numQHeads: spec.nqh }, ws);
+  }, 'pagedAttn: out too small');
+  throws(function () { att.pagedAttn(cache, batch, { q: qOut, out: out, numQHeads: spec.nqh }, newCtx); }, 'short workspace');
+  const outs = [out, lp.logprobs, lp.entropy, lp.topIds, lp.topLogprobs, newCtx, cache.kPool, cache.vPool];
+  let total = 0;
+  for (const o of outs) total += o.size;
+  const res = new Uint8Array(total);
+  let off = 0;
+  for (const o of outs) {
+    att.readBuffer(o, 0, res.subarray(off, off + o.size));
+    off += o.size;
+  }
+  fs.writeFileSync(path.join(dir, 'out.bin'), res);
+  for (const b of bufs) att.destroyBuffer(b);
+  att.dispose();
+  return ['paged: append, attention, log probabilities, commit', 'results written'];
 }
 
 interface PromptPrepSpec {
@@ -819,8 +922,9 @@ export function main(argv: string[]): void {
   else if (mode === 'head') done = head(argv[1]);
   else if (mode === 'prefill') done = prefill(argv[1]);
   else if (mode === 'promptprep') done = promptPrep(argv[1]);
+  else if (mode === 'paged') done = paged(argv[1]);
   else if (mode === 'linear') done = linear(argv[1]);
   else if (mode === 'qkvprep') done = qkvPrep(argv[1]);
-  else fail(`usage: run.js cpu | layer <dir> | prefill <dir> | promptprep <dir> | head <dir> | linear <dir> | qkvprep <dir> | capture <dir> | batch <dir> | readback <dir> | profile`);
+  else fail(`usage: run.js cpu | layer <dir> | prefill <dir> | promptprep <dir> | paged <dir> | head <dir> | linear <dir> | qkvprep <dir> | capture <dir> | batch <dir> | readback <dir> | profile`);
   process.stdout.write(JSON.stringify({ ok: true, checks: done }) + '\n');
 }
