@@ -7,9 +7,9 @@
 // Bound by the logits' bytes, read once: a workgroup takes a chunk of consecutive
 // logits of a row into registers, so the maximum, the sums and the selection all
 // work on what one pass has loaded. z is monotone in x, so maxima and ranks are
-// taken on x itself and each element's z is evaluated once: 2 transcendental
-// operations less one with a cap of 3 an element, and 6 plain ones (9 with a cap),
-// which the loads of the other workgroups on a CU cover.
+// taken on x itself and each element's z is evaluated once: one transcendental
+// operation an element (three with a cap) and six plain ones (nine), which the
+// loads of the other workgroups on a CU cover.
 //
 // Selection: candidates are 64-bit keys (order-preserving logit in the high half,
 // inverted index in the low half), all different, so equal logits rank by index.
@@ -44,7 +44,7 @@ struct LogprobsArgs {
     uint64_t* __restrict__ cand;   // [rows][chunks][k]
     uint64_t row_stride;
     uint32_t vocab, chunks, k;
-    float cap, cap_exp;  // and 2 log2(e) / cap
+    float cap, cap_exp, cap_inv;  // and 2 log2(e) / cap, 1 / cap
     float slope;         // log2(e) / temperature
 };
 
@@ -64,14 +64,26 @@ __device__ __forceinline__ float logit_f32(typename LogitType<DT>::T v) {
     else return __uint_as_float((uint32_t)v << 16);
 }
 
-// cap tanh(x / cap) = cap - 2 cap / (e^(2 x / cap) + 1), to a few half-steps of cap. A mask of -inf stays
-// one, and +inf too (it makes the row's sums NaN).
+// cap tanh(x / cap). A mask of -inf stays one, and +inf too (it makes the row's sums NaN).
+// Up to kLpNearCap as cap - 2 cap / (e^(2 x / cap) + 1), which is off by a few half-steps of the cap: 1e-5 at
+// most, about what f32 logits near the cap are rounded by. Above it to a few half-steps of the value (half as
+// many operations again).
+constexpr float kLpNearCap = 64.0f;
+template <bool NEAR>
 __device__ __forceinline__ float logit_capped(float x, const LogprobsArgs& a) {
-    const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * a.cap_exp) + 1.0f);
-    const float z = __builtin_fmaf(-2.0f * a.cap, r, a.cap);
+    float z;
+    if constexpr (NEAR) {
+        const float r = __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * a.cap_exp) + 1.0f);
+        z = __builtin_fmaf(-2.0f * a.cap, r, a.cap);
+    } else {
+        z = a.cap * tanh_f32(x * a.cap_inv);
+    }
     return fabsf(x) == INFINITY ? x : z;
 }
-__device__ __forceinline__ float logit_z(float x, const LogprobsArgs& a) { return a.cap > 0.0f ? logit_capped(x, a) : x; }
+__device__ __forceinline__ float logit_z(float x, const LogprobsArgs& a) {
+    if (a.cap > kLpNearCap) return logit_capped<false>(x, a);
+    return a.cap > 0.0f ? logit_capped<true>(x, a) : x;
+}
 
 // Key of logit x at index i: larger first, equal ones by lower index; 0 for none.
 __device__ __forceinline__ uint32_t logit_order(float x) {
@@ -280,21 +292,17 @@ __global__ __launch_bounds__(kLpThreads, E <= 32 ? 4 : 3) void k_logprobs(const 
     const float m = xmax == -INFINITY ? 0.0f : logit_z(xmax, a);
     float S = 0.0f, U = 0.0f;
     // 2^t is 0 from -200 on, where t 2^t must not become -inf times 0; a NaN goes on in S.
-    if (a.cap > 0.0f) {
+    auto sums = [&](auto&& z) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < E; i++) {
-            const float d = (logit_capped(logit(i), a) - m) * a.slope, e = __builtin_amdgcn_exp2f(d);
+            const float d = (z(logit(i)) - m) * a.slope, e = __builtin_amdgcn_exp2f(d);
             S += e;
             U = __builtin_fmaf(e, fmaxf(d, -200.0f), U);
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < E; i++) {
-            const float d = (logit(i) - m) * a.slope, e = __builtin_amdgcn_exp2f(d);
-            S += e;
-            U = __builtin_fmaf(e, fmaxf(d, -200.0f), U);
-        }
-    }
+    };
+    if (a.cap > kLpNearCap) sums([&](float x) __attribute__((always_inline)) { return logit_capped<false>(x, a); });
+    else if (a.cap > 0.0f) sums([&](float x) __attribute__((always_inline)) { return logit_capped<true>(x, a); });
+    else sums([](float x) __attribute__((always_inline)) { return x; });
     S = lp_wave_sum(S);
     U = lp_wave_sum(U);
     if (lane == 0) {
@@ -505,6 +513,7 @@ int g4_token_logprobs(const void* logits, const int32_t* tokens, float* logprobs
     a.k = p->top_k;
     a.cap = p->cap;
     a.cap_exp = p->cap > 0.0f ? 2.0f * kLog2e / p->cap : 0.0f;
+    a.cap_inv = p->cap > 0.0f ? 1.0f / p->cap : 0.0f;
     a.slope = kLog2e / p->temperature;
     const bool vec = !((reinterpret_cast<uintptr_t>(logits) | (a.row_stride * elem)) & 15);
     hipStream_t st = as_stream(stream);

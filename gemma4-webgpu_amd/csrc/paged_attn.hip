@@ -295,17 +295,6 @@ __device__ __forceinline__ void paged_load_v(const char* base0, const char* base
             vr[b][t] = ldg_stream<u32x4>((t < 4 ? base0 : base1) + (off + (uint32_t)(t & 3) * row_bytes + b * 256u));
 }
 
-// tanh(x) to f32 accuracy (logprobs.hip has the derivation).
-__device__ __forceinline__ float paged_tanh(float x) {
-    const float ax = fabsf(x), z = x * x;
-    const float t = __builtin_amdgcn_exp2f(-2.0f * kLog2e * ax);
-    const bool small = ax < 0.5f;
-    const float num = small ? ax * (945.0f + z * (105.0f + z)) : 1.0f - t;
-    const float den = small ? 945.0f + z * (420.0f + 15.0f * z) : 1.0f + t;
-    const float y = __builtin_amdgcn_rcpf(den), q = num * y;
-    return copysignf(__builtin_fmaf(__builtin_fmaf(-q, den, num), y, q), x);
-}
-
 // O^T += V^T P^T for piece block b of V, all query groups. Word w of a row's piece holds
 // elements (2w, 2w + 1) (f16) or 4w .. 4w + 3 (e4m3): acc tile b E + e takes element e of
 // every lane's piece, so its rows are d = 16 E b + E (row) + e.
@@ -510,7 +499,7 @@ __device__ __forceinline__ void paged_softmax(const PagedAttnArgs& a, const f32x
         for (int x = 0; x < NX; x++) {
             if (a.cap_log2 > 0.0f) {  // uniform, once a tile
 #pragma unroll
-                for (int i = 0; i < 8; i++) sv[x][i] = a.cap_log2 * paged_tanh(sc[x][c][i >> 2][i & 3] * a.cap_scale);
+                for (int i = 0; i < 8; i++) sv[x][i] = a.cap_log2 * tanh_f32(sc[x][c][i >> 2][i & 3] * a.cap_scale);
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; i++) sv[x][i] = sc[x][c][i >> 2][i & 3] * a.qscale;

@@ -800,14 +800,14 @@ int g4_paged_append(const g4_paged_cache* cache, const g4_paged_batch* batch, co
  * not attend do not reach it, whatever they hold. q: f16 [n_tokens][num_q_heads]
  * [head_dim]; out: f32, the same shape, 16-byte aligned; num_q_heads up to 8 times
  * num_kv_heads. The workspace (g4_paged_attn_workspace_size: it depends on the
- * head layout, head_dim, n_seqs and max_tokens alone) holds partial results within
+ * head layout, head_dim and max_tokens alone) holds partial results within
  * a call; calls that overlap need one each. Results do not depend on scheduling:
  * the same call gives the same bits. */
 typedef struct g4_paged_attn_params {
     uint32_t num_q_heads;
-    uint32_t sliding_window;
+    uint32_t sliding_window; /* positions, the token's own included; 0: no limit */
     float scale;
-    float softcap;
+    float softcap;           /* 0: none; else 1e-6 to 1e30 */
 } g4_paged_attn_params;
 int g4_paged_attn_workspace_size(const g4_paged_cache* cache, const g4_paged_batch* batch, uint32_t num_q_heads,
                                  size_t* bytes);
@@ -846,13 +846,13 @@ int g4_paged_commit(const g4_paged_cache* caches, uint32_t n_caches, const g4_pa
 #define G4_LOGITS_BF16 2
 #define G4_LOGPROBS_MAX_TOP 64
 typedef struct g4_token_logprobs_params {
-    uint32_t rows;
+    uint32_t rows;        /* at most 65535 */
     uint32_t vocab;       /* 1 .. 2^24 */
     uint64_t row_stride;  /* elements from row to row, at least vocab; 0: vocab */
     uint32_t dtype;
     uint32_t top_k;       /* 0 .. min(vocab, 64) */
-    float cap;            /* 0: none */
-    float temperature;    /* above 0 */
+    float cap;            /* 0: none; else 1e-6 to 1e30 */
+    float temperature;    /* 1e-6 to 1e6 */
 } g4_token_logprobs_params;
 int g4_token_logprobs_workspace_size(const g4_token_logprobs_params* p, size_t* bytes);
 int g4_token_logprobs(const void* logits, const int32_t* tokens, float* logprobs, float* entropy, int32_t* top_ids,

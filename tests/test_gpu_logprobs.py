@@ -174,3 +174,18 @@ def test_parts_asked_for_alone_streams_and_replays(dev):
         torch.cuda.synchronize()
         want = call(y, u, 5)
         assert all(torch.equal(a, b) for a, b in zip((only, ent, i2, t2), want))
+
+
+@pytest.mark.parametrize("cap", [64.0, 65.0, 1000.0, 1e6, 1e30])
+def test_caps_far_above_the_logits(dev, cap):
+    """A cap's rounding is the logits', not the cap's (which would leave 0.06 at 1e6): up to 64, where the sums take a
+    shorter form, 4 half-steps of the cap, above it within the tolerance of every other case."""
+    announce(f"tokenLogprobs cap={cap}")
+    x, tokens = inputs(dev, 90, 5, 5000, "f32", spread=1.0)
+    if cap > 64:
+        check(x, tokens, 7, cap=cap)
+        return
+    lp, _, _, _ = call(x, tokens, 0, cap=cap)
+    want = torch.log_softmax(cap * torch.tanh(x.double() / cap), -1).gather(1, tokens.long()[:, None])[:, 0]
+    # z of the token and of the sum: two differences, each 4 half-steps of the cap.
+    assert ((lp - want).abs() <= 2 * 4 * cap * 2.0 ** -24 + 64 * 2.0 ** -24 + want.abs() * 2.0 ** -22).all()
