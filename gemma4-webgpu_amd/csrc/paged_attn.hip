@@ -75,13 +75,19 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedAttnArgs& a, const Pa
     return s;
 }
 
-__device__ __forceinline__ unsigned wave_scan(unsigned x, unsigned lane) {  // inclusive
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const unsigned y = __shfl_up(x, d);
-        if (lane >= (unsigned)d) x += y;
-    }
-    return x;
+// Inclusive sum over the wave's lanes: shifts within rows of 16 lanes, then a row's (two rows') last sum
+// into the rows behind it.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned scan_dpp(unsigned x) {  // 0 where no lane is read
+    return (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, true);
+}
+__device__ __forceinline__ unsigned wave_scan(unsigned x) {
+    x += scan_dpp<0x111, 0xf>(x);  // row_shr:1
+    x += scan_dpp<0x112, 0xf>(x);
+    x += scan_dpp<0x114, 0xf>(x);
+    x += scan_dpp<0x118, 0xf>(x);
+    x += scan_dpp<0x142, 0xa>(x);  // row_bcast:15, rows 1 and 3
+    return x + scan_dpp<0x143, 0xc>(x);  // row_bcast:31, rows 2 and 3
 }
 __device__ __forceinline__ unsigned lane_value(unsigned x, unsigned lane) {
     return __builtin_amdgcn_readlane(x, lane);
@@ -113,7 +119,7 @@ struct PagedScan {
             head = paged_span<MQ, UR>(a, sq, one ? 0u : i % a.q_tiles).n;
         }
         tiles = head * a.nkh;
-        incl = wave_scan(tiles, lane);
+        incl = wave_scan(tiles);
     }
     __device__ __forceinline__ void run(const PagedAttnArgs& a, unsigned lane) {
         for (unsigned i0 = 0; i0 < items(a); i0 += 64) {
@@ -137,7 +143,7 @@ struct PagedPieces {
     unsigned n, per, first;  // pieces a kv head, tiles a piece, the first piece's workgroup
 
     template <int MQ, int UR>
-    __device__ __forceinline__ void run(const PagedAttnArgs& a, const PagedScan<MQ, UR>& scan, unsigned share, unsigned lane) {
+    __device__ __forceinline__ void run(const PagedAttnArgs& a, const PagedScan<MQ, UR>& scan, unsigned share) {
         fit = false;
         if (scan.items(a) > 64) return;  // uniform
         n = (scan.head + share - 1) / share;
@@ -146,7 +152,7 @@ struct PagedPieces {
             n = (n + 7) & ~7u;
             per = n ? (scan.head + n - 1) / n : 1u;
         }
-        const unsigned incl = wave_scan(n * a.nkh, lane);
+        const unsigned incl = wave_scan(n * a.nkh);
         first = incl - n * a.nkh;
         fit = lane_value(incl, 63) <= a.wgs;
     }
@@ -198,7 +204,7 @@ __device__ __forceinline__ bool paged_begin(const PagedAttnArgs& a, unsigned lan
     scan.run(a, lane);
     const unsigned share = scan.share(a);
     PagedPieces pc;
-    pc.run(a, scan, share, lane);
+    pc.run(a, scan, share);
     if (pc.fit) {
         const uint64_t there = __ballot(pc.n && pc.first <= blockIdx.x);
         if (!there) return false;
@@ -1141,7 +1147,7 @@ __global__ __launch_bounds__(256) void k_paged_join(const PagedAttnArgs a) {
     const unsigned share = scan.share(a);
     unsigned w0 = base / share, w1 = (base + mine - 1) / share;
     PagedPieces pc;
-    pc.run(a, scan, share, lane);
+    pc.run(a, scan, share);
     if (pc.fit) {
         w0 = lane_value(pc.first, i) + kvh * lane_value(pc.n, i);
         w1 = w0 + (mine - 1) / lane_value(pc.per, i);
