@@ -243,6 +243,25 @@ using namespace g4;
 
 namespace {
 
+// Whether two arrays of 4-byte elements share one.
+bool overlap(const int32_t* x, uint64_t nx, const int32_t* y, uint64_t ny) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(x), b = reinterpret_cast<uintptr_t>(y);
+    return a < b + ny * 4 && b < a + nx * 4;
+}
+// Whether two of n pools are one, by open addressing over twice as many places as there may be pools.
+bool repeated(const CommitPool* pool, uint32_t n) {
+    constexpr uint32_t PLACES = 4 * G4_COMMIT_MAX_CACHES;
+    const void* seen[PLACES] = {};
+    for (uint32_t i = 0; i < n; i++) {
+        uint32_t at = (uint32_t)((reinterpret_cast<uintptr_t>(pool[i].p) >> 4) * 0x9E3779B97F4A7C15ull >> 56);
+        static_assert(PLACES == 256, "the hash's top byte");
+        for (; seen[at]; at = (at + 1) % PLACES)
+            if (seen[at] == pool[i].p) return true;
+        seen[at] = pool[i].p;
+    }
+    return false;
+}
+
 // The pools go by value in the kernel arguments: a block for up to 16 caches (a launch's cost grows with
 // its size), and one for the most there may be.
 template <int N>
@@ -266,6 +285,12 @@ int commit(const g4_paged_cache* caches, uint32_t n_caches, const g4_paged_batch
         if (row_bytes / 16 > most) most = row_bytes / 16;
     }
     if (new_ctx_lens == batch->ctx_lens) return fail(G4_EINVAL, "pagedCommit: new_ctx_lens is ctx_lens itself");
+    // Written while other workgroups still read these.
+    const uint64_t seqs = batch->n_seqs;
+    if (overlap(new_ctx_lens, seqs, batch->ctx_lens, seqs) || overlap(new_ctx_lens, seqs, n_accepted, seqs) ||
+        overlap(new_ctx_lens, seqs, path, seqs * path_stride))
+        return fail(G4_EINVAL, "pagedCommit: new_ctx_lens lies over ctx_lens, n_accepted or path");
+    if (repeated(a.pool, 2 * n_caches)) return fail(G4_EINVAL, "pagedCommit: a pool is named twice (its rows would move twice)");
     a.path = path;
     a.accepted = n_accepted;
     a.new_ctx = new_ctx_lens;

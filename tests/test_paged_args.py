@@ -184,3 +184,32 @@ def test_tensor_wrappers_refuse_host_tensors_and_shapes():
         ops.token_logprobs(torch.zeros(2, 8), None, None, None, None)
     with pytest.raises(ValueError, match="rows, vocab"):
         ops.token_logprobs(torch.zeros(8), None, None, None, None)
+
+
+def test_commit_refuses_a_pool_twice_and_outputs_over_inputs():
+    """Layers that share a cache name it once: two workgroups moving the same rows would each undo what the other
+    relies on."""
+    lib = abi.load()
+
+    def call(caches, **kw):
+        a = dict(b=batch(), path=0x10000, stride=4, acc=0x20000, new=0x30000)
+        a.update(kw)
+        c = (abi.PagedCache * len(caches))(*caches)
+        st = lib.g4_paged_commit(c, len(caches), a["b"], a["path"], a["stride"], a["acc"], a["new"], None)
+        return st, lib.g4_last_error().decode()
+
+    apart = [cache(k_pool=0x1000000 * (2 * i + 1), v_pool=0x1000000 * (2 * i + 2)) for i in range(64)]
+    for n, i, j in [(2, 0, 1), (17, 3, 16), (64, 0, 63), (64, 62, 63)]:
+        for what in ("k_pool", "v_pool"):
+            cs = [abi.PagedCache.from_buffer_copy(c) for c in apart[:n]]
+            setattr(cs[j], what, getattr(cs[i], what))
+            st, msg = call(cs)
+            assert st == abi.G4_EINVAL and "twice" in msg, (n, i, j, what, msg)
+    one = abi.PagedCache.from_buffer_copy(apart[0])
+    one.v_pool = one.k_pool
+    assert "twice" in call([one])[1]
+    n = batch().n_seqs
+    for kw in [dict(new=0x20000), dict(new=0x10000 + 4 * (4 * n - 1)), dict(new=0x20000 - 4 * (n - 1)),
+               dict(acc=0x30000 + 4 * (n - 1)), dict(path=0x30000)]:
+        st, msg = call(apart[:1], **kw)
+        assert st == abi.G4_EINVAL and "lies over" in msg, (kw, msg)
