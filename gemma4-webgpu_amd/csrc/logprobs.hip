@@ -26,8 +26,9 @@
 namespace g4 {
 
 constexpr unsigned kLpThreads = 256;
-constexpr unsigned kLpShort = 2048;  // logits of a chunk where rows are few: more workgroups, shorter chains
-constexpr unsigned kLpLong = 8192;   // and where they are many (twice as many logits of 16 bits)
+constexpr unsigned kLpShort = 2048, kLpMiddle = 4096;  // logits of a chunk where rows are few: more workgroups,
+                                                       // shorter chains
+constexpr unsigned kLpLong = 8192;                     // and where they are many (twice as many logits of 16 bits)
 constexpr unsigned kLpMaxK = G4_LOGPROBS_MAX_TOP;
 constexpr unsigned kLpGroups = 64;  // at least kLpMaxK
 constexpr unsigned kLpCandidates = 1024;
@@ -418,28 +419,31 @@ __global__ __launch_bounds__(kLpThreads) void k_logprobs_join(const LogprobsArgs
     lp_finish<DT>(a, sh, row, mx, S, U);
 }
 
-// Short chunks while the long ones leave CUs idle.
-static bool lp_short(uint32_t rows, uint32_t vocab) {
-    return (uint64_t)rows * ((vocab + kLpLong - 1) / kLpLong) < device_cus();
+// Long chunks where they fill the chip twice; else shorter ones, as long as a row has at most 64 for the second
+// launch to join. (Chunks of 2048 / 4096 / 8192 logits: a row of 50257 10.4 / 11.7 / 13.5 us, one of 262144
+// 12.6 / 10.8 / 11.8, 64 of those 33.8 / 25.5 / 24.8.)
+static uint32_t lp_chunk(uint32_t rows, uint32_t vocab) {
+    if ((uint64_t)rows * ((vocab + kLpLong - 1) / kLpLong) >= 2 * (uint64_t)device_cus()) return kLpLong;
+    return vocab <= 64 * kLpShort ? kLpShort : kLpMiddle;
+}
+
+template <int DT, int E>
+void launch_chunks(const LogprobsArgs& a, uint32_t rows, bool vec, hipStream_t st) {
+    const dim3 grid(a.chunks, rows), block(kLpThreads);
+    if (vec) G4_LAUNCH((k_logprobs<DT, true, E>), grid, block, 0, st, a);
+    else G4_LAUNCH((k_logprobs<DT, false, E>), grid, block, 0, st, a);
 }
 
 template <int DT>
 void launch_logprobs(LogprobsArgs& a, uint32_t rows, bool vec, hipStream_t st) {
     constexpr int P = DT == G4_LOGITS_F32 ? 1 : 2;
-    constexpr int LONG = (int)(kLpLong * P / kLpThreads), SHORT = (int)(kLpShort / kLpThreads);
-    const bool brief = lp_short(rows, a.vocab);
-    const uint32_t chunk = brief ? kLpShort : kLpLong * P;
+    const uint32_t least = lp_chunk(rows, a.vocab), chunk = least == kLpLong ? kLpLong * P : least;
     a.chunks = (a.vocab + chunk - 1) / chunk;
     a.cand = reinterpret_cast<uint64_t*>(a.part + (uint64_t)rows * a.chunks * 4);
-    const dim3 grid(a.chunks, rows), block(kLpThreads);
-    if (brief) {
-        if (vec) G4_LAUNCH((k_logprobs<DT, true, SHORT>), grid, block, 0, st, a);
-        else G4_LAUNCH((k_logprobs<DT, false, SHORT>), grid, block, 0, st, a);
-    } else {
-        if (vec) G4_LAUNCH((k_logprobs<DT, true, LONG>), grid, block, 0, st, a);
-        else G4_LAUNCH((k_logprobs<DT, false, LONG>), grid, block, 0, st, a);
-    }
-    if (a.chunks > 1) G4_LAUNCH((k_logprobs_join<DT>), dim3(rows), block, 0, st, a);
+    if (least == kLpShort) launch_chunks<DT, kLpShort / kLpThreads>(a, rows, vec, st);
+    else if (least == kLpMiddle) launch_chunks<DT, kLpMiddle / kLpThreads>(a, rows, vec, st);
+    else launch_chunks<DT, kLpLong * P / kLpThreads>(a, rows, vec, st);
+    if (a.chunks > 1) G4_LAUNCH((k_logprobs_join<DT>), dim3(rows), dim3(kLpThreads), 0, st, a);
 }
 
 }  // namespace g4
@@ -467,7 +471,7 @@ int logprobs_check(const g4_token_logprobs_params* p) {
 
 // Room for the chunks of any type and alignment.
 size_t logprobs_bytes(const g4_token_logprobs_params* p) {
-    const uint64_t chunk = lp_short(p->rows, p->vocab) ? kLpShort : kLpLong, chunks = (p->vocab + chunk - 1) / chunk;
+    const uint64_t chunk = lp_chunk(p->rows, p->vocab), chunks = (p->vocab + chunk - 1) / chunk;
     return (size_t)p->rows * chunks * (16 + 8ull * p->top_k) + 16;
 }
 
