@@ -45,7 +45,7 @@ struct PagedAttnArgs {
     int32_t window;               // 0: none
     float qscale;                 // scale * log2(e)
     float cap_scale, cap_log2;    // scale / cap and cap * log2(e); 0: no cap
-    uint32_t wgs, min_share;      // workgroups of the attention launch; least tiles a workgroup takes
+    uint32_t wgs;                 // workgroups of the attention launch
     uint32_t whole;               // 1: a workgroup an item, nothing is cut
     PagedBatchDev b;
 };
@@ -129,7 +129,7 @@ struct PagedScan {
     }
     // Tiles a workgroup takes (the last one fewer).
     __device__ __forceinline__ unsigned share(const PagedAttnArgs& a) const {
-        return max((total + a.wgs - 1) / a.wgs, a.min_share);
+        return max((total + a.wgs - 1) / a.wgs, 1u);
     }
 };
 
@@ -1234,14 +1234,19 @@ static bool paged_whole(uint64_t rows, uint64_t items, unsigned cus) {
     return rows <= 256 || (rows <= 2048 && 2 * items >= cus);
 }
 
+// How the records are joined: few an item, its thread's rows in turn; many, in 16 groups, or in 4 where an item's
+// rows fill the chip already. (64 sequences of 8 tokens, 1 / 16 groups: 212 / 240 us; 26 tokens over 8192 rows at
+// head_dim 512, 1 / 4 / 16: 37.1 / 34.6 / 36.8; 8 over 32768 rows 43.1 / 33.0 / 29.3; one over 8192 24.2 / 16.9 / 13.4.)
 template <int HD, int MQ, int UR>
 static void launch_join(const PagedAttnArgs& a, hipStream_t st) {
     if (a.whole) return;
     const unsigned items = a.b.n_seqs * a.q_tiles * a.nkh;
-    if (items * 16 >= a.wgs) {  // few records an item
+    if (items * 16 >= a.wgs) {
         G4_LAUNCH((k_paged_join<HD, MQ, UR, 1, HD>), dim3(items, MQ * HD / 4 / 256), dim3(256), 0, st, a);
-    } else {
+    } else if (MQ <= 32 || items * 128 <= a.wgs) {
         G4_LAUNCH((k_paged_join<HD, MQ, UR, 16, 64>), dim3(items, MQ, HD / 64), dim3(256), 0, st, a);
+    } else {
+        if constexpr (MQ > 32) G4_LAUNCH((k_paged_join<HD, MQ, UR, 4, 64>), dim3(items, MQ / 4, HD / 64), dim3(256), 0, st, a);
     }
 }
 
@@ -1339,7 +1344,6 @@ int g4_paged_attn(const g4_paged_cache* cache, const g4_paged_batch* batch, cons
     a.cap_scale = p->softcap > 0.0f ? p->scale / p->softcap : 0.0f;
     a.cap_log2 = p->softcap * kLog2e;
     a.wgs = plan.wgs;
-    a.min_share = plan.mq <= 32 ? kPagedWaves : 1;
     const uint64_t cap = (uint64_t)batch->table_stride * cache->page_size;
     const uint64_t span = a.window ? (uint64_t)a.window + a.b.max_tokens : cap;
     a.whole = paged_whole(span < cap ? span : cap, (uint64_t)a.b.n_seqs * a.q_tiles * a.nkh, device_cus());
