@@ -504,8 +504,19 @@ __device__ __forceinline__ void paged_softmax(const PagedAttnArgs& a, const f32x
 #pragma unroll
         for (int x = 0; x < NX; x++) {
             if (a.cap_log2 > 0.0f) {  // uniform, once a tile
+                float far = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 8; i++) sv[x][i] = a.cap_log2 * tanh_f32(sc[x][c][i >> 2][i & 3] * a.cap_scale);
+                for (int i = 0; i < 8; i++) {
+                    sv[x][i] = sc[x][c][i >> 2][i & 3] * a.cap_scale;
+                    far = fmaxf(far, fabsf(sv[x][i]));
+                }
+                if (__any(far >= 0.5f)) {  // scores beyond half the cap are few
+#pragma unroll
+                    for (int i = 0; i < 8; i++) sv[x][i] = a.cap_log2 * tanh_f32(sv[x][i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) sv[x][i] = a.cap_log2 * tanh_near(sv[x][i]);
+                }
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; i++) sv[x][i] = sc[x][c][i >> 2][i & 3] * a.qscale;
