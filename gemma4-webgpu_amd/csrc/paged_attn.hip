@@ -4,7 +4,7 @@
 // Per query row r = (token, query head of a kv head) and attended cache row i:
 //   s_i = scale q.k_i (capped: softcap tanh(s / softcap)), p_i = e^(s_i - m),
 //   out = sum p_i v_i / sum p_i, with the running maximum m and sum of an online
-//   softmax, f32 throughout; K and V are read once per tile of 16 C query rows.
+//   softmax, f32 throughout; K and V are read once per tile of query rows.
 //
 // MFMA mapping (v_mfma_f32_16x16x32_f16; lane = 16 g + n), for each 32-row tile of
 // the cache, per group of 16 query rows:
@@ -16,16 +16,19 @@
 //     an f32 result keeps f32 accuracy (one f16 P alone leaves 2e-4).
 // e4m3 pools are widened to f16 in registers, which is exact.
 //
-// Two forms: at most 16 query rows a kv head (k_paged_few: the workgroup's waves take
-// different cache rows, K and V go from memory to registers) and more (k_paged_tile:
-// the waves take different query rows of one tile, K and V rows shared through LDS).
+// Two forms. Few query rows a kv head (up to 16, at head_dim 256 up to 32; k_paged_few): the workgroup's
+// waves take different cache rows, K and V go from memory to registers, and the cache's bytes bound it. More
+// (k_paged_tile): the waves take different query rows of one tile and share K and V rows through LDS, whose
+// reads, with the softmax and the transposition, then bound it.
 //
 // Work split: a (sequence, tile of query rows, kv head) is an item of ceil(rows / 32)
 // row tiles; all items' tiles in order are cut into equal shares, one a workgroup,
 // whatever the lengths, so a ragged batch fills the chip and one long sequence does
-// too. Lengths are read on the device (a captured launch serves the next step's),
-// every workgroup finds its share by a scan over the items. An item cut between
-// workgroups leaves (m, l, o) records that a second launch joins in a fixed order.
+// too; few items are cut each by itself (PagedPieces), and short ones not at all
+// (paged_whole). Lengths are read on the device (a captured launch serves the next
+// step's), every workgroup finds its share by a scan over the items. An item cut
+// between workgroups leaves (m, l, o) records that a second launch joins in a fixed
+// order.
 #include "decode_core.h"
 #include "paged.h"
 
@@ -137,7 +140,7 @@ struct PagedScan {
 // workgroup takes the end of one item and the beginning of the next (which costs it the query, the page
 // ids, the pipeline's start and a record once more). Lane l: query tile l's. Several query tiles of the same
 // cache rows have pieces in a multiple of the XCDs, so that the pieces of the same rows meet in one L2.
-// (26 tokens over 8192 rows at head_dim 512: 52 pieces of 5 tiles an item 39 us, without them 48.)
+// (26 tokens over 8192 rows at head_dim 512: 48 us in shares, 41 in pieces, 56 of 5 tiles an item.)
 struct PagedPieces {
     bool fit;
     unsigned n, per, first;  // pieces a kv head, tiles a piece, the first piece's workgroup
@@ -595,8 +598,9 @@ __device__ __forceinline__ float paged_inverse(float L) { return L > 0.0f ? 1.0f
 // workgroup has whole, takes half as many in turn.
 // Measured: 64 sequences of 1024 to 32768 rows, one token: f16 187 us, 6.1 TB/s; e4m3 106 us, 5.4 TB/s (both read 0.83
 // to 0.9 of what a plain read stream does, the rest are ~20 us at the two launches' ends); head_dim 512 f16 205 us,
-// 5.8 TB/s; one sequence of 400000 f16 rows 77 us, 5.3 TB/s; four tokens over 4 x 100000 e4m3 rows (32 query rows, twice
-// the work a byte) 78 us, 4.7 TB/s.
+// 5.8 TB/s; one sequence of 400000 f16 rows 77 us, 5.3 TB/s; five tokens of four heads (20 query rows) and a
+// softcap over three sequences of 100001 to 131072 e4m3 rows 77 us, 4.8 TB/s, where the work on a tile, 8000 cycles a
+// wave, is the bound: twice the tiles in flight gave nothing (86 us).
 template <int HD, int C, int W>
 struct PagedFewSmem {
     f16x8 q[C][HD / 32][64];      // score operand, lane-major
@@ -822,12 +826,22 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_paged_few(const PagedAttnArgs
 
 // ---- more query rows -----------------------------------------------------------------
 
-// WQ x WK waves: 16 of the tile's 16 WQ query rows each (the query in registers), and every WK-th part
-// of a row tile of 32 TS rows, with maxima and sums of their own. K and V come to LDS by DMA, a row
-// tile's K or its V a slot, NS slots in a ring: K, V, K of the next tile and so on, NS - 1 requested
-// ahead; one barrier a slot. A row's 16-byte pieces are stored at piece ^ (row % 16), which spreads
-// both operands' reads over all banks (sixteen lanes read sixteen rows of K, or sixteen pieces of one
-// row of V). NT: the rows are read by one workgroup alone and bypass the caches.
+// WQ x WK x WD waves: 16 of the tile's 16 WQ query rows each (the query in registers), every WK-th part of a
+// row tile of 32 TS rows, with maxima and sums of their own, and a WD-th part of the head: a pair's scores are
+// added through LDS, each keeps half of the outputs, so at head_dim 512 two waves fit a SIMD (26 tokens over 8192
+// rows 41 -> 37 us). K and V come to LDS by DMA, a row tile's K or its V a slot, NS slots in a ring: K, V, K of
+// the next tile and so on, NS - 1 requested ahead; one barrier a slot. A row's 16-byte pieces are stored at
+// piece ^ (row % 16), which spreads both operands' reads over all banks (sixteen lanes read sixteen rows of K, or
+// sixteen pieces of one row of V). NT: the rows are read by one workgroup alone and bypass the caches (64
+// sequences of 8 tokens, pages of 1024, 223 us, without 238).
+//
+// Measured: 1024 tokens of 8 heads over 7001 rows 138 us, 456 TFLOP/s (0.68 PFLOP/s with the two products of P). A
+// tile of 128 query rows and 64 cache rows takes 8600 cycles: 4400 of reading K and V from LDS (128 bytes a
+// cycle; each wave reads them whole), of MFMA 3100 beside it, 1150 of softmax, and the rest are the barriers'
+// skew and the DMA's issue. 32 query rows a wave would halve the LDS reads, but one wave a SIMD overlaps
+// nothing (160 us); scores of the next tile beside this one's softmax (one barrier a tile, half of the waves
+// in each order) lost to the lookahead that it takes from the ring (150). 64 sequences of 8 tokens (64 query rows)
+// read 5.4 TB/s (209 us).
 template <int HD, bool F8, int TS, int NS, int PW>
 struct PagedTileSmem {
     unsigned char t[NS][32 * TS][HD * (F8 ? 1 : 2)];
@@ -1153,6 +1167,8 @@ __global__ __launch_bounds__(64 * WQ * WK * WD, WQ * WK * WD / 4) void k_paged_t
 // The records of an item that was cut, in P groups of consecutive ones, added in order: the records of
 // a group in turn, then the groups. A workgroup takes COLS columns (COLS / 4 threads a group) of
 // R = 256 / (P COLS / 4) query rows. Items that are none and items that one workgroup had leave at once.
+// Bound by the records' bytes (22 MB of 26 tokens over 8192 rows at head_dim 512: 8 us), or for few of them
+// by a launch's start and two dependent reads (4 us).
 template <int HD, int MQ, int UR, int P, int COLS>
 __global__ __launch_bounds__(256) void k_paged_join(const PagedAttnArgs a) {
     constexpr unsigned TPG = COLS / 4, R = 256 / (P * TPG);
@@ -1244,6 +1260,9 @@ struct PagedPlan {
     uint64_t q_tiles;  // of a sequence and kv head, at most
     size_t bytes;
 };
+// Query rows of a tile: 32 (K and V in registers) against a tile of 64 (through LDS), 64 sequences of 4 tokens, e4m3: 142
+// and 192 us; 64 against 128, 64 sequences of 8 tokens: 223 and 250 us; 128 against 64, 1024 tokens over 7001 rows: 137 and
+// 175 us. At head_dim 512 the registers hold no more than 16 and 64.
 static PagedPlan paged_plan(unsigned head_dim, unsigned num_kv_heads, unsigned num_q_heads, const PagedBatchDev& b) {
     PagedPlan p;
     const uint64_t rows = (uint64_t)b.max_tokens * (num_q_heads / num_kv_heads);
@@ -1254,10 +1273,11 @@ static PagedPlan paged_plan(unsigned head_dim, unsigned num_kv_heads, unsigned n
     return p;
 }
 
-// Whether every item goes to one workgroup: its rows are few for certain (by the window, or the block
-// table's size), and there are items for the CUs or one tile a wave, so that cutting them and joining the
-// parts in a second launch would cost more. (One token over a window of 512, whole / cut: 16.3 / 13.8 us;
-// 512 sequences of 100 to 300 rows 34 / 55 us.)
+// Whether every item goes to one workgroup: its rows are few for certain (by the window, or the block table's
+// size), and there are items for half the CUs or one tile a wave, so that cutting them and joining the parts in a
+// second launch would cost more. (512 sequences of 100 to 300 rows, whole / cut: 34 / 55 us; one token over a window
+// of 512, which this leaves to be cut: 16 / 12 us.) At head_dim 256 with eight waves, which have a tile each at
+// once: 34.3 us for the 512 sequences, 35.0 with four.
 static bool paged_whole(uint64_t rows, uint64_t items, unsigned cus) {
     return rows <= 256 || (rows <= 2048 && 2 * items >= cus);
 }

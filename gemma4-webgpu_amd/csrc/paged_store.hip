@@ -13,7 +13,9 @@ namespace g4 {
 // token: its threads evaluate the cos and sin of the token's angles (in f64, as
 // the other preps do), its four waves take the head slots (q heads, k heads, v
 // heads) in turn. A wave requests its first row before it looks for the token's
-// sequence, page and position, which are three dependent loads.
+// sequence, page and position, which are three dependent loads. Bound by its
+// bytes (four prompts of 1000 tokens, e4m3, head_dim 512: 21 us at the rate of
+// a large copy), and for few tokens by those loads: 512 tokens take 5.4 us.
 struct AppendArgs {
     const float* __restrict__ q;
     const float* __restrict__ k;
@@ -137,7 +139,9 @@ __global__ __launch_bounds__(kWG) void k_paged_append(const AppendArgs a) {
 // One thread a (sequence, 16-byte column of a row) of a pool. It reads a batch of
 // the path's rows before it writes any. That is enough: the path ascends, so
 // path[d] >= d, and a row written at step d is no later step's source (those
-// are above path[d]); other columns belong to other threads.
+// are above path[d]); other columns belong to other threads. Bound by its
+// dependent loads (lengths, path, page, row: 5 us for one sequence in 15 layers,
+// 8 for 64 in 10), which a batch of eight rows has side by side.
 struct CommitPool {
     void* p;
     uint32_t row_bytes;
