@@ -147,9 +147,8 @@ struct CommitPool {
     uint32_t row_bytes;
     uint32_t pieces;  // row_bytes / 16
 };
-template <int N>
 struct CommitArgs {
-    CommitPool pool[2 * N];
+    CommitPool pool[2 * G4_COMMIT_MAX_CACHES];
     const int32_t* __restrict__ path;
     const int32_t* __restrict__ accepted;
     int32_t* __restrict__ new_ctx;
@@ -159,8 +158,7 @@ struct CommitArgs {
 
 constexpr int kCommitBatch = 8;
 
-template <int N>
-__global__ __launch_bounds__(kWG) void k_paged_commit(const CommitArgs<N> a) {
+__global__ __launch_bounds__(kWG) void k_paged_commit(const CommitArgs a) {
     const CommitPool pool = a.pool[blockIdx.y];
     const unsigned i = blockIdx.x * kWG + threadIdx.x;  // below 2^31 (checked on the host)
     const unsigned s = i / pool.pieces, piece = i % pool.pieces;
@@ -266,12 +264,10 @@ bool repeated(const CommitPool* pool, uint32_t n) {
     return false;
 }
 
-// The pools go by value in the kernel arguments: a block for up to 16 caches (a launch's cost grows with
-// its size), and one for the most there may be.
-template <int N>
+// The pools go by value in the kernel arguments.
 int commit(const g4_paged_cache* caches, uint32_t n_caches, const g4_paged_batch* batch, const int32_t* path,
            uint32_t path_stride, const int32_t* n_accepted, int32_t* new_ctx_lens, void* stream) {
-    CommitArgs<N> a;
+    CommitArgs a;
     uint32_t most = 0;
     for (uint32_t i = 0; i < n_caches; i++) {
         const g4_paged_cache& c = caches[i];
@@ -301,7 +297,7 @@ int commit(const g4_paged_cache* caches, uint32_t n_caches, const g4_paged_batch
     a.path_stride = path_stride;
     const uint64_t threads = (uint64_t)batch->n_seqs * most;
     if (threads > 0x7fffff00u) return fail(G4_EINVAL, "pagedCommit: %u sequences of %u-byte rows are too many", batch->n_seqs, most * 16);
-    G4_LAUNCH(k_paged_commit<N>, dim3((uint32_t)((threads + kWG - 1) / kWG), 2 * n_caches), dim3(kWG), 0, as_stream(stream), a);
+    G4_LAUNCH(k_paged_commit, dim3((uint32_t)((threads + kWG - 1) / kWG), 2 * n_caches), dim3(kWG), 0, as_stream(stream), a);
     G4_CHECK_LAUNCH("pagedCommit");
     return G4_OK;
 }
@@ -368,9 +364,7 @@ int g4_paged_commit(const g4_paged_cache* caches, uint32_t n_caches, const g4_pa
         return fail(G4_EINVAL, "pagedCommit: %u caches (1 to %d)", n_caches, G4_COMMIT_MAX_CACHES);
     if (!path || !n_accepted || !new_ctx_lens) return fail(G4_EINVAL, "pagedCommit: NULL path, n_accepted or new_ctx_lens");
     if (path_stride == 0 || path_stride > (1u << 30)) return fail(G4_EINVAL, "pagedCommit: path_stride %u", path_stride);
-    static_assert(G4_COMMIT_MAX_CACHES == 64, "the largest argument block");
-    return n_caches <= 16 ? commit<16>(caches, n_caches, batch, path, path_stride, n_accepted, new_ctx_lens, stream)
-                          : commit<64>(caches, n_caches, batch, path, path_stride, n_accepted, new_ctx_lens, stream);
+    return commit(caches, n_caches, batch, path, path_stride, n_accepted, new_ctx_lens, stream);
 }
 
 }  // extern "C"

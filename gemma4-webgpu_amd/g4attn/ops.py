@@ -729,6 +729,7 @@ class PagedCache:
         f8 = k_pool.dtype == torch.float8_e4m3fn
         self.c = abi.PagedCache(k_pool.data_ptr(), v_pool.data_ptr(), self.num_pages, self.page_size,
                                 self.num_kv_heads, self.head_dim, abi.G4_KV_E4M3 if f8 else abi.G4_KV_F16, 0)
+        self.record = bytes(self.c)
 
 
 class PagedBatch:
@@ -855,7 +856,7 @@ class PagedCaches:
         for i, c in enumerate(self.caches):
             if c.device != self.device:
                 raise ValueError(f"caches[{i}]: on cuda:{c.device}, expected cuda:{self.device}")
-        self.c = (abi.PagedCache * len(self.caches))(*[c.c for c in self.caches])
+        self.c = (abi.PagedCache * len(self.caches)).from_buffer_copy(b"".join([c.record for c in self.caches]))
 
 
 def paged_commit(caches, batch, path, n_accepted, new_ctx_lens, stream=None):
