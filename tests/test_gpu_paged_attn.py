@@ -278,3 +278,25 @@ def test_random_batches(dev, case):
               parents=[random_parents(r, t) for t in new] if tree else None)
     announce(f"pagedAttn random {case}: hd={hd} heads={nqh}/{nkh} ctx={ctx} new={new} tree={tree} kv={p.kv} {kw}")
     run(p, **kw)
+
+
+@pytest.mark.parametrize("ctx,new,nqh,nkh,hd,kv", [
+    ([5000, 10, 700], [40, 1, 0], 8, 2, 512, "f16"),        # three query tiles of two kv heads, some of no tokens
+    ([9000, 10], [130, 1], 8, 1, 256, "f16"),               # nine query tiles, eight of them of one sequence
+    ([3000, 2999, 1, 0], [33, 17, 33, 1], 8, 4, 256, "e4m3"),
+    ([16000], [26], 8, 1, 512, "e4m3"),
+    ([12000], [1], 1, 1, 256, "f16"),                       # more pieces than a join's group has records
+    ([1500] * 60, [2] * 60, 8, 4, 256, "f16"),              # items fit one scan, their pieces do not fit the workgroups
+    ([400, 300, 200], [300, 200, 100], 8, 1, 256, "f16"),   # query tiles that end at different rows
+])
+def test_pieces_of_items(dev, ctx, new, nqh, nkh, hd, kv):
+    announce(f"pagedAttn pieces hd={hd} heads={nqh}/{nkh} {kv} ctx={ctx[:4]} new={new[:4]}")
+    run(Paged(dev, 60 + len(ctx), ctx, new, nqh=nqh, nkh=nkh, hd=hd, kv=kv, page=32))
+
+
+@pytest.mark.parametrize("softcap", [5.0, 50.0, 1e6])
+def test_softcaps_on_both_sides_of_the_polynomial(dev, softcap):
+    """Scores up to about 8: beyond half of a cap of 5 in every tile, of 50 in none, and tiny against 1e6."""
+    announce(f"pagedAttn softcap={softcap} both forms")
+    run(Paged(dev, 71, [700, 90], [3, 5], page=64), softcap=softcap)
+    run(Paged(dev, 72, [300], [30], hd=512, page=64), softcap=softcap)

@@ -270,3 +270,66 @@ def test_a_drafted_step_equals_the_tokens_one_by_one(dev, hd):
     _, tol = p.expected()
     for d, j in enumerate(path):
         assert (tree_out[j] - outs[d]).abs().max().item() <= 2 * tol[j]
+
+
+@pytest.mark.parametrize("hd,kv,seqs", [(256, "f16", 3), (512, "e4m3", 2), (256, "e4m3", 70)])
+def test_a_captured_step_serves_later_steps(dev, hd, kv, seqs):
+    """Append, attention, log probabilities and commit captured once, then replayed with other lengths, paths and inputs
+    written in place: every replay gives the eager calls' bits, in the outputs and in the pools. 70 sequences of
+    a query tile each are more than a wave's scan holds at once."""
+    r = np.random.default_rng(seqs)
+    longest = [int(x) for x in r.integers(40, 700, seqs)]
+    parents = [random_parents(r, 5) for _ in range(seqs)]
+    p = Paged(dev, 50, longest, [5] * seqs, hd=hd, page=16, kv=kv, parents=parents)
+    p.upload()
+    a = Append(dev, p, 51)
+    n, vocab, top = p.tokens, 700, 3
+    out = torch.zeros(n, p.nqh, hd, device=dev)
+    ws = torch.empty(ops.paged_attn_workspace_bytes(p.cache, p.batch, p.nqh), dtype=torch.uint8, device=dev)
+    logits = torch.zeros(n, vocab, device=dev)
+    tokens = torch.arange(n, dtype=torch.int32, device=dev) % vocab
+    lp, ent, tops = torch.zeros(n, device=dev), torch.zeros(n, device=dev), torch.zeros(n, top, device=dev)
+    ids = torch.zeros(n, top, dtype=torch.int32, device=dev)
+    lws = torch.empty(ops.token_logprobs_workspace_bytes(n, vocab, top), dtype=torch.uint8, device=dev)
+    path = torch.zeros(seqs, 5, dtype=torch.int32, device=dev)
+    accepted = torch.zeros(seqs, dtype=torch.int32, device=dev)
+    new_ctx = torch.zeros(seqs, dtype=torch.int32, device=dev)
+    caches = ops.PagedCaches([p.cache])
+    results = (a.q_out, out, lp, ent, ids, tops, new_ctx, p.d_k, p.d_v)
+
+    def step():
+        ops.paged_append(p.cache, p.batch, **a.d, q_out=a.q_out, eps=EPS)
+        ops.paged_attn(p.cache, p.batch, a.q_out, out, ws, sliding_window=256)
+        ops.token_logprobs(logits, tokens, lp, ent, lws, ids, tops, cap=30.0)
+        ops.paged_commit(caches, p.batch, path, accepted, new_ctx)
+
+    announce(f"captured drafted step hd={hd} {kv} {seqs} sequences")
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    k0, v0 = p.d_k.clone(), p.d_v.clone()
+    depth = p.batch.tensors[3] - p.d_ctx.repeat_interleave(5)
+    for turn in range(4):
+        ctx = torch.tensor([int(r.integers(0, x + 1)) for x in longest], dtype=torch.int32, device=dev)
+        p.d_ctx.copy_(ctx)
+        p.batch.tensors[3].copy_(ctx.repeat_interleave(5) + depth)
+        for s in range(seqs):
+            m = int(r.integers(0, 6))
+            accepted[s] = m
+            path[s, :m] = torch.tensor(sorted(r.choice(5, m, replace=False).tolist()), dtype=torch.int32, device=dev)
+        for t in (a.d["q"], a.d["k"], a.d["v"], logits):
+            t.normal_(generator=torch.Generator(device=dev).manual_seed(turn))
+        got = []
+        for run in (step, graph.replay):
+            p.d_k.copy_(k0)
+            p.d_v.copy_(v0)
+            for t in results[:-2]:
+                t.zero_()
+            run()
+            torch.cuda.synchronize()
+            got.append([t.clone() for t in results])
+        for x, y in zip(*got):
+            assert torch.equal(x.view(torch.uint8), y.view(torch.uint8)), turn
+        assert torch.equal(new_ctx, ctx + accepted)
