@@ -761,7 +761,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_paged_few(const PagedAttnArgs
                 if (t + W < seg) tile(1, it + 1, t + W);
         }
 
-        // The four waves' states joined: maxima first, then a query group's outputs at a time.
+        // The waves' states joined: maxima first, then a query group's outputs at a time.
         const bool whole = seg == sp.n;
         const unsigned slot = 2 * blockIdx.x + (off ? 0u : 1u);  // a part that continues its item, or begins it
         const int el = not_hoisted(lane), en = el & 15, eg = el >> 4;
