@@ -593,7 +593,7 @@ __device__ __forceinline__ float paged_inverse(float L) { return L > 0.0f ? 1.0f
 // Bound by the cache's bytes: the W waves of a workgroup take every W-th row tile of its share, each
 // with a tile's K and V in registers. With four waves (512 registers each) the next tile's K is
 // requested when the scores have used this one's, its V when the products have (two tiles ahead for e4m3 at
-// head_dim 512, whose tiles' work is long next to their bytes: 64 sequences of one token 134 -> 124 us; at 256 it
+// head_dim 512, whose tiles' work is long next to their bytes: 64 sequences of one token 134 -> 126 us; at 256 it
 // gives nothing); with eight (256 registers) a wave requests a tile at a time, and a short item, which one
 // workgroup has whole, takes half as many in turn.
 // Measured: 64 sequences of 1024 to 32768 rows, one token: f16 187 us, 6.1 TB/s; e4m3 106 us, 5.4 TB/s (both read 0.83
@@ -761,10 +761,39 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_paged_few(const PagedAttnArgs
                 if (t + W < seg) tile(1, it + 1, t + W);
         }
 
-        // The waves' states joined: maxima first, then a query group's outputs at a time.
         const bool whole = seg == sp.n;
         const unsigned slot = 2 * blockIdx.x + (off ? 0u : 1u);  // a part that continues its item, or begins it
         const int el = not_hoisted(lane), en = el & 15, eg = el >> 4;
+        if (seg == 1) {  // one wave had it all (short sequences: one token over 2048 rows 10.7 us, by way of LDS 11.7)
+            if (wave == 0) {
+#pragma unroll
+                for (int c = 0; c < C; c++) {
+                    float L = add_xor16(l_run[c]);
+                    L = add_xor32(L);
+                    const unsigned r = qt * MQ + 16 * c + en, rec = 16 * c + en;
+                    if (r < rows) {
+                        const float inv = whole ? paged_inverse(L) : 1.0f;
+                        float* dst = whole ? a.out + ((uint64_t)(sq.start + r / G) * (a.nkh * G) + kvh * G + r % G) * HD
+                                           : a.part_o + ((uint64_t)slot * MQ + rec) * HD;
+                        if (!whole && eg == 0) stg<f32x2>(a.part_ml + ((uint64_t)slot * MQ + rec) * 2, f32x2{m_run[c], L});
+#pragma unroll
+                        for (int b = 0; b < D::VP; b++)
+#pragma unroll
+                            for (int j = 0; j < 4; j++)
+#pragma unroll
+                                for (int e = 0; e < D::E; e += 4) {
+                                    const int x = b * D::E + e;
+                                    stg<f32x4>(dst + 16 * D::E * b + D::E * (4 * eg + j) + e,
+                                               f32x4{acc[c][x][j], acc[c][x + 1][j], acc[c][x + 2][j], acc[c][x + 3][j]} * inv);
+                                }
+                    }
+                }
+            }
+            u += seg;
+            if (u < u_end) paged_next<MQ, UR>(a, at);
+            continue;
+        }
+        // The waves' states joined: maxima first, then a query group's outputs at a time.
 #pragma unroll
         for (int c = 0; c < C; c++) {
             float l = add_xor16(l_run[c]);
@@ -1276,7 +1305,7 @@ static PagedPlan paged_plan(unsigned head_dim, unsigned num_kv_heads, unsigned n
 // Whether every item goes to one workgroup: its rows are few for certain (by the window, or the block table's
 // size), and there are items for half the CUs or one tile a wave, so that cutting them and joining the parts in a
 // second launch would cost more. (512 sequences of 100 to 300 rows, whole / cut: 34 / 55 us; one token over a window
-// of 512, which this leaves to be cut: 16 / 12 us.) At head_dim 256 with eight waves, which have a tile each at
+// of 512, which this leaves to be cut: 16 / 11 us.) At head_dim 256 with eight waves, which have a tile each at
 // once: 34.3 us for the 512 sequences, 35.0 with four.
 static bool paged_whole(uint64_t rows, uint64_t items, unsigned cus) {
     return rows <= 256 || (rows <= 2048 && 2 * items >= cus);
