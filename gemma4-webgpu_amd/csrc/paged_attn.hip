@@ -763,16 +763,19 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_paged_few(const PagedAttnArgs
 
         const bool whole = seg == sp.n;
         const unsigned slot = 2 * blockIdx.x + (off ? 0u : 1u);  // a part that continues its item, or begins it
-        const int el = not_hoisted(lane), en = el & 15, eg = el >> 4;
         if (seg == 1) {  // one wave had it all (short sequences: one token over 2048 rows 10.7 us, by way of LDS 11.7)
             if (wave == 0) {
+                const int el = not_hoisted(lane), en = el & 15, eg = el >> 4;
 #pragma unroll
                 for (int c = 0; c < C; c++) {
                     float L = add_xor16(l_run[c]);
                     L = add_xor32(L);
                     const unsigned r = qt * MQ + 16 * c + en, rec = 16 * c + en;
                     if (r < rows) {
-                        const float inv = whole ? paged_inverse(L) : 1.0f;
+                        if (whole) {
+#pragma unroll
+                            for (int x = 0; x < D::NO; x++) acc[c][x] *= paged_inverse(L);
+                        }
                         float* dst = whole ? a.out + ((uint64_t)(sq.start + r / G) * (a.nkh * G) + kvh * G + r % G) * HD
                                            : a.part_o + ((uint64_t)slot * MQ + rec) * HD;
                         if (!whole && eg == 0) stg<f32x2>(a.part_ml + ((uint64_t)slot * MQ + rec) * 2, f32x2{m_run[c], L});
@@ -784,7 +787,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_paged_few(const PagedAttnArgs
                                 for (int e = 0; e < D::E; e += 4) {
                                     const int x = b * D::E + e;
                                     stg<f32x4>(dst + 16 * D::E * b + D::E * (4 * eg + j) + e,
-                                               f32x4{acc[c][x][j], acc[c][x + 1][j], acc[c][x + 2][j], acc[c][x + 3][j]} * inv);
+                                               f32x4{acc[c][x][j], acc[c][x + 1][j], acc[c][x + 2][j], acc[c][x + 3][j]});
                                 }
                     }
                 }
@@ -794,6 +797,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_paged_few(const PagedAttnArgs
             continue;
         }
         // The waves' states joined: maxima first, then a query group's outputs at a time.
+        const int el = not_hoisted(lane), en = el & 15, eg = el >> 4;
 #pragma unroll
         for (int c = 0; c < C; c++) {
             float l = add_xor16(l_run[c]);
