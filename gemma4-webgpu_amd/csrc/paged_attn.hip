@@ -967,7 +967,8 @@ __global__ __launch_bounds__(64 * WQ * WK * WD, WQ * WK * WD / 4) void k_paged_t
         const unsigned j0 = w0 / G, j1 = min((w0 + 15) / G, sq.n - 1);
         const unsigned wave_hi = !work ? 0u : a.b.mask ? sp.hi : min(sq.ctx + j1 + 1, sp.hi);
         const unsigned clear_lo = !a.window ? 0u : a.b.positions ? ~0u : (unsigned)max((int)(sq.ctx + j1 + 1) - a.window, 0);
-        const unsigned clear_hi = a.b.mask ? sq.ctx : sq.ctx + min(j0 + 1, sq.n);
+        // sp.hi: a chain may run past the block table, whose last page then ends in the middle of a row tile.
+        const unsigned clear_hi = a.b.mask ? sq.ctx : min(sq.ctx + min(j0 + 1, sq.n), sp.hi);
 
         // The query first: its wait, before the page ids', would otherwise be one for the requests below too.
         f16x8 qr[D::NC];
