@@ -12,8 +12,9 @@
 //     straight from the cache; the query is f16, so products are exact.
 //   O^T[16 d x 16 q] += V^T[16 d x 32 rows] P^T: lane (n, g) holds V pieces of rows
 //     4g..4g+3 and 16+4g..16+4g+3, the rows whose scores it has, and transposes them in
-//     registers. P goes in twice, as its f16 value and the f16 residual: 22 bits, so that
-//     an f32 result keeps f32 accuracy (one f16 P alone leaves 2e-4).
+//     registers. P goes in twice, as its f16 value and the f16 residual, so that an f32 result
+//     keeps f32 accuracy (one f16 P alone leaves 2e-4): off by 2^-24 of a weight down to 2^-8 of
+//     the largest one, from there on by 2^-32 of that (paged_softmax).
 // e4m3 pools are widened to f16 in registers, which is exact.
 //
 // Two forms. Few query rows a kv head (up to 16, at head_dim 256 up to 32; k_paged_few): the workgroup's
@@ -494,8 +495,16 @@ struct PagedCols {
 // How a wave takes a 32-row tile: not at all, as it is, or masked.
 enum PagedTake { kSkip, kClear, kMasked };
 
-// The online softmax of NX tiles' scores (log2 units), together: the running maximum moves once a
-// score is 8 above it (P stays within f16), P leaves as f16 and its residual.
+// The online softmax of NX tiles' scores (log2 units), together; P leaves as f16 and its residual, both
+// rounded to nearest. P is 2^(score - m_run), and m_run lies kPagedLift below the maximum that it was set at and
+// moves once a score is kPagedMove above that: P stays within f16 (2^15 at most), and half of f16's least step,
+// 2^-25, is at most 2^-32 of the largest weight. That counts where many rows lie far below the largest, as behind
+// an attention sink: 2^17 of them are off by 3e-5 in all at most, and as P is rounded to nearest mostly by far less
+// (relative to the maximum itself and truncated, the weights of 16384 rows 17 nats below one lost 6e-4 of the output).
+// A larger lift leaves less to the move, and outputs are rescaled more often (64 sequences of 8 tokens, 1024 tokens over
+// 7001 rows: 7 and 8 take 0 and 1 % longer than no lift, 11 and 4 2.5 %). The factor is the same in l, o and the records, and falls out of
+// their quotient.
+constexpr float kPagedLift = 7.0f, kPagedMove = 8.0f;
 template <int HD, int C, bool F8, int NX>
 __device__ __forceinline__ void paged_softmax(const PagedAttnArgs& a, const f32x4 (&sc)[NX][C][2], const unsigned (&seen)[NX][C],
                                               const PagedTake (&how)[NX], float (&m_run)[C], float (&l_run)[C],
@@ -534,9 +543,9 @@ __device__ __forceinline__ void paged_softmax(const PagedAttnArgs& a, const f32x
         }
         tmax = max_xor16(tmax);  // the column's rows lie in four lane groups
         tmax = max_xor32(tmax);
-        const bool move = tmax > m_run[c] + 8.0f;
+        const bool move = tmax > m_run[c] + (kPagedLift + kPagedMove);
         if (__any(move)) {
-            const float m_new = move ? tmax : m_run[c];
+            const float m_new = move ? tmax - kPagedLift : m_run[c];
             const float alpha = move ? __builtin_amdgcn_exp2f(m_run[c] - m_new) : 1.0f;
             m_run[c] = m_new;
             l_run[c] *= alpha;
@@ -550,8 +559,8 @@ __device__ __forceinline__ void paged_softmax(const PagedAttnArgs& a, const f32x
             for (int i = 0; i < 8; i += 2) {
                 const float p0 = __builtin_amdgcn_exp2f(sv[x][i] - base), p1 = __builtin_amdgcn_exp2f(sv[x][i + 1] - base);
                 l_run[c] += p0 + p1;
-                const f16x2 h = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(p0, p1));
-                const f16x2 r = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(p0 - (float)h[0], p1 - (float)h[1]));
+                const f16x2 h = __builtin_convertvector((f32x2{p0, p1}), f16x2);
+                const f16x2 r = __builtin_convertvector((f32x2{p0 - (float)h[0], p1 - (float)h[1]}), f16x2);
                 hi[x][c][i] = h[0];
                 hi[x][c][i + 1] = h[1];
                 lo[x][c][i] = r[0];

@@ -1,9 +1,11 @@
-"""g4_paged_attn at edges of its tiles, windows and number formats: chains that run past the block table, against the
-definition in 64 bits. Tolerances are derived in paged_helpers.Paged.expected, or where a test stands."""
+"""g4_paged_attn at edges of its tiles, windows and number formats: chains that run past the block table, weights far below
+the largest, against the definition in 64 bits. Tolerances are derived in paged_helpers.Paged.expected, or where a test stands."""
+import numpy as np
 import pytest
 import torch
 
 from conftest import announce
+from g4attn import ops
 from paged_helpers import Paged
 
 pytestmark = pytest.mark.gpu
@@ -26,3 +28,63 @@ def test_chains_past_the_block_table(dev, hd, nqh, new, kv, window, ctx):
     p = Paged(dev, ctx + new, [ctx, 20], [new, 1], hd=hd, nqh=nqh, kv=kv, page=16)
     p.table = p.table[:, :7].copy()
     run(p, window=window)
+
+
+# ---- weights far below the largest ------------------------------------------------------
+
+@pytest.mark.parametrize("kv", ["f16", "e4m3"])
+@pytest.mark.parametrize("hd,new,rows,sinks", [
+    (256, 1, 32768, [0, 32, 64, 96]),  # every fourth tile a wave
+    (512, 1, 32768, [0, 32, 64, 96]),
+    (256, 4, 32768, [0, 32, 64, 96]),  # 32 query rows
+    (256, 8, 16384, [0, 32]),          # 64, two waves a tile
+    (256, 16, 16384, [0]),             # 128
+    (512, 8, 16384, [0]),
+])
+def test_weights_far_below_the_largest_add_up(dev, hd, new, rows, sinks, kv):
+    """A row 11 to 17 nats above all others, as an attention sink has it, in each wave's share, V of one sign: what
+    thousands of small weights add is not lost, nor one-sided. Scores are exact (one element of q and k each), and
+    a sequence a compute unit keeps all rows of one in one running state.
+
+    The bound, in units of the largest |v| = 1. Weights: scale and log2(e) round the score twice, the difference from
+    the maximum once more (it is at most 2 X + 16 ln 2 nats for scores up to X), the exponent is good to a
+    step: (4 X + 14) 2^-24, in the numerator and the denominator. Eight factors of states that are joined: 16. The two
+    f16 of a weight: 2^-22 of it, and a row at most 2^-32 of the largest weight (half of f16's least step, if that
+    weight is 2^7 or more in f16). Sums: the numerator takes two products a tile of
+    32 rows, the denominator four terms, each off by half a step of the partial sum."""
+    announce(f"pagedAttn sink hd={hd} new={new} rows={rows} kv={kv}")
+    r = np.random.default_rng(hd + new)
+    seqs = torch.cuda.get_device_properties(dev).multi_processor_count
+    page, nqh = 64, 8
+    dt = torch.float8_e4m3fn if kv == "e4m3" else torch.float16
+    order = r.permutation(rows // page)
+    low = -6.0 if kv == "e4m3" else -5.6875  # 2^-24 times 0.7 and 0.95
+    score = np.where(r.random(rows) < 0.75, low, 0.0)
+    score[sinks] = 11.0
+    v = np.where(r.random((rows, hd)) < 0.5, 1.0, 0.75)
+    v[sinks] = 0.0
+    k = torch.zeros(rows, hd)
+    k[:, 0] = torch.from_numpy(score).float()
+    # Row i of every sequence lies in page order[i // page].
+    pool = lambda x: torch.empty(rows // page, page, 1, hd).index_copy_(  # noqa: E731
+        0, torch.from_numpy(order), x.float().view(rows // page, page, 1, hd)).to(dt).to(dev)
+    cache = ops.PagedCache(pool(k), pool(torch.from_numpy(v)))
+    i32 = lambda a: torch.from_numpy(np.ascontiguousarray(a, np.int32)).to(dev)  # noqa: E731
+    batch = ops.PagedBatch(i32(np.tile(order, (seqs, 1))), i32(np.arange(seqs + 1) * new), i32(np.full(seqs, rows - new)),
+                           seqs * new, max_tokens=new)
+    factor = np.array([1.0, 1.0, 0.75, 1.0, 0.625, 1.0, 0.5, 0.875])
+    q = torch.zeros(seqs * new, nqh, hd)
+    q[:, :, 0] = torch.from_numpy(factor).float()
+    out = torch.full((seqs * new, nqh, hd), -123.0, device=dev)
+    ws = torch.empty(ops.paged_attn_workspace_bytes(cache, batch, nqh), dtype=torch.uint8, device=dev)
+    ops.paged_attn(cache, batch, q.half().to(dev), out, ws)
+    torch.cuda.synchronize()
+    got = out.cpu().double().numpy().reshape(seqs, new, nqh, hd)
+    tiles = rows // 32 // (4 if len(sinks) == 4 else len(sinks))
+    bound = (2 * (4 * 11.0 + 14) + 16 + 4 + 6 * tiles) * 2.0 ** -24 + rows * 2.0 ** -32
+    for j in range(new):
+        n = rows - new + j + 1
+        p = np.exp(factor[:, None] * (score[None, :n] - 11.0))
+        want = (p / p.sum(-1, keepdims=True)) @ v[:n]
+        err = np.abs(got[:, j] - want).max()
+        assert err <= bound, f"token {j}: off by {err:.3e}, bound {bound:.3e}"
