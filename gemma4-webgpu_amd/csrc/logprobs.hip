@@ -431,6 +431,19 @@ static uint32_t lp_chunk(uint32_t rows, uint32_t vocab) {
     if ((uint64_t)rows * ((vocab + kLpLong - 1) / kLpLong) >= 2 * (uint64_t)device_cus()) return kLpLong;
     return vocab <= 64 * kLpShort ? kLpShort : kLpMiddle;
 }
+static uint64_t lp_chunks(uint32_t rows, uint32_t vocab) {
+    const uint64_t chunk = lp_chunk(rows, vocab);
+    return (vocab + chunk - 1) / chunk;
+}
+// The most chunks that a call of at most this many rows and logits has, all rows together: fewer rows or logits may
+// be cut shorter. Cut long, a call has at most rows * long; cut short, fewer than 2 CUs long chunks' worth of logits
+// (or it would be cut long), of four short chunks each.
+static uint64_t lp_most_chunks(uint32_t rows, uint32_t vocab) {
+    const uint64_t longs = (vocab + kLpLong - 1) / kLpLong, middles = (vocab + kLpMiddle - 1) / kLpMiddle;
+    const uint64_t shorts = vocab <= 64 * kLpShort ? (vocab + kLpShort - 1) / kLpShort : 64;
+    const uint64_t cut_short = rows * (shorts > middles ? shorts : middles), least = 8ull * (uint64_t)device_cus();
+    return cut_short <= least ? cut_short : rows * longs > least ? rows * longs : least;
+}
 
 template <int DT, int E>
 void launch_chunks(const LogprobsArgs& a, uint32_t rows, bool vec, hipStream_t st) {
@@ -474,10 +487,9 @@ int logprobs_check(const g4_token_logprobs_params* p) {
     return G4_OK;
 }
 
-// Room for the chunks of any type and alignment.
-size_t logprobs_bytes(const g4_token_logprobs_params* p) {
-    const uint64_t chunk = lp_chunk(p->rows, p->vocab), chunks = (p->vocab + chunk - 1) / chunk;
-    return (size_t)p->rows * chunks * (16 + 8ull * p->top_k) + 16;
+// Room for so many chunks, of any type and alignment.
+size_t logprobs_bytes(const g4_token_logprobs_params* p, uint64_t chunks) {
+    return (size_t)chunks * (16 + 8ull * p->top_k) + 16;
 }
 
 }  // namespace
@@ -488,7 +500,7 @@ int g4_token_logprobs_workspace_size(const g4_token_logprobs_params* p, size_t* 
     if (!bytes) return fail(G4_EINVAL, "g4_token_logprobs_workspace_size: bytes is NULL");
     const int rc = logprobs_check(p);
     if (rc) return rc;
-    *bytes = logprobs_bytes(p);
+    *bytes = logprobs_bytes(p, lp_most_chunks(p->rows, p->vocab));
     return G4_OK;
 }
 
@@ -506,8 +518,9 @@ int g4_token_logprobs(const void* logits, const int32_t* tokens, float* logprobs
     if (reinterpret_cast<uintptr_t>(logits) & (elem - 1)) return fail(G4_EINVAL, "tokenLogprobs: misaligned logits");
     if (reinterpret_cast<uintptr_t>(workspace) & 15)
         return fail(G4_EINVAL, "tokenLogprobs: workspace must be 16-byte aligned");
-    if (workspace_bytes < logprobs_bytes(p))
-        return fail(G4_ENOSPC, "tokenLogprobs: workspace %zu bytes < %zu needed", workspace_bytes, logprobs_bytes(p));
+    const size_t need = logprobs_bytes(p, p->rows * lp_chunks(p->rows, p->vocab));
+    if (workspace_bytes < need)
+        return fail(G4_ENOSPC, "tokenLogprobs: workspace %zu bytes < %zu needed", workspace_bytes, need);
     if (p->rows == 0) return G4_OK;
     LogprobsArgs a = {};
     a.logits = logits;

@@ -881,6 +881,7 @@ LOGIT_TYPES = {torch.float32: abi.G4_LOGITS_F32, torch.float16: abi.G4_LOGITS_F1
 
 
 def token_logprobs_workspace_bytes(rows, vocab, top_k) -> int:
+    """Bytes that serve every call of at most so many rows, logits and alternatives."""
     n = C.c_size_t(0)
     p = abi.TokenLogprobsParams(rows, vocab, 0, abi.G4_LOGITS_F32, top_k, 0.0, 1.0)
     abi.call("g4_token_logprobs_workspace_size", p, C.byref(n))

@@ -840,7 +840,9 @@ int g4_paged_commit(const g4_paged_cache* caches, uint32_t n_caches, const g4_pa
  * (its top ids as said, NaN never among them). logits: f32, f16 or bf16, row r
  * at r * row_stride elements. logprobs and tokens may be NULL together, and so
  * entropy, and top_ids and top_logprobs (with top_k 0). The workspace holds
- * partial results within a call; calls that overlap need one each. */
+ * partial results within a call; calls that overlap need one each. Its size
+ * (g4_token_logprobs_workspace_size) serves every call of no more rows, logits
+ * and alternatives: a loop sizes it for its largest batch. */
 #define G4_LOGITS_F32 0
 #define G4_LOGITS_F16 1
 #define G4_LOGITS_BF16 2

@@ -189,3 +189,19 @@ def test_caps_far_above_the_logits(dev, cap):
     want = torch.log_softmax(cap * torch.tanh(x.double() / cap), -1).gather(1, tokens.long()[:, None])[:, 0]
     # z of the token and of the sum: two differences, each 4 half-steps of the cap.
     assert ((lp - want).abs() <= 2 * 4 * cap * 2.0 ** -24 + 64 * 2.0 ** -24 + want.abs() * 2.0 ** -22).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("vocab,most", [(262144, 16), (50257, 74), (151936, 27)])
+def test_one_workspace_for_a_batch_that_shrinks(dev, dtype, vocab, most):
+    """A loop sizes its workspace for its largest batch and goes on with it as sequences end."""
+    announce(f"tokenLogprobs shrinking batch vocab={vocab} most={most} {dtype}")
+    x, tokens = inputs(dev, vocab, most, vocab, dtype)
+    ws = torch.empty(ops.token_logprobs_workspace_bytes(most, vocab, 20), dtype=torch.uint8, device=dev)
+    for rows in (most, most - 1, most // 2, 1):
+        want = call(x[:rows], tokens[:rows], 20)
+        lp, ent, ids, tops = (torch.empty_like(a) for a in want)
+        ws.fill_(0xff)
+        ops.token_logprobs(x[:rows], tokens[:rows], lp, ent, ws, ids, tops)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip((lp, ent, ids, tops), want)), rows

@@ -213,3 +213,24 @@ def test_commit_refuses_a_pool_twice_and_outputs_over_inputs():
                dict(acc=0x30000 + 4 * (n - 1)), dict(path=0x30000)]:
         st, msg = call(apart[:1], **kw)
         assert st == abi.G4_EINVAL and "lies over" in msg, (kw, msg)
+
+
+@pytest.mark.parametrize("vocab", [1000, 50257, 131072, 131073, 151936, 262144, 1 << 20])
+@pytest.mark.parametrize("k", [0, 5, 20, 64])
+def test_a_workspace_serves_every_smaller_call(vocab, k):
+    """A step with fewer rows, a smaller vocabulary or fewer alternatives than the workspace was sized for is not
+    refused: the size never falls as one of them grows, over the row counts at which the chunks' length changes. (What
+    a call needs is at most its own size.)"""
+    lib = abi.load()
+
+    def size(rows, v=vocab, top=k):
+        n = C.c_size_t(0)
+        assert lib.g4_token_logprobs_workspace_size(abi.TokenLogprobsParams(rows, v, 0, 0, top, 0.0, 1.0), C.byref(n)) == 0
+        return n.value
+
+    sizes = [size(r) for r in range(1, 600)] + [size(65535)]
+    assert sizes == sorted(sizes)
+    for r in (1, 3, 15, 16, 73, 74, 300, 600):
+        by_vocab = [size(r, v) for v in sorted({1000, vocab // 2, vocab - 1, vocab, vocab + 1, 2 * vocab, 65536, 131072, 131073})]
+        assert by_vocab == sorted(by_vocab), r
+        assert size(r, top=k // 2) <= size(r)
