@@ -70,9 +70,9 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedAttnArgs& a, const Pa
     const unsigned j1 = min((qt * MQ + MQ - 1) / a.group, sq.n - 1);
     s.hi = min(sq.ctx + (a.b.mask ? sq.n : j1 + 1), paged_rows(a.b));
     unsigned lo = 0;
-    if (a.window) {  // positions are at least ctx (a chain's: ctx + j)
-        const int at = (int)(sq.ctx + (a.b.positions || a.b.mask ? 0u : j0)) - a.window + 1;
-        lo = min((unsigned)max(at, 0), sq.ctx);
+    if (a.window) {  // a token's position is its row, or given and then at least ctx
+        const int at = (int)(sq.ctx + (a.b.positions ? 0u : j0)) - a.window + 1;
+        lo = (unsigned)max(at, 0);
     }
     s.first = min(lo, s.hi - 1) / UR;
     s.n = (s.hi + UR - 1) / UR - s.first;

@@ -1,5 +1,6 @@
-"""g4_paged_attn at edges of its tiles, windows and number formats: chains that run past the block table, weights far below
-the largest, against the definition in 64 bits. Tolerances are derived in paged_helpers.Paged.expected, or where a test stands."""
+"""g4_paged_attn at edges of its tiles, windows and number formats: chains that run past the block table, weights far
+below the largest, chunks of several windows, against the definition in 64 bits. Tolerances are derived in
+paged_helpers.Paged.expected, or where a test stands."""
 import numpy as np
 import pytest
 import torch
@@ -88,3 +89,45 @@ def test_weights_far_below_the_largest_add_up(dev, hd, new, rows, sinks, kv):
         want = (p / p.sum(-1, keepdims=True)) @ v[:n]
         err = np.abs(got[:, j] - want).max()
         assert err <= bound, f"token {j}: off by {err:.3e}, bound {bound:.3e}"
+
+
+# ---- windows much shorter than a chunk ----------------------------------------------------
+
+@pytest.mark.parametrize("hd,nqh,nkh", [(256, 8, 1), (256, 8, 2), (512, 8, 1)])
+@pytest.mark.parametrize("form", ["chain", "mask", "positions"])
+@pytest.mark.parametrize("ctx,new,window", [(0, 300, 40), (70, 300, 33), (0, 129, 1), (500, 200, 100)])
+def test_chunks_of_several_windows(dev, hd, nqh, nkh, form, ctx, new, window):
+    """A chain as such, as a mask of rows that are their own positions, and with positions given."""
+    announce(f"pagedAttn chunk hd={hd} heads={nqh}/{nkh} {form} ctx={ctx} new={new} window={window}")
+    masks = None if form == "chain" else [set(range(j + 1)) for j in range(new)] + [{0}]
+    positions = [ctx + j for j in range(new)] + [9] if form == "positions" else None
+    run(Paged(dev, new + window, [ctx, 9], [new, 1], hd=hd, nqh=nqh, nkh=nkh, page=16, masks=masks, positions=positions),
+        window=window)
+
+
+def test_work_on_a_windowed_chunk_grows_with_its_length(dev):
+    """Tokens far into a chunk leave its first rows alone: four times the tokens take about four times as long, not the
+    sixteen of a full chunk (a factor of 8 lies between)."""
+    announce("pagedAttn windowed chunk, time by length")
+    hd, nqh, page = 256, 8, 64
+    took = []
+    for new in (4096, 16384):
+        pages = new // page
+        pool = [torch.randn(pages, page, 1, hd, device=dev).half() for _ in range(2)]
+        i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device=dev)  # noqa: E731
+        cache = ops.PagedCache(*pool)
+        batch = ops.PagedBatch(torch.arange(pages, dtype=torch.int32, device=dev).view(1, -1), i32(0, new), i32(0), new)
+        q = torch.randn(new, nqh, hd, device=dev).half()
+        out = torch.empty(new, nqh, hd, device=dev)
+        ws = torch.empty(ops.paged_attn_workspace_bytes(cache, batch, nqh), dtype=torch.uint8, device=dev)
+        best = float("inf")
+        for _ in range(8):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            ops.paged_attn(cache, batch, q, out, ws, scale=0.0625, sliding_window=512)
+            b.record()
+            b.synchronize()
+            best = min(best, a.elapsed_time(b))
+        took.append(best)
+    print(f"4096 tokens {1e3 * took[0]:.0f} us, 16384 tokens {1e3 * took[1]:.0f} us", flush=True)
+    assert took[1] < 8 * took[0], took
