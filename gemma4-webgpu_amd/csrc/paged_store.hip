@@ -288,8 +288,9 @@ int commit(const g4_paged_cache* caches, uint32_t n_caches, const g4_paged_batch
     // Written while other workgroups still read these.
     const uint64_t seqs = batch->n_seqs;
     if (overlap(new_ctx_lens, seqs, batch->ctx_lens, seqs) || overlap(new_ctx_lens, seqs, n_accepted, seqs) ||
-        overlap(new_ctx_lens, seqs, path, seqs * path_stride))
-        return fail(G4_EINVAL, "pagedCommit: new_ctx_lens lies over ctx_lens, n_accepted or path");
+        overlap(new_ctx_lens, seqs, path, seqs * path_stride) || overlap(new_ctx_lens, seqs, batch->token_start, seqs + 1) ||
+        overlap(new_ctx_lens, seqs, batch->block_table, seqs * batch->table_stride))
+        return fail(G4_EINVAL, "pagedCommit: new_ctx_lens lies over ctx_lens, token_start, block_table, n_accepted or path");
     if (repeated(a.pool, 2 * n_caches)) return fail(G4_EINVAL, "pagedCommit: a pool is named twice (its rows would move twice)");
     a.path = path;
     a.accepted = n_accepted;

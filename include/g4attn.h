@@ -821,7 +821,7 @@ int g4_paged_attn(const g4_paged_cache* cache, const g4_paged_batch* batch, cons
  * sequence (a tree's ancestors come before their descendants); n_accepted: DEVICE
  * [n_seqs], cut to [0, path_stride]. An index that is negative, not above the one before it, or
  * not below the sequence's new tokens ends its sequence's path there.
- * new_ctx_lens (DEVICE [n_seqs], apart from ctx_lens, n_accepted and path) receives ctx_lens + the
+ * new_ctx_lens (DEVICE [n_seqs], apart from path, n_accepted and the batch's arrays) receives ctx_lens + the
  * length of the path. Of the batch, positions and tree_mask are not read. */
 #define G4_COMMIT_MAX_CACHES 64
 int g4_paged_commit(const g4_paged_cache* caches, uint32_t n_caches, const g4_paged_batch* batch, const int32_t* path,

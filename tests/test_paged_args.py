@@ -234,3 +234,13 @@ def test_a_workspace_serves_every_smaller_call(vocab, k):
         by_vocab = [size(r, v) for v in sorted({1000, vocab // 2, vocab - 1, vocab, vocab + 1, 2 * vocab, 65536, 131072, 131073})]
         assert by_vocab == sorted(by_vocab), r
         assert size(r, top=k // 2) <= size(r)
+
+
+def test_commit_refuses_new_lengths_over_what_other_workgroups_read():
+    """One workgroup writes the lengths while others still look their sequence and their pages up."""
+    lib = abi.load()
+    b = batch(token_start=0x40000, block_table=0x50000, ctx_lens=0x60000)
+    for new in (0x40000, 0x40000 + 4 * b.n_seqs, 0x40000 - 4 * (b.n_seqs - 1), 0x50000,
+                0x50000 + 4 * (b.n_seqs * b.table_stride - 1), 0x50000 - 4 * (b.n_seqs - 1)):
+        st = lib.g4_paged_commit(cache(k_pool=0x1000000, v_pool=0x2000000), 1, b, 0x10000, 4, 0x20000, new, None)
+        assert st == abi.G4_EINVAL and "lies over" in lib.g4_last_error().decode(), hex(new)
