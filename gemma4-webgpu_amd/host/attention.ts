@@ -340,8 +340,16 @@ export interface TokenLogprobs {
   temperature?: number;
 }
 
+const KV_DTYPES: Record<string, number> = { f16: 0, e4m3: 1 };
 const LOGIT_DTYPES: Record<string, number> = { f32: 0, f16: 1, bf16: 2 };
 const LOGIT_BYTES: Record<string, number> = { f32: 4, f16: 2, bf16: 2 };
+
+// The number of a type's name. The sources run without a type check, and another name would pass every size check.
+function dtypeCode(codes: Record<string, number>, dtype: string, what: string): number {
+  const code = codes[dtype];
+  if (typeof code !== 'number') throw new TypeError(what + ': dtype ' + dtype + ', expected ' + Object.keys(codes).join(', '));
+  return code;
+}
 
 export interface StepShape {
   numQHeads: number;
@@ -837,12 +845,13 @@ export class HipAttention {
     const bytes = new Uint8Array(REC * caches.length);
     const dv = new DataView(bytes.buffer);
     caches.forEach(function (c, i) {
-      const need = c.numPages * c.pageSize * c.numKvHeads * c.headDim * (c.dtype === 'e4m3' ? 1 : 2);
+      const dtype = dtypeCode(KV_DTYPES, c.dtype || 'f16', 'paged cache ' + i);
+      const need = c.numPages * c.pageSize * c.numKvHeads * c.headDim * (dtype === KV_DTYPES.e4m3 ? 1 : 2);
       if (c.kPool.size < need || c.vPool.size < need) throw new RangeError('paged cache ' + i + ': pools too small');
       const o = i * REC;
       dv.setBigUint64(o, c.kPool.ptr, true);
       dv.setBigUint64(o + 8, c.vPool.ptr, true);
-      [c.numPages, c.pageSize, c.numKvHeads, c.headDim, c.dtype === 'e4m3' ? 1 : 0, 0].forEach(function (x, j) {
+      [c.numPages, c.pageSize, c.numKvHeads, c.headDim, dtype, 0].forEach(function (x, j) {
         dv.setUint32(o + 16 + 4 * j, x, true);
       });
     });
@@ -955,7 +964,7 @@ export class HipAttention {
     dv.setUint32(0, p.rows, true);
     dv.setUint32(4, p.vocab, true);
     dv.setBigUint64(8, BigInt(p.rowStride || 0), true);
-    dv.setUint32(16, LOGIT_DTYPES[p.dtype || 'f32'], true);
+    dv.setUint32(16, dtypeCode(LOGIT_DTYPES, p.dtype || 'f32', 'tokenLogprobs'), true);
     dv.setUint32(20, p.topK || 0, true);
     dv.setFloat32(24, p.cap || 0, true);
     dv.setFloat32(28, p.temperature === undefined ? 1.0 : p.temperature, true);
@@ -967,6 +976,7 @@ export class HipAttention {
   }
 
   tokenLogprobs(p: TokenLogprobs, workspace: DeviceBuffer): void {
+    const params = HipAttention.tokenLogprobsParams(p);
     const k = p.topK || 0;
     const need: [DeviceBuffer | undefined, number, string][] = [
       [p.logits, p.rows ? ((p.rows - 1) * (p.rowStride || p.vocab) + p.vocab) * LOGIT_BYTES[p.dtype || 'f32'] : 0, 'logits'],
@@ -974,7 +984,6 @@ export class HipAttention {
       [p.topIds, p.rows * k * 4, 'topIds'], [p.topLogprobs, p.rows * k * 4, 'topLogprobs']];
     for (const n of need) if (n[0] && n[0].size < n[1]) throw new RangeError('tokenLogprobs: ' + n[2] + ' too small');
     function ptr(b: DeviceBuffer | undefined): bigint | null { return b ? b.ptr : null; }
-    const params = HipAttention.tokenLogprobsParams(p);
     const slot = this.beginPass(PASS_LABELS.tokenLogprobs);
     try {
       this.g4.tokenLogprobs(p.logits.ptr, ptr(p.tokens), ptr(p.logprobs), ptr(p.entropy), ptr(p.topIds), ptr(p.topLogprobs),

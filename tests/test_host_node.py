@@ -73,3 +73,32 @@ def test_host_cpu_checks():
     assert r.returncode == 0, r.stderr
     res = json.loads(r.stdout.strip().splitlines()[-1])
     assert res["ok"] and "uniform layout" in res["checks"]
+
+
+def test_names_of_types_that_are_none_are_refused():
+    """The sources run with their types erased: a name that is no type passed the size checks and was taken for f32 logits
+    (of a buffer half that long) or f16 rows."""
+    script = (
+        "require('./gemma4-webgpu_amd/host/ts_register').register();"
+        "const {HipAttention} = require('./gemma4-webgpu_amd/host/attention.ts');"
+        "const buf = (size) => ({ptr: BigInt(4096), size});"
+        "const out = [];"
+        "const tried = (f) => { try { f(); out.push('taken'); } catch (e) { out.push(String(e.message)); } };"
+        "const cache = {kPool: buf(1 << 20), vPool: buf(1 << 20), numPages: 4, pageSize: 32, numKvHeads: 1, headDim: 256};"
+        "for (const dtype of ['fp8', 'bf16', 'F16', 'constructor']) {"
+        "  tried(() => HipAttention.pagedCacheBytes([Object.assign({dtype}, cache)]));"
+        "  tried(() => HipAttention.tokenLogprobsParams({logits: buf(2000), rows: 1, vocab: 1000,"
+        "    dtype: dtype === 'bf16' ? 'bfloat16' : dtype}));"
+        "  const self = {g4: {tokenLogprobs: () => {}}, beginPass: () => 0, endPass: () => {}};"
+        "  tried(() => HipAttention.prototype.tokenLogprobs.call(self, {logits: buf(2000), rows: 1, vocab: 1000,"
+        "    dtype: dtype === 'bf16' ? 'bfloat16' : dtype}, buf(1 << 20)));"
+        "}"
+        "for (const dtype of [undefined, 'f16', 'e4m3']) HipAttention.pagedCacheBytes([Object.assign({}, cache, {dtype})]);"
+        "for (const dtype of [undefined, 'f32', 'f16', 'bf16'])"
+        "  HipAttention.tokenLogprobsParams({logits: buf(4000), rows: 1, vocab: 1000, dtype});"
+        "console.log(JSON.stringify(out));"
+    )
+    r = run_node("-e", script)
+    assert r.returncode == 0, r.stderr
+    out = json.loads(r.stdout)
+    assert len(out) == 12 and all("dtype" in msg and "expected f" in msg for msg in out), out
