@@ -1429,7 +1429,7 @@ int g4_paged_attn(const g4_paged_cache* cache, const g4_paged_batch* batch, cons
     a.part_ml = a.part_o + (size_t)2 * plan.wgs * plan.mq * cache->head_dim;
     a.nkh = cache->num_kv_heads;
     a.group = p->num_q_heads / cache->num_kv_heads;
-    a.window = p->sliding_window > (1u << 30) ? 0 : (int32_t)p->sliding_window;  // positions are below 2^31 - 2^30
+    a.window = p->sliding_window > 0x7fffffffu ? 0 : (int32_t)p->sliding_window;  // no position is further on
     a.q_tiles = (uint32_t)plan.q_tiles;
     a.qscale = p->scale * kLog2e;
     a.cap_scale = p->softcap > 0.0f ? p->scale / p->softcap : 0.0f;

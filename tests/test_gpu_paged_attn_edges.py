@@ -131,3 +131,11 @@ def test_work_on_a_windowed_chunk_grows_with_its_length(dev):
         took.append(best)
     print(f"4096 tokens {1e3 * took[0]:.0f} us, 16384 tokens {1e3 * took[1]:.0f} us", flush=True)
     assert took[1] < 8 * took[0], took
+
+
+@pytest.mark.parametrize("window", [2 ** 30, 2 ** 30 + 1, 2 ** 31 - 3, 2 ** 31 - 1, 2 ** 31, 2 ** 32 - 1])
+def test_windows_and_positions_up_to_the_largest(dev, window):
+    """A position of 2^31 - 2 leaves rows behind for every window that is shorter."""
+    announce(f"pagedAttn far position window={window}")
+    far = 2 ** 31 - 2
+    run(Paged(dev, 5, [40, 33], [2, 20], page=16, positions=[far - 1, far] + [far - 19 + j for j in range(20)]), window=window)
