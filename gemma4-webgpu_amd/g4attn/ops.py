@@ -750,8 +750,8 @@ class PagedBatch:
             raise ValueError(f"n_tokens {n_tokens}, max_tokens {max_tokens}")
         words = 0
         if tree_mask is not None:
-            if tree_mask.dim() != 2:
-                raise ValueError("tree_mask: expected [n_tokens, words]")
+            if tree_mask.dim() != 2 or tree_mask.shape[1] == 0:  # an empty tensor's pointer would mean no mask: a chain
+                raise ValueError(f"tree_mask: shape {tuple(tree_mask.shape)}, expected [n_tokens, words]")
             words = int(tree_mask.shape[1])
         self.device = dev = block_table.get_device()
         self.tensors = (block_table, token_start, ctx_lens, positions, tree_mask)

@@ -139,3 +139,11 @@ def test_windows_and_positions_up_to_the_largest(dev, window):
     announce(f"pagedAttn far position window={window}")
     far = 2 ** 31 - 2
     run(Paged(dev, 5, [40, 33], [2, 20], page=16, positions=[far - 1, far] + [far - 19 + j for j in range(20)]), window=window)
+
+
+def test_a_mask_of_no_words_is_refused(dev):
+    """Its pointer is NULL, which stands for a chain: each token would attend those before it."""
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device=dev)  # noqa: E731
+    for shape in ((3, 0), (3,)):
+        with pytest.raises(ValueError, match="tree_mask"):
+            ops.PagedBatch(i32([0]), i32(0, 3), i32(0), 3, tree_mask=torch.zeros(shape, dtype=torch.int64, device=dev))
