@@ -1,13 +1,13 @@
 """g4_paged_attn at edges of its tiles, windows and number formats: chains that run past the block table, weights far
-below the largest, chunks of several windows, against the definition in 64 bits. Tolerances are derived in
-paged_helpers.Paged.expected, or where a test stands."""
+below the largest, chunks of several windows, shares of hundreds of tiles, mixed batches, against the definition in 64 bits. Tolerances
+are derived in paged_helpers.Paged.expected, or where a test stands."""
 import numpy as np
 import pytest
 import torch
 
 from conftest import announce
 from g4attn import ops
-from paged_helpers import Paged
+from paged_helpers import Paged, normed
 
 pytestmark = pytest.mark.gpu
 
@@ -147,3 +147,71 @@ def test_a_mask_of_no_words_is_refused(dev):
     for shape in ((3, 0), (3,)):
         with pytest.raises(ValueError, match="tree_mask"):
             ops.PagedBatch(i32([0]), i32(0, 3), i32(0), 3, tree_mask=torch.zeros(shape, dtype=torch.int64, device=dev))
+
+
+# ---- long shares ------------------------------------------------------------------------
+
+@pytest.mark.parametrize("hd,new,kv", [(256, 1, "f16"), (512, 1, "e4m3"), (256, 4, "e4m3"), (256, 8, "f16"), (256, 16, "f16"),
+                                       (512, 8, "f16")])
+def test_workgroups_that_read_page_ids_several_times(dev, hd, new, kv):
+    """Five sequences of 524288 rows, 320 tiles of 32 rows a workgroup: page ids are held for 64 of a wave's tiles. All
+    rows lie in 64 pages, so the definition is a sum over 1024 rows and how often a sequence names them. A page's V has
+    an offset of its own, and the pages change every few tiles, so that ids of other tiles would show."""
+    announce(f"pagedAttn long shares hd={hd} new={new} kv={kv}")
+    r = np.random.default_rng(hd + new)
+    seqs, rows, page, pages, nqh = 5, 524288, 16, 64, 8
+    dt = torch.float8_e4m3fn if kv == "e4m3" else torch.float16
+    k = torch.from_numpy(normed(r.standard_normal((pages, page, 1, hd)), 0.125)).to(dt)
+    v = torch.from_numpy(normed(r.standard_normal((pages, page, 1, hd))) + r.choice([-1.0, 1.0], (pages, 1, 1, 1))).to(dt)
+    # 11 pages of rows (176 rows, no multiple of a tile) from a page on, then from another.
+    i = np.arange(rows // page)
+    table = np.stack([(r.integers(0, pages, len(i))[i // 11] + i % 3) % pages for _ in range(seqs)]).astype(np.int32)
+    q = normed(r.standard_normal((seqs * new, nqh, hd))).astype(np.float16)
+    i32 = lambda a: torch.from_numpy(np.ascontiguousarray(a, np.int32)).to(dev)  # noqa: E731
+    cache = ops.PagedCache(k.to(dev), v.to(dev))
+    batch = ops.PagedBatch(i32(table), i32(np.arange(seqs + 1) * new), i32(np.full(seqs, rows - new)), seqs * new,
+                           max_tokens=new)
+    out = torch.full((seqs * new, nqh, hd), -123.0, device=dev)
+    ws = torch.empty(ops.paged_attn_workspace_bytes(cache, batch, nqh), dtype=torch.uint8, device=dev)
+    ops.paged_attn(cache, batch, torch.from_numpy(q).to(dev), out, ws)
+    torch.cuda.synchronize()
+    got = out.cpu().double().numpy()
+    kk, vv = k.double().numpy().reshape(-1, hd), v.double().numpy().reshape(-1, hd)
+    for s in range(seqs):
+        at = table[s, np.arange(rows) // page].astype(np.int64) * page + np.arange(rows) % page
+        for j in range(new):
+            count = np.bincount(at[:rows - new + j + 1], minlength=pages * page)
+            x = q[s * new + j].astype(np.float64) @ kk.T
+            p = count * np.exp(x - x.max(-1, keepdims=True))
+            want = (p / p.sum(-1, keepdims=True)) @ vv
+            # As in Paged.expected, with the sums of 320 tiles at most (two products and four terms a tile) and of
+            # the records of 52 workgroups; the weights that two f16 leave out are below 2^-32 of the largest.
+            mag = (np.abs(q[s * new + j].astype(np.float64)) @ np.abs(kk).T).max()
+            ds = ((hd / 32 + 32) * mag + 8 * np.abs(x).max()) * 2.0 ** -24
+            bound = (2 * ds + 2.0 ** -22 + rows * 2.0 ** -32 + (6 * 320 + 64) * 2.0 ** -24) * 2 * np.abs(vv).max()
+            err = np.abs(got[s * new + j] - want).max()
+            assert err <= bound, f"sequence {s} token {j}: off by {err:.3e}, bound {bound:.3e}"
+
+
+@pytest.mark.parametrize("form", ["one call", "two calls"])
+def test_a_chunk_beside_single_tokens(dev, form):
+    """In one batch, or as two over the same token buffers: tokens of no sequence are left alone."""
+    announce(f"pagedAttn chunk and single tokens, {form}")
+    new = [150] + [1] * 20
+    p = Paged(dev, 31, [70] + [5 * i for i in range(20)], new, page=16).upload()
+    if form == "one call":
+        p.check(p.attn())
+        return
+    out = torch.full((p.tokens, p.nqh, p.hd), -123.0, device=dev)
+    whole = p.batch
+    parts = [ops.PagedBatch(p.d_table[a:b].contiguous(), p.d_start[a:b + 1].contiguous(), p.d_ctx[a:b].contiguous(), p.tokens,
+                            max_tokens=most) for a, b, most in ((0, 1, 150), (1, 21, 1))]
+    p.batch = parts[0]
+    p.attn(out=out)
+    torch.cuda.synchronize()
+    assert (out[150:] == -123.0).all()
+    p.batch = parts[1]
+    p.attn(out=out)
+    p.batch = whole
+    torch.cuda.synchronize()
+    p.check(out)
