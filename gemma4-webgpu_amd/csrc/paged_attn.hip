@@ -601,10 +601,8 @@ __device__ __forceinline__ float paged_inverse(float L) { return L > 0.0f ? 1.0f
 
 // Bound by the cache's bytes: the W waves of a workgroup take every W-th row tile of its share, each
 // with a tile's K and V in registers. With four waves (512 registers each) the next tile's K is
-// requested when the scores have used this one's, its V when the products have (two tiles ahead for e4m3 at
-// head_dim 512, whose tiles' work is long next to their bytes: 64 sequences of one token 134 -> 126 us; at 256 it
-// gives nothing); with eight (256 registers) a wave requests a tile at a time, and a short item, which one
-// workgroup has whole, takes half as many in turn.
+// requested when the scores have used this one's, its V when the products have; with eight (256 registers) a wave
+// requests a tile at a time, and a short item, which one workgroup has whole, takes half as many in turn.
 // Measured: 64 sequences of 1024 to 32768 rows, one token: f16 187 us, 6.1 TB/s; e4m3 106 us, 5.4 TB/s (both read 0.83
 // to 0.9 of what a plain read stream does, the rest are ~20 us at the two launches' ends); head_dim 512 f16 205 us,
 // 5.8 TB/s; one sequence of 400000 f16 rows 77 us, 5.3 TB/s; five tokens of four heads (20 query rows) and a
@@ -620,7 +618,6 @@ struct PagedFewSmem {
 template <int HD, int C, bool F8, int W>
 __global__ __launch_bounds__(64 * W, W / 4) void k_paged_few(const PagedAttnArgs a) {
     constexpr bool AHEAD = W == 4;
-    constexpr int S = AHEAD && F8 && HD == 512 ? 2 : 1;  // tiles in registers
     using D = PagedDims<HD, F8>;
     constexpr int MQ = 16 * C, UR = 32;
     __shared__ PagedFewSmem<HD, C, W> sm;
@@ -646,28 +643,26 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_paged_few(const PagedAttnArgs
         const uint32_t head_off = kvh * HD * D::ES;
         const int32_t* table = a.b.table + (uint64_t)s * a.b.table_stride;
 
-        // The wave's first tiles are requested before the query is read.
+        // The wave's first tile is requested before the query is read.
         PagedPages pages;
-        u32x4 kr[S][2][D::KP];
-        PagedV<HD, F8> vr[S];
-        PagedAt pa[S] = {};
-        auto load_k = [&](int i, const PagedAt& p) __attribute__((always_inline)) {  // i: a constant
-            paged_load_k<HD, F8>(a.k + p.half0, row_bytes, n, g, kr[i][0]);
-            paged_load_k<HD, F8>(a.k + p.half1, row_bytes, n, g, kr[i][1]);
+        u32x4 kr[2][D::KP];
+        PagedV<HD, F8> vr;
+        PagedAt pa{};
+        auto load_k = [&](const PagedAt& p) __attribute__((always_inline)) {
+            paged_load_k<HD, F8>(a.k + p.half0, row_bytes, n, g, kr[0]);
+            paged_load_k<HD, F8>(a.k + p.half1, row_bytes, n, g, kr[1]);
         };
-        auto load_v = [&](int i, const PagedAt& p) __attribute__((always_inline)) {
-            paged_load_v<HD, F8>(a.v + p.half0, a.v + p.half1, row_bytes, n, g, vr[i]);
+        auto load_v = [&](const PagedAt& p) __attribute__((always_inline)) {
+            paged_load_v<HD, F8>(a.v + p.half0, a.v + p.half1, row_bytes, n, g, vr);
         };
-        if ((unsigned)wave < seg) pages.load(a, table, sp.first + off + wave, W, sp.hi, lane);
-#pragma unroll
-        for (int i = 0; i < S; i++)
-            if (wave + i * W < seg) {
-                pa[i] = paged_at(a, pages, i, (sp.first + off + wave + i * W) * 32, row_bytes, head_off);
-                if constexpr (AHEAD) {
-                    load_k(i, pa[i]);
-                    load_v(i, pa[i]);
-                }
+        if ((unsigned)wave < seg) {
+            pages.load(a, table, sp.first + off + wave, W, sp.hi, lane);
+            pa = paged_at(a, pages, 0, (sp.first + off + wave) * 32, row_bytes, head_off);
+            if constexpr (AHEAD) {
+                load_k(pa);
+                load_v(pa);
             }
+        }
         if (again) __syncthreads();  // the last segment's combine has read sm
         again = true;
         for (int x = not_hoisted(threadIdx.x); x < C * D::NC * 64; x += 64 * W) {
@@ -695,11 +690,11 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_paged_few(const PagedAttnArgs
         // Rows that every column attends: committed, and above every window's start.
         const unsigned clear_lo = !a.window ? 0u : a.b.positions ? sq.ctx : (unsigned)max((int)(sq.ctx + sq.n) - a.window, 0);
 
-        auto tile = [&](int i, unsigned it, unsigned t) __attribute__((always_inline)) {  // i: a constant, the registers
+        for (unsigned it = 0, t = wave; t < seg; it++, t += W) {
             const unsigned kt0 = (sp.first + off + t) * 32;
             if constexpr (!AHEAD) {
-                load_k(i, pa[i]);
-                load_v(i, pa[i]);
+                load_k(pa);
+                load_v(pa);
             }
             f32x4 sc[1][C][2];
 #pragma unroll
@@ -708,7 +703,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_paged_few(const PagedAttnArgs
                 for (int h = 0; h < 2; h++) sc[0][c][h] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int ch = 0; ch < D::NC; ch++) {
-                const f16x8 k0 = paged_k_chunk<HD, F8>(kr[i][0], ch), k1 = paged_k_chunk<HD, F8>(kr[i][1], ch);
+                const f16x8 k0 = paged_k_chunk<HD, F8>(kr[0], ch), k1 = paged_k_chunk<HD, F8>(kr[1], ch);
 #pragma unroll
                 for (int c = 0; c < C; c++) {
                     const f16x8 qv = sm.q[c][ch][lane];
@@ -717,24 +712,24 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_paged_few(const PagedAttnArgs
                 }
             }
             // The next K into the registers just used (behind a masked tile's work: that needs some).
-            const bool more = t + S * W < seg;
+            const bool more = t + W < seg;
             PagedAt pn{};
             if (more) {
-                if (((it + S) & 63) == 0) pages.load(a, table, sp.first + off + t + S * W, W, sp.hi, lane);
-                pn = paged_at(a, pages, (it + S) & 63, kt0 + S * W * 32, row_bytes, head_off);
+                if (((it + 1) & 63) == 0) pages.load(a, table, sp.first + off + t + W, W, sp.hi, lane);
+                pn = paged_at(a, pages, (it + 1) & 63, kt0 + W * 32, row_bytes, head_off);
             }
-            const bool clear = kt0 >= clear_lo && kt0 + 32 <= sq.ctx && pa[i].ok0 && pa[i].ok1;
+            const bool clear = kt0 >= clear_lo && kt0 + 32 <= sq.ctx && pa.ok0 && pa.ok1;
             unsigned seen[1][C], dead = 0;
             if (!clear) {
-                cols.look(a, sq, sp.hi, kt0, g, pa[i].ok0, pa[i].ok1, seen[0], dead);
+                cols.look(a, sq, sp.hi, kt0, g, pa.ok0, pa.ok1, seen[0], dead);
 #pragma unroll
                 for (int t8 = 0; t8 < 8; t8++)
                     if (dead >> t8 & 1) {
 #pragma unroll
-                        for (int b = 0; b < D::VP; b++) vr[i][b][t8] = u32x4{0u, 0u, 0u, 0u};
+                        for (int b = 0; b < D::VP; b++) vr[b][t8] = u32x4{0u, 0u, 0u, 0u};
                     }
             }
-            if (AHEAD && clear && more) load_k(i, pn);
+            if (AHEAD && clear && more) load_k(pn);
             f16x8 hi[1][C], lo[1][C];
             const PagedTake how[1] = {clear ? kClear : kMasked};
             paged_softmax<HD, C, F8, 1>(a, sc, seen, how, m_run, l_run, acc, hi, lo);
@@ -743,11 +738,11 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_paged_few(const PagedAttnArgs
             uint32_t odd_rows = 0;
             if (!clear) {
 #pragma unroll
-                for (int b = 0; b < D::VP; b++) odd_rows |= paged_take_odd<F8>(vr[i][b]);
+                for (int b = 0; b < D::VP; b++) odd_rows |= paged_take_odd<F8>(vr[b]);
             }
 #pragma unroll
             for (int b = 0; b < D::VP; b++) {
-                paged_pv<HD, C, F8>(b, vr[i][b], hi[0], lo[0], acc);
+                paged_pv<HD, C, F8>(b, vr[b], hi[0], lo[0], acc);
                 if constexpr (HD == 512) __builtin_amdgcn_sched_barrier(0);  // block by block: registers
             }
             while (odd_rows) {
@@ -755,19 +750,14 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_paged_few(const PagedAttnArgs
                 odd_rows &= odd_rows - 1;
 #pragma unroll
                 for (int c = 0; c < C; c++)
-                    paged_add_odd<HD, F8>(a.v + (t8 < 4 ? pa[i].half0 : pa[i].half1) + (uint32_t)(4 * gg + (t8 & 3)) * row_bytes, g,
+                    paged_add_odd<HD, F8>(a.v + (t8 < 4 ? pa.half0 : pa.half1) + (uint32_t)(4 * gg + (t8 & 3)) * row_bytes, g,
                                           __shfl(seen[0][c], 16 * gg + n) >> t8 & 1, acc[c]);
             }
             if (AHEAD && more) {
-                if (!clear) load_k(i, pn);
-                load_v(i, pn);
+                if (!clear) load_k(pn);
+                load_v(pn);
             }
-            pa[i] = pn;
-        };
-        for (unsigned it = 0, t = wave; t < seg; it += S, t += S * W) {
-            tile(0, it, t);
-            if constexpr (S == 2)
-                if (t + W < seg) tile(1, it + 1, t + W);
+            pa = pn;
         }
 
         const bool whole = seg == sp.n;
