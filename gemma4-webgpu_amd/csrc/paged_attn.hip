@@ -35,7 +35,7 @@
 
 namespace g4 {
 
-constexpr int kPagedWaves = 4;  // of k_paged_few where items are cut
+constexpr int kPagedWaves = 4;  // of k_paged_few
 
 struct PagedAttnArgs {
     const uint16_t* __restrict__ q;
@@ -599,28 +599,28 @@ __device__ __forceinline__ float paged_inverse(float L) { return L > 0.0f ? 1.0f
 
 // ---- at most 32 query rows --------------------------------------------------------
 
-// Bound by the cache's bytes: the W waves of a workgroup take every W-th row tile of its share, each
-// with a tile's K and V in registers. With four waves (512 registers each) the next tile's K is
-// requested when the scores have used this one's, its V when the products have; with eight (256 registers) a wave
-// requests a tile at a time, and a short item, which one workgroup has whole, takes half as many in turn.
+// Bound by the cache's bytes: the four waves of a workgroup (512 registers each) take every fourth row tile of its
+// share, each with a tile's K and V in registers. The next tile's K is requested when the scores have used this one's,
+// its V when the products have. (Eight waves of 256 registers, a tile at a time, for short items that one workgroup has
+// whole: 512 sequences of 200 rows f16 31.1 against 29.5 us, e4m3 21.4 against 15.9.)
 // Measured: 64 sequences of 1024 to 32768 rows, one token: f16 187 us, 6.1 TB/s; e4m3 106 us, 5.4 TB/s (both read 0.83
 // to 0.9 of what a plain read stream does, the rest are ~20 us at the two launches' ends); head_dim 512 f16 205 us,
 // 5.8 TB/s; one sequence of 400000 f16 rows 77 us, 5.3 TB/s; five tokens of four heads (20 query rows) and a
 // softcap over three sequences of 100001 to 131072 e4m3 rows 77 us, 4.8 TB/s, where the work on a tile, 8000 cycles a
 // wave, is the bound: twice the tiles in flight gave nothing (86 us).
-template <int HD, int C, int W>
+template <int HD, int C>
 struct PagedFewSmem {
-    f16x8 q[C][HD / 32][64];      // score operand, lane-major
-    float o[W][HD / 16 * 4][64];  // one query group's outputs, per wave
-    float m[W][16 * C], l[W][16 * C];
+    f16x8 q[C][HD / 32][64];                // score operand, lane-major
+    float o[kPagedWaves][HD / 16 * 4][64];  // one query group's outputs, per wave
+    float m[kPagedWaves][16 * C], l[kPagedWaves][16 * C];
 };
 
-template <int HD, int C, bool F8, int W>
-__global__ __launch_bounds__(64 * W, W / 4) void k_paged_few(const PagedAttnArgs a) {
-    constexpr bool AHEAD = W == 4;
+template <int HD, int C, bool F8>
+__global__ __launch_bounds__(64 * kPagedWaves, 1) void k_paged_few(const PagedAttnArgs a) {
     using D = PagedDims<HD, F8>;
-    constexpr int MQ = 16 * C, UR = 32;
-    __shared__ PagedFewSmem<HD, C, W> sm;
+    constexpr int W = kPagedWaves, MQ = 16 * C, UR = 32;
+    static_assert(W == 4, "a wave a row of every four of an output tile");
+    __shared__ PagedFewSmem<HD, C> sm;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, g = lane >> 4;
@@ -658,10 +658,8 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_paged_few(const PagedAttnArgs
         if ((unsigned)wave < seg) {
             pages.load(a, table, sp.first + off + wave, W, sp.hi, lane);
             pa = paged_at(a, pages, 0, (sp.first + off + wave) * 32, row_bytes, head_off);
-            if constexpr (AHEAD) {
-                load_k(pa);
-                load_v(pa);
-            }
+            load_k(pa);
+            load_v(pa);
         }
         if (again) __syncthreads();  // the last segment's combine has read sm
         again = true;
@@ -692,10 +690,6 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_paged_few(const PagedAttnArgs
 
         for (unsigned it = 0, t = wave; t < seg; it++, t += W) {
             const unsigned kt0 = (sp.first + off + t) * 32;
-            if constexpr (!AHEAD) {
-                load_k(pa);
-                load_v(pa);
-            }
             f32x4 sc[1][C][2];
 #pragma unroll
             for (int c = 0; c < C; c++)
@@ -729,7 +723,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_paged_few(const PagedAttnArgs
                         for (int b = 0; b < D::VP; b++) vr[b][t8] = u32x4{0u, 0u, 0u, 0u};
                     }
             }
-            if (AHEAD && clear && more) load_k(pn);
+            if (clear && more) load_k(pn);
             f16x8 hi[1][C], lo[1][C];
             const PagedTake how[1] = {clear ? kClear : kMasked};
             paged_softmax<HD, C, F8, 1>(a, sc, seen, how, m_run, l_run, acc, hi, lo);
@@ -753,7 +747,7 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_paged_few(const PagedAttnArgs
                     paged_add_odd<HD, F8>(a.v + (t8 < 4 ? pa.half0 : pa.half1) + (uint32_t)(4 * gg + (t8 & 3)) * row_bytes, g,
                                           __shfl(seen[0][c], 16 * gg + n) >> t8 & 1, acc[c]);
             }
-            if (AHEAD && more) {
+            if (more) {
                 if (!clear) load_k(pn);
                 load_v(pn);
             }
@@ -829,23 +823,16 @@ __global__ __launch_bounds__(64 * W, W / 4) void k_paged_few(const PagedAttnArgs
                 float* dst = whole ? a.out + ((uint64_t)(sq.start + r / G) * (a.nkh * G) + kvh * G + r % G) * HD
                                    : a.part_o + ((uint64_t)slot * MQ + rec) * HD;
                 if (!whole && wave == 0 && eg == 0) stg<f32x2>(a.part_ml + ((uint64_t)slot * MQ + rec) * 2, f32x2{M, L});
-                // Of the 4 rows 4g + j of every output tile, j = wave % 4; eight waves share its elements too.
-                const int j = wave & 3;
-                constexpr int PART = D::E * 4 / W;
-                const int e0 = (wave >> 2) * PART;
+                const int j = wave;  // of the 4 rows 4g + j of every output tile
 #pragma unroll
                 for (int b = 0; b < D::VP; b++)
 #pragma unroll
-                    for (int e1 = 0; e1 < PART; e1 += 4) {
-                        const int e = e0 + e1;
+                    for (int e = 0; e < D::E; e += 4) {
                         f32x4 x;
 #pragma unroll
                         for (int y = 0; y < 4; y++) {
                             const int k = (b * D::E + e + y) * 4 + j;
-                            float sum = (sm.o[0][k][el] + sm.o[1][k][el]) + (sm.o[2][k][el] + sm.o[3][k][el]);
-                            if constexpr (W == 8)
-                                sum += (sm.o[4][k][el] + sm.o[5][k][el]) + (sm.o[6][k][el] + sm.o[7][k][el]);
-                            x[y] = sum * inv;
+                            x[y] = ((sm.o[0][k][el] + sm.o[1][k][el]) + (sm.o[2][k][el] + sm.o[3][k][el])) * inv;
                         }
                         stg<f32x4>(dst + 16 * D::E * b + D::E * (4 * eg + j) + e, x);
                     }
@@ -1309,8 +1296,7 @@ static PagedPlan paged_plan(unsigned head_dim, unsigned num_kv_heads, unsigned n
 // Whether every item goes to one workgroup: its rows are few for certain (by the window, or the block table's
 // size), and there are items for half the CUs or one tile a wave, so that cutting them and joining the parts in a
 // second launch would cost more. (512 sequences of 100 to 300 rows, whole / cut: 34 / 55 us; one token over a window
-// of 512, which this leaves to be cut: 16 / 11 us.) At head_dim 256 with eight waves, which have a tile each at
-// once: 34.3 us for the 512 sequences, 35.0 with four.
+// of 512, which this leaves to be cut: 16 / 11 us.)
 static bool paged_whole(uint64_t rows, uint64_t items, unsigned cus) {
     return rows <= 256 || (rows <= 2048 && 2 * items >= cus);
 }
@@ -1335,11 +1321,7 @@ template <int HD, bool F8>
 static void launch_paged(const PagedAttnArgs& a, const PagedPlan& p, hipStream_t st) {
     const dim3 grid(a.whole ? a.b.n_seqs * a.q_tiles * a.nkh : p.wgs);
     if (p.mq == 16) {
-        if (HD == 256 && a.whole) {
-            if constexpr (HD == 256) G4_LAUNCH((k_paged_few<256, 1, F8, 8>), grid, dim3(512), 0, st, a);
-        } else {
-            G4_LAUNCH((k_paged_few<HD, 1, F8, kPagedWaves>), grid, dim3(64 * kPagedWaves), 0, st, a);
-        }
+        G4_LAUNCH((k_paged_few<HD, 1, F8>), grid, dim3(64 * kPagedWaves), 0, st, a);
         launch_join<HD, 16, 32>(a, st);
     } else if constexpr (HD == 512) {
         constexpr int TS = F8 ? 2 : 1;
@@ -1349,7 +1331,7 @@ static void launch_paged(const PagedAttnArgs& a, const PagedPlan& p, hipStream_t
             G4_LAUNCH((k_paged_tile<512, 4, 1, 2, TS, 4, F8, false>), grid, dim3(512), 0, st, a);
         launch_join<HD, 64, 32 * TS>(a, st);
     } else if (p.mq == 32) {
-        G4_LAUNCH((k_paged_few<256, 2, F8, kPagedWaves>), grid, dim3(64 * kPagedWaves), 0, st, a);
+        G4_LAUNCH((k_paged_few<256, 2, F8>), grid, dim3(64 * kPagedWaves), 0, st, a);
         launch_join<HD, 32, 32>(a, st);
     } else if (p.mq == 64) {
         G4_LAUNCH((k_paged_tile<256, 4, 2, 1, 2, F8 ? 10 : 5, F8, true>), grid, dim3(512), 0, st, a);
