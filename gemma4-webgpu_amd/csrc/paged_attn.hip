@@ -1294,11 +1294,14 @@ static PagedPlan paged_plan(unsigned head_dim, unsigned num_kv_heads, unsigned n
 }
 
 // Whether every item goes to one workgroup: its rows are few for certain (by the window, or the block table's
-// size), and there are items for half the CUs or one tile a wave, so that cutting them and joining the parts in a
-// second launch would cost more. (512 sequences of 100 to 300 rows, whole / cut: 34 / 55 us; one token over a window
-// of 512, which this leaves to be cut: 16 / 11 us.)
+// size), and there are items for the CUs, or for half of them and half as many rows, or one tile or two a wave, so
+// that cutting them and joining the parts in a second launch would cost more. (One token, f16, whole / cut: 512
+// sequences of 200 rows 30 / 39 us, 256 of a window of 1024 50 / 55, of 200 to 1500 rows 55 / 57; 128 of a window of 512
+// 26 / 28, of 1024 43 / 37 but e4m3 27 / 29, four tokens 47 / 49, eight 51 / 56; of 200 to 1500 rows 49 / 34, e4m3 31 / 28,
+// four tokens 38 / 43; one sequence over a window of 512 16 / 11, of 1024 31 / 11.)
 static bool paged_whole(uint64_t rows, uint64_t items, unsigned cus) {
-    return rows <= 256 || (rows <= 2048 && 2 * items >= cus);
+    if (items >= cus) return rows <= 2048;
+    return rows <= (2 * items >= cus ? 1088 : 256);
 }
 
 // How the records are joined: few an item, its thread's rows in turn; many, in 16 groups, or in 4 where an item's
