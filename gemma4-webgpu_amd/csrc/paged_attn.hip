@@ -24,12 +24,14 @@
 //
 // Work split: a (sequence, tile of query rows, kv head) is an item of ceil(rows / 32)
 // row tiles; all items' tiles in order are cut into equal shares, one a workgroup,
-// whatever the lengths, so a ragged batch fills the chip and one long sequence does
+// whatever the rows, so a ragged batch fills the chip and one long sequence does
 // too; few items are cut each by itself (PagedPieces), and short ones not at all
 // (paged_whole). Lengths are read on the device (a captured launch serves the next
 // step's), every workgroup finds its share by a scan over the items. An item cut
 // between workgroups leaves (m, l, o) records that a second launch joins in a fixed
-// order.
+// order. The host knows the longest sequence's new tokens alone, so every sequence
+// has that many query tiles in the scan and in the join's grid: one chunk of 1024
+// tokens beside 63 single ones (4096 rows each) takes 395 us, as two calls 157.
 #include "decode_core.h"
 #include "paged.h"
 
@@ -446,7 +448,7 @@ struct PagedCols {
                 s = in0 | in1 << 4;
                 s |= (bits_from(word[c], row0 - ctx) & ~in0) | (bits_from(word[c], row1 - ctx) & ~in1) << 4;
             } else {
-                const int end = ctx + (int)j[c] + 1;  // past a column that is none: below 0
+                const int end = ctx + (int)j[c] + 1;  // ctx for a column that is none, which the last line clears
                 s = rows_below(end - row0) | rows_below(end - row1) << 4;
             }
             if (a.window) {
@@ -603,11 +605,11 @@ __device__ __forceinline__ float paged_inverse(float L) { return L > 0.0f ? 1.0f
 // share, each with a tile's K and V in registers. The next tile's K is requested when the scores have used this one's,
 // its V when the products have. (Eight waves of 256 registers, a tile at a time, for short items that one workgroup has
 // whole: 512 sequences of 200 rows f16 31.1 against 29.5 us, e4m3 21.4 against 15.9.)
-// Measured: 64 sequences of 1024 to 32768 rows, one token: f16 187 us, 6.1 TB/s; e4m3 106 us, 5.4 TB/s (both read 0.83
-// to 0.9 of what a plain read stream does, the rest are ~20 us at the two launches' ends); head_dim 512 f16 205 us,
-// 5.8 TB/s; one sequence of 400000 f16 rows 77 us, 5.3 TB/s; five tokens of four heads (20 query rows) and a
-// softcap over three sequences of 100001 to 131072 e4m3 rows 77 us, 4.8 TB/s, where the work on a tile, 8000 cycles a
-// wave, is the bound: twice the tiles in flight gave nothing (86 us).
+// Measured: 64 sequences of 1024 to 32768 rows, one token: f16 183 us, 6.3 TB/s; e4m3 104 us, 5.5 TB/s (both read 0.83
+// to 0.9 of what a plain read stream does, the rest are ~20 us at the two launches' ends); head_dim 512 f16 364 us,
+// 6.3 TB/s, e4m3 194 us, 5.9 TB/s (201 with two tiles ahead); one sequence of 400000 f16 rows 75 us, 5.5 TB/s; five
+// tokens of four heads (20 query rows) and a softcap over three sequences of 100001 to 131072 e4m3 rows 75 us, 4.9 TB/s,
+// where the work on a tile, 8000 cycles a wave, is the bound: twice the tiles in flight gave nothing (86 us).
 template <int HD, int C>
 struct PagedFewSmem {
     f16x8 q[C][HD / 32][64];                // score operand, lane-major
@@ -852,9 +854,9 @@ __global__ __launch_bounds__(64 * kPagedWaves, 1) void k_paged_few(const PagedAt
 // the next tile and so on, NS - 1 requested ahead; one barrier a slot. A row's 16-byte pieces are stored at
 // piece ^ (row % 16), which spreads both operands' reads over all banks (sixteen lanes read sixteen rows of K, or
 // sixteen pieces of one row of V). NT: the rows are read by one workgroup alone and bypass the caches (64
-// sequences of 8 tokens, pages of 1024, 223 us, without 238).
+// sequences of 8 tokens, pages of 1024, 214 us, without 231).
 //
-// Measured: 1024 tokens of 8 heads over 7001 rows 138 us, 456 TFLOP/s (0.68 PFLOP/s with the two products of P). A
+// Measured: 1024 tokens of 8 heads over 7001 rows 139 us, 452 TFLOP/s (0.68 PFLOP/s with the two products of P). A
 // tile of 128 query rows and 64 cache rows takes 8600 cycles: 4400 of reading K and V from LDS (128 bytes a
 // cycle; each wave reads them whole), of MFMA 3100 beside it, 1150 of softmax, and the rest are the barriers'
 // skew and the DMA's issue. 32 query rows a wave would halve the LDS reads, but one wave a SIMD overlaps
@@ -1280,9 +1282,9 @@ struct PagedPlan {
     uint64_t q_tiles;  // of a sequence and kv head, at most
     size_t bytes;
 };
-// Query rows of a tile: 32 (K and V in registers) against a tile of 64 (through LDS), 64 sequences of 4 tokens, e4m3: 142
-// and 192 us; 64 against 128, 64 sequences of 8 tokens: 223 and 250 us; 128 against 64, 1024 tokens over 7001 rows: 137 and
-// 175 us. At head_dim 512 the registers hold no more than 16 and 64.
+// Query rows of a tile: 32 (K and V in registers) against a tile of 64 (through LDS), 64 sequences of 4 tokens, e4m3: 122
+// and 170 us (f16 195 and 191); 64 against 128, 64 sequences of 8 tokens: 214 and 242 us; 128 against 64, 1024 tokens over
+// 7001 rows: 137 and 175 us. At head_dim 512 the registers hold no more than 16 and 64.
 static PagedPlan paged_plan(unsigned head_dim, unsigned num_kv_heads, unsigned num_q_heads, const PagedBatchDev& b) {
     PagedPlan p;
     const uint64_t rows = (uint64_t)b.max_tokens * (num_q_heads / num_kv_heads);

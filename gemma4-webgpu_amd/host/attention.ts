@@ -294,7 +294,7 @@ export interface PagedBatch {
   nSeqs: number;
   tableStride: number;
   nTokens: number;            // of the token buffers, padding included
-  maxTokens: number;          // at least the longest sequence's new tokens
+  maxTokens: number;          // at least the longest sequence's new tokens; no more where time counts
   maskWords?: number;         // with treeMask: at least ceil(maxTokens / 64)
 }
 

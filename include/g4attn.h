@@ -766,7 +766,10 @@ typedef struct g4_paged_batch {
     uint32_t n_seqs;            /* 1 .. 65535 */
     uint32_t table_stride;      /* pages a sequence can name; table_stride * page_size <= 2^30 */
     uint32_t n_tokens;          /* tokens of the batch's buffers (padding included), at most 2^22 */
-    uint32_t max_tokens;        /* at least the longest sequence's new tokens */
+    uint32_t max_tokens;        /* at least the longest sequence's new tokens; no more, and alike lengths, where time
+                                   counts: the attention plans as many for every sequence. A long chunk beside many
+                                   single tokens is faster as two batches over the same token buffers (the other's
+                                   tokens are padding to each) */
     uint32_t mask_words;        /* with tree_mask: at least ceil(max_tokens / 64) */
     uint32_t reserved;          /* 0 */
 } g4_paged_batch;
@@ -793,11 +796,14 @@ int g4_paged_append(const g4_paged_cache* cache, const g4_paged_batch* batch, co
 
 /* Attention of every new token over its sequence's rows: committed rows and the
  * new tokens' rows its mask names (stored before, by g4_paged_append), all
- * limited to positions above its own minus sliding_window (0: no limit).
+ * limited to positions above its own minus sliding_window (0, or 2^31 and above: no limit).
  * score = scale * q . k, then softcap * tanh(score / softcap) where softcap > 0;
  * softmax and products in f32 (the probabilities enter the matrix products as the
- * sum of two f16). A token that attends nothing gets 0; rows that a token does
- * not attend do not reach it, whatever they hold. q: f16 [n_tokens][num_q_heads]
+ * sum of two f16: off by 2^-24 of themselves, or by 2^-32 of the token's largest
+ * one where that is more). A token that attends nothing gets 0; rows that a token
+ * does not attend do not reach it, whatever they hold. Rows that it attends are
+ * taken to be finite, as normed ones are: an Inf or NaN among them reaches its
+ * outputs as one of the two, not always the definition's. q: f16 [n_tokens][num_q_heads]
  * [head_dim]; out: f32, the same shape, 16-byte aligned; num_q_heads up to 8 times
  * num_kv_heads. The workspace (g4_paged_attn_workspace_size: it depends on the
  * head layout, head_dim and max_tokens alone) holds partial results within
@@ -833,7 +839,8 @@ int g4_paged_commit(const g4_paged_cache* caches, uint32_t n_caches, const g4_pa
  * lse = log(sum exp(z)); logprob = z[token] - lse of the given token; entropy =
  * lse - sum p z; and the top_k logits' indices with their log probabilities,
  * by descending logit, equal logits (cap and temperature aside) by ascending
- * index. A token outside [0, vocab) gets logprob 0 (padding). Logits of -inf
+ * index. z is off by a few 2^-24 of itself, with a cap up to 64 of the cap.
+ * A token outside [0, vocab) gets logprob 0 (padding). Logits of -inf
  * have probability 0 and are never among the top; where fewer than top_k logits
  * are above -inf, the rest have id -1 and logprob -inf. A row with a NaN or
  * +inf logit, or with -inf alone, has NaN as logprob, entropy and top_logprobs
