@@ -1,0 +1,69 @@
+// Types of a served batch's rows (rownorm.hip, linear8.hip, lora.hip) and the
+// checks that their entry points share.
+#pragma once
+
+#include "common.h"
+
+namespace g4 {
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef int32_t i32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+constexpr uint32_t kMaxRows = 1u << 22;  // tokens of a batch's buffers
+
+inline uint32_t type_bytes(uint32_t type) { return type == G4_F32 ? 4 : type == G4_E4M3 ? 1 : 2; }
+inline bool aligned(const void* p, uint64_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+
+__device__ __forceinline__ uint16_t f2bf(float x) { return __builtin_bit_cast(uint16_t, static_cast<__bf16>(x)); }
+__device__ __forceinline__ float bf2f(uint16_t x) { return __uint_as_float((uint32_t)x << 16); }
+
+// Two f32 as e4m3, nearest even, in the low half; values past 448 become 448 (the conversion alone makes them NaN).
+__device__ __forceinline__ uint32_t e4m3_pair(float x, float y) {
+    x = __builtin_amdgcn_fmed3f(x, -448.0f, 448.0f);
+    y = __builtin_amdgcn_fmed3f(y, -448.0f, 448.0f);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x, y, 0, false) & 0xFFFFu;
+}
+
+// Four outputs of a row in the row's type: one store where the row allows it, else one each of those below `left`.
+__device__ __forceinline__ void store4(void* out, uint32_t type, uint64_t at, f32x4 v, bool wide, unsigned left) {
+    if (type == G4_F32) {
+        float* o = static_cast<float*>(out) + at;
+        if (wide && left >= 4) stg<f32x4>(o, v);
+        else
+            for (unsigned i = 0; i < 4; i++)
+                if (i < left) stg<float>(o + i, v[i]);
+        return;
+    }
+    u16x4 h;
+#pragma unroll
+    for (int i = 0; i < 4; i++) h[i] = type == G4_F16 ? f2h(v[i]) : f2bf(v[i]);
+    uint16_t* o = static_cast<uint16_t*>(out) + at;
+    if (wide && left >= 4) stg<u16x4>(o, h);
+    else
+        for (unsigned i = 0; i < 4; i++)
+            if (i < left) stg<uint16_t>(o + i, h[i]);
+}
+__device__ __forceinline__ f32x4 load4(const void* in, uint32_t type, uint64_t at, bool wide, unsigned left) {
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (type == G4_F32) {
+        const float* p = static_cast<const float*>(in) + at;
+        if (wide && left >= 4) return ldg<f32x4>(p);
+        for (unsigned i = 0; i < 4; i++)
+            if (i < left) v[i] = ldg<float>(p + i);
+        return v;
+    }
+    const uint16_t* p = static_cast<const uint16_t*>(in) + at;
+    u16x4 h = {0, 0, 0, 0};
+    if (wide && left >= 4) h = ldg<u16x4>(p);
+    else
+        for (unsigned i = 0; i < 4; i++)
+            if (i < left) h[i] = ldg<uint16_t>(p + i);
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = type == G4_F16 ? h2f(h[i]) : bf2f(h[i]);
+    return v;
+}
+
+}  // namespace g4

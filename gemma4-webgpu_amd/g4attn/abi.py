@@ -171,6 +171,37 @@ class TokenLogprobsParams(C.Structure):
                 ("top_k", C.c_uint32), ("cap", C.c_float), ("temperature", C.c_float)]
 
 
+G4_F32, G4_F16, G4_BF16, G4_E4M3 = 0, 1, 2, 3
+
+
+class AddRmsNormParams(C.Structure):
+    _fields_ = [("rows", C.c_uint32), ("n", C.c_uint32), ("x_type", C.c_uint32), ("residual_type", C.c_uint32),
+                ("weight_type", C.c_uint32), ("out_type", C.c_uint32), ("eps", C.c_float), ("reserved", C.c_uint32),
+                ("x_stride", C.c_uint64), ("residual_stride", C.c_uint64), ("residual_out_stride", C.c_uint64),
+                ("out_stride", C.c_uint64)]
+
+
+class QuantizeRowsParams(C.Structure):
+    _fields_ = [("rows", C.c_uint32), ("n", C.c_uint32), ("x_type", C.c_uint32), ("reserved", C.c_uint32),
+                ("x_stride", C.c_uint64), ("out_stride", C.c_uint64)]
+
+
+class Lora(C.Structure):
+    _fields_ = [("a", C.c_void_p), ("b", C.c_void_p), ("scales", C.c_void_p), ("n_adapters", C.c_uint32),
+                ("rank", C.c_uint32), ("n", C.c_uint32), ("n_segs", C.c_uint32), ("widths", C.c_uint32 * 4),
+                ("type", C.c_uint32), ("reserved", C.c_uint32)]
+
+
+class LinearE4m3Params(C.Structure):
+    _fields_ = [("n_tokens", C.c_uint32), ("rows", C.c_uint32), ("n", C.c_uint32), ("out_type", C.c_uint32),
+                ("x_stride", C.c_uint64), ("out_stride", C.c_uint64)]
+
+
+class LoraAddParams(C.Structure):
+    _fields_ = [("n_tokens", C.c_uint32), ("x_type", C.c_uint32), ("out_type", C.c_uint32), ("reserved", C.c_uint32),
+                ("x_stride", C.c_uint64), ("base_stride", C.c_uint64), ("out_stride", C.c_uint64)]
+
+
 _P = C.c_void_p
 _U32 = C.c_uint32
 _SZ = C.c_size_t
@@ -260,6 +291,12 @@ SIGNATURES: dict[str, list] = {
     "g4_paged_commit": [C.POINTER(PagedCache), _U32, C.POINTER(PagedBatch), _P, _U32, _P, _P, _P],
     "g4_token_logprobs_workspace_size": [C.POINTER(TokenLogprobsParams), C.POINTER(C.c_size_t)],
     "g4_token_logprobs": [_P, _P, _P, _P, _P, _P, C.POINTER(TokenLogprobsParams), _P, _SZ, _P],
+    "g4_add_rms_norm": [_P, _P, _P, _P, _P, _P, _P, C.POINTER(AddRmsNormParams), _P],
+    "g4_quantize_rows": [_P, _P, _P, C.POINTER(QuantizeRowsParams), _P],
+    "g4_linear_e4m3_workspace_size": [C.POINTER(LinearE4m3Params), C.POINTER(Lora), C.POINTER(C.c_size_t)],
+    "g4_linear_e4m3": [_P, _P, _P, _P, C.POINTER(Lora), _P, _P, C.POINTER(LinearE4m3Params), _P, _SZ, _P],
+    "g4_lora_workspace_size": [C.POINTER(Lora), _U32, C.POINTER(C.c_size_t)],
+    "g4_lora_add": [C.POINTER(Lora), _P, _P, _P, _P, _P, C.POINTER(LoraAddParams), _P, _SZ, _P],
 }
 STRING_FUNCS = ("g4_last_error", "g4_version")
 

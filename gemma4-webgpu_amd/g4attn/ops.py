@@ -923,3 +923,179 @@ def token_logprobs(logits, tokens, logprobs, entropy, workspace, top_ids=None, t
              abi.TokenLogprobsParams(rows, vocab, logits.stride(0) if rows > 1 else 0, LOGIT_TYPES[logits.dtype], k, cap,
                                      temperature),
              _at(workspace, "workspace", torch.uint8, 0, dev), workspace.numel(), _stream(stream))
+
+
+# ---- between two attention blocks of a served batch -----------------------------------
+
+ROW_TYPES = {torch.float32: abi.G4_F32, torch.float16: abi.G4_F16, torch.bfloat16: abi.G4_BF16,
+             torch.float8_e4m3fn: abi.G4_E4M3}
+_WIDE_TYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _rows_of(t, name, types, device, shape=None):
+    """A [rows, n] tensor whose rows may lie apart: (pointer, type, elements from row to row)."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a tensor")
+    if t.get_device() != device or not t.is_cuda:
+        raise ValueError(f"{name}: must be on the GPU cuda:{device}, got {t.device}")
+    if t.dtype not in types:
+        raise TypeError(f"{name}: dtype {t.dtype} not in {types}")
+    if t.dim() != 2 or shape is not None and t.shape != shape:
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {'[rows, n]' if shape is None else tuple(shape)}")
+    if t.is_contiguous():
+        return t.data_ptr(), ROW_TYPES[t.dtype], 0
+    rows, n = t.shape
+    if n > 1 and t.stride(1) != 1 or rows > 1 and t.stride(0) < n:
+        raise ValueError(f"{name}: a row's elements must be contiguous, and rows apart")
+    return t.data_ptr(), ROW_TYPES[t.dtype], t.stride(0) if rows > 1 else 0
+
+
+def _device_of(t, name):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name}: must be on the GPU, got {t.device}")
+    return _call_device(t.get_device())
+
+
+def _norm_weight(t, name, n, device):
+    """A norm's weights: f32, bf16 or f16 (or its bits, as the other norms take them)."""
+    kind = torch.float16 if t.dtype in F16_TYPES else t.dtype
+    if kind not in _WIDE_TYPES:
+        raise TypeError(f"{name}: dtype {t.dtype} not in {_WIDE_TYPES}")
+    if t.numel() != n:
+        raise ValueError(f"{name}: {t.numel()} elements, expected {n}")
+    return _at(t, name, kind, n, device), ROW_TYPES[kind]
+
+
+def add_rms_norm(x, weight, out, scales=None, residual=None, residual_out=None, post_weight=None, eps=1e-6, stream=None):
+    """The residual's addition and the norm of a batch's rows (g4_add_rms_norm). x: [rows, n], f32, f16 or bf16;
+    residual and residual_out: one type of those three; post_weight: of the branch's own norm, before the addition; weight
+    (None: a norm without) and out, any of those types or float8_e4m3fn with scales f32 [rows]; out None: only the
+    addition. Rows may lie apart; residual_out may be residual."""
+    dev = _device_of(x, "x")
+    xp, xt, xs = _rows_of(x, "x", _WIDE_TYPES, dev)
+    rows, n = x.shape
+    rp, rt, rs, sp, ss = None, None, 0, None, 0
+    if residual is not None:
+        rp, rt, rs = _rows_of(residual, "residual", _WIDE_TYPES, dev, x.shape)
+    if residual_out is not None:
+        sp, st, ss = _rows_of(residual_out, "residual_out", _WIDE_TYPES, dev, x.shape)
+        if rt is not None and st != rt:
+            raise TypeError(f"residual_out: dtype {residual_out.dtype}, residual's is {residual.dtype}")
+        rt = st
+    op, ot, os_ = (None, xt, 0) if out is None else _rows_of(out, "out", tuple(ROW_TYPES), dev, x.shape)
+    pp = wp = wt = None
+    if post_weight is not None:
+        pp, wt = _norm_weight(post_weight, "post_weight", n, dev)
+    if weight is not None:
+        wp, kind = _norm_weight(weight, "weight", n, dev)
+        if wt is not None and kind != wt:
+            raise TypeError(f"weight: dtype {weight.dtype}, post_weight's is {post_weight.dtype}")
+        wt = kind
+    cp = None if scales is None else _at(scales, "scales", torch.float32, rows, dev)
+    if rows == 0:
+        return
+    abi.call("g4_add_rms_norm", xp, rp, pp, wp, sp, op, cp,
+             abi.AddRmsNormParams(rows, n, xt, xt if rt is None else rt, wt or 0, ot, eps, 0, xs, rs, ss, os_), _stream(stream))
+
+
+def quantize_rows(x, out, scales, stream=None):
+    """Rows in 8 bits (g4_quantize_rows). x: [rows, n], f32, f16 or bf16; out: float8_e4m3fn, the same shape; scales: f32
+    [rows]. Rows may lie apart."""
+    dev = _device_of(x, "x")
+    xp, xt, xs = _rows_of(x, "x", _WIDE_TYPES, dev)
+    op, _, os_ = _rows_of(out, "out", (torch.float8_e4m3fn,), dev, x.shape)
+    rows, n = x.shape
+    cp = _at(scales, "scales", torch.float32, rows, dev)
+    if rows == 0:
+        return
+    abi.call("g4_quantize_rows", xp, op, cp, abi.QuantizeRowsParams(rows, n, xt, 0, xs, os_), _stream(stream))
+
+
+class LoraAdapters:
+    """The low-rank adapters of a projection: a [adapters, segments * rank, n] and b [adapters, outputs, rank], float16 or
+    bfloat16, scales f32 [adapters] or None (1 each), widths the outputs of each segment of a fused projection (q, k and v;
+    None: one segment). Keeps the tensors alive; describe a projection's adapters once and pass it to every call."""
+
+    def __init__(self, a, b, scales=None, widths=None):
+        dev = _device_of(a, "a")
+        if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0]:
+            raise ValueError(f"a, b: shapes {tuple(a.shape)} and {tuple(b.shape)}, expected [adapters, segments * rank, n] and "
+                             "[adapters, outputs, rank]")
+        if a.dtype not in (torch.float16, torch.bfloat16) or b.dtype != a.dtype:
+            raise TypeError(f"a, b: dtypes {a.dtype} and {b.dtype}, expected float16 or bfloat16 for both")
+        self.n_adapters, down, self.n = (int(v) for v in a.shape)
+        self.rows, self.rank = int(b.shape[1]), int(b.shape[2])
+        self.widths = (self.rows,) if widths is None else tuple(int(w) for w in widths)
+        if not 1 <= len(self.widths) <= 4 or min(self.widths) < 1 or sum(self.widths) != self.rows:
+            raise ValueError(f"widths: {self.widths} for {self.rows} outputs (1 to 4 segments)")
+        if down != len(self.widths) * self.rank:
+            raise ValueError(f"a: {down} rows, expected {len(self.widths)} segments of rank {self.rank}")
+        self.a, self.b, self.scales, self.device = a, b, scales, dev
+        self.c = abi.Lora(_at(a, "a", a.dtype, 1, dev), _at(b, "b", a.dtype, 1, dev),
+                          None if scales is None else _at(scales, "scales", torch.float32, self.n_adapters, dev),
+                          self.n_adapters, self.rank, self.n, len(self.widths), (C.c_uint32 * 4)(*self.widths),
+                          ROW_TYPES[a.dtype], 0)
+
+
+def linear_e4m3_workspace_bytes(n_tokens, rows, n, lora=None) -> int:
+    """Bytes that serve every call of at most so many tokens with this projection and these adapters (or none)."""
+    size = C.c_size_t(0)
+    abi.call("g4_linear_e4m3_workspace_size", abi.LinearE4m3Params(n_tokens, rows, n, abi.G4_F32, 0, 0),
+             None if lora is None else lora.c, C.byref(size))
+    return size.value
+
+
+def linear_e4m3(x, x_scales, weight, weight_scales, out, workspace, lora=None, adapter_ids=None, stream=None):
+    """Projection of 8-bit rows (g4_linear_e4m3). x: float8_e4m3fn [n_tokens, n] with f32 scales [n_tokens], tokens may lie
+    apart; weight: float8_e4m3fn [rows, n] with f32 scales [rows]; out: [n_tokens, rows], f32, f16 or bf16, tokens may lie
+    apart. lora: a LoraAdapters of n inputs and rows outputs, with adapter_ids int32 [n_tokens] (outside the adapters: none).
+    workspace: uint8, linear_e4m3_workspace_bytes."""
+    dev = _device_of(x, "x")
+    e4m3, f32 = torch.float8_e4m3fn, torch.float32
+    xp, _, xs = _rows_of(x, "x", (e4m3,), dev)
+    tokens, n = x.shape
+    if weight.dim() != 2 or weight.shape[1] != n:
+        raise ValueError(f"weight: shape {tuple(weight.shape)}, expected [rows, {n}]")
+    rows = weight.shape[0]
+    op, ot, os_ = _rows_of(out, "out", _WIDE_TYPES, dev, (tokens, rows))
+    if (lora is None) != (adapter_ids is None):
+        raise ValueError("lora and adapter_ids go together")
+    if lora is not None and lora.device != dev:
+        raise ValueError(f"lora: on cuda:{lora.device}, expected cuda:{dev}")
+    if tokens == 0:
+        return
+    abi.call("g4_linear_e4m3", xp, _at(x_scales, "x_scales", f32, tokens, dev), _at(weight, "weight", e4m3, rows * n, dev),
+             _at(weight_scales, "weight_scales", f32, rows, dev), None if lora is None else lora.c,
+             None if lora is None else _at(adapter_ids, "adapter_ids", torch.int32, tokens, dev), op,
+             abi.LinearE4m3Params(tokens, rows, n, ot, xs, os_), _at(workspace, "workspace", torch.uint8, 0, dev),
+             workspace.numel(), _stream(stream))
+
+
+def lora_workspace_bytes(lora, n_tokens) -> int:
+    """Bytes that serve every lora_add of at most so many tokens with these adapters."""
+    size = C.c_size_t(0)
+    abi.call("g4_lora_workspace_size", lora.c, n_tokens, C.byref(size))
+    return size.value
+
+
+def lora_add(lora, adapter_ids, x, base, out, workspace, x_scales=None, stream=None):
+    """out = base + the adapters' part, beside a projection of x made elsewhere (g4_lora_add). adapter_ids: int32
+    [n_tokens]; x: [n_tokens, n], f32, f16, bf16, or float8_e4m3fn with x_scales; base and out: [n_tokens, rows] of one type,
+    f32, f16 or bf16 (may be the same tensor). Tokens may lie apart. workspace: uint8, lora_workspace_bytes."""
+    dev = _call_device(lora.device)
+    xp, xt, xs = _rows_of(x, "x", tuple(ROW_TYPES), dev)
+    tokens = x.shape[0]
+    if x.shape[1] != lora.n:
+        raise ValueError(f"x: shape {tuple(x.shape)}, expected [n_tokens, {lora.n}]")
+    bp, bt, bs = _rows_of(base, "base", _WIDE_TYPES, dev, (tokens, lora.rows))
+    op, ot, os_ = _rows_of(out, "out", (base.dtype,), dev, (tokens, lora.rows))
+    if (x.dtype == torch.float8_e4m3fn) != (x_scales is not None):
+        raise ValueError("x_scales go with a float8_e4m3fn x")
+    if tokens == 0:
+        return
+    abi.call("g4_lora_add", lora.c, _at(adapter_ids, "adapter_ids", torch.int32, tokens, dev), xp,
+             None if x_scales is None else _at(x_scales, "x_scales", torch.float32, tokens, dev), bp, op,
+             abi.LoraAddParams(tokens, xt, ot, 0, xs, bs, os_), _at(workspace, "workspace", torch.uint8, 0, dev),
+             workspace.numel(), _stream(stream))

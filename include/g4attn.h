@@ -868,6 +868,123 @@ int g4_token_logprobs(const void* logits, const int32_t* tokens, float* logprobs
                       float* top_logprobs, const g4_token_logprobs_params* p, void* workspace, size_t workspace_bytes,
                       void* stream);
 
+/* ---- between two attention blocks of a served batch -----------------------
+ * The rows of a batch's tokens from one attention block to the next: the
+ * residual's addition and the norms, rows in 8 bits, projections of them, and
+ * the requests' low-rank adapters beside a projection. The engine runs these
+ * for one token, as rmsNorm, fusedNormAdd and add (src/engine.ts:2044,
+ * 2099-2103, 2140-2161) and as GEMVs (:2045-2051, 2096); adapters and batches
+ * have no counterpart there. g4_paged_append takes such a projection's q, k and
+ * v, g4_quantize_rows g4_paged_attn's outputs for the next.
+ *
+ * Element types: */
+#define G4_F32 0
+#define G4_F16 1
+#define G4_BF16 2
+#define G4_E4M3 3 /* OCP e4m3, with one f32 scale a row: the row is scale * codes */
+
+/* Per row: b = x, or post_weight * x / sqrt(mean x^2 + eps); r = residual + b
+ * (or b), rounded to residual_type and written to residual_out; out = weight *
+ * r / sqrt(mean r^2 + eps). post_weight, residual and residual_out may be NULL;
+ * weight NULL: a norm without weights; out NULL (with weight NULL): only the
+ * addition. residual_out may be residual, and out may be x where they have one
+ * type and stride. Sums in f32 (elements up to 1e16 in magnitude).
+ * out_type G4_E4M3: scales[row] = max |out| / 448, codes of out / scale to nearest
+ * even; rows all below 2^-100 are scaled as rows of that size; a row with an Inf
+ * or NaN has scale NaN and NaN codes. scales: NULL with the other types. Strides:
+ * elements from row to row, 0 for contiguous rows. Rows aligned to 16 bytes of n a
+ * multiple of 8 are the fast ones. */
+typedef struct g4_add_rms_norm_params {
+    uint32_t rows;          /* at most 2^22 */
+    uint32_t n;             /* elements of a row, at most 32768 */
+    uint32_t x_type;        /* G4_F32, G4_F16 or G4_BF16 */
+    uint32_t residual_type; /* of residual and residual_out */
+    uint32_t weight_type;   /* of post_weight and weight */
+    uint32_t out_type;      /* any */
+    float eps;              /* 0 to 1 */
+    uint32_t reserved;      /* 0 */
+    uint64_t x_stride;
+    uint64_t residual_stride;
+    uint64_t residual_out_stride;
+    uint64_t out_stride;
+} g4_add_rms_norm_params;
+int g4_add_rms_norm(const void* x, const void* residual, const void* post_weight, const void* weight, void* residual_out,
+                    void* out, float* scales, const g4_add_rms_norm_params* p, void* stream);
+
+/* Rows in 8 bits, as g4_add_rms_norm's G4_E4M3 out: an attention's or
+ * activation's outputs before the next projection; a projection's weights, once. */
+typedef struct g4_quantize_rows_params {
+    uint32_t rows;      /* at most 2^22 */
+    uint32_t n;         /* at most 32768 */
+    uint32_t x_type;    /* G4_F32, G4_F16 or G4_BF16 */
+    uint32_t reserved;  /* 0 */
+    uint64_t x_stride;
+    uint64_t out_stride;
+} g4_quantize_rows_params;
+int g4_quantize_rows(const void* x, uint8_t* out, float* scales, const g4_quantize_rows_params* p, void* stream);
+
+/* Low-rank adapters of a projection, all of one rank (pad with zeros). A fused
+ * projection has a segment of outputs for each of its parts (q, k and v: one
+ * down product of n_segs * rank rows); a single one has one. Token t has adapter
+ * adapter_ids[t] (DEVICE, read when the kernels run), or none where that is not
+ * in [0, n_adapters): what the other adapters hold does not reach it. With o in
+ * segment s, its adapter adds
+ *   scales[a] * sum_j (sum_k x[t][k] a[a][s * rank + j][k]) * b[a][o][j]
+ * (sums in f32; the inner sums enter the second product off by 2^-23 of themselves
+ * or 2^-39 of the token's largest). An Inf or NaN among a token's inner sums
+ * makes outputs of that token Inf or NaN. */
+typedef struct g4_lora {
+    const void* a;          /* [n_adapters][n_segs * rank][n], 16-byte aligned */
+    const void* b;          /* [n_adapters][sum of widths][rank], 16-byte aligned */
+    const float* scales;    /* DEVICE [n_adapters], or NULL: 1 */
+    uint32_t n_adapters;    /* 1 .. 65535 */
+    uint32_t rank;          /* a multiple of 8, at most 128 */
+    uint32_t n;             /* inputs: a multiple of 16, at most 65536 */
+    uint32_t n_segs;        /* 1 .. 4 */
+    uint32_t widths[4];     /* outputs of each segment */
+    uint32_t type;          /* of a and b: G4_F16 or G4_BF16 */
+    uint32_t reserved;      /* 0 */
+} g4_lora;
+
+/* out[t][o] = x_scales[t] * weight_scales[o] * sum_k x[t][k] weight[o][k] of e4m3
+ * rows (sums in f32), with the adapters' part added before the rounding where
+ * lora is given. x: [n_tokens][n], as g4_add_rms_norm or g4_quantize_rows leave
+ * it; weight: [rows][n], its scales one a row. Rows 16-byte aligned. The workspace
+ * holds partial results within a call; calls that overlap need one each, and a
+ * size (g4_linear_e4m3_workspace_size) serves every call of no more tokens with
+ * the same projection and adapters. The same call gives the same bits. */
+typedef struct g4_linear_e4m3_params {
+    uint32_t n_tokens;   /* at most 2^22 */
+    uint32_t rows;       /* outputs, at most 2^20 */
+    uint32_t n;          /* inputs: a multiple of 16, at most 65536 */
+    uint32_t out_type;   /* G4_F32, G4_F16 or G4_BF16 */
+    uint64_t x_stride;   /* elements from token to token; 0: n */
+    uint64_t out_stride; /* 0: rows */
+} g4_linear_e4m3_params;
+int g4_linear_e4m3_workspace_size(const g4_linear_e4m3_params* p, const g4_lora* lora, size_t* bytes);
+int g4_linear_e4m3(const uint8_t* x, const float* x_scales, const uint8_t* weight, const float* weight_scales,
+                   const g4_lora* lora, const int32_t* adapter_ids, void* out, const g4_linear_e4m3_params* p,
+                   void* workspace, size_t workspace_bytes, void* stream);
+
+/* out = base + the adapters' part, beside a projection made elsewhere (of
+ * g4_linear_f16, g4_linear_quant, ...). x: [n_tokens][n], the projection's input, of
+ * any type (x_scales with G4_E4M3, else NULL); f16 x with f16 adapters, bf16 with
+ * bf16 and e4m3 with either are the fast ones. base and out: [n_tokens][outputs] of
+ * out_type; base may be out (with one stride). Tokens without an adapter: out =
+ * base. x's rows 16-byte aligned. Workspace as above. */
+typedef struct g4_lora_add_params {
+    uint32_t n_tokens;    /* at most 2^22 */
+    uint32_t x_type;
+    uint32_t out_type;    /* G4_F32, G4_F16 or G4_BF16 */
+    uint32_t reserved;    /* 0 */
+    uint64_t x_stride;    /* elements from token to token; 0: contiguous */
+    uint64_t base_stride;
+    uint64_t out_stride;
+} g4_lora_add_params;
+int g4_lora_workspace_size(const g4_lora* lora, uint32_t n_tokens, size_t* bytes);
+int g4_lora_add(const g4_lora* lora, const int32_t* adapter_ids, const void* x, const float* x_scales, const void* base,
+                void* out, const g4_lora_add_params* p, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
