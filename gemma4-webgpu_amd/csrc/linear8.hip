@@ -6,6 +6,8 @@
 // rows: a sum of 128 is off by 1.4e-5 of itself, at most 2^-12.3 of the largest product). Elements widened to
 // f16, which is exact, give sums in f32. Weight rows are the matrix operand's rows, tokens its columns: a lane
 // ends with four consecutive outputs of one token.
+#include <utility>
+
 #include "lora.h"
 
 namespace g4 {
@@ -32,12 +34,12 @@ __device__ __forceinline__ Row32 row32(const uint8_t* p, unsigned k, unsigned n)
     if (k + 16 < n) r.v[1] = ldg<u32x4>(p + k + 16);
     return r;
 }
-// Eight of them (q: 0 to 3) as f16, exactly.
-__device__ __forceinline__ f16x8 widen8(const Row32& r, int q) {
+// Eight e4m3 as f16, exactly.
+__device__ __forceinline__ f16x8 widen8(uint32_t a, uint32_t b) {
     f16x8 h;
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-        const uint32_t w = r.v[q / 2][2 * (q & 1) + i];
+        const uint32_t w = i ? b : a;
         const auto lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false), hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true);
         h[4 * i] = lo[0];
         h[4 * i + 1] = lo[1];
@@ -47,20 +49,25 @@ __device__ __forceinline__ f16x8 widen8(const Row32& r, int q) {
     return h;
 }
 
+__device__ __forceinline__ f16x8 widen8(const Row32& r, int q) {  // the q-th eight of 32
+    return widen8(r.v[q / 2][2 * (q & 1)], r.v[q / 2][2 * (q & 1) + 1]);
+}
+
 // Sums of one 16-output tile: scales, adapters, the store.
 __device__ __forceinline__ void finish(const Linear8Args& a, f32x4 sum, unsigned o0, unsigned t) {
     const unsigned lane = threadIdx.x & 63, g = lane >> 4, o = o0 + 4 * g;
     const bool valid = t < a.n_tokens;
     const float xs = valid ? a.x_scales[t] : 0.0f;
-    f32x4 acc[1];
+    f32x4 y;
 #pragma unroll
-    for (int i = 0; i < 4; i++) acc[0][i] = sum[i] * xs * (o + i < a.rows ? a.w_scales[o + i] : 0.0f);
+    for (int i = 0; i < 4; i++) y[i] = sum[i] * xs * (o + i < a.rows ? a.w_scales[o + i] : 0.0f);
     if (a.low) {
         const int id = lora_id(a.l, t, valid);
-        if (a.low == G4_F16) lora_up<1, false>(acc, a.l, o0, t, id);
-        else lora_up<1, true>(acc, a.l, o0, t, id);
+        auto add = [&](int, int i, float v) __attribute__((always_inline)) { y[i] += v; };
+        if (a.low == G4_F16) lora_up<16, 1, false>(a.l, o0, t, id, add);
+        else lora_up<16, 1, true>(a.l, o0, t, id, add);
     }
-    if (valid && o < a.rows) store4(a.out, a.out_type, t * a.out_stride + o, acc[0], a.wide, a.rows - o);
+    if (valid && o < a.rows) store4(a.out, a.out_type, t * a.out_stride + o, y, a.wide, a.rows - o);
 }
 
 // Few tokens: 16 outputs by 16 CT tokens a workgroup, its waves take every Wth 128 of k.
@@ -98,6 +105,287 @@ __global__ __launch_bounds__(W * 64) void k_linear8_few(const Linear8Args a) {
     }
 }
 
+
+// ---- many tokens ---------------------------------------------------------------------
+//
+// 64 RT outputs by 64 CT tokens a workgroup of four waves, two by two, a wave 2 RT x 2 CT / 4 tiles of 32 x 32. Both
+// operands come to LDS by DMA, 64 k a stage, four stages; a wave reads the next stage's operands into registers
+// while it multiplies this one's, so LDS, the DMA and the matrix unit work at once, with one barrier a stage. The
+// workgroup goes on to its next tile without a pause: the DMA runs up to four stages ahead, across the tiles' ends.
+//
+// A stage holds 64 bytes a row, 16-byte piece c of row r at r * 64 + (c ^ (r / 4) % 4) * 16: sixteen lanes that read one
+// piece of sixteen rows meet all 64 banks.
+constexpr unsigned kStageK = 64;
+__device__ __attribute__((aligned(16))) const uint32_t kZeros[4] = {0, 0, 0, 0};
+
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // M0 is a reserved register: clobbering it is what is meant
+// 16 bytes a lane from base + its offset, or from its address, to LDS lds + at + 16 lane. No memory clobber: it writes a
+// stage that nothing reads before the barrier that waits for it, and reads of other stages may pass it.
+template <unsigned AT>
+__device__ __forceinline__ void stage_dma(const void* base, uint32_t off, uint32_t lds) {
+    asm volatile("s_add_u32 m0, %2, %3\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds), "n"(AT) : "m0", "scc");
+}
+template <unsigned AT>
+__device__ __forceinline__ void stage_dma(const void* from, uint32_t lds) {
+    asm volatile("s_add_u32 m0, %1, %2\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(lds), "n"(AT) : "m0", "scc");
+}
+// Four bytes a lane to LDS lds + 4 lane.
+__device__ __forceinline__ void scale_dma(const void* from, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(lds) : "m0");
+}
+#pragma clang diagnostic pop
+// All but the N newest requests have come, the wave's LDS reads too; then every wave's.
+template <int N>
+__device__ __forceinline__ void stage_barrier() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+struct TileArgs {
+    Linear8Args a;
+    uint32_t o_tiles, t_tiles;
+};
+
+// Tiles in an order that keeps the 32 workgroups of an XCD (workgroup b: XCD b % 8) on few rows of both operands at a
+// time: each XCD has a run of the order, in which eight token tiles go together.
+struct TileOrder {
+    uint32_t o_tiles, t_tiles, at, end, step;
+    __device__ TileOrder(uint32_t o, uint32_t t) : o_tiles(o), t_tiles(t) {
+        const uint32_t n = o * t, b = blockIdx.x;
+        if (gridDim.x % 8 == 0) {
+            at = n / 8 * (b % 8) + min(b % 8, n % 8) + b / 8;
+            end = n / 8 * (b % 8 + 1) + min(b % 8 + 1, n % 8);
+            step = gridDim.x / 8;
+        } else {
+            at = b;
+            end = n;
+            step = gridDim.x;
+        }
+    }
+    __device__ void place(uint32_t i, uint32_t& o, uint32_t& t) const {
+        const uint32_t group = i / (8 * o_tiles), r = i - group * 8 * o_tiles, wide = min(8u, t_tiles - group * 8);
+        o = r / wide;
+        t = group * 8 + r - o * wide;
+    }
+};
+
+// f(0), f(1) .. f(N - 1), the numbers as types: what depends on them is settled when it is compiled.
+template <int... I, typename F>
+__device__ __forceinline__ void each_of(std::integer_sequence<int, I...>, F&& f) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void each_of(F&& f) {
+    each_of(std::make_integer_sequence<int, N>{}, f);
+}
+
+template <int WO, int WT, int RT, int CT, int kStages, uint32_t OT, bool LOW>
+__global__ __launch_bounds__(64 * WO * WT, RT * CT >= 16 ? 1 : 2) void k_linear8_tiles(const TileArgs ta) {
+    constexpr bool WIDE = OT == G4_F32;
+    constexpr int W = WO * WT, OPS = RT + CT, READS = 2 * OPS, PAIRS = RT * CT;
+    constexpr unsigned BO = 32 * WO * RT, BT = 32 * WT * CT, STAGE = (BO + BT) * kStageK;
+    constexpr int DW = BO / 16 / W, DX = BT / 16 / W, DMAS = DW + DX;  // requests a wave and stage
+    static_assert(BO % (16 * W) == 0 && BT % (16 * W) == 0, "even shares");
+    constexpr unsigned SLOTS = 4, SCALES = kStages * STAGE;  // scales of up to four tiles: the DMA is two tiles ahead at most
+    static_assert(BO % 64 == 0 && (BO + BT) % (64 * W) == 0, "whole waves of scales");
+    __shared__ __attribute__((aligned(16))) uint8_t s_mem[SCALES + SLOTS * (BO + BT) * 4];
+    const Linear8Args& a = ta.a;
+    const unsigned lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, g = lane >> 5;
+    const unsigned wo = wave / WT * 32 * RT, wt = wave % WT * 32 * CT;
+    const uint32_t lds = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)s_mem);
+    TileOrder order(ta.o_tiles, ta.t_tiles);
+    if (order.at >= order.end) return;
+    const unsigned stages = ((a.n + 2 * kStageK - 1) / (2 * kStageK)) * 2;  // of a tile; even
+
+    // The DMA's side: pieces of 16 rows, DW of the weights' and DX of the tokens' a wave; a lane's offset from the tile.
+    const unsigned piece = ((lane & 3) ^ ((lane >> 4) & 3)) * 16;
+    const uint8_t *d_w, *d_x;  // the tile's rows at the stage's k
+    uint32_t from[DMAS];
+    unsigned d_k = 0, d_tile = order.at, d_slot = 0;
+    uint32_t d_lds = 0;
+    auto aim = [&]() __attribute__((always_inline)) {
+        uint32_t o, t;
+        order.place(d_tile, o, t);
+        d_w = a.w + (uint64_t)(o * BO) * a.n;
+        d_x = a.x + (uint64_t)(t * BT) * a.x_stride;
+#pragma unroll
+        for (int j = 0; j < DMAS; j++) {
+            const unsigned r = 16 * (j < DW ? wave * DW + j : wave * DX + j - DW) + (lane >> 2);
+            from[j] = (j < DW ? min(r, a.rows - 1 - o * BO) * a.n : min(r, a.n_tokens - 1 - t * BT) * (uint32_t)a.x_stride) + piece;
+        }
+#pragma unroll
+        for (unsigned first = wave * 64; first < BO + BT; first += 64 * W) {  // 64 of the weights' or of the tokens'
+            const unsigned i = first + lane;
+            scale_dma(first < BO ? a.w_scales + min(o * BO + i, a.rows - 1) : a.x_scales + min(t * BT + i - BO, a.n_tokens - 1),
+                      __builtin_amdgcn_readfirstlane(lds + SCALES + (d_slot * (BO + BT) + first) * 4));
+        }
+        d_slot = (d_slot + 1) % SLOTS;
+    };
+    auto request = [&](auto j) __attribute__((always_inline)) {
+        constexpr unsigned at = j < DW ? j * 1024 : BO * kStageK + (j - DW) * 1024;
+        const uint8_t* base = j < DW ? d_w : d_x;
+        const uint32_t to = lds + d_lds + wave * (j < DW ? DW : DX) * 1024;
+        if (d_k + kStageK <= a.n) {  // uniform
+            stage_dma<at>(uniform_ptr(reinterpret_cast<const char*>(base)), from[j], to);
+        } else {
+            const uint8_t* p = base + from[j];
+            if (d_k + piece >= a.n) p = reinterpret_cast<const uint8_t*>(kZeros);
+            stage_dma<at>(p, to);
+        }
+    };
+    auto requested = [&]() __attribute__((always_inline)) {  // a stage's; past the last tile the same tile's come again
+        d_lds = d_lds == (kStages - 1) * STAGE ? 0 : d_lds + STAGE;
+        d_k += kStageK;
+        d_w += kStageK;
+        d_x += kStageK;
+        if (d_k == stages * kStageK) {
+            d_k = 0;
+            if (d_tile + order.step < order.end) d_tile += order.step;
+            aim();
+        }
+    };
+    aim();
+#pragma unroll 1
+    for (int s = 0; s < kStages; s++) {
+        each_of<DMAS>(request);
+        requested();
+    }
+
+    // The matrix unit's side.
+    const unsigned swz = (col >> 2) & 3;
+    const unsigned off0 = col * kStageK + ((2 * g) ^ swz) * 16, off1 = col * kStageK + ((2 * g + 1) ^ swz) * 16;
+    i32x8 reg[2][OPS];
+    unsigned r_lds = 0;
+    auto read = [&](i32x8 (&to)[OPS], auto i) __attribute__((always_inline)) {
+        constexpr int j = i / 2, h = i % 2;
+        const unsigned base = r_lds + (j < RT ? wo * kStageK + j * 32 * kStageK : (BO + wt) * kStageK + (j - RT) * 32 * kStageK);
+        const u32x4 v = *reinterpret_cast<const u32x4*>(s_mem + base + (h ? off1 : off0));
+#pragma unroll
+        for (int e = 0; e < 4; e++) to[j][4 * h + e] = (int)v[e];
+    };
+    stage_barrier<(kStages - 1) * DMAS>();
+    each_of<READS>([&](auto i) __attribute__((always_inline)) { read(reg[0], i); });
+    r_lds = STAGE;
+    stage_barrier<(kStages - 2) * DMAS>();
+
+    f32x16 acc[RT][CT];
+    bool stored = false;  // whether the tile before left PAIRS * (4 or 2) stores, all of them
+    unsigned slot = 0;
+    auto stage = [&](const i32x8 (&now)[OPS], i32x8 (&next)[OPS], auto first, auto early) __attribute__((always_inline)) {
+        constexpr int SUBS = WIDE ? 4 : 1, STEPS = PAIRS * SUBS;
+        f16x8 half[2][OPS];
+        auto widen = [&](auto j, auto q) __attribute__((always_inline)) { half[q & 1][j] = widen8(now[j][2 * q], now[j][2 * q + 1]); };
+        if constexpr (WIDE) each_of<OPS>([&](auto j) __attribute__((always_inline)) { widen(j, std::integral_constant<int, 0>{}); });
+        each_of<STEPS>([&](auto m) __attribute__((always_inline)) {
+            constexpr int q = m / PAIRS, pair = m % PAIRS, rt = pair / CT, ct = rt & 1 ? CT - 1 - pair % CT : pair % CT;
+            f32x16 c = acc[rt][ct];
+            if constexpr (first && q == 0) c = f32x16{0};
+            if constexpr (WIDE) acc[rt][ct] = __builtin_amdgcn_mfma_f32_32x32x16_f16(half[q & 1][rt], half[q & 1][RT + ct], c, 0, 0, 0);
+            else acc[rt][ct] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(now[rt], now[RT + ct], c, 0, 0, 0, 0, 0, 0);
+            if constexpr (WIDE && q < 3) {
+                // The next quarter's elements, evenly over this one's products.
+                constexpr int w0 = pair * OPS / PAIRS, w1 = (pair + 1) * OPS / PAIRS;
+                each_of<w1 - w0>([&](auto j) __attribute__((always_inline)) {
+                    widen(std::integral_constant<int, w0 + j>{}, std::integral_constant<int, q + 1>{});
+                });
+            }
+            // The reads in the first part, the DMA's requests all along.
+            constexpr int by = STEPS * 3 / 4;
+            constexpr int r0 = m < by ? m * READS / by : READS, r1 = m + 1 < by ? (m + 1) * READS / by : READS;
+            each_of<r1 - r0>([&](auto i) __attribute__((always_inline)) { read(next, std::integral_constant<int, r0 + i>{}); });
+            constexpr int d0 = m * DMAS / STEPS, d1 = (m + 1) * DMAS / STEPS;
+            each_of<d1 - d0>([&](auto j) __attribute__((always_inline)) { request(std::integral_constant<int, d0 + j>{}); });
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        requested();
+        r_lds = r_lds == (kStages - 1) * STAGE ? 0 : r_lds + STAGE;
+        // The last tile's stores are younger than the stages that the first two barriers wait for: they may go on.
+        constexpr int AFTER = (kStages - 2) * DMAS + PAIRS * (WIDE ? 4 : 2);  // the counter's most is 63
+        if (decltype(early)::value && stored) stage_barrier<AFTER < 63 ? AFTER : 63>();
+        else stage_barrier<(kStages - 2) * DMAS>();
+    };
+    constexpr std::true_type kFirst{};  // of a tile: nothing to add to; the tile before may have left stores
+    constexpr std::false_type kLater{};
+
+    for (unsigned i = order.at; i < order.end; i += order.step) {
+        stage(reg[0], reg[1], kFirst, kFirst);
+        stage(reg[1], reg[0], kLater, kFirst);
+#pragma unroll 1
+        for (unsigned s = 2; s < stages; s += 2) {
+            stage(reg[0], reg[1], kLater, kLater);
+            stage(reg[1], reg[0], kLater, kLater);
+        }
+        uint32_t ot, tt;
+        order.place(i, ot, tt);
+        const unsigned o0 = ot * BO + wo, t0 = tt * BT + wt;
+        const float* scales = reinterpret_cast<const float*>(s_mem + SCALES) + slot * (BO + BT);
+        slot = (slot + 1) % SLOTS;
+        stored = a.wide && o0 + 32 * RT <= a.rows && t0 + 32 * CT <= a.n_tokens;  // uniform: every lane stores whole pieces
+        each_of<CT>([&](auto ct) __attribute__((always_inline)) {
+            const unsigned t = t0 + 32 * ct + col;
+            const float xs = scales[BO + wt + 32 * ct + col];
+            const int id = LOW ? lora_id(a.l, t, t < a.n_tokens) : -1;
+            each_of<RT>([&](auto rt) __attribute__((always_inline)) {
+                const unsigned o = o0 + 32 * rt;
+                f32x4 y[4];
+                each_of<4>([&](auto q) __attribute__((always_inline)) {
+                    const f32x4 ws = *reinterpret_cast<const f32x4*>(scales + wo + 32 * rt + 8 * q + 4 * g);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) y[q][e] = acc[rt][ct][4 * q + e] * xs * ws[e];
+                });
+                if constexpr (LOW) {
+                    auto add = [&](int, int i, float v) __attribute__((always_inline)) { y[i / 4][i % 4] += v; };
+                    if (a.low == G4_F16) lora_up<32, 1, false>(a.l, o, t, id, add);
+                    else lora_up<32, 1, true>(a.l, o, t, id, add);
+                }
+                if (!stored) {
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        const unsigned oq = o + 8 * q + 4 * g;
+                        if (t < a.n_tokens && oq < a.rows)
+                            store4(a.out, OT, t * a.out_stride + oq, y[q], a.wide, a.rows - oq);
+                    }
+                } else if constexpr (WIDE) {
+                    float* out = static_cast<float*>(a.out) + t * a.out_stride + o + 4 * g;
+#pragma unroll
+                    for (int q = 0; q < 4; q++) stg<f32x4>(out + 8 * q, y[q]);
+                } else {
+                    // Lane halves exchange, so that a lane has eight outputs one after the other: the lower half's of every
+                    // even eight, the upper's of the odd.
+                    uint16_t* out = static_cast<uint16_t*>(a.out) + t * a.out_stride + o + 8 * g;
+#pragma unroll
+                    for (int q = 0; q < 4; q += 2) {
+                        uint32_t w[2][2];
+#pragma unroll
+                        for (int p = 0; p < 2; p++)
+#pragma unroll
+                            for (int e = 0; e < 2; e++) w[p][e] = pair16(y[q + p][2 * e], y[q + p][2 * e + 1], OT);
+                        u32x4 v;
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const auto sw = __builtin_amdgcn_permlane32_swap(w[0][e], w[1][e], false, false);
+                            v[e] = sw[0];
+                            v[2 + e] = sw[1];
+                        }
+                        stg<u32x4>(out + 8 * q, v);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);  // tile by tile: the registers hold no more
+            });
+        });
+        if (!stored) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // an unknown number of stores: the counts begin anew
+        if constexpr (LOW) {  // the next tile's first operands once more: the adapters need the registers in between
+            asm volatile("" ::: "memory");
+            const unsigned ahead = r_lds;
+            r_lds = ahead == 0 ? (kStages - 1) * STAGE : ahead - STAGE;
+            each_of<READS>([&](auto j) __attribute__((always_inline)) { read(reg[0], j); });
+            r_lds = ahead;
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // the next stage's requests go where these lay
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no DMA into LDS that is another workgroup's by then
+}
+
 }  // namespace g4
 
 using namespace g4;
@@ -123,6 +411,22 @@ int linear8_check(const g4_linear_e4m3_params* p, const g4_lora* lora) {
         return fail(G4_EINVAL, "%s: adapters of %u inputs and %u outputs beside a projection of %u and %u", what, lora->n, rows, p->n,
                     p->rows);
     return G4_OK;
+}
+
+template <int WO, int WT, int RT, int CT, int NS>
+void launch_tiles(const Linear8Args& a, hipStream_t st) {
+    constexpr uint32_t BO = 32 * WO * RT, BT = 32 * WT * CT;
+    TileArgs t = {a, (a.rows + BO - 1) / BO, (a.n_tokens + BT - 1) / BT};
+    const uint32_t n = t.o_tiles * t.t_tiles, most = device_cus() * (WO * WT == 8 ? 1 : 2);
+    const dim3 grid(n < most ? n : most), block(64 * WO * WT);
+    auto launch = [&](auto type) {
+        constexpr uint32_t OT = decltype(type)::value;
+        if (a.low) G4_LAUNCH((k_linear8_tiles<WO, WT, RT, CT, NS, OT, true>), grid, block, 0, st, t);
+        else G4_LAUNCH((k_linear8_tiles<WO, WT, RT, CT, NS, OT, false>), grid, block, 0, st, t);
+    };
+    if (a.out_type == G4_F32) launch(std::integral_constant<uint32_t, G4_F32>{});
+    else if (a.out_type == G4_F16) launch(std::integral_constant<uint32_t, G4_F16>{});
+    else launch(std::integral_constant<uint32_t, G4_BF16>{});
 }
 
 template <int CT, int W>
@@ -183,7 +487,9 @@ int g4_linear_e4m3(const uint8_t* x, const float* x_scales, const uint8_t* weigh
         G4_CHECK_LAUNCH("k_lora_down");
     }
     if (p->n_tokens <= 16) launch_few<1, 4>(a, st);
-    else launch_few<4, 4>(a, st);
+    else if (p->n_tokens <= 96 || xs >= (1u << 24)) launch_few<4, 4>(a, st);
+    else if ((uint64_t)((a.rows + 255) / 256) * ((a.n_tokens + 255) / 256) >= device_cus() / 2) launch_tiles<2, 4, 4, 2, 4>(a, st);
+    else launch_tiles<2, 2, 2, 2, 4>(a, st);
     G4_CHECK_LAUNCH("k_linear8");
     return G4_OK;
 }

@@ -35,11 +35,34 @@ __device__ __forceinline__ int lora_id(const LoraDev& l, unsigned t, bool valid)
     return (unsigned)id < l.n_adapters ? id : -1;
 }
 
-// Adds a 16-token column tile's adapters to NRT 16-row tiles of outputs from o0 on. Lane: token column lane % 16 (its token
-// `t`, its adapter `id`, -1 none), outputs 16 rt + 4 (lane / 16) + i. BF: bf16 adapters.
-template <int NRT, bool BF>
-__device__ __forceinline__ void lora_up(f32x4 (&acc)[NRT], const LoraDev& l, unsigned o0, unsigned t, int id) {
-    const unsigned lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+// The up product's tile: M outputs by M tokens. A lane holds, of token column lane % M, outputs 4 group + i % 4 + 8 (i / 4)
+// with M 32, 4 group + i with M 16, where group = lane / M; its operands hold eight j of every STEP from 8 group on.
+template <int M>
+struct LoraTile;
+template <>
+struct LoraTile<16> {
+    typedef f32x4 acc;
+    static constexpr unsigned STEP = 32;
+    static __device__ __forceinline__ acc mfma(f16x8 a, f16x8 b, acc c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ acc mfma(bf16x8 a, bf16x8 b, acc c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ float most(float x) { return max_xor32(max_xor16(x)); }
+};
+template <>
+struct LoraTile<32> {
+    typedef f32x16 acc;
+    static constexpr unsigned STEP = 16;
+    static __device__ __forceinline__ acc mfma(f16x8 a, f16x8 b, acc c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ acc mfma(bf16x8 a, bf16x8 b, acc c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ float most(float x) { return max_xor32(x); }
+};
+
+// Adds a column tile's adapters to NRT row tiles of outputs from o0 on, through add(rt, i, value) for each element of the
+// lane's: token `t` of column lane % M, its adapter `id`, -1 none. BF: bf16 adapters.
+template <int M, int NRT, bool BF, typename ADD>
+__device__ __forceinline__ void lora_up(const LoraDev& l, unsigned o0, unsigned t, int id, ADD&& add) {
+    using T = LoraTile<M>;
+    constexpr int N = sizeof(typename T::acc) / 4;
+    const unsigned lane = threadIdx.x & 63, col = lane % M, g = lane / M;
     uint64_t left = __ballot(id >= 0);
     while (left) {  // an adapter of the tile at a time; uniform
         const int a = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
@@ -51,11 +74,13 @@ __device__ __forceinline__ void lora_up(f32x4 (&acc)[NRT], const LoraDev& l, uns
 #pragma unroll 1
         for (unsigned s = 0; s < l.n_segs; s++) {  // uniform
             const unsigned end = l.ends[s];
-            if (end > o0 && first < o0 + 16 * NRT) {
-                const unsigned steps = (l.rank + 31) / 32;
-                f32x4 d[NRT];
+            if (end > o0 && first < o0 + M * NRT) {
+                const unsigned steps = (l.rank + T::STEP - 1) / T::STEP;
+                typename T::acc d[NRT];
 #pragma unroll
-                for (int rt = 0; rt < NRT; rt++) d[rt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                for (int rt = 0; rt < NRT; rt++)
+#pragma unroll
+                    for (int i = 0; i < N; i++) d[rt][i] = 0.0f;
                 const float* u = l.u + (uint64_t)t * l.down + s * l.rank;
                 const uint64_t piece = (uint64_t)l.n_tokens * l.down;
                 auto part = [&](unsigned j) __attribute__((always_inline)) {  // u[j .. j + 8)
@@ -72,17 +97,16 @@ __device__ __forceinline__ void lora_up(f32x4 (&acc)[NRT], const LoraDev& l, uns
                 if constexpr (!BF) {
                     float m = 0.0f;
                     for (unsigned st = 0; st < steps; st++) {
-                        const auto v = part(32 * st + 8 * g);
+                        const auto v = part(T::STEP * st + 8 * g);
 #pragma unroll
                         for (int i = 0; i < 4; i++) m = fmaxf(m, fmaxf(fabsf(v.a[i]), fabsf(v.b[i])));
                     }
-                    m = max_xor32(max_xor16(m));
-                    const unsigned e = max(__float_as_uint(m) >> 23, 15u);
+                    const unsigned e = max(__float_as_uint(T::most(m)) >> 23, 15u);
                     up = __uint_as_float((268u - e) << 23);
                     down = __uint_as_float((e - 14u) << 23);
                 }
                 for (unsigned st = 0; st < steps; st++) {
-                    const unsigned j = 32 * st + 8 * g;
+                    const unsigned j = T::STEP * st + 8 * g;
                     const auto v = part(j);
                     float x[8];
 #pragma unroll
@@ -93,7 +117,7 @@ __device__ __forceinline__ void lora_up(f32x4 (&acc)[NRT], const LoraDev& l, uns
                     u32x4 w[NRT];
 #pragma unroll
                     for (int rt = 0; rt < NRT; rt++) {
-                        const unsigned o = o0 + 16 * rt + col;
+                        const unsigned o = o0 + M * rt + col;
                         w[rt] = u32x4{0, 0, 0, 0};
                         if (o >= first && o < end && j < l.rank) w[rt] = ldg<u32x4>(b + (uint64_t)o * l.rank + j);
                     }
@@ -109,9 +133,9 @@ __device__ __forceinline__ void lora_up(f32x4 (&acc)[NRT], const LoraDev& l, uns
 #pragma unroll
                         for (int rt = 0; rt < NRT; rt++) {
                             const bf16x8 wb = __builtin_bit_cast(bf16x8, w[rt]);
-                            d[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb, p2, d[rt], 0, 0, 0);
-                            d[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb, p1, d[rt], 0, 0, 0);
-                            d[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb, p0, d[rt], 0, 0, 0);
+                            d[rt] = T::mfma(wb, p2, d[rt]);
+                            d[rt] = T::mfma(wb, p1, d[rt]);
+                            d[rt] = T::mfma(wb, p0, d[rt]);
                         }
                     } else {
                         f16x8 p0, p1;
@@ -123,8 +147,8 @@ __device__ __forceinline__ void lora_up(f32x4 (&acc)[NRT], const LoraDev& l, uns
 #pragma unroll
                         for (int rt = 0; rt < NRT; rt++) {
                             const f16x8 wh = __builtin_bit_cast(f16x8, w[rt]);
-                            d[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh, p1, d[rt], 0, 0, 0);
-                            d[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh, p0, d[rt], 0, 0, 0);
+                            d[rt] = T::mfma(wh, p1, d[rt]);
+                            d[rt] = T::mfma(wh, p0, d[rt]);
                         }
                     }
                 }
@@ -132,7 +156,8 @@ __device__ __forceinline__ void lora_up(f32x4 (&acc)[NRT], const LoraDev& l, uns
 #pragma unroll
                 for (int rt = 0; rt < NRT; rt++) {
 #pragma unroll
-                    for (int i = 0; i < 4; i++) acc[rt][i] = mine ? __builtin_fmaf(d[rt][i], f, acc[rt][i]) : acc[rt][i];
+                    for (int i = 0; i < N; i++)
+                        if (mine) add(rt, i, d[rt][i] * f);
                 }
             }
             first = end;

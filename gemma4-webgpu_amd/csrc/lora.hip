@@ -170,7 +170,7 @@ __global__ __launch_bounds__(kUpWaves * 64) void k_lora_up(const UpArgs a) {
         const unsigned o = o0 + 16 * rt + 4 * g;
         acc[rt] = valid && o < l.rows ? load4(a.base, a.type, t * a.base_stride + o, a.wide, l.rows - o) : f32x4{0, 0, 0, 0};
     }
-    lora_up<kUpTiles, BF>(acc, l, o0, t, id);
+    lora_up<16, kUpTiles, BF>(l, o0, t, id, [&](int rt, int i, float v) __attribute__((always_inline)) { acc[rt][i] += v; });
 #pragma unroll
     for (int rt = 0; rt < kUpTiles; rt++) {
         const unsigned o = o0 + 16 * rt + 4 * g;

@@ -11,6 +11,7 @@ typedef int32_t i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 constexpr uint32_t kMaxRows = 1u << 22;  // tokens of a batch's buffers
 
@@ -27,6 +28,15 @@ __device__ __forceinline__ uint32_t e4m3_pair(float x, float y) {
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x, y, 0, false) & 0xFFFFu;
 }
 
+// Two f32 in one of the 16-bit types. Each is rounded to f32 where it was computed: fused with the product before it,
+// the rounding to f16 would differ from that of other stores of the same value.
+__device__ __forceinline__ uint32_t pair16(float x, float y, uint32_t type) {
+    asm("" : "+v"(x), "+v"(y));
+    const f32x2 v = {x, y};
+    return type == G4_F16 ? __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2))
+                          : __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
+}
+
 // Four outputs of a row in the row's type: one store where the row allows it, else one each of those below `left`.
 __device__ __forceinline__ void store4(void* out, uint32_t type, uint64_t at, f32x4 v, bool wide, unsigned left) {
     if (type == G4_F32) {
@@ -37,12 +47,12 @@ __device__ __forceinline__ void store4(void* out, uint32_t type, uint64_t at, f3
                 if (i < left) stg<float>(o + i, v[i]);
         return;
     }
-    u16x4 h;
-#pragma unroll
-    for (int i = 0; i < 4; i++) h[i] = type == G4_F16 ? f2h(v[i]) : f2bf(v[i]);
+    const uint32_t lo = pair16(v[0], v[1], type), hi = pair16(v[2], v[3], type);
+    const u16x4 h = {(uint16_t)lo, (uint16_t)(lo >> 16), (uint16_t)hi, (uint16_t)(hi >> 16)};
     uint16_t* o = static_cast<uint16_t*>(out) + at;
     if (wide && left >= 4) stg<u16x4>(o, h);
     else
+#pragma unroll
         for (unsigned i = 0; i < 4; i++)
             if (i < left) stg<uint16_t>(o + i, h[i]);
 }
@@ -51,6 +61,7 @@ __device__ __forceinline__ f32x4 load4(const void* in, uint32_t type, uint64_t a
     if (type == G4_F32) {
         const float* p = static_cast<const float*>(in) + at;
         if (wide && left >= 4) return ldg<f32x4>(p);
+#pragma unroll
         for (unsigned i = 0; i < 4; i++)
             if (i < left) v[i] = ldg<float>(p + i);
         return v;
@@ -59,6 +70,7 @@ __device__ __forceinline__ f32x4 load4(const void* in, uint32_t type, uint64_t a
     u16x4 h = {0, 0, 0, 0};
     if (wide && left >= 4) h = ldg<u16x4>(p);
     else
+#pragma unroll
         for (unsigned i = 0; i < 4; i++)
             if (i < left) h[i] = ldg<uint16_t>(p + i);
 #pragma unroll

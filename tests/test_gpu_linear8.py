@@ -31,7 +31,7 @@ def check(dev, seed, tokens, rows, n, kind="f32"):
     announce(f"linearE4m3 {tokens} x {rows} x {n} {kind}")
     x, xs, w, ws = make(dev, seed, tokens, rows, n)
     got = call(x, xs, w, ws, kind)
-    want, tol = linear(*(t.cpu().float() for t in (x, xs, w, ws)))
+    want, tol = linear(*(t.cpu().float() for t in (x, xs, w, ws)), kind)
     within(got.cpu(), want, tol + rounding(want, kind), "out")
 
 
@@ -61,6 +61,13 @@ def test_types(dev, kind, tokens, rows, n):
 @pytest.mark.parametrize("tokens,rows,n", [(5, 65536, 64), (3, 8, 65536), (1, 16, 65536), (4200, 24, 128), (2049, 4112, 144)])
 def test_long_sides(dev, tokens, rows, n):
     check(dev, 4, tokens, rows, n)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("tokens,rows,n", [(4500, 4100, 64), (4352, 4352, 128), (4400, 4104, 336)])
+def test_more_tiles_than_compute_units(dev, kind, tokens, rows, n):
+    """Workgroups that go on from tile to tile, whole ones and cut ones, over one to six stages each."""
+    check(dev, 5, tokens, rows, n, kind)
 
 
 @pytest.mark.parametrize("tokens", [1, 30, 260])

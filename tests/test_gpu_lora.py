@@ -68,7 +68,7 @@ def check_fused(dev, seed, tokens, n, low, kind="f32", runs=None):
     x, xs, ids = batch(dev, seed, tokens, n, "e4m3", low.n_adapters, runs)
     w, ws = (t.to(dev) for t in in_8_bits(torch.randn(low.rows, n, generator=g) * n ** -0.5))
     got = fused(low, ids, x, xs, w, ws, kind).cpu()
-    y, off = linear(*(t.cpu().float() for t in (x, xs, w, ws)))
+    y, off = linear(*(t.cpu().float() for t in (x, xs, w, ws)), kind)
     part, tol = lora(ids.cpu(), x.cpu().double() * xs.cpu().double()[:, None], *cpu(low))
     want = y + part
     within(got, want, off + tol + (y.abs() + part.abs()) * 4 * E + rounding(want, kind), "out")
@@ -125,6 +125,13 @@ def test_sixty_four_requests_of_forty_adapters(dev):
     announce("lora 64 requests")
     low = adapters(dev, 64, 40, 16, (2048, 256, 256), 1536)
     check_fused(dev, 64, 64, 1536, low)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_more_tiles_than_compute_units(dev, kind):
+    announce(f"lora many tiles {kind}")
+    low = adapters(dev, 65, 5, 24, (4000, 56, 300), 128, "bf16" if kind == "f32" else "f16")
+    check_fused(dev, 66, 4360, 128, low, kind, runs=11)
 
 
 @pytest.mark.parametrize("kind", ["f16", "bf16"])
