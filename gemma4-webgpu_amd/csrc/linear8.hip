@@ -70,41 +70,49 @@ __device__ __forceinline__ void finish(const Linear8Args& a, f32x4 sum, unsigned
     if (valid && o < a.rows) store4(a.out, a.out_type, t * a.out_stride + o, y, a.wide, a.rows - o);
 }
 
-// Few tokens: 16 outputs by 16 CT tokens a workgroup, its waves take every Wth 128 of k.
-template <int CT, int W>
+// Few tokens: 16 RT outputs by 16 CT tokens a workgroup, its waves take every Wth 128 of k.
+template <int RT, int CT, int W>
 __global__ __launch_bounds__(W * 64) void k_linear8_few(const Linear8Args a) {
-    __shared__ f32x4 s_sum[W][CT][64];
+    __shared__ f32x4 s_sum[W][RT * CT][64];
     const unsigned lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
-    const unsigned o0 = blockIdx.y * 16, t0 = blockIdx.x * (16 * CT);
-    const uint8_t* w = a.w + (uint64_t)min(o0 + col, a.rows - 1) * a.n;
-    f32x4 acc[CT];
+    const unsigned o0 = blockIdx.x * (16 * RT), t0 = blockIdx.y * (16 * CT);
+    f32x4 acc[RT][CT];
 #pragma unroll
-    for (int ct = 0; ct < CT; ct++) acc[ct] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) acc[rt][ct] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     for (unsigned k0 = wave * 128; k0 < a.n; k0 += W * 128) {
         const unsigned k = k0 + 32 * g;
-        const Row32 wv = row32(w, k, a.n);
-        f16x8 wh[4];
+        Row32 w[RT], x[CT];
 #pragma unroll
-        for (int q = 0; q < 4; q++) wh[q] = widen8(wv, q);
+        for (int rt = 0; rt < RT; rt++) w[rt] = row32(a.w + (uint64_t)min(o0 + 16 * rt + col, a.rows - 1) * a.n, k, a.n);
 #pragma unroll
-        for (int ct = 0; ct < CT; ct++) {
-            const unsigned t = min(t0 + 16 * ct + col, a.n_tokens - 1);
-            const Row32 xv = row32(a.x + t * a.x_stride, k, a.n);
+        for (int ct = 0; ct < CT; ct++) x[ct] = row32(a.x + min(t0 + 16 * ct + col, a.n_tokens - 1) * a.x_stride, k, a.n);
 #pragma unroll
-            for (int q = 0; q < 4; q++) acc[ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh[q], widen8(xv, q), acc[ct], 0, 0, 0);
+        for (int q = 0; q < 4; q++) {
+            f16x8 wh[RT];
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) wh[rt] = widen8(w[rt], q);
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++) {
+                const f16x8 xh = widen8(x[ct], q);
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++) acc[rt][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh[rt], xh, acc[rt][ct], 0, 0, 0);
+            }
         }
     }
 #pragma unroll
-    for (int ct = 0; ct < CT; ct++) s_sum[wave][ct][lane] = acc[ct];
-    __syncthreads();
-    for (unsigned ct = wave; ct < CT; ct += W) {
-        f32x4 s = s_sum[0][ct][lane];
+    for (int rt = 0; rt < RT; rt++)
 #pragma unroll
-        for (int i = 1; i < W; i++) s += s_sum[i][ct][lane];
-        finish(a, s, o0, t0 + 16 * ct + col);
+        for (int ct = 0; ct < CT; ct++) s_sum[wave][rt * CT + ct][lane] = acc[rt][ct];
+    __syncthreads();
+    for (unsigned i = wave; i < RT * CT; i += W) {
+        f32x4 s = s_sum[0][i][lane];
+#pragma unroll
+        for (int w = 1; w < W; w++) s += s_sum[w][i][lane];
+        finish(a, s, o0 + 16 * (i / CT), t0 + 16 * (i % CT) + col);
     }
 }
-
 
 // ---- many tokens ---------------------------------------------------------------------
 //
@@ -148,26 +156,11 @@ struct TileArgs {
 
 // Tiles in an order that keeps the 32 workgroups of an XCD (workgroup b: XCD b % 8) on few rows of both operands at a
 // time: each XCD has a run of the order, in which eight token tiles go together.
-struct TileOrder {
-    uint32_t o_tiles, t_tiles, at, end, step;
-    __device__ TileOrder(uint32_t o, uint32_t t) : o_tiles(o), t_tiles(t) {
-        const uint32_t n = o * t, b = blockIdx.x;
-        if (gridDim.x % 8 == 0) {
-            at = n / 8 * (b % 8) + min(b % 8, n % 8) + b / 8;
-            end = n / 8 * (b % 8 + 1) + min(b % 8 + 1, n % 8);
-            step = gridDim.x / 8;
-        } else {
-            at = b;
-            end = n;
-            step = gridDim.x;
-        }
-    }
-    __device__ void place(uint32_t i, uint32_t& o, uint32_t& t) const {
-        const uint32_t group = i / (8 * o_tiles), r = i - group * 8 * o_tiles, wide = min(8u, t_tiles - group * 8);
-        o = r / wide;
-        t = group * 8 + r - o * wide;
-    }
-};
+__device__ __forceinline__ uint32_t tile_begin(uint32_t n, uint32_t part) { return n / 8 * part + min(part, n % 8); }
+__device__ __forceinline__ uint2 tile_place(uint32_t i, uint32_t o_tiles, uint32_t t_tiles) {  // x: outputs', y: tokens'
+    const uint32_t group = i / (8 * o_tiles), r = i - group * 8 * o_tiles, wide = min(8u, t_tiles - group * 8), o = r / wide;
+    return make_uint2(o, group * 8 + r - o * wide);
+}
 
 // f(0), f(1) .. f(N - 1), the numbers as types: what depends on them is settled when it is compiled.
 template <int... I, typename F>
@@ -179,7 +172,7 @@ __device__ __forceinline__ void each_of(F&& f) {
     each_of(std::make_integer_sequence<int, N>{}, f);
 }
 
-template <int WO, int WT, int RT, int CT, int kStages, uint32_t OT, bool LOW>
+template <int WO, int WT, int RT, int CT, int kStages, uint32_t OT, uint32_t LOW>  // LOW: the adapters' type, 0 none
 __global__ __launch_bounds__(64 * WO * WT, RT * CT >= 16 ? 1 : 2) void k_linear8_tiles(const TileArgs ta) {
     constexpr bool WIDE = OT == G4_F32;
     constexpr int W = WO * WT, OPS = RT + CT, READS = 2 * OPS, PAIRS = RT * CT;
@@ -190,32 +183,37 @@ __global__ __launch_bounds__(64 * WO * WT, RT * CT >= 16 ? 1 : 2) void k_linear8
     static_assert(BO % 64 == 0 && (BO + BT) % (64 * W) == 0, "whole waves of scales");
     __shared__ __attribute__((aligned(16))) uint8_t s_mem[SCALES + SLOTS * (BO + BT) * 4];
     const Linear8Args& a = ta.a;
-    const unsigned lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 31, g = lane >> 5;
+    const unsigned lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const unsigned wo = wave / WT * 32 * RT, wt = wave % WT * 32 * CT;
     const uint32_t lds = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)s_mem);
-    TileOrder order(ta.o_tiles, ta.t_tiles);
-    if (order.at >= order.end) return;
+    const uint32_t tiles = ta.o_tiles * ta.t_tiles, xcd = blockIdx.x % 8;
+    const bool even = gridDim.x % 8 == 0;
+    const uint32_t tile_0 = even ? tile_begin(tiles, xcd) + blockIdx.x / 8 : blockIdx.x;
+    const uint32_t tile_end = even ? tile_begin(tiles, xcd + 1) : tiles, tile_step = even ? gridDim.x / 8 : gridDim.x;
+    if (tile_0 >= tile_end) return;
     const unsigned stages = ((a.n + 2 * kStageK - 1) / (2 * kStageK)) * 2;  // of a tile; even
 
     // The DMA's side: pieces of 16 rows, DW of the weights' and DX of the tokens' a wave; a lane's offset from the tile.
-    const unsigned piece = ((lane & 3) ^ ((lane >> 4) & 3)) * 16;
     const uint8_t *d_w, *d_x;  // the tile's rows at the stage's k
     uint32_t from[DMAS];
-    unsigned d_k = 0, d_tile = order.at, d_slot = 0;
+    unsigned d_k = 0, d_tile = tile_0, d_slot = 0;
     uint32_t d_lds = 0;
     auto aim = [&]() __attribute__((always_inline)) {
-        uint32_t o, t;
-        order.place(d_tile, o, t);
+        const uint2 at = tile_place(d_tile, ta.o_tiles, ta.t_tiles);
+        const unsigned o = at.x, t = at.y;
+        unsigned l = lane;
+        asm volatile("" : "+v"(l));
+        const unsigned piece = ((l & 3) ^ ((l >> 4) & 3)) * 16;
         d_w = a.w + (uint64_t)(o * BO) * a.n;
         d_x = a.x + (uint64_t)(t * BT) * a.x_stride;
 #pragma unroll
         for (int j = 0; j < DMAS; j++) {
-            const unsigned r = 16 * (j < DW ? wave * DW + j : wave * DX + j - DW) + (lane >> 2);
+            const unsigned r = 16 * (j < DW ? wave * DW + j : wave * DX + j - DW) + (l >> 2);
             from[j] = (j < DW ? min(r, a.rows - 1 - o * BO) * a.n : min(r, a.n_tokens - 1 - t * BT) * (uint32_t)a.x_stride) + piece;
         }
 #pragma unroll
         for (unsigned first = wave * 64; first < BO + BT; first += 64 * W) {  // 64 of the weights' or of the tokens'
-            const unsigned i = first + lane;
+            const unsigned i = first + l;
             scale_dma(first < BO ? a.w_scales + min(o * BO + i, a.rows - 1) : a.x_scales + min(t * BT + i - BO, a.n_tokens - 1),
                       __builtin_amdgcn_readfirstlane(lds + SCALES + (d_slot * (BO + BT) + first) * 4));
         }
@@ -229,7 +227,9 @@ __global__ __launch_bounds__(64 * WO * WT, RT * CT >= 16 ? 1 : 2) void k_linear8
             stage_dma<at>(uniform_ptr(reinterpret_cast<const char*>(base)), from[j], to);
         } else {
             const uint8_t* p = base + from[j];
-            if (d_k + piece >= a.n) p = reinterpret_cast<const uint8_t*>(kZeros);
+            unsigned l = lane;
+            asm volatile("" : "+v"(l));
+            if (d_k + ((l & 3) ^ ((l >> 4) & 3)) * 16 >= a.n) p = reinterpret_cast<const uint8_t*>(kZeros);
             stage_dma<at>(p, to);
         }
     };
@@ -240,7 +240,7 @@ __global__ __launch_bounds__(64 * WO * WT, RT * CT >= 16 ? 1 : 2) void k_linear8
         d_x += kStageK;
         if (d_k == stages * kStageK) {
             d_k = 0;
-            if (d_tile + order.step < order.end) d_tile += order.step;
+            if (d_tile + tile_step < tile_end) d_tile += tile_step;
             aim();
         }
     };
@@ -252,8 +252,15 @@ __global__ __launch_bounds__(64 * WO * WT, RT * CT >= 16 ? 1 : 2) void k_linear8
     }
 
     // The matrix unit's side.
-    const unsigned swz = (col >> 2) & 3;
-    const unsigned off0 = col * kStageK + ((2 * g) ^ swz) * 16, off1 = col * kStageK + ((2 * g + 1) ^ swz) * 16;
+    unsigned off0, off1;  // of the lane's two pieces of a row
+    auto place = [&]() __attribute__((always_inline)) {
+        unsigned l = lane;
+        asm volatile("" : "+v"(l));
+        const unsigned col = l & 31, g = l >> 5, swz = (col >> 2) & 3;
+        off0 = col * kStageK + ((2 * g) ^ swz) * 16;
+        off1 = col * kStageK + ((2 * g + 1) ^ swz) * 16;
+    };
+    place();
     i32x8 reg[2][OPS];
     unsigned r_lds = 0;
     auto read = [&](i32x8 (&to)[OPS], auto i) __attribute__((always_inline)) {
@@ -307,7 +314,7 @@ __global__ __launch_bounds__(64 * WO * WT, RT * CT >= 16 ? 1 : 2) void k_linear8
     constexpr std::true_type kFirst{};  // of a tile: nothing to add to; the tile before may have left stores
     constexpr std::false_type kLater{};
 
-    for (unsigned i = order.at; i < order.end; i += order.step) {
+    for (unsigned i = tile_0; i < tile_end; i += tile_step) {
         stage(reg[0], reg[1], kFirst, kFirst);
         stage(reg[1], reg[0], kLater, kFirst);
 #pragma unroll 1
@@ -315,9 +322,11 @@ __global__ __launch_bounds__(64 * WO * WT, RT * CT >= 16 ? 1 : 2) void k_linear8
             stage(reg[0], reg[1], kLater, kLater);
             stage(reg[1], reg[0], kLater, kLater);
         }
-        uint32_t ot, tt;
-        order.place(i, ot, tt);
-        const unsigned o0 = ot * BO + wo, t0 = tt * BT + wt;
+        const uint2 at = tile_place(i, ta.o_tiles, ta.t_tiles);
+        const unsigned o0 = at.x * BO + wo, t0 = at.y * BT + wt;
+        unsigned el = lane;  // what follows from it is not kept beside the next tile's sums
+        asm volatile("" : "+v"(el));
+        const unsigned col = el & 31, g = el >> 5;
         const float* scales = reinterpret_cast<const float*>(s_mem + SCALES) + slot * (BO + BT);
         slot = (slot + 1) % SLOTS;
         stored = a.wide && o0 + 32 * RT <= a.rows && t0 + 32 * CT <= a.n_tokens;  // uniform: every lane stores whole pieces
@@ -333,10 +342,9 @@ __global__ __launch_bounds__(64 * WO * WT, RT * CT >= 16 ? 1 : 2) void k_linear8
 #pragma unroll
                     for (int e = 0; e < 4; e++) y[q][e] = acc[rt][ct][4 * q + e] * xs * ws[e];
                 });
-                if constexpr (LOW) {
+                if constexpr (LOW != 0) {
                     auto add = [&](int, int i, float v) __attribute__((always_inline)) { y[i / 4][i % 4] += v; };
-                    if (a.low == G4_F16) lora_up<32, 1, false>(a.l, o, t, id, add);
-                    else lora_up<32, 1, true>(a.l, o, t, id, add);
+                    lora_up<32, 1, LOW == G4_BF16, (PAIRS < 8)>(a.l, o, t, id, add);
                 }
                 if (!stored) {
 #pragma unroll
@@ -374,8 +382,9 @@ __global__ __launch_bounds__(64 * WO * WT, RT * CT >= 16 ? 1 : 2) void k_linear8
             });
         });
         if (!stored) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // an unknown number of stores: the counts begin anew
-        if constexpr (LOW) {  // the next tile's first operands once more: the adapters need the registers in between
+        if constexpr (LOW != 0) {  // the next tile's first operands once more: the adapters need the registers in between
             asm volatile("" ::: "memory");
+            place();
             const unsigned ahead = r_lds;
             r_lds = ahead == 0 ? (kStages - 1) * STAGE : ahead - STAGE;
             each_of<READS>([&](auto j) __attribute__((always_inline)) { read(reg[0], j); });
@@ -417,21 +426,23 @@ template <int WO, int WT, int RT, int CT, int NS>
 void launch_tiles(const Linear8Args& a, hipStream_t st) {
     constexpr uint32_t BO = 32 * WO * RT, BT = 32 * WT * CT;
     TileArgs t = {a, (a.rows + BO - 1) / BO, (a.n_tokens + BT - 1) / BT};
-    const uint32_t n = t.o_tiles * t.t_tiles, most = device_cus() * (WO * WT == 8 ? 1 : 2);
+    const uint32_t n = t.o_tiles * t.t_tiles, most = device_cus() * (BO * BT >= 65536 ? 1 : BO * BT >= 16384 ? 2 : 4);
     const dim3 grid(n < most ? n : most), block(64 * WO * WT);
     auto launch = [&](auto type) {
         constexpr uint32_t OT = decltype(type)::value;
-        if (a.low) G4_LAUNCH((k_linear8_tiles<WO, WT, RT, CT, NS, OT, true>), grid, block, 0, st, t);
-        else G4_LAUNCH((k_linear8_tiles<WO, WT, RT, CT, NS, OT, false>), grid, block, 0, st, t);
+        if (a.low == G4_F16) G4_LAUNCH((k_linear8_tiles<WO, WT, RT, CT, NS, OT, G4_F16>), grid, block, 0, st, t);
+        else if (a.low) G4_LAUNCH((k_linear8_tiles<WO, WT, RT, CT, NS, OT, G4_BF16>), grid, block, 0, st, t);
+        else G4_LAUNCH((k_linear8_tiles<WO, WT, RT, CT, NS, OT, 0>), grid, block, 0, st, t);
     };
     if (a.out_type == G4_F32) launch(std::integral_constant<uint32_t, G4_F32>{});
     else if (a.out_type == G4_F16) launch(std::integral_constant<uint32_t, G4_F16>{});
     else launch(std::integral_constant<uint32_t, G4_BF16>{});
 }
 
-template <int CT, int W>
+template <int RT, int CT, int W>
 void launch_few(const Linear8Args& a, hipStream_t st) {
-    G4_LAUNCH((k_linear8_few<CT, W>), dim3((a.n_tokens + 16 * CT - 1) / (16 * CT), (a.rows + 15) / 16), dim3(W * 64), 0, st, a);
+    const dim3 grid((a.rows + 16 * RT - 1) / (16 * RT), (a.n_tokens + 16 * CT - 1) / (16 * CT));
+    G4_LAUNCH((k_linear8_few<RT, CT, W>), grid, dim3(W * 64), 0, st, a);
 }
 
 }  // namespace
@@ -442,7 +453,7 @@ int g4_linear_e4m3_workspace_size(const g4_linear_e4m3_params* p, const g4_lora*
     if (!bytes) return fail(G4_EINVAL, "g4_linear_e4m3_workspace_size: bytes is NULL");
     const int rc = linear8_check(p, lora);
     if (rc) return rc;
-    *bytes = 16 + (lora ? lora_most_bytes(lora, p->n_tokens) : 0);
+    *bytes = 16 + (lora ? lora_bytes(lora, p->n_tokens) : 0);
     return G4_OK;
 }
 
@@ -486,8 +497,8 @@ int g4_linear_e4m3(const uint8_t* x, const float* x_scales, const uint8_t* weigh
         lora_launch_down(a.l, lora->type, x, G4_E4M3, xs, x_scales, st);
         G4_CHECK_LAUNCH("k_lora_down");
     }
-    if (p->n_tokens <= 16) launch_few<1, 4>(a, st);
-    else if (p->n_tokens <= 96 || xs >= (1u << 24)) launch_few<4, 4>(a, st);
+    if (p->n_tokens <= 16) launch_few<1, 1, 8>(a, st);
+    else if (p->n_tokens <= 96 || xs >= (1u << 24)) launch_few<2, 4, 8>(a, st);
     else if ((uint64_t)((a.rows + 255) / 256) * ((a.n_tokens + 255) / 256) >= device_cus() / 2) launch_tiles<2, 4, 4, 2, 4>(a, st);
     else launch_tiles<2, 2, 2, 2, 4>(a, st);
     G4_CHECK_LAUNCH("k_linear8");

@@ -3,12 +3,14 @@
 // [0, n_adapters).
 //
 // Two products. Down: u[t][i] = sum_k x[t][k] A[a][i][k], i over the segments' rank rows each,
-// left in the workspace as f32 partial sums of pieces of k (lora.hip). Up, here, as an
-// epilogue of whatever made the token's outputs: acc[o] += scale[a] sum_j u[s(o)][j] B[a][o][j].
+// left in the workspace in f32 (lora.hip). Up, here, as an epilogue of whatever made the token's
+// outputs: acc[o] += scale[a] sum_j u[s(o)][j] B[a][o][j].
 //
-// The up product runs on the 16-bit MFMA: u enters as the f16 parts of u 2^e (2^e: the token's
+// Where a tile's tokens share an adapter or two, the up product runs on the 16-bit MFMA: u enters as the f16 parts of u 2^e (2^e: the token's
 // largest |u| comes to lie in [2^14, 2^15)) and of what the first leaves, off by 2^-23 of itself or 2^-39
 // of the largest; with bf16 adapters as three bf16 parts, off by 2^-25. f32 products take eight times the cycles.
+// Where they have more, an adapter after the other would wait for memory each time (64 requests of 40 adapters: 43 us);
+// then every lane takes its own token's rows and adds the products in f32, all loads independent of each other.
 #pragma once
 
 #include "decode_core.h"
@@ -23,11 +25,11 @@ struct LoraDev {
     const void* __restrict__ b;        // [n_adapters][rows][rank]
     const float* __restrict__ scales;  // [n_adapters] or nullptr: 1
     const int32_t* __restrict__ ids;   // [n_tokens]
-    float* __restrict__ u;             // [splits][n_tokens][down]
+    float* __restrict__ u;             // [n_tokens][down]
     uint32_t n_adapters, rank, n, n_segs;
     uint32_t ends[4];                  // of the segments' outputs; those past n_segs as the last
     uint32_t rows, down;               // outputs; n_segs * rank
-    uint32_t splits, n_tokens;
+    uint32_t n_tokens;
 };
 
 __device__ __forceinline__ int lora_id(const LoraDev& l, unsigned t, bool valid) {
@@ -56,15 +58,70 @@ struct LoraTile<32> {
     static __device__ __forceinline__ float most(float x) { return max_xor32(x); }
 };
 
+constexpr int kLoraShared = 2;  // adapters of a tile that are taken one after the other
+
+template <bool BF>
+__device__ __forceinline__ float lora_dot8(u32x4 w, f32x4 x, f32x4 y, float sum) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float lo = BF ? __uint_as_float(w[i] << 16) : h2f((uint16_t)w[i]), hi = BF ? __uint_as_float(w[i] & 0xFFFF0000u) : h2f((uint16_t)(w[i] >> 16));
+        sum = __builtin_fmaf(lo, i < 2 ? x[2 * i] : y[2 * i - 4], sum);
+        sum = __builtin_fmaf(hi, i < 2 ? x[2 * i + 1] : y[2 * i - 3], sum);
+    }
+    return sum;
+}
+
 // Adds a column tile's adapters to NRT row tiles of outputs from o0 on, through add(rt, i, value) for each element of the
-// lane's: token `t` of column lane % M, its adapter `id`, -1 none. BF: bf16 adapters.
-template <int M, int NRT, bool BF, typename ADD>
+// lane's: token `t` of column lane % M, its adapter `id`, -1 none. BF: bf16 adapters. AHEAD: the next step's operands are
+// requested before this one's products, where the registers allow it.
+template <int M, int NRT, bool BF, bool AHEAD = true, typename ADD>
 __device__ __forceinline__ void lora_up(const LoraDev& l, unsigned o0, unsigned t, int id, ADD&& add) {
     using T = LoraTile<M>;
     constexpr int N = sizeof(typename T::acc) / 4;
-    const unsigned lane = threadIdx.x & 63, col = lane % M, g = lane / M;
+    unsigned lane = threadIdx.x & 63;
+    if constexpr (M == 32) asm volatile("" : "+v"(lane));  // what follows from it is not kept from call to call
+    const unsigned col = lane % M, g = lane / M;
     uint64_t left = __ballot(id >= 0);
-    while (left) {  // an adapter of the tile at a time; uniform
+    int others = 0;
+    for (uint64_t rest = left; rest && others <= kLoraShared; others++)  // uniform, as all below
+        rest &= ~__ballot(id == __builtin_amdgcn_readlane(id, __builtin_ctzll(rest)));
+    if (others > kLoraShared) {
+        const float alpha = id < 0 ? 0.0f : l.scales ? l.scales[id] : 1.0f;
+        const uint16_t* b = static_cast<const uint16_t*>(l.b) + (uint64_t)max(id, 0) * l.rows * l.rank;
+        unsigned first = 0;
+#pragma unroll 1
+        for (unsigned s = 0; s < l.n_segs; s++) {
+            const unsigned end = l.ends[s];
+            if (end > o0 && first < o0 + M * NRT) {
+                const float* u = l.u + (uint64_t)t * l.down + s * l.rank;
+                constexpr int P = AHEAD ? 4 : 2;  // outputs at a time
+#pragma unroll
+                for (int q = 0; q < NRT * N / P; q++) {
+                    const int rt = P * q / N, i = P * q % N;
+                    const unsigned o = o0 + M * rt + 8 * (i / 4) + 4 * g + i % 4;
+                    float sum[P] = {};
+                    const bool some = id >= 0 && o < end && o + P > first;
+#pragma unroll AHEAD ? 2 : 1
+                    for (unsigned j = 0; j < l.rank; j += 8) {
+                        if (!some) continue;
+                        const f32x4 x = ldg<f32x4>(u + j), y = ldg<f32x4>(u + j + 4);
+                        u32x4 w[P];
+#pragma unroll
+                        for (int e = 0; e < P; e++) w[e] = ldg<u32x4>(b + (uint64_t)min(o + e, l.rows - 1) * l.rank + j);
+#pragma unroll
+                        for (int e = 0; e < P; e++) sum[e] = lora_dot8<BF>(w[e], x, y, sum[e]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < P; e++)
+                        if (some && o + e >= first && o + e < end) add(rt, i + e, sum[e] * alpha);
+                    if constexpr (!AHEAD) __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            first = end;
+        }
+        return;
+    }
+    while (left) {  // an adapter of the tile at a time
         const int a = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
         left &= ~__ballot(id == a);
         const bool mine = id == a;
@@ -72,54 +129,65 @@ __device__ __forceinline__ void lora_up(const LoraDev& l, unsigned o0, unsigned 
         const uint16_t* b = static_cast<const uint16_t*>(l.b) + (uint64_t)a * l.rows * l.rank;
         unsigned first = 0;
 #pragma unroll 1
-        for (unsigned s = 0; s < l.n_segs; s++) {  // uniform
+        for (unsigned s = 0; s < l.n_segs; s++) {
             const unsigned end = l.ends[s];
             if (end > o0 && first < o0 + M * NRT) {
                 const unsigned steps = (l.rank + T::STEP - 1) / T::STEP;
+                const float* u = l.u + (uint64_t)t * l.down + s * l.rank + 8 * g;
                 typename T::acc d[NRT];
 #pragma unroll
                 for (int rt = 0; rt < NRT; rt++)
 #pragma unroll
                     for (int i = 0; i < N; i++) d[rt][i] = 0.0f;
-                const float* u = l.u + (uint64_t)t * l.down + s * l.rank;
-                const uint64_t piece = (uint64_t)l.n_tokens * l.down;
-                auto part = [&](unsigned j) __attribute__((always_inline)) {  // u[j .. j + 8)
-                    struct { f32x4 a, b; } v = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+                struct Ops {
+                    f32x4 x, y;
+                    u32x4 w[NRT];
+                };
+                auto fetch = [&](unsigned st) __attribute__((always_inline)) {
+                    const unsigned j = T::STEP * st + 8 * g;
+                    Ops r;
+                    r.x = f32x4{0, 0, 0, 0};
+                    r.y = f32x4{0, 0, 0, 0};
                     if (mine && j < l.rank) {
-                        for (unsigned p = 0; p < l.splits; p++) {
-                            v.a += ldg<f32x4>(u + p * piece + j);
-                            v.b += ldg<f32x4>(u + p * piece + j + 4);
-                        }
+                        r.x = ldg<f32x4>(u + T::STEP * st);
+                        r.y = ldg<f32x4>(u + T::STEP * st + 4);
                     }
-                    return v;
+#pragma unroll
+                    for (int rt = 0; rt < NRT; rt++) {
+                        const unsigned o = o0 + M * rt + col;
+                        r.w[rt] = u32x4{0, 0, 0, 0};
+                        if (o >= first && o < end && j < l.rank) r.w[rt] = ldg<u32x4>(b + (uint64_t)o * l.rank + j);
+                    }
+                    return r;
                 };
                 float up = 1.0f, down = 1.0f;
+                Ops held;
+                if constexpr (AHEAD) held = fetch(0);
                 if constexpr (!BF) {
                     float m = 0.0f;
+#pragma unroll M == 32 ? 2 : 4
                     for (unsigned st = 0; st < steps; st++) {
-                        const auto v = part(T::STEP * st + 8 * g);
+                        f32x4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
+                        if (mine && T::STEP * st + 8 * g < l.rank) {
+                            x = ldg<f32x4>(u + T::STEP * st);
+                            y = ldg<f32x4>(u + T::STEP * st + 4);
+                        }
 #pragma unroll
-                        for (int i = 0; i < 4; i++) m = fmaxf(m, fmaxf(fabsf(v.a[i]), fabsf(v.b[i])));
+                        for (int i = 0; i < 4; i++) m = fmaxf(m, fmaxf(fabsf(x[i]), fabsf(y[i])));
                     }
                     const unsigned e = max(__float_as_uint(T::most(m)) >> 23, 15u);
                     up = __uint_as_float((268u - e) << 23);
                     down = __uint_as_float((e - 14u) << 23);
                 }
+#pragma unroll 1
                 for (unsigned st = 0; st < steps; st++) {
-                    const unsigned j = T::STEP * st + 8 * g;
-                    const auto v = part(j);
+                    const Ops now = AHEAD ? held : fetch(st);
+                    if constexpr (AHEAD) held = fetch(st + 1);  // past the last: zeros
                     float x[8];
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        x[i] = v.a[i] * up;
-                        x[4 + i] = v.b[i] * up;
-                    }
-                    u32x4 w[NRT];
-#pragma unroll
-                    for (int rt = 0; rt < NRT; rt++) {
-                        const unsigned o = o0 + M * rt + col;
-                        w[rt] = u32x4{0, 0, 0, 0};
-                        if (o >= first && o < end && j < l.rank) w[rt] = ldg<u32x4>(b + (uint64_t)o * l.rank + j);
+                        x[i] = now.x[i] * up;
+                        x[4 + i] = now.y[i] * up;
                     }
                     if constexpr (BF) {
                         bf16x8 p0, p1, p2;
@@ -132,7 +200,7 @@ __device__ __forceinline__ void lora_up(const LoraDev& l, unsigned o0, unsigned 
                         }
 #pragma unroll
                         for (int rt = 0; rt < NRT; rt++) {
-                            const bf16x8 wb = __builtin_bit_cast(bf16x8, w[rt]);
+                            const bf16x8 wb = __builtin_bit_cast(bf16x8, now.w[rt]);
                             d[rt] = T::mfma(wb, p2, d[rt]);
                             d[rt] = T::mfma(wb, p1, d[rt]);
                             d[rt] = T::mfma(wb, p0, d[rt]);
@@ -146,7 +214,7 @@ __device__ __forceinline__ void lora_up(const LoraDev& l, unsigned o0, unsigned 
                         }
 #pragma unroll
                         for (int rt = 0; rt < NRT; rt++) {
-                            const f16x8 wh = __builtin_bit_cast(f16x8, w[rt]);
+                            const f16x8 wh = __builtin_bit_cast(f16x8, now.w[rt]);
                             d[rt] = T::mfma(wh, p1, d[rt]);
                             d[rt] = T::mfma(wh, p0, d[rt]);
                         }
@@ -168,10 +236,7 @@ __device__ __forceinline__ void lora_up(const LoraDev& l, unsigned o0, unsigned 
 // The description checked and brought into the kernels' form; `what` names the call.
 int lora_check(const char* what, const g4_lora* l);
 LoraDev lora_dev(const g4_lora* l, uint32_t n_tokens);
-// Pieces of k that the down product takes, the bytes of its sums, and those that serve every call of no more tokens.
-uint32_t lora_splits(const g4_lora* l, uint32_t n_tokens);
-size_t lora_bytes(const g4_lora* l, uint32_t n_tokens);
-size_t lora_most_bytes(const g4_lora* l, uint32_t n_tokens);
+size_t lora_bytes(const g4_lora* l, uint32_t n_tokens);  // of u
 // The down product of every token that has an adapter; d.u and d.ids set. x: rows of x_type, x_scales with e4m3.
 void lora_launch_down(const LoraDev& d, uint32_t lora_type, const void* x, uint32_t x_type, uint64_t x_stride,
                       const float* x_scales, hipStream_t st);

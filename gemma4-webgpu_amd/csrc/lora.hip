@@ -1,5 +1,7 @@
 // Low-rank adapters of many requests beside a projection made elsewhere
 // (g4_lora_add), and the down product that linear8.hip shares.
+#include <type_traits>
+
 #include "lora.h"
 
 namespace g4 {
@@ -34,121 +36,189 @@ __device__ __forceinline__ u32x4 e4m3_wide(u32x2 q) {
     return r;
 }
 
-constexpr int kDownWaves = 4;
+// Sixteen elements of a row as f32.
+__device__ __forceinline__ void wide16(f32x4 (&v)[4], const void* row, uint32_t type, unsigned k, bool in) {
+    const bool full = type == G4_F32;
+    const char* p = static_cast<const char*>(row) + (full ? 4 * k : 2 * k);
+    u32x4 r[4];
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        r[q] = u32x4{0, 0, 0, 0};
+        if (in && (full || q < 2)) r[q] = ldg<u32x4>(p + 16 * q);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+        const uint32_t w = r[i / 8][i % 8 / 2];
+        const float h = h2f((uint16_t)(w >> (16 * (i & 1)))), b = __uint_as_float((i & 1) ? w & 0xFFFF0000u : w << 16);
+        v[i / 4][i % 4] = full ? __uint_as_float(r[i / 4][i % 4]) : type == G4_F16 ? h : b;
+    }
+}
 
-// 16 CT tokens by groups of RT 16-row tiles of the adapters' down rows; blockIdx: (token tile, piece of k, which of the
-// tile's adapters). The four waves take every fourth 64-element chunk of the piece.
-template <int MODE, int CT, int RT>
+// Few tokens: a wave takes four down rows of one token, its lanes eight k at a time; no adapter waits for another.
+constexpr int kFewRows = 4, kFewWaves = 4;
+template <uint32_t XT, bool BF>
+__global__ __launch_bounds__(kFewWaves * 64) void k_lora_down_few(const DownArgs a) {
+    const LoraDev& l = a.l;
+    const unsigned lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = blockIdx.x;
+    const unsigned r0 = (blockIdx.y * kFewWaves + wave) * kFewRows;
+    const int id = lora_id(l, t, true);
+    if (id < 0 || r0 >= l.down) return;
+    const uint16_t* rows = static_cast<const uint16_t*>(l.a) + ((uint64_t)id * l.down + r0) * l.n;  // l.down: a multiple of 4
+    const char* x = static_cast<const char*>(a.x) + t * a.x_stride * (XT == G4_F32 ? 4 : XT == G4_E4M3 ? 1 : 2);
+    float sum[kFewRows] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 2
+    for (unsigned k0 = 0; k0 < l.n; k0 += 512) {
+        const unsigned k = k0 + 8 * lane;
+        if (k >= l.n) continue;
+        u32x4 w[kFewRows];
+#pragma unroll
+        for (int r = 0; r < kFewRows; r++) w[r] = ldg<u32x4>(rows + (uint64_t)r * l.n + k);
+        f32x4 lo, hi;
+        if constexpr (XT == G4_F32) {
+            lo = ldg<f32x4>(x + 4 * k);
+            hi = ldg<f32x4>(x + 4 * k + 16);
+        } else if constexpr (XT == G4_E4M3) {
+            const u32x2 q = ldg<u32x2>(x + k);
+            const auto a0 = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[0], false), a1 = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[0], true);
+            const auto b0 = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[1], false), b1 = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[1], true);
+            lo = f32x4{a0[0], a0[1], a1[0], a1[1]};
+            hi = f32x4{b0[0], b0[1], b1[0], b1[1]};
+        } else {
+            const u32x4 q = ldg<u32x4>(x + 2 * k);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float e = XT == G4_F16 ? h2f((uint16_t)q[i]) : __uint_as_float(q[i] << 16);
+                const float o = XT == G4_F16 ? h2f((uint16_t)(q[i] >> 16)) : __uint_as_float(q[i] & 0xFFFF0000u);
+                (i < 2 ? lo : hi)[2 * (i & 1)] = e;
+                (i < 2 ? lo : hi)[2 * (i & 1) + 1] = o;
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < kFewRows; r++) sum[r] = lora_dot8<BF>(w[r], lo, hi, sum[r]);
+    }
+#pragma unroll
+    for (int r = 0; r < kFewRows; r++) {
+#pragma unroll
+        for (int m = 1; m < 16; m <<= 1) sum[r] += __shfl_xor(sum[r], m);
+        sum[r] = add_xor32(add_xor16(sum[r]));
+    }
+    if (lane == 0) {
+        const float xs = a.x_scales ? a.x_scales[t] : 1.0f;
+        stg<f32x4>(l.u + (uint64_t)t * l.down + r0, f32x4{sum[0] * xs, sum[1] * xs, sum[2] * xs, sum[3] * xs});
+    }
+}
+
+// Many tokens: 32 tokens by 64 down rows a workgroup, whose eight waves take every eighth 64 k; the tile's adapters one
+// after the other.
+constexpr int kDownWaves = 8, kDownCols = 2, kDownRows = 4;  // 16-wide tiles
+template <int MODE>
 __global__ __launch_bounds__(kDownWaves * 64) void k_lora_down(const DownArgs a) {
+    constexpr int CT = kDownCols, RT = kDownRows;
     __shared__ f32x4 s_sum[kDownWaves][RT * CT][64];
     __shared__ int s_id[64];
     const LoraDev& l = a.l;
     const unsigned lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
-    const unsigned t0 = blockIdx.x * (16 * CT);
+    const unsigned t0 = blockIdx.x * (16 * CT), r0 = blockIdx.y * (16 * RT);
     // Lane: token of the tile. One wave's reading for all, so that they agree whatever happens to the array meanwhile.
     if (wave == 0) s_id[lane] = lora_id(l, t0 + lane, lane < 16 * CT && t0 + lane < l.n_tokens);
     __syncthreads();
     const int id = s_id[lane];
     uint64_t left = __ballot(id >= 0);
     const unsigned chunks = (l.n + 63) / 64;
-    unsigned nth = 0;
     while (left) {  // uniform over the workgroup
         const int ad = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
         const uint64_t with = __ballot(id == ad);
         left &= ~with;
-        if (nth++ % gridDim.z != blockIdx.z) continue;
-        for (unsigned r0 = 0; r0 < l.down; r0 += 16 * RT) {
-            f32x4 acc[RT][CT];
+        f32x4 acc[RT][CT];
 #pragma unroll
-            for (int rt = 0; rt < RT; rt++)
+        for (int rt = 0; rt < RT; rt++)
 #pragma unroll
-                for (int ct = 0; ct < CT; ct++) acc[rt][ct] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            for (unsigned c = blockIdx.y * kDownWaves + wave; c < chunks; c += gridDim.y * kDownWaves) {
-                const unsigned k = c * 64 + g * 16;  // the lane's 16 elements
-                const bool in = k < l.n;
-                if constexpr (MODE == kDownF32) {
-                    f32x4 w[RT][4];
+            for (int ct = 0; ct < CT; ct++) acc[rt][ct] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (unsigned c = wave; c < chunks; c += kDownWaves) {
+            const unsigned k = c * 64 + g * 16;  // the lane's 16 elements
+            const bool in = k < l.n;
+            if constexpr (MODE == kDownF32) {
+                f32x4 x[CT][4];
 #pragma unroll
-                    for (int rt = 0; rt < RT; rt++) {
-                        const unsigned row = min(r0 + 16 * rt + col, l.down - 1);
-                        const uint64_t at = ((uint64_t)ad * l.down + row) * l.n + k;
+                for (int ct = 0; ct < CT; ct++) {
+                    const unsigned t = min(t0 + 16 * ct + col, l.n_tokens - 1);
+                    wide16(x[ct], static_cast<const char*>(a.x) + t * a.x_stride * (a.x_type == G4_F32 ? 4 : 2), a.x_type, k, in);
+                }
 #pragma unroll
-                        for (int q = 0; q < 4; q++) w[rt][q] = in ? load4(l.a, a.a_type, at + 4 * q, true, 4) : f32x4{0, 0, 0, 0};
+                for (int rt = 0; rt < RT; rt++) {
+                    const unsigned row = min(r0 + 16 * rt + col, l.down - 1);
+                    f32x4 w[4];
+                    wide16(w, static_cast<const uint16_t*>(l.a) + ((uint64_t)ad * l.down + row) * l.n, a.a_type, k, in);
+#pragma unroll
+                    for (int e = 0; e < 16; e++)
+#pragma unroll
+                        for (int ct = 0; ct < CT; ct++)
+                            acc[rt][ct] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[e / 4][e % 4], x[ct][e / 4][e % 4], acc[rt][ct], 0, 0, 0);
+                }
+            } else {
+                constexpr bool BF = MODE == kDownBf16 || MODE == kDownE4m3Bf16;
+                u32x4 w[RT][2], x[CT][2];
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++) {
+                    const unsigned row = min(r0 + 16 * rt + col, l.down - 1);
+                    const uint16_t* p = static_cast<const uint16_t*>(l.a) + ((uint64_t)ad * l.down + row) * l.n + k;
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        w[rt][h] = u32x4{0, 0, 0, 0};
+                        if (in) w[rt][h] = ldg<u32x4>(p + 8 * h);
                     }
+                }
 #pragma unroll
-                    for (int ct = 0; ct < CT; ct++) {
-                        if (!((with >> (16 * ct)) & 0xFFFF)) continue;
-                        const unsigned t = min(t0 + 16 * ct + col, l.n_tokens - 1);
-                        f32x4 x[4];
-#pragma unroll
-                        for (int q = 0; q < 4; q++)
-                            x[q] = in ? load4(a.x, a.x_type, t * a.x_stride + k + 4 * q, true, 4) : f32x4{0, 0, 0, 0};
-#pragma unroll
-                        for (int rt = 0; rt < RT; rt++)
-#pragma unroll
-                            for (int e = 0; e < 16; e++)
-                                acc[rt][ct] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[rt][e / 4][e % 4], x[e / 4][e % 4], acc[rt][ct], 0, 0, 0);
+                for (int ct = 0; ct < CT; ct++) {
+                    const unsigned t = min(t0 + 16 * ct + col, l.n_tokens - 1);
+                    x[ct][0] = x[ct][1] = u32x4{0, 0, 0, 0};
+                    if constexpr (MODE == kDownE4m3F16 || MODE == kDownE4m3Bf16) {
+                        u32x4 q = {0, 0, 0, 0};
+                        if (in) q = ldg<u32x4>(static_cast<const uint8_t*>(a.x) + t * a.x_stride + k);
+                        x[ct][0] = e4m3_wide<BF>(u32x2{q[0], q[1]});
+                        x[ct][1] = e4m3_wide<BF>(u32x2{q[2], q[3]});
+                    } else {
+                        const uint16_t* p = static_cast<const uint16_t*>(a.x) + t * a.x_stride + k;
+                        if (in) x[ct][0] = ldg<u32x4>(p);
+                        if (in) x[ct][1] = ldg<u32x4>(p + 8);
                     }
-                } else {
-                    constexpr bool BF = MODE == kDownBf16 || MODE == kDownE4m3Bf16;
-                    u32x4 w[RT][2];
+                }
 #pragma unroll
-                    for (int rt = 0; rt < RT; rt++) {
-                        const unsigned row = min(r0 + 16 * rt + col, l.down - 1);
-                        const uint16_t* p = static_cast<const uint16_t*>(l.a) + ((uint64_t)ad * l.down + row) * l.n + k;
-                        w[rt][0] = in ? ldg<u32x4>(p) : u32x4{0, 0, 0, 0};
-                        w[rt][1] = in ? ldg<u32x4>(p + 8) : u32x4{0, 0, 0, 0};
-                    }
+                for (int h = 0; h < 2; h++)
 #pragma unroll
-                    for (int ct = 0; ct < CT; ct++) {
-                        if (!((with >> (16 * ct)) & 0xFFFF)) continue;
-                        const unsigned t = min(t0 + 16 * ct + col, l.n_tokens - 1);
-                        u32x4 x[2];
-                        if constexpr (MODE == kDownE4m3F16 || MODE == kDownE4m3Bf16) {
-                            const u32x4 q = in ? ldg<u32x4>(static_cast<const uint8_t*>(a.x) + t * a.x_stride + k) : u32x4{0, 0, 0, 0};
-                            x[0] = e4m3_wide<BF>(u32x2{q[0], q[1]});
-                            x[1] = e4m3_wide<BF>(u32x2{q[2], q[3]});
-                        } else {
-                            const uint16_t* p = static_cast<const uint16_t*>(a.x) + t * a.x_stride + k;
-                            x[0] = in ? ldg<u32x4>(p) : u32x4{0, 0, 0, 0};
-                            x[1] = in ? ldg<u32x4>(p + 8) : u32x4{0, 0, 0, 0};
+                    for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                        for (int ct = 0; ct < CT; ct++) {
+                            if constexpr (BF)
+                                acc[rt][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                                    __builtin_bit_cast(bf16x8, w[rt][h]), __builtin_bit_cast(bf16x8, x[ct][h]), acc[rt][ct], 0, 0, 0);
+                            else
+                                acc[rt][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                    __builtin_bit_cast(f16x8, w[rt][h]), __builtin_bit_cast(f16x8, x[ct][h]), acc[rt][ct], 0, 0, 0);
                         }
-#pragma unroll
-                        for (int rt = 0; rt < RT; rt++)
-#pragma unroll
-                            for (int h = 0; h < 2; h++) {
-                                if constexpr (BF)
-                                    acc[rt][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                                        __builtin_bit_cast(bf16x8, w[rt][h]), __builtin_bit_cast(bf16x8, x[h]), acc[rt][ct], 0, 0, 0);
-                                else
-                                    acc[rt][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                                        __builtin_bit_cast(f16x8, w[rt][h]), __builtin_bit_cast(f16x8, x[h]), acc[rt][ct], 0, 0, 0);
-                            }
-                    }
-                }
             }
-#pragma unroll
-            for (int rt = 0; rt < RT; rt++)
-#pragma unroll
-                for (int ct = 0; ct < CT; ct++) s_sum[wave][rt * CT + ct][lane] = acc[rt][ct];
-            __syncthreads();
-            for (unsigned i = wave; i < RT * CT; i += kDownWaves) {
-                const unsigned rt = i / CT, ct = i % CT, t = t0 + 16 * ct + col, row = r0 + 16 * rt + 4 * g;
-                f32x4 s = s_sum[0][i][lane];
-#pragma unroll
-                for (int w = 1; w < kDownWaves; w++) s += s_sum[w][i][lane];
-                if (((with >> (16 * ct + col)) & 1) && row < l.down) {  // down and row: multiples of 4
-                    if (a.x_scales) s *= a.x_scales[t];
-                    stg<f32x4>(l.u + ((uint64_t)blockIdx.y * l.n_tokens + t) * l.down + row, s);
-                }
-            }
-            __syncthreads();
         }
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++) s_sum[wave][rt * CT + ct][lane] = acc[rt][ct];
+        __syncthreads();
+        for (unsigned i = wave; i < RT * CT; i += kDownWaves) {
+            const unsigned rt = i / CT, ct = i % CT, t = t0 + 16 * ct + col, row = r0 + 16 * rt + 4 * g;
+            f32x4 s = s_sum[0][i][lane];
+#pragma unroll
+            for (int w = 1; w < kDownWaves; w++) s += s_sum[w][i][lane];
+            if (((with >> (16 * ct + col)) & 1) && row < l.down) {  // down and row: multiples of 4
+                if (a.x_scales) s *= a.x_scales[t];
+                stg<f32x4>(l.u + (uint64_t)t * l.down + row, s);
+            }
+        }
+        __syncthreads();
     }
 }
 
-// out = base + the adapters' part. A wave: 16 tokens by 64 outputs.
-constexpr int kUpTiles = 4, kUpWaves = 4;
+// out = base + the adapters' part. A wave: 16 tokens by TILES * 16 outputs.
+constexpr int kUpWaves = 4;
 struct UpArgs {
     LoraDev l;
     const void* base;  // may be out
@@ -156,23 +226,23 @@ struct UpArgs {
     uint64_t base_stride, out_stride;
     uint32_t type, wide;
 };
-template <bool BF>
+template <int TILES, bool BF>
 __global__ __launch_bounds__(kUpWaves * 64) void k_lora_up(const UpArgs a) {
     const LoraDev& l = a.l;
     const unsigned lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
-    const unsigned t = blockIdx.x * 16 + (lane & 15), o0 = (blockIdx.y * kUpWaves + wave) * (16 * kUpTiles);
+    const unsigned t = blockIdx.x * 16 + (lane & 15), o0 = (blockIdx.y * kUpWaves + wave) * (16 * TILES);
     if (o0 >= l.rows) return;
     const bool valid = t < l.n_tokens;
     const int id = lora_id(l, t, valid);
-    f32x4 acc[kUpTiles];
+    f32x4 acc[TILES];
 #pragma unroll
-    for (int rt = 0; rt < kUpTiles; rt++) {
+    for (int rt = 0; rt < TILES; rt++) {
         const unsigned o = o0 + 16 * rt + 4 * g;
         acc[rt] = valid && o < l.rows ? load4(a.base, a.type, t * a.base_stride + o, a.wide, l.rows - o) : f32x4{0, 0, 0, 0};
     }
-    lora_up<16, kUpTiles, BF>(l, o0, t, id, [&](int rt, int i, float v) __attribute__((always_inline)) { acc[rt][i] += v; });
+    lora_up<16, TILES, BF>(l, o0, t, id, [&](int rt, int i, float v) __attribute__((always_inline)) { acc[rt][i] += v; });
 #pragma unroll
-    for (int rt = 0; rt < kUpTiles; rt++) {
+    for (int rt = 0; rt < TILES; rt++) {
         const unsigned o = o0 + 16 * rt + 4 * g;
         if (valid && o < l.rows) store4(a.out, a.type, t * a.out_stride + o, acc[rt], a.wide, l.rows - o);
     }
@@ -213,42 +283,36 @@ LoraDev lora_dev(const g4_lora* l, uint32_t n_tokens) {
     d.rows = end;
     d.down = l->n_segs * l->rank;
     d.n_tokens = n_tokens;
-    d.splits = lora_splits(l, n_tokens);
     return d;
 }
 
-uint32_t lora_splits(const g4_lora* l, uint32_t n_tokens) {
-    if (n_tokens == 0) return 1;
-    const uint32_t per = n_tokens > 256 ? 64 : 16, tiles = (n_tokens + per - 1) / per, chunks = (l->n + 63) / 64;
-    uint32_t splits = (chunks + kDownWaves - 1) / kDownWaves;  // a chunk a wave at least
-    const uint32_t fill = (device_cus() + tiles - 1) / tiles;
-    if (splits > fill) splits = fill;
-    if (splits > 8) splits = 8;
-    return splits;
-}
-size_t lora_bytes(const g4_lora* l, uint32_t n_tokens) {
-    return ((size_t)lora_splits(l, n_tokens) * n_tokens * l->n_segs * l->rank * 4 + 15) & ~(size_t)15;
-}
-// splits * n <= 64 (CUs + tiles - 1) for every n up to n_tokens, and splits <= 8.
-size_t lora_most_bytes(const g4_lora* l, uint32_t n_tokens) {
-    const uint64_t few = 8ull * n_tokens, many = 64ull * device_cus() + n_tokens + 64;
-    return (size_t)(few < many ? few : many) * l->n_segs * l->rank * 4 + 16;
-}
+size_t lora_bytes(const g4_lora* l, uint32_t n_tokens) { return (size_t)n_tokens * l->n_segs * l->rank * 4 + 16; }
+
+// Few tokens: a wave a token and four rows reads its rows and no others' (64 requests of 40 adapters, n 1536); from
+// some hundred tokens on, the matrix units' tiles read an adapter once for 32 of them.
+constexpr uint32_t kLoraFewTokens = 128;
 
 template <int MODE>
 static void launch_down(const DownArgs& a, hipStream_t st) {
-    const uint32_t T = a.l.n_tokens;
-    if (T > 256) {
-        G4_LAUNCH((k_lora_down<MODE, 4, 2>), dim3((T + 63) / 64, a.l.splits, 1), dim3(kDownWaves * 64), 0, st, a);
-    } else {
-        G4_LAUNCH((k_lora_down<MODE, 1, 4>), dim3((T + 15) / 16, a.l.splits, T < 16 ? T : 16), dim3(kDownWaves * 64), 0, st, a);
-    }
+    const dim3 grid((a.l.n_tokens + 16 * kDownCols - 1) / (16 * kDownCols), (a.l.down + 16 * kDownRows - 1) / (16 * kDownRows));
+    G4_LAUNCH((k_lora_down<MODE>), grid, dim3(kDownWaves * 64), 0, st, a);
+}
+template <uint32_t XT>
+static void launch_down_few(const DownArgs& a, hipStream_t st) {
+    const dim3 grid(a.l.n_tokens, (a.l.down + kFewRows * kFewWaves - 1) / (kFewRows * kFewWaves));
+    if (a.a_type == G4_BF16) G4_LAUNCH((k_lora_down_few<XT, true>), grid, dim3(kFewWaves * 64), 0, st, a);
+    else G4_LAUNCH((k_lora_down_few<XT, false>), grid, dim3(kFewWaves * 64), 0, st, a);
 }
 
 void lora_launch_down(const LoraDev& d, uint32_t lora_type, const void* x, uint32_t x_type, uint64_t x_stride,
                       const float* x_scales, hipStream_t st) {
-    DownArgs a = {d, x, x_scales, x_stride, x_type, lora_type};
-    if (x_type == G4_E4M3) {
+    const DownArgs a = {d, x, x_scales, x_stride, x_type, lora_type};
+    if (d.n_tokens <= kLoraFewTokens) {
+        if (x_type == G4_F32) launch_down_few<G4_F32>(a, st);
+        else if (x_type == G4_F16) launch_down_few<G4_F16>(a, st);
+        else if (x_type == G4_BF16) launch_down_few<G4_BF16>(a, st);
+        else launch_down_few<G4_E4M3>(a, st);
+    } else if (x_type == G4_E4M3) {
         if (lora_type == G4_F16) launch_down<kDownE4m3F16>(a, st);
         else launch_down<kDownE4m3Bf16>(a, st);
     } else if (x_type == lora_type) {
@@ -270,7 +334,7 @@ int g4_lora_workspace_size(const g4_lora* lora, uint32_t n_tokens, size_t* bytes
     const int rc = lora_check("loraAdd", lora);
     if (rc) return rc;
     if (n_tokens > kMaxRows) return fail(G4_EINVAL, "loraAdd: %u tokens (at most 2^22)", n_tokens);
-    *bytes = lora_most_bytes(lora, n_tokens);
+    *bytes = lora_bytes(lora, n_tokens);
     return G4_OK;
 }
 
@@ -311,9 +375,14 @@ int g4_lora_add(const g4_lora* lora, const int32_t* adapter_ids, const void* x, 
     a.out_stride = os;
     a.type = p->out_type;
     a.wide = aligned(base, 4 * width) && aligned(out, 4 * width) && bs % 4 == 0 && os % 4 == 0;
-    const dim3 grid((p->n_tokens + 15) / 16, (d.rows + 16 * kUpTiles * kUpWaves - 1) / (16 * kUpTiles * kUpWaves));
-    if (lora->type == G4_F16) G4_LAUNCH((k_lora_up<false>), grid, dim3(kUpWaves * 64), 0, as_stream(stream), a);
-    else G4_LAUNCH((k_lora_up<true>), grid, dim3(kUpWaves * 64), 0, as_stream(stream), a);
+    auto launch = [&](auto tiles) {
+        constexpr int TILES = decltype(tiles)::value, per = 16 * TILES * kUpWaves;
+        const dim3 grid((p->n_tokens + 15) / 16, (d.rows + per - 1) / per), block(kUpWaves * 64);
+        if (lora->type == G4_F16) G4_LAUNCH((k_lora_up<TILES, false>), grid, block, 0, as_stream(stream), a);
+        else G4_LAUNCH((k_lora_up<TILES, true>), grid, block, 0, as_stream(stream), a);
+    };
+    if (p->n_tokens <= kLoraFewTokens) launch(std::integral_constant<int, 1>{});  // more waves, each waiting for less
+    else launch(std::integral_constant<int, 4>{});
     G4_CHECK_LAUNCH("k_lora_up");
     return G4_OK;
 }
