@@ -53,14 +53,26 @@ __device__ __forceinline__ f16x8 widen8(const Row32& r, int q) {  // the q-th ei
     return widen8(r.v[q / 2][2 * (q & 1)], r.v[q / 2][2 * (q & 1) + 1]);
 }
 
-// Sums of one 16-output tile: scales, adapters, the store.
-__device__ __forceinline__ void finish(const Linear8Args& a, f32x4 sum, unsigned o0, unsigned t) {
-    const unsigned lane = threadIdx.x & 63, g = lane >> 4, o = o0 + 4 * g;
+// The scales of a 16-output tile's element of the lane's.
+struct TileScales {
+    float x;
+    f32x4 w;
+};
+__device__ __forceinline__ TileScales tile_scales(const Linear8Args& a, unsigned o0, unsigned t) {
+    const unsigned o = o0 + 4 * ((threadIdx.x & 63) >> 4);
+    TileScales s;
+    s.x = a.x_scales[min(t, a.n_tokens - 1)];
+#pragma unroll
+    for (int i = 0; i < 4; i++) s.w[i] = a.w_scales[min(o + i, a.rows - 1)];
+    return s;
+}
+// Its sums scaled, the adapters' part added, and stored.
+__device__ __forceinline__ void finish(const Linear8Args& a, f32x4 sum, const TileScales& s, unsigned o0, unsigned t) {
+    const unsigned o = o0 + 4 * ((threadIdx.x & 63) >> 4);
     const bool valid = t < a.n_tokens;
-    const float xs = valid ? a.x_scales[t] : 0.0f;
     f32x4 y;
 #pragma unroll
-    for (int i = 0; i < 4; i++) y[i] = sum[i] * xs * (o + i < a.rows ? a.w_scales[o + i] : 0.0f);
+    for (int i = 0; i < 4; i++) y[i] = sum[i] * s.x * s.w[i];
     if (a.low) {
         const int id = lora_id(a.l, t, valid);
         auto add = [&](int, int i, float v) __attribute__((always_inline)) { y[i] += v; };
@@ -81,21 +93,35 @@ __global__ __launch_bounds__(W * 64) void k_linear8_few(const Linear8Args a) {
     for (int rt = 0; rt < RT; rt++)
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) acc[rt][ct] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (unsigned k0 = wave * 128; k0 < a.n; k0 += W * 128) {
-        const unsigned k = k0 + 32 * g;
+    const uint8_t *wp[RT], *xp[CT];
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) wp[rt] = a.w + (uint64_t)min(o0 + 16 * rt + col, a.rows - 1) * a.n;
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) xp[ct] = a.x + min(t0 + 16 * ct + col, a.n_tokens - 1) * a.x_stride;
+    struct Operands {
         Row32 w[RT], x[CT];
+    };
+    auto fetch = [&](unsigned k) __attribute__((always_inline)) {
+        Operands r;
 #pragma unroll
-        for (int rt = 0; rt < RT; rt++) w[rt] = row32(a.w + (uint64_t)min(o0 + 16 * rt + col, a.rows - 1) * a.n, k, a.n);
+        for (int rt = 0; rt < RT; rt++) r.w[rt] = row32(wp[rt], k, a.n);
 #pragma unroll
-        for (int ct = 0; ct < CT; ct++) x[ct] = row32(a.x + min(t0 + 16 * ct + col, a.n_tokens - 1) * a.x_stride, k, a.n);
+        for (int ct = 0; ct < CT; ct++) r.x[ct] = row32(xp[ct], k, a.n);
+        return r;
+    };
+    // The end's scales come with the first operands.
+    const unsigned first = wave < RT * CT ? wave : 0;
+    const TileScales scales = tile_scales(a, o0 + 16 * (first / CT), t0 + 16 * (first % CT) + col);
+    for (unsigned k0 = wave * 128; k0 < a.n; k0 += W * 128) {
+        const Operands now = fetch(k0 + 32 * g);
 #pragma unroll
         for (int q = 0; q < 4; q++) {
             f16x8 wh[RT];
 #pragma unroll
-            for (int rt = 0; rt < RT; rt++) wh[rt] = widen8(w[rt], q);
+            for (int rt = 0; rt < RT; rt++) wh[rt] = widen8(now.w[rt], q);
 #pragma unroll
             for (int ct = 0; ct < CT; ct++) {
-                const f16x8 xh = widen8(x[ct], q);
+                const f16x8 xh = widen8(now.x[ct], q);
 #pragma unroll
                 for (int rt = 0; rt < RT; rt++) acc[rt][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh[rt], xh, acc[rt][ct], 0, 0, 0);
             }
@@ -110,7 +136,8 @@ __global__ __launch_bounds__(W * 64) void k_linear8_few(const Linear8Args a) {
         f32x4 s = s_sum[0][i][lane];
 #pragma unroll
         for (int w = 1; w < W; w++) s += s_sum[w][i][lane];
-        finish(a, s, o0 + 16 * (i / CT), t0 + 16 * (i % CT) + col);
+        const unsigned o = o0 + 16 * (i / CT), t = t0 + 16 * (i % CT) + col;
+        finish(a, s, i == wave ? scales : tile_scales(a, o, t), o, t);
     }
 }
 
@@ -180,7 +207,7 @@ __global__ __launch_bounds__(64 * WO * WT, RT * CT >= 16 ? 1 : 2) void k_linear8
     constexpr int DW = BO / 16 / W, DX = BT / 16 / W, DMAS = DW + DX;  // requests a wave and stage
     static_assert(BO % (16 * W) == 0 && BT % (16 * W) == 0, "even shares");
     constexpr unsigned SLOTS = 4, SCALES = kStages * STAGE;  // scales of up to four tiles: the DMA is two tiles ahead at most
-    static_assert(BO % 64 == 0 && (BO + BT) % (64 * W) == 0, "whole waves of scales");
+    static_assert(BO % 64 == 0 && BT % 64 == 0, "whole waves of scales");
     __shared__ __attribute__((aligned(16))) uint8_t s_mem[SCALES + SLOTS * (BO + BT) * 4];
     const Linear8Args& a = ta.a;
     const unsigned lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -297,7 +324,7 @@ __global__ __launch_bounds__(64 * WO * WT, RT * CT >= 16 ? 1 : 2) void k_linear8
                 });
             }
             // The reads in the first part, the DMA's requests all along.
-            constexpr int by = STEPS * 3 / 4;
+            constexpr int by = STEPS > 1 ? STEPS * 3 / 4 : 1;
             constexpr int r0 = m < by ? m * READS / by : READS, r1 = m + 1 < by ? (m + 1) * READS / by : READS;
             each_of<r1 - r0>([&](auto i) __attribute__((always_inline)) { read(next, std::integral_constant<int, r0 + i>{}); });
             constexpr int d0 = m * DMAS / STEPS, d1 = (m + 1) * DMAS / STEPS;
@@ -445,6 +472,22 @@ void launch_few(const Linear8Args& a, hipStream_t st) {
     G4_LAUNCH((k_linear8_few<RT, CT, W>), grid, dim3(W * 64), 0, st, a);
 }
 
+// The largest tile that there are about enough of for the compute units, as long as there are; else tiles of 16 or 32
+// whose waves share k (us, n 1536; tiles of 256 / 128 / 64 / few): 1024 tokens by 12288 outputs 29.4 / 33.6 / 40.5 / -,
+// 256 by 12288 22.5 / 12.7 / 14.7 / 36.6, 1024 by 2560 (f32) 43 / 22.9 / 17.8 / 30.7, 64 by 12288 19.2 / 11.1 / 7.1 / 12.2,
+// 256 by 2560 - / 21.8 / 11.0 / 11.4, 128 by 2560 - / 21.2 / 10.6 / 7.6, 64 by 2560 - / 20.3 / 10.6 / 5.8.
+void launch_linear8(const Linear8Args& a, hipStream_t st) {
+    auto tiles = [&](uint32_t side) { return (uint64_t)((a.rows + side - 1) / side) * ((a.n_tokens + side - 1) / side); };
+    const uint64_t cus = device_cus();
+    const bool staged = a.x_stride < (1u << 24);  // a tile's offsets fit 32 bits
+    if (staged && tiles(256) >= cus * 3 / 4) launch_tiles<2, 4, 4, 2, 4>(a, st);
+    else if (staged && tiles(128) >= cus * 3 / 4) launch_tiles<2, 2, 2, 2, 4>(a, st);
+    else if (staged && tiles(64) >= cus * 5 / 8) launch_tiles<2, 2, 1, 1, 4>(a, st);
+    else if (a.n_tokens <= 16) launch_few<1, 1, 8>(a, st);
+    else if (a.n_tokens <= 96) launch_few<2, 2, 8>(a, st);
+    else launch_few<2, 4, 8>(a, st);
+}
+
 }  // namespace
 
 extern "C" {
@@ -497,10 +540,7 @@ int g4_linear_e4m3(const uint8_t* x, const float* x_scales, const uint8_t* weigh
         lora_launch_down(a.l, lora->type, x, G4_E4M3, xs, x_scales, st);
         G4_CHECK_LAUNCH("k_lora_down");
     }
-    if (p->n_tokens <= 16) launch_few<1, 1, 8>(a, st);
-    else if (p->n_tokens <= 96 || xs >= (1u << 24)) launch_few<2, 4, 8>(a, st);
-    else if ((uint64_t)((a.rows + 255) / 256) * ((a.n_tokens + 255) / 256) >= device_cus() / 2) launch_tiles<2, 4, 4, 2, 4>(a, st);
-    else launch_tiles<2, 2, 2, 2, 4>(a, st);
+    launch_linear8(a, st);
     G4_CHECK_LAUNCH("k_linear8");
     return G4_OK;
 }
