@@ -361,29 +361,35 @@ __global__ __launch_bounds__(64 * WO * WT, RT * CT >= 16 ? 1 : 2) void k_linear8
             const unsigned t = t0 + 32 * ct + col;
             const float xs = scales[BO + wt + 32 * ct + col];
             const int id = LOW ? lora_id(a.l, t, t < a.n_tokens) : -1;
+            constexpr int TOGETHER = LOW != 0 && PAIRS < 8 ? RT : 1;  // row tiles that share the adapters' sums of a token
+            f32x4 y[TOGETHER][4];
             each_of<RT>([&](auto rt) __attribute__((always_inline)) {
                 const unsigned o = o0 + 32 * rt;
-                f32x4 y[4];
-                each_of<4>([&](auto q) __attribute__((always_inline)) {
-                    const f32x4 ws = *reinterpret_cast<const f32x4*>(scales + wo + 32 * rt + 8 * q + 4 * g);
+                if constexpr (rt % TOGETHER == 0) {
+                    each_of<TOGETHER>([&](auto r) __attribute__((always_inline)) {
+                        each_of<4>([&](auto q) __attribute__((always_inline)) {
+                            const f32x4 ws = *reinterpret_cast<const f32x4*>(scales + wo + 32 * (rt + r) + 8 * q + 4 * g);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) y[q][e] = acc[rt][ct][4 * q + e] * xs * ws[e];
-                });
-                if constexpr (LOW != 0) {
-                    auto add = [&](int, int i, float v) __attribute__((always_inline)) { y[i / 4][i % 4] += v; };
-                    lora_up<32, 1, LOW == G4_BF16, (PAIRS < 8)>(a.l, o, t, id, add);
+                            for (int e = 0; e < 4; e++) y[r][q][e] = acc[rt + r][ct][4 * q + e] * xs * ws[e];
+                        });
+                    });
+                    if constexpr (LOW != 0) {
+                        auto add = [&](int r, int i, float v) __attribute__((always_inline)) { y[r][i / 4][i % 4] += v; };
+                        lora_up<32, TOGETHER, LOW == G4_BF16, (PAIRS < 8)>(a.l, o, t, id, add);
+                    }
                 }
+                const f32x4(&yr)[4] = y[rt % TOGETHER];
                 if (!stored) {
 #pragma unroll
                     for (int q = 0; q < 4; q++) {
                         const unsigned oq = o + 8 * q + 4 * g;
                         if (t < a.n_tokens && oq < a.rows)
-                            store4(a.out, OT, t * a.out_stride + oq, y[q], a.wide, a.rows - oq);
+                            store4(a.out, OT, t * a.out_stride + oq, yr[q], a.wide, a.rows - oq);
                     }
                 } else if constexpr (WIDE) {
                     float* out = static_cast<float*>(a.out) + t * a.out_stride + o + 4 * g;
 #pragma unroll
-                    for (int q = 0; q < 4; q++) stg<f32x4>(out + 8 * q, y[q]);
+                    for (int q = 0; q < 4; q++) stg<f32x4>(out + 8 * q, yr[q]);
                 } else {
                     // Lane halves exchange, so that a lane has eight outputs one after the other: the lower half's of every
                     // even eight, the upper's of the odd.
@@ -394,7 +400,7 @@ __global__ __launch_bounds__(64 * WO * WT, RT * CT >= 16 ? 1 : 2) void k_linear8
 #pragma unroll
                         for (int p = 0; p < 2; p++)
 #pragma unroll
-                            for (int e = 0; e < 2; e++) w[p][e] = pair16(y[q + p][2 * e], y[q + p][2 * e + 1], OT);
+                            for (int e = 0; e < 2; e++) w[p][e] = pair16(yr[q + p][2 * e], yr[q + p][2 * e + 1], OT);
                         u32x4 v;
 #pragma unroll
                         for (int e = 0; e < 2; e++) {

@@ -72,8 +72,8 @@ __device__ __forceinline__ float lora_dot8(u32x4 w, f32x4 x, f32x4 y, float sum)
 }
 
 // Adds a column tile's adapters to NRT row tiles of outputs from o0 on, through add(rt, i, value) for each element of the
-// lane's: token `t` of column lane % M, its adapter `id`, -1 none. BF: bf16 adapters. AHEAD: the next step's operands are
-// requested before this one's products, where the registers allow it.
+// lane's: token `t` of column lane % M, its adapter `id`, -1 none. BF: bf16 adapters. AHEAD: more operands are
+// requested at once, where the registers allow it.
 template <int M, int NRT, bool BF, bool AHEAD = true, typename ADD>
 __device__ __forceinline__ void lora_up(const LoraDev& l, unsigned o0, unsigned t, int id, ADD&& add) {
     using T = LoraTile<M>;
@@ -143,80 +143,93 @@ __device__ __forceinline__ void lora_up(const LoraDev& l, unsigned o0, unsigned 
                     f32x4 x, y;
                     u32x4 w[NRT];
                 };
+                constexpr unsigned BATCH = AHEAD ? 4 : 1;  // steps whose operands are requested at once
                 auto fetch = [&](unsigned st) __attribute__((always_inline)) {
                     const unsigned j = T::STEP * st + 8 * g;
-                    Ops r;
-                    r.x = f32x4{0, 0, 0, 0};
-                    r.y = f32x4{0, 0, 0, 0};
+                    f32x4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
                     if (mine && j < l.rank) {
-                        r.x = ldg<f32x4>(u + T::STEP * st);
-                        r.y = ldg<f32x4>(u + T::STEP * st + 4);
+                        x = ldg<f32x4>(u + T::STEP * st);
+                        y = ldg<f32x4>(u + T::STEP * st + 4);
                     }
+                    Ops r;
+                    r.x = x;
+                    r.y = y;
 #pragma unroll
                     for (int rt = 0; rt < NRT; rt++) {
                         const unsigned o = o0 + M * rt + col;
-                        r.w[rt] = u32x4{0, 0, 0, 0};
-                        if (o >= first && o < end && j < l.rank) r.w[rt] = ldg<u32x4>(b + (uint64_t)o * l.rank + j);
+                        u32x4 w = {0, 0, 0, 0};
+                        if (o >= first && o < end && j < l.rank) w = ldg<u32x4>(b + (uint64_t)o * l.rank + j);
+                        r.w[rt] = w;
                     }
                     return r;
                 };
+                auto most = [](float m, const f32x4& x, const f32x4& y) __attribute__((always_inline)) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) m = fmaxf(m, fmaxf(fabsf(x[i]), fabsf(y[i])));
+                    return m;
+                };
                 float up = 1.0f, down = 1.0f;
-                Ops held;
-                if constexpr (AHEAD) held = fetch(0);
-                if constexpr (!BF) {
-                    float m = 0.0f;
-#pragma unroll M == 32 ? 2 : 4
-                    for (unsigned st = 0; st < steps; st++) {
-                        f32x4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
-                        if (mine && T::STEP * st + 8 * g < l.rank) {
-                            x = ldg<f32x4>(u + T::STEP * st);
-                            y = ldg<f32x4>(u + T::STEP * st + 4);
-                        }
-#pragma unroll
-                        for (int i = 0; i < 4; i++) m = fmaxf(m, fmaxf(fabsf(x[i]), fabsf(y[i])));
-                    }
-                    const unsigned e = max(__float_as_uint(T::most(m)) >> 23, 15u);
-                    up = __uint_as_float((268u - e) << 23);
-                    down = __uint_as_float((e - 14u) << 23);
-                }
 #pragma unroll 1
-                for (unsigned st = 0; st < steps; st++) {
-                    const Ops now = AHEAD ? held : fetch(st);
-                    if constexpr (AHEAD) held = fetch(st + 1);  // past the last: zeros
-                    float x[8];
+                for (unsigned st0 = 0; st0 < steps; st0 += BATCH) {
+                    Ops ops[BATCH];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        x[i] = now.x[i] * up;
-                        x[4 + i] = now.y[i] * up;
+                    for (unsigned i = 0; i < BATCH; i++) ops[i] = fetch(st0 + i);  // past the last: zeros
+                    if (!BF && st0 == 0) {  // the token's largest, of these and of the others
+                        float m = 0.0f;
+#pragma unroll
+                        for (unsigned i = 0; i < BATCH; i++) m = most(m, ops[i].x, ops[i].y);
+#pragma unroll 2
+                        for (unsigned st = BATCH; st < steps; st++) {
+                            f32x4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
+                            if (mine && T::STEP * st + 8 * g < l.rank) {
+                                x = ldg<f32x4>(u + T::STEP * st);
+                                y = ldg<f32x4>(u + T::STEP * st + 4);
+                            }
+                            m = most(m, x, y);
+                        }
+                        const unsigned e = max(__float_as_uint(T::most(m)) >> 23, 15u);
+                        up = __uint_as_float((268u - e) << 23);
+                        down = __uint_as_float((e - 14u) << 23);
                     }
-                    if constexpr (BF) {
-                        bf16x8 p0, p1, p2;
 #pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            p0[i] = (__bf16)x[i];
-                            const float r = x[i] - (float)p0[i];
-                            p1[i] = (__bf16)r;
-                            p2[i] = (__bf16)(r - (float)p1[i]);
+                    for (unsigned b4 = 0; b4 < BATCH; b4++) {
+                        const Ops& now = ops[b4];
+                        if (st0 + b4 >= steps) continue;
+                        float x[8];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            x[i] = now.x[i] * up;
+                            x[4 + i] = now.y[i] * up;
                         }
+                        if constexpr (BF) {
+                            bf16x8 p0, p1, p2;
 #pragma unroll
-                        for (int rt = 0; rt < NRT; rt++) {
-                            const bf16x8 wb = __builtin_bit_cast(bf16x8, now.w[rt]);
-                            d[rt] = T::mfma(wb, p2, d[rt]);
-                            d[rt] = T::mfma(wb, p1, d[rt]);
-                            d[rt] = T::mfma(wb, p0, d[rt]);
-                        }
-                    } else {
-                        f16x8 p0, p1;
+                            for (int i = 0; i < 8; i++) {
+                                p0[i] = (__bf16)x[i];
+                                const float r = x[i] - (float)p0[i];
+                                p1[i] = (__bf16)r;
+                                p2[i] = (__bf16)(r - (float)p1[i]);
+                            }
 #pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            p0[i] = (f16)x[i];
-                            p1[i] = (f16)(x[i] - (float)p0[i]);
-                        }
+                            for (int rt = 0; rt < NRT; rt++) {
+                                const bf16x8 wb = __builtin_bit_cast(bf16x8, now.w[rt]);
+                                d[rt] = T::mfma(wb, p2, d[rt]);
+                                d[rt] = T::mfma(wb, p1, d[rt]);
+                                d[rt] = T::mfma(wb, p0, d[rt]);
+                            }
+                        } else {
+                            f16x8 p0, p1;
 #pragma unroll
-                        for (int rt = 0; rt < NRT; rt++) {
-                            const f16x8 wh = __builtin_bit_cast(f16x8, now.w[rt]);
-                            d[rt] = T::mfma(wh, p1, d[rt]);
-                            d[rt] = T::mfma(wh, p0, d[rt]);
+                            for (int i = 0; i < 8; i++) {
+                                p0[i] = (f16)x[i];
+                                p1[i] = (f16)(x[i] - (float)p0[i]);
+                            }
+#pragma unroll
+                            for (int rt = 0; rt < NRT; rt++) {
+                                const f16x8 wh = __builtin_bit_cast(f16x8, now.w[rt]);
+                                d[rt] = T::mfma(wh, p1, d[rt]);
+                                d[rt] = T::mfma(wh, p0, d[rt]);
+                            }
                         }
                     }
                 }

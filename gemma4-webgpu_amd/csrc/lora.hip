@@ -108,12 +108,12 @@ __global__ __launch_bounds__(kFewWaves * 64) void k_lora_down_few(const DownArgs
     }
 }
 
-// Many tokens: 32 tokens by 64 down rows a workgroup, whose eight waves take every eighth 64 k; the tile's adapters one
+// Many tokens: 16 CT tokens by 64 down rows a workgroup, whose eight waves take every eighth 64 k; the tile's adapters one
 // after the other.
-constexpr int kDownWaves = 8, kDownCols = 2, kDownRows = 4;  // 16-wide tiles
-template <int MODE>
+constexpr int kDownWaves = 8, kDownRows = 4;  // 16-wide tiles
+template <int MODE, int CT>
 __global__ __launch_bounds__(kDownWaves * 64) void k_lora_down(const DownArgs a) {
-    constexpr int CT = kDownCols, RT = kDownRows;
+    constexpr int RT = kDownRows;
     __shared__ f32x4 s_sum[kDownWaves][RT * CT][64];
     __shared__ int s_id[64];
     const LoraDev& l = a.l;
@@ -134,10 +134,10 @@ __global__ __launch_bounds__(kDownWaves * 64) void k_lora_down(const DownArgs a)
         for (int rt = 0; rt < RT; rt++)
 #pragma unroll
             for (int ct = 0; ct < CT; ct++) acc[rt][ct] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        for (unsigned c = wave; c < chunks; c += kDownWaves) {
-            const unsigned k = c * 64 + g * 16;  // the lane's 16 elements
-            const bool in = k < l.n;
-            if constexpr (MODE == kDownF32) {
+        if constexpr (MODE == kDownF32) {
+            for (unsigned c = wave; c < chunks; c += kDownWaves) {
+                const unsigned k = c * 64 + g * 16;  // the lane's 16 elements
+                const bool in = k < l.n;
                 f32x4 x[CT][4];
 #pragma unroll
                 for (int ct = 0; ct < CT; ct++) {
@@ -155,47 +155,66 @@ __global__ __launch_bounds__(kDownWaves * 64) void k_lora_down(const DownArgs a)
                         for (int ct = 0; ct < CT; ct++)
                             acc[rt][ct] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[e / 4][e % 4], x[ct][e / 4][e % 4], acc[rt][ct], 0, 0, 0);
                 }
-            } else {
-                constexpr bool BF = MODE == kDownBf16 || MODE == kDownE4m3Bf16;
-                u32x4 w[RT][2], x[CT][2];
+            }
+        } else {
+            constexpr bool BF = MODE == kDownBf16 || MODE == kDownE4m3Bf16, E4M3 = MODE == kDownE4m3F16 || MODE == kDownE4m3Bf16;
+            struct Operands {
+                u32x4 w[RT][2], x[CT][E4M3 ? 1 : 2];
+            };
+            const uint16_t* wp[RT];
+            const char* xp[CT];
 #pragma unroll
-                for (int rt = 0; rt < RT; rt++) {
-                    const unsigned row = min(r0 + 16 * rt + col, l.down - 1);
-                    const uint16_t* p = static_cast<const uint16_t*>(l.a) + ((uint64_t)ad * l.down + row) * l.n + k;
+            for (int rt = 0; rt < RT; rt++)
+                wp[rt] = static_cast<const uint16_t*>(l.a) + ((uint64_t)ad * l.down + min(r0 + 16 * rt + col, l.down - 1)) * l.n + g * 16;
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++)
+                xp[ct] = static_cast<const char*>(a.x) + (min(t0 + 16 * ct + col, l.n_tokens - 1) * a.x_stride + g * 16) * (E4M3 ? 1 : 2);
+            auto fetch = [&](unsigned c) __attribute__((always_inline)) {
+                Operands r;
+                const unsigned k = c * 64;
+                const bool in = k + g * 16 < l.n;
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++)
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        w[rt][h] = u32x4{0, 0, 0, 0};
-                        if (in) w[rt][h] = ldg<u32x4>(p + 8 * h);
+                        u32x4 v = {0, 0, 0, 0};
+                        if (in) v = ldg<u32x4>(wp[rt] + k + 8 * h);
+                        r.w[rt][h] = v;
                     }
-                }
 #pragma unroll
-                for (int ct = 0; ct < CT; ct++) {
-                    const unsigned t = min(t0 + 16 * ct + col, l.n_tokens - 1);
-                    x[ct][0] = x[ct][1] = u32x4{0, 0, 0, 0};
-                    if constexpr (MODE == kDownE4m3F16 || MODE == kDownE4m3Bf16) {
-                        u32x4 q = {0, 0, 0, 0};
-                        if (in) q = ldg<u32x4>(static_cast<const uint8_t*>(a.x) + t * a.x_stride + k);
-                        x[ct][0] = e4m3_wide<BF>(u32x2{q[0], q[1]});
-                        x[ct][1] = e4m3_wide<BF>(u32x2{q[2], q[3]});
-                    } else {
-                        const uint16_t* p = static_cast<const uint16_t*>(a.x) + t * a.x_stride + k;
-                        if (in) x[ct][0] = ldg<u32x4>(p);
-                        if (in) x[ct][1] = ldg<u32x4>(p + 8);
+                for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+                    for (int h = 0; h < (E4M3 ? 1 : 2); h++) {
+                        u32x4 v = {0, 0, 0, 0};
+                        if (in) v = ldg<u32x4>(xp[ct] + k * (E4M3 ? 1 : 2) + 16 * h);
+                        r.x[ct][h] = v;
                     }
-                }
+                return r;
+            };
+            Operands now = fetch(wave);
+            for (unsigned c = wave; c < chunks; c += kDownWaves) {
+                const Operands next = fetch(c + kDownWaves);  // past the end: zeros
 #pragma unroll
-                for (int h = 0; h < 2; h++)
+                for (int h = 0; h < 2; h++) {
+                    u32x4 x[CT];
+#pragma unroll
+                    for (int ct = 0; ct < CT; ct++) {
+                        if constexpr (E4M3) x[ct] = e4m3_wide<BF>(u32x2{now.x[ct][0][2 * h], now.x[ct][0][2 * h + 1]});
+                        else x[ct] = now.x[ct][h];
+                    }
 #pragma unroll
                     for (int rt = 0; rt < RT; rt++)
 #pragma unroll
                         for (int ct = 0; ct < CT; ct++) {
                             if constexpr (BF)
                                 acc[rt][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                                    __builtin_bit_cast(bf16x8, w[rt][h]), __builtin_bit_cast(bf16x8, x[ct][h]), acc[rt][ct], 0, 0, 0);
+                                    __builtin_bit_cast(bf16x8, now.w[rt][h]), __builtin_bit_cast(bf16x8, x[ct]), acc[rt][ct], 0, 0, 0);
                             else
                                 acc[rt][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                                    __builtin_bit_cast(f16x8, w[rt][h]), __builtin_bit_cast(f16x8, x[ct][h]), acc[rt][ct], 0, 0, 0);
+                                    __builtin_bit_cast(f16x8, now.w[rt][h]), __builtin_bit_cast(f16x8, x[ct]), acc[rt][ct], 0, 0, 0);
                         }
+                }
+                now = next;
             }
         }
 #pragma unroll
@@ -294,8 +313,10 @@ constexpr uint32_t kLoraFewTokens = 128;
 
 template <int MODE>
 static void launch_down(const DownArgs& a, hipStream_t st) {
-    const dim3 grid((a.l.n_tokens + 16 * kDownCols - 1) / (16 * kDownCols), (a.l.down + 16 * kDownRows - 1) / (16 * kDownRows));
-    G4_LAUNCH((k_lora_down<MODE>), grid, dim3(kDownWaves * 64), 0, st, a);
+    const uint32_t groups = (a.l.down + 16 * kDownRows - 1) / (16 * kDownRows), pairs = (a.l.n_tokens + 31) / 32;
+    // Tiles of 32 tokens read an adapter half as often; of 16 where those would leave compute units idle.
+    if (pairs * groups >= device_cus()) G4_LAUNCH((k_lora_down<MODE, 2>), dim3(pairs, groups), dim3(kDownWaves * 64), 0, st, a);
+    else G4_LAUNCH((k_lora_down<MODE, 1>), dim3((a.l.n_tokens + 15) / 16, groups), dim3(kDownWaves * 64), 0, st, a);
 }
 template <uint32_t XT>
 static void launch_down_few(const DownArgs& a, hipStream_t st) {

@@ -9,6 +9,8 @@
 // those. The largest |y| is the largest |r w2| times one factor, so the second
 // norm and the scale share one reduction, and a row of one wave has no barrier
 // at all.
+#include <type_traits>
+
 #include "decode_core.h"
 #include "rows.h"
 
@@ -75,16 +77,17 @@ __device__ __forceinline__ void nr_reduce(float& sum, uint32_t& top, float (&s_s
 }
 
 // NV * 8 elements of a row as they lie: 16-bit ones fill the first half of each eight. Elements past n are 0. Element i of a
-// thread is (i / 8 * TPR + t) * 8 + i % 8 of the row with VEC, else i * TPR + t.
-template <int NV>
+// thread is (i / 8 * TPR + t) * 8 + i % 8 of the row with VEC, else i * TPR + t. WIDTH: the bytes of an element, 0 known
+// only at run time (with the registers of four).
+template <int NV, int WIDTH>
 struct RawRow {
-    u32x4 a[NV], b[NV];
+    u32x4 a[NV], b[WIDTH == 2 ? 1 : NV];
 };
-template <int TPR, int NV, bool VEC>
-__device__ __forceinline__ RawRow<NV> nr_load(const void* p, uint32_t type, unsigned t, unsigned n) {
-    RawRow<NV> r;
+template <int TPR, int NV, bool VEC, int WIDTH>
+__device__ __forceinline__ RawRow<NV, WIDTH> nr_load(const void* p, uint32_t type, unsigned t, unsigned n) {
+    RawRow<NV, WIDTH> r;
     const char* base = static_cast<const char*>(p);
-    const bool full = type == G4_F32;
+    const bool full = WIDTH == 0 ? type == G4_F32 : WIDTH == 4;
     if constexpr (VEC) {
 #pragma unroll
         for (int i = 0; i < NV; i++) {
@@ -93,9 +96,10 @@ __device__ __forceinline__ RawRow<NV> nr_load(const void* p, uint32_t type, unsi
             if (at < n) a = ldg<u32x4>(base + (full ? 4 * at : 2 * at));
             if (at < n && full) b = ldg<u32x4>(base + 4 * at + 16);
             r.a[i] = a;
-            r.b[i] = b;
+            if constexpr (WIDTH != 2) r.b[i] = b;
         }
     } else {
+        static_assert(WIDTH == 0, "one element a load: any type");
         uint32_t e[NV * 8];
 #pragma unroll
         for (int i = 0; i < NV * 8; i++) {
@@ -118,13 +122,14 @@ __device__ __forceinline__ RawRow<NV> nr_load(const void* p, uint32_t type, unsi
     return r;
 }
 // f(i, element i).
-template <int NV, typename F>
-__device__ __forceinline__ void nr_each(const RawRow<NV>& r, uint32_t type, F&& f) {
+template <int NV, int WIDTH, typename F>
+__device__ __forceinline__ void nr_each(const RawRow<NV, WIDTH>& r, uint32_t type, F&& f) {
 #pragma unroll
     for (int i = 0; i < NV * 8; i++) {
-        const uint32_t word = i % 8 < 4 ? r.a[i / 8][i % 4] : r.b[i / 8][i % 4], pair = r.a[i / 8][i % 8 / 2];
+        const uint32_t pair = r.a[i / 8][i % 8 / 2], word = WIDTH == 2 ? 0 : i % 8 < 4 ? r.a[i / 8][i % 4] : r.b[WIDTH == 2 ? 0 : i / 8][i % 4];
         const float h = h2f((uint16_t)(pair >> (16 * (i & 1)))), b = __uint_as_float((i & 1) ? pair & 0xFFFF0000u : pair << 16);
-        f(i, type == G4_F32 ? __uint_as_float(word) : type == G4_F16 ? h : b);
+        const float half = type == G4_F16 ? h : b;
+        f(i, WIDTH == 4 ? __uint_as_float(word) : WIDTH == 2 ? half : type == G4_F32 ? __uint_as_float(word) : half);
     }
 }
 template <int E>
@@ -181,22 +186,26 @@ __device__ __forceinline__ const void* nr_row(const void* p, uint32_t type, uint
 }
 
 // TPR threads a row, NV * 8 elements a thread. VEC: 8 elements a load (16 or 32 bytes; rows aligned, n a multiple of 8).
-template <int TPR, int NV, bool VEC>
+// XW, RW, WW: the widths of x, the residual and the weights.
+template <int TPR, int NV, bool VEC, int XW, int RW, int WW>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_rows(const NormRowsArgs a) {
     constexpr int E = NV * 8, W = TPR / 64;
+    constexpr bool LATE = TPR == 1024;  // 128 registers a wave: each operand only when the one before is done with
     __shared__ float s_sum[2][W];
     __shared__ uint32_t s_top[2][W];
     const unsigned row = TPR < 256 ? blockIdx.x * (256 / TPR) + threadIdx.x / TPR : blockIdx.x;
     const unsigned t = TPR < 256 ? threadIdx.x % TPR : threadIdx.x;
     if (row >= a.rows) return;  // whole waves, of a kernel without barriers
     const unsigned n = a.n;
-    const RawRow<NV> x = nr_load<TPR, NV, VEC>(nr_row(a.x, a.x_type, row * a.x_stride), a.x_type, t, n);
-    constexpr bool LATE = TPR == 1024;  // 128 registers a wave: the residual only when x is done with
     auto load_residual = [&]() __attribute__((always_inline)) {
-        return nr_load<TPR, NV, VEC>(nr_row(a.residual, a.residual_type, row * a.residual_stride), a.residual_type, t, n);
+        return nr_load<TPR, NV, VEC, RW>(nr_row(a.residual, a.residual_type, row * a.residual_stride), a.residual_type, t, n);
     };
-    RawRow<NV> res = x;
+    const auto x = nr_load<TPR, NV, VEC, XW>(nr_row(a.x, a.x_type, row * a.x_stride), a.x_type, t, n);
+    RawRow<NV, RW> res = {};
     if (!LATE && a.residual) res = load_residual();
+    // The next norm's weights are requested early too: behind the sums they would be waited for.
+    RawRow<NV, WW> w2 = {};
+    if (!LATE && a.weight) w2 = nr_load<TPR, NV, VEC, WW>(a.weight, a.weight_type, t, n);
     float v[E];
     nr_each(x, a.x_type, [&](int i, float e) __attribute__((always_inline)) { v[i] = e; });
     if (a.post) {
@@ -204,7 +213,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_rows(const NormR
         uint32_t top = 0;
 #pragma unroll
         for (int i = 0; i < E; i++) sum = __builtin_fmaf(v[i], v[i], sum);
-        const RawRow<NV> w = nr_load<TPR, NV, VEC>(a.post, a.weight_type, t, n);
+        const auto w = nr_load<TPR, NV, VEC, WW>(a.post, a.weight_type, t, n);
         nr_reduce<W>(sum, top, s_sum[0], s_top[0]);
         const float inv = 1.0f / sqrtf(sum * a.inv_n + a.eps);
         nr_each(w, a.weight_type, [&](int i, float e) __attribute__((always_inline)) { v[i] *= e * inv; });
@@ -227,8 +236,9 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_rows(const NormR
         for (int i = 0; i < E; i++) sum = __builtin_fmaf(v[i], v[i], sum);
     }
     if (a.weight) {
-        const RawRow<NV> w = nr_load<TPR, NV, VEC>(a.weight, a.weight_type, t, n);
-        nr_each(w, a.weight_type, [&](int i, float e) __attribute__((always_inline)) { v[i] *= e; });
+        auto times = [&](int i, float e) __attribute__((always_inline)) { v[i] *= e; };
+        if constexpr (LATE) nr_each(nr_load<TPR, NV, VEC, WW>(a.weight, a.weight_type, t, n), a.weight_type, times);
+        else nr_each(w2, a.weight_type, times);
     }
     if (a.out_type == G4_E4M3) {
 #pragma unroll
@@ -256,19 +266,38 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_rows(const NormR
 
 constexpr uint32_t kNormMaxN = 32768;
 
-template <bool VEC>
+// Eight elements a load would not fit the registers.
+void launch_longest(const NormRowsArgs& a, hipStream_t st) {
+    G4_LAUNCH((k_norm_rows<1024, 4, false, 0, 0, 0>), dim3(a.rows), dim3(1024), 0, st, a);
+}
+template <bool VEC, int XW, int RW, int WW>
 void launch_norm_rows(const NormRowsArgs& a, hipStream_t st) {
-    const dim3 four((a.rows + 3) / 4), one(a.rows);
+    auto launch = [&](auto tpr, auto nv) {
+        constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value;
+        constexpr uint32_t PER = TPR < 256 ? 256 / TPR : 1;
+        const dim3 grid((a.rows + PER - 1) / PER), block(TPR * PER);
+        G4_LAUNCH((k_norm_rows<TPR, NV, VEC, XW, RW, WW>), grid, block, 0, st, a);
+    };
+#define G4_NORM(TPR, NV) launch(std::integral_constant<int, TPR>{}, std::integral_constant<int, NV>{})
     // A wave a row where the rows fill the chip with waves; else four waves a row.
     const bool many = a.rows >= 8 * device_cus();
-    if (many && a.n <= 512) G4_LAUNCH((k_norm_rows<64, 1, VEC>), four, dim3(256), 0, st, a);
-    else if (many && a.n <= 1024) G4_LAUNCH((k_norm_rows<64, 2, VEC>), four, dim3(256), 0, st, a);
-    else if (many && a.n <= 2048) G4_LAUNCH((k_norm_rows<64, 4, VEC>), four, dim3(256), 0, st, a);
-    else if (a.n <= 2048) G4_LAUNCH((k_norm_rows<256, 1, VEC>), one, dim3(256), 0, st, a);
-    else if (a.n <= 4096) G4_LAUNCH((k_norm_rows<256, 2, VEC>), one, dim3(256), 0, st, a);
-    else if (a.n <= 8192) G4_LAUNCH((k_norm_rows<256, 4, VEC>), one, dim3(256), 0, st, a);
-    else if (a.n <= 16384) G4_LAUNCH((k_norm_rows<512, 4, VEC>), one, dim3(512), 0, st, a);
-    else G4_LAUNCH((k_norm_rows<1024, 4, false>), one, dim3(1024), 0, st, a);  // eight-element loads would spill
+    if (many && a.n <= 512) G4_NORM(64, 1);
+    else if (many && a.n <= 1024) G4_NORM(64, 2);
+    else if (many && a.n <= 1536) G4_NORM(64, 3);
+    else if (a.n <= 2048) G4_NORM(256, 1);
+    else if (a.n <= 4096) G4_NORM(256, 2);
+    else if (a.n <= 6144) G4_NORM(256, 3);
+    else if (a.n <= 8192) G4_NORM(256, 4);
+    else if (a.n <= 16384) G4_NORM(512, 4);
+    else launch_longest(a, st);
+#undef G4_NORM
+}
+void launch_norm_rows(const NormRowsArgs& a, bool vec, hipStream_t st) {
+    if (!vec) return launch_norm_rows<false, 0, 0, 0>(a, st);
+    const bool w4 = (a.post || a.weight) && a.weight_type == G4_F32, r4 = a.residual && a.residual_type == G4_F32;
+    if (w4) return launch_norm_rows<true, 0, 0, 0>(a, st);
+    if (a.x_type == G4_F32) return r4 ? launch_norm_rows<true, 4, 4, 2>(a, st) : launch_norm_rows<true, 4, 2, 2>(a, st);
+    return r4 ? launch_norm_rows<true, 2, 4, 2>(a, st) : launch_norm_rows<true, 2, 2, 2>(a, st);
 }
 
 }  // namespace g4
@@ -354,8 +383,7 @@ int g4_add_rms_norm(const void* x, const void* residual, const void* post_weight
     const bool wide = p->n % 8 == 0 && wide_rows(x, a.x_type, a.x_stride) && wide_rows(residual, a.residual_type, a.residual_stride) &&
                       wide_rows(residual_out, a.residual_type, a.residual_out_stride) && wide_rows(post_weight, a.weight_type, 0) &&
                       wide_rows(weight, a.weight_type, 0) && wide_rows(out, a.out_type, a.out_stride);
-    if (wide) launch_norm_rows<true>(a, as_stream(stream));
-    else launch_norm_rows<false>(a, as_stream(stream));
+    launch_norm_rows(a, wide, as_stream(stream));
     G4_CHECK_LAUNCH("k_norm_rows");
     return G4_OK;
 }
@@ -382,8 +410,7 @@ int g4_quantize_rows(const void* x, uint8_t* out, float* scales, const g4_quanti
     a.x_type = p->x_type;
     a.out_type = G4_E4M3;
     const bool wide = p->n % 8 == 0 && wide_rows(x, a.x_type, a.x_stride) && wide_rows(out, G4_E4M3, a.out_stride);
-    if (wide) launch_norm_rows<true>(a, as_stream(stream));
-    else launch_norm_rows<false>(a, as_stream(stream));
+    launch_norm_rows(a, wide, as_stream(stream));
     G4_CHECK_LAUNCH("k_norm_rows");
     return G4_OK;
 }
