@@ -151,25 +151,6 @@ __global__ __launch_bounds__(W * 64) void k_linear8_few(const Linear8Args a) {
 // A stage holds 64 bytes a row, 16-byte piece c of row r at r * 64 + (c ^ (r / 4) % 4) * 16: sixteen lanes that read one
 // piece of sixteen rows meet all 64 banks.
 constexpr unsigned kStageK = 64;
-__device__ __attribute__((aligned(16))) const uint32_t kZeros[4] = {0, 0, 0, 0};
-
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"  // M0 is a reserved register: clobbering it is what is meant
-// 16 bytes a lane from base + its offset, or from its address, to LDS lds + at + 16 lane. No memory clobber: it writes a
-// stage that nothing reads before the barrier that waits for it, and reads of other stages may pass it.
-template <unsigned AT>
-__device__ __forceinline__ void stage_dma(const void* base, uint32_t off, uint32_t lds) {
-    asm volatile("s_add_u32 m0, %2, %3\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds), "n"(AT) : "m0", "scc");
-}
-template <unsigned AT>
-__device__ __forceinline__ void stage_dma(const void* from, uint32_t lds) {
-    asm volatile("s_add_u32 m0, %1, %2\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(lds), "n"(AT) : "m0", "scc");
-}
-// Four bytes a lane to LDS lds + 4 lane.
-__device__ __forceinline__ void scale_dma(const void* from, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(lds) : "m0");
-}
-#pragma clang diagnostic pop
 // All but the N newest requests have come, the wave's LDS reads too; then every wave's.
 template <int N>
 __device__ __forceinline__ void stage_barrier() {

@@ -24,13 +24,14 @@ __device__ __forceinline__ u32x4 e4m3_wide(u32x2 q) {
     u32x4 r;
 #pragma unroll
     for (int w = 0; w < 2; w++) {
-        const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[w], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[w], true);
         if constexpr (BF) {
-            r[2 * w] = (uint32_t)f2bf(lo[0]) | (uint32_t)f2bf(lo[1]) << 16;
-            r[2 * w + 1] = (uint32_t)f2bf(hi[0]) | (uint32_t)f2bf(hi[1]) << 16;
+            const auto lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[w], 1.0f, false), hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[w], 1.0f, true);
+            r[2 * w] = __builtin_bit_cast(uint32_t, lo);
+            r[2 * w + 1] = __builtin_bit_cast(uint32_t, hi);
         } else {
-            r[2 * w] = (uint32_t)f2h(lo[0]) | (uint32_t)f2h(lo[1]) << 16;
-            r[2 * w + 1] = (uint32_t)f2h(hi[0]) | (uint32_t)f2h(hi[1]) << 16;
+            const auto lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(q[w], 1.0f, false), hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(q[w], 1.0f, true);
+            r[2 * w] = __builtin_bit_cast(uint32_t, lo);
+            r[2 * w + 1] = __builtin_bit_cast(uint32_t, hi);
         }
     }
     return r;
@@ -108,17 +109,31 @@ __global__ __launch_bounds__(kFewWaves * 64) void k_lora_down_few(const DownArgs
     }
 }
 
-// Many tokens: 16 CT tokens by 64 down rows a workgroup, whose eight waves take every eighth 64 k; the tile's adapters one
-// after the other.
-constexpr int kDownWaves = 8, kDownRows = 4;  // 16-wide tiles
+// Many tokens: 16 CT tokens by 64 down rows a workgroup; the tile's adapters one after the other.
+//
+// Each wave takes every Wth 64 k and brings both operands of it to LDS by DMA, one chunk ahead: loaded straight into the matrix
+// unit's layout, in which neighbouring lanes lie in different rows, every lane's 16 bytes are an access of their own (4003
+// tokens, n 2048, rank 64: 21 us). Piece c (16 bytes) of row r lies at c ^ r % 8 of its 128 bytes, c ^ r / 2 % 4 of its 64.
+constexpr int kDownWaves = 4, kDownRows = 4;  // 16-wide tiles
+template <int N>
+__device__ __forceinline__ void down_wait() {  // all but the N newest requests of the wave
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
 template <int MODE, int CT>
 __global__ __launch_bounds__(kDownWaves * 64) void k_lora_down(const DownArgs a) {
     constexpr int RT = kDownRows;
-    __shared__ f32x4 s_sum[kDownWaves][RT * CT][64];
+    constexpr bool BF = MODE == kDownBf16 || MODE == kDownE4m3Bf16, E4M3 = MODE == kDownE4m3F16 || MODE == kDownE4m3Bf16;
+    constexpr unsigned XROW = E4M3 ? 64 : 128, WBYTES = RT * 16 * 128, CHUNK = WBYTES + CT * 16 * XROW;
+    constexpr int DMAS = CHUNK / 1024;
+    constexpr unsigned SUMS = RT * CT * 1024;
+    constexpr unsigned AREA = MODE == kDownF32 ? SUMS : 2 * CHUNK;  // a wave's: two chunks, then its sums
+    static_assert(AREA >= SUMS, "the sums take the chunks' place");
+    __shared__ __attribute__((aligned(16))) uint8_t s_mem[kDownWaves * AREA];
     __shared__ int s_id[64];
     const LoraDev& l = a.l;
-    const unsigned lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
+    const unsigned lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
     const unsigned t0 = blockIdx.x * (16 * CT), r0 = blockIdx.y * (16 * RT);
+    uint8_t* const mine = s_mem + wave * AREA;
     // Lane: token of the tile. One wave's reading for all, so that they agree whatever happens to the array meanwhile.
     if (wave == 0) s_id[lane] = lora_id(l, t0 + lane, lane < 16 * CT && t0 + lane < l.n_tokens);
     __syncthreads();
@@ -157,76 +172,87 @@ __global__ __launch_bounds__(kDownWaves * 64) void k_lora_down(const DownArgs a)
                 }
             }
         } else {
-            constexpr bool BF = MODE == kDownBf16 || MODE == kDownE4m3Bf16, E4M3 = MODE == kDownE4m3F16 || MODE == kDownE4m3Bf16;
-            struct Operands {
-                u32x4 w[RT][2], x[CT][E4M3 ? 1 : 2];
+            const uint32_t lds = __builtin_amdgcn_readfirstlane(
+                (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)mine));
+            const char* from[DMAS];  // at k = 0
+            unsigned at[DMAS];       // the lane's first element of a chunk
+#pragma unroll
+            for (int j = 0; j < DMAS; j++) {
+                if (j < RT * 2) {  // eight rows of 128 bytes
+                    const unsigned r = 8 * j + (lane >> 3), piece = (lane & 7) ^ (r & 7);
+                    at[j] = piece * 8;
+                    from[j] = reinterpret_cast<const char*>(static_cast<const uint16_t*>(l.a) +
+                                                            ((uint64_t)ad * l.down + min(r0 + r, l.down - 1)) * l.n + at[j]);
+                } else if (E4M3) {  // sixteen rows of 64
+                    const unsigned r = 16 * (j - RT * 2) + (lane >> 2), piece = (lane & 3) ^ ((r >> 1) & 3);
+                    at[j] = piece * 16;
+                    from[j] = static_cast<const char*>(a.x) + min(t0 + r, l.n_tokens - 1) * a.x_stride + at[j];
+                } else {
+                    const unsigned r = 8 * (j - RT * 2) + (lane >> 3), piece = (lane & 7) ^ (r & 7);
+                    at[j] = piece * 8;
+                    from[j] = static_cast<const char*>(a.x) + 2 * (min(t0 + r, l.n_tokens - 1) * a.x_stride + at[j]);
+                }
+            }
+            // A chunk into half `half` of the wave's; past the end, and lanes past n, zeros.
+            auto request = [&](unsigned c, unsigned half) __attribute__((always_inline)) {
+#pragma unroll
+                for (int j = 0; j < DMAS; j++) {
+                    const char* p = from[j] + (uint64_t)c * ((j < RT * 2 || !E4M3) ? 128 : 64);
+                    if (c * 64 + at[j] >= l.n) p = reinterpret_cast<const char*>(kZeros);
+                    stage_dma<0>(p, lds + half * CHUNK + j * 1024);
+                }
             };
-            const uint16_t* wp[RT];
-            const char* xp[CT];
+            unsigned half = 0;
+            request(wave, 0);
+            for (unsigned c = wave; c < chunks; c += kDownWaves, half ^= 1) {
+                request(c + kDownWaves, half ^ 1);
+                down_wait<DMAS>();
+                const uint8_t* w = mine + half * CHUNK;
+                const uint8_t* x = w + WBYTES;
+                u32x4 wv[RT][2], xv[CT][2];
 #pragma unroll
-            for (int rt = 0; rt < RT; rt++)
-                wp[rt] = static_cast<const uint16_t*>(l.a) + ((uint64_t)ad * l.down + min(r0 + 16 * rt + col, l.down - 1)) * l.n + g * 16;
+                for (int h = 0; h < 2; h++) {  // k 32 h + 8 g of the chunk
 #pragma unroll
-            for (int ct = 0; ct < CT; ct++)
-                xp[ct] = static_cast<const char*>(a.x) + (min(t0 + 16 * ct + col, l.n_tokens - 1) * a.x_stride + g * 16) * (E4M3 ? 1 : 2);
-            auto fetch = [&](unsigned c) __attribute__((always_inline)) {
-                Operands r;
-                const unsigned k = c * 64;
-                const bool in = k + g * 16 < l.n;
-#pragma unroll
-                for (int rt = 0; rt < RT; rt++)
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        u32x4 v = {0, 0, 0, 0};
-                        if (in) v = ldg<u32x4>(wp[rt] + k + 8 * h);
-                        r.w[rt][h] = v;
-                    }
-#pragma unroll
-                for (int ct = 0; ct < CT; ct++)
-#pragma unroll
-                    for (int h = 0; h < (E4M3 ? 1 : 2); h++) {
-                        u32x4 v = {0, 0, 0, 0};
-                        if (in) v = ldg<u32x4>(xp[ct] + k * (E4M3 ? 1 : 2) + 16 * h);
-                        r.x[ct][h] = v;
-                    }
-                return r;
-            };
-            Operands now = fetch(wave);
-            for (unsigned c = wave; c < chunks; c += kDownWaves) {
-                const Operands next = fetch(c + kDownWaves);  // past the end: zeros
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    u32x4 x[CT];
+                    for (int rt = 0; rt < RT; rt++)
+                        wv[rt][h] = *reinterpret_cast<const u32x4*>(w + (16 * rt + col) * 128 + ((4 * h + g) ^ (col & 7)) * 16);
 #pragma unroll
                     for (int ct = 0; ct < CT; ct++) {
-                        if constexpr (E4M3) x[ct] = e4m3_wide<BF>(u32x2{now.x[ct][0][2 * h], now.x[ct][0][2 * h + 1]});
-                        else x[ct] = now.x[ct][h];
+                        if constexpr (E4M3) {
+                            const unsigned piece = (2 * h + (g >> 1)) ^ ((col >> 1) & 3);
+                            xv[ct][h] = e4m3_wide<BF>(*reinterpret_cast<const u32x2*>(x + (16 * ct + col) * 64 + piece * 16 + 8 * (g & 1)));
+                        } else {
+                            xv[ct][h] = *reinterpret_cast<const u32x4*>(x + (16 * ct + col) * 128 + ((4 * h + g) ^ (col & 7)) * 16);
+                        }
                     }
+                }
+#pragma unroll
+                for (int h = 0; h < 2; h++)
 #pragma unroll
                     for (int rt = 0; rt < RT; rt++)
 #pragma unroll
                         for (int ct = 0; ct < CT; ct++) {
                             if constexpr (BF)
                                 acc[rt][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                                    __builtin_bit_cast(bf16x8, now.w[rt][h]), __builtin_bit_cast(bf16x8, x[ct]), acc[rt][ct], 0, 0, 0);
+                                    __builtin_bit_cast(bf16x8, wv[rt][h]), __builtin_bit_cast(bf16x8, xv[ct][h]), acc[rt][ct], 0, 0, 0);
                             else
                                 acc[rt][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                                    __builtin_bit_cast(f16x8, now.w[rt][h]), __builtin_bit_cast(f16x8, x[ct]), acc[rt][ct], 0, 0, 0);
+                                    __builtin_bit_cast(f16x8, wv[rt][h]), __builtin_bit_cast(f16x8, xv[ct][h]), acc[rt][ct], 0, 0, 0);
                         }
-                }
-                now = next;
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read: the next request but one goes here
             }
+            down_wait<0>();  // the last, of zeros, has come too: its place is the sums'
         }
+        f32x4* sums = reinterpret_cast<f32x4*>(mine);
 #pragma unroll
         for (int rt = 0; rt < RT; rt++)
 #pragma unroll
-            for (int ct = 0; ct < CT; ct++) s_sum[wave][rt * CT + ct][lane] = acc[rt][ct];
+            for (int ct = 0; ct < CT; ct++) sums[(rt * CT + ct) * 64 + lane] = acc[rt][ct];
         __syncthreads();
         for (unsigned i = wave; i < RT * CT; i += kDownWaves) {
             const unsigned rt = i / CT, ct = i % CT, t = t0 + 16 * ct + col, row = r0 + 16 * rt + 4 * g;
-            f32x4 s = s_sum[0][i][lane];
+            f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int w = 1; w < kDownWaves; w++) s += s_sum[w][i][lane];
+            for (int w = 0; w < kDownWaves; w++) s += reinterpret_cast<const f32x4*>(s_mem + w * AREA)[i * 64 + lane];
             if (((with >> (16 * ct + col)) & 1) && row < l.down) {  // down and row: multiples of 4
                 if (a.x_scales) s *= a.x_scales[t];
                 stg<f32x4>(l.u + (uint64_t)t * l.down + row, s);
