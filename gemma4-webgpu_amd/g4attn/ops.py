@@ -11,6 +11,7 @@ current stream only; all arithmetic runs in libg4attn.so.
 from __future__ import annotations
 
 import ctypes as C
+from functools import lru_cache
 
 import torch
 
@@ -934,6 +935,9 @@ _WIDE_TYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 def _rows_of(t, name, types, device, shape=None):
     """A [rows, n] tensor whose rows may lie apart: (pointer, type, elements from row to row)."""
+    if isinstance(t, torch.Tensor) and t.dtype in types and t.get_device() == device and t.is_contiguous() and (
+            t.dim() == 2 if shape is None else t.shape == shape):
+        return t.data_ptr(), ROW_TYPES[t.dtype], 0
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a tensor")
     if t.get_device() != device or not t.is_cuda:
@@ -942,24 +946,32 @@ def _rows_of(t, name, types, device, shape=None):
         raise TypeError(f"{name}: dtype {t.dtype} not in {types}")
     if t.dim() != 2 or shape is not None and t.shape != shape:
         raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {'[rows, n]' if shape is None else tuple(shape)}")
-    if t.is_contiguous():
-        return t.data_ptr(), ROW_TYPES[t.dtype], 0
     rows, n = t.shape
     if n > 1 and t.stride(1) != 1 or rows > 1 and t.stride(0) < n:
         raise ValueError(f"{name}: a row's elements must be contiguous, and rows apart")
     return t.data_ptr(), ROW_TYPES[t.dtype], t.stride(0) if rows > 1 else 0
 
 
+# A call's sizes and types as the C ABI takes them, built once for each set of them (a loop's calls repeat theirs).
+_norm_params = lru_cache(256)(abi.AddRmsNormParams)
+_quantize_params = lru_cache(256)(abi.QuantizeRowsParams)
+_linear_params = lru_cache(256)(abi.LinearE4m3Params)
+_lora_params = lru_cache(256)(abi.LoraAddParams)
+_ALL_TYPES, _E4M3 = tuple(ROW_TYPES), (torch.float8_e4m3fn,)
+
+
 def _device_of(t, name):
+    if isinstance(t, torch.Tensor) and t.is_cuda:
+        return _call_device(t.get_device())
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a tensor")
-    if not t.is_cuda:
-        raise ValueError(f"{name}: must be on the GPU, got {t.device}")
-    return _call_device(t.get_device())
+    raise ValueError(f"{name}: must be on the GPU, got {t.device}")
 
 
 def _norm_weight(t, name, n, device):
     """A norm's weights: f32, bf16 or f16 (or its bits, as the other norms take them)."""
+    if t.dtype in _WIDE_TYPES and t.get_device() == device and t.numel() == n and t.is_contiguous():
+        return t.data_ptr(), ROW_TYPES[t.dtype]
     kind = torch.float16 if t.dtype in F16_TYPES else t.dtype
     if kind not in _WIDE_TYPES:
         raise TypeError(f"{name}: dtype {t.dtype} not in {_WIDE_TYPES}")
@@ -984,7 +996,7 @@ def add_rms_norm(x, weight, out, scales=None, residual=None, residual_out=None, 
         if rt is not None and st != rt:
             raise TypeError(f"residual_out: dtype {residual_out.dtype}, residual's is {residual.dtype}")
         rt = st
-    op, ot, os_ = (None, xt, 0) if out is None else _rows_of(out, "out", tuple(ROW_TYPES), dev, x.shape)
+    op, ot, os_ = (None, xt, 0) if out is None else _rows_of(out, "out", _ALL_TYPES, dev, x.shape)
     pp = wp = wt = None
     if post_weight is not None:
         pp, wt = _norm_weight(post_weight, "post_weight", n, dev)
@@ -997,7 +1009,7 @@ def add_rms_norm(x, weight, out, scales=None, residual=None, residual_out=None, 
     if rows == 0:
         return
     abi.call("g4_add_rms_norm", xp, rp, pp, wp, sp, op, cp,
-             abi.AddRmsNormParams(rows, n, xt, xt if rt is None else rt, wt or 0, ot, eps, 0, xs, rs, ss, os_), _stream(stream))
+             _norm_params(rows, n, xt, xt if rt is None else rt, wt or 0, ot, eps, 0, xs, rs, ss, os_), _stream(stream))
 
 
 def quantize_rows(x, out, scales, stream=None):
@@ -1005,12 +1017,12 @@ def quantize_rows(x, out, scales, stream=None):
     [rows]. Rows may lie apart."""
     dev = _device_of(x, "x")
     xp, xt, xs = _rows_of(x, "x", _WIDE_TYPES, dev)
-    op, _, os_ = _rows_of(out, "out", (torch.float8_e4m3fn,), dev, x.shape)
+    op, _, os_ = _rows_of(out, "out", _E4M3, dev, x.shape)
     rows, n = x.shape
     cp = _at(scales, "scales", torch.float32, rows, dev)
     if rows == 0:
         return
-    abi.call("g4_quantize_rows", xp, op, cp, abi.QuantizeRowsParams(rows, n, xt, 0, xs, os_), _stream(stream))
+    abi.call("g4_quantize_rows", xp, op, cp, _quantize_params(rows, n, xt, 0, xs, os_), _stream(stream))
 
 
 class LoraAdapters:
@@ -1054,7 +1066,7 @@ def linear_e4m3(x, x_scales, weight, weight_scales, out, workspace, lora=None, a
     workspace: uint8, linear_e4m3_workspace_bytes."""
     dev = _device_of(x, "x")
     e4m3, f32 = torch.float8_e4m3fn, torch.float32
-    xp, _, xs = _rows_of(x, "x", (e4m3,), dev)
+    xp, _, xs = _rows_of(x, "x", _E4M3, dev)
     tokens, n = x.shape
     if weight.dim() != 2 or weight.shape[1] != n:
         raise ValueError(f"weight: shape {tuple(weight.shape)}, expected [rows, {n}]")
@@ -1069,7 +1081,7 @@ def linear_e4m3(x, x_scales, weight, weight_scales, out, workspace, lora=None, a
     abi.call("g4_linear_e4m3", xp, _at(x_scales, "x_scales", f32, tokens, dev), _at(weight, "weight", e4m3, rows * n, dev),
              _at(weight_scales, "weight_scales", f32, rows, dev), None if lora is None else lora.c,
              None if lora is None else _at(adapter_ids, "adapter_ids", torch.int32, tokens, dev), op,
-             abi.LinearE4m3Params(tokens, rows, n, ot, xs, os_), _at(workspace, "workspace", torch.uint8, 0, dev),
+             _linear_params(tokens, rows, n, ot, xs, os_), _at(workspace, "workspace", torch.uint8, 0, dev),
              workspace.numel(), _stream(stream))
 
 
@@ -1085,7 +1097,7 @@ def lora_add(lora, adapter_ids, x, base, out, workspace, x_scales=None, stream=N
     [n_tokens]; x: [n_tokens, n], f32, f16, bf16, or float8_e4m3fn with x_scales; base and out: [n_tokens, rows] of one type,
     f32, f16 or bf16 (may be the same tensor). Tokens may lie apart. workspace: uint8, lora_workspace_bytes."""
     dev = _call_device(lora.device)
-    xp, xt, xs = _rows_of(x, "x", tuple(ROW_TYPES), dev)
+    xp, xt, xs = _rows_of(x, "x", _ALL_TYPES, dev)
     tokens = x.shape[0]
     if x.shape[1] != lora.n:
         raise ValueError(f"x: shape {tuple(x.shape)}, expected [n_tokens, {lora.n}]")
@@ -1097,5 +1109,5 @@ def lora_add(lora, adapter_ids, x, base, out, workspace, x_scales=None, stream=N
         return
     abi.call("g4_lora_add", lora.c, _at(adapter_ids, "adapter_ids", torch.int32, tokens, dev), xp,
              None if x_scales is None else _at(x_scales, "x_scales", torch.float32, tokens, dev), bp, op,
-             abi.LoraAddParams(tokens, xt, ot, 0, xs, bs, os_), _at(workspace, "workspace", torch.uint8, 0, dev),
+             _lora_params(tokens, xt, ot, 0, xs, bs, os_), _at(workspace, "workspace", torch.uint8, 0, dev),
              workspace.numel(), _stream(stream))
