@@ -1466,6 +1466,103 @@ napi_value TokenLogprobs(napi_env env, napi_callback_info info) {
     return undefined(env);
 }
 
+// ---- between two attention blocks of a batch --------------------------------------
+
+// addRmsNorm(x, residual, postWeight, weight, residualOut, out, scales, params, stream)
+napi_value AddRmsNorm(napi_env env, napi_callback_info info) {
+    Args a(env, info, 9);
+    void* d[7];
+    for (int i = 0; i < 7; i++) d[i] = a.ptr(i);
+    g4_add_rms_norm_params p;
+    a.params(7, &p);
+    void* s = a.ptr(8);
+    if (!a.ok) return nullptr;
+    CALL(env, g4_add_rms_norm(d[0], d[1], d[2], d[3], d[4], d[5], (float*)d[6], &p, s));
+    return undefined(env);
+}
+
+// quantizeRows(x, out, scales, params, stream)
+napi_value QuantizeRows(napi_env env, napi_callback_info info) {
+    Args a(env, info, 5);
+    void* d[3];
+    for (int i = 0; i < 3; i++) d[i] = a.ptr(i);
+    g4_quantize_rows_params p;
+    a.params(3, &p);
+    void* s = a.ptr(4);
+    if (!a.ok) return nullptr;
+    CALL(env, g4_quantize_rows(d[0], (uint8_t*)d[1], (float*)d[2], &p, s));
+    return undefined(env);
+}
+
+// A g4_lora record, or null for none.
+const g4_lora* lora_arg(Args& a, size_t i, g4_lora* l) {
+    if (!a.ok) return nullptr;
+    napi_valuetype t;
+    napi_typeof(a.env, a.v[i], &t);
+    if (t == napi_null || t == napi_undefined) return nullptr;
+    return a.params(i, l) ? l : nullptr;
+}
+
+napi_value LinearE4m3WorkspaceSize(napi_env env, napi_callback_info info) {
+    Args a(env, info, 2);  // params, lora
+    g4_linear_e4m3_params p;
+    g4_lora l;
+    a.params(0, &p);
+    const g4_lora* lora = lora_arg(a, 1, &l);
+    if (!a.ok) return nullptr;
+    size_t bytes = 0;
+    CALL(env, g4_linear_e4m3_workspace_size(&p, lora, &bytes));
+    return number(env, (double)bytes);
+}
+
+// linearE4m3(x, xScales, weight, weightScales, lora, adapterIds, out, params, workspace, workspaceBytes, stream)
+napi_value LinearE4m3(napi_env env, napi_callback_info info) {
+    Args a(env, info, 11);
+    void* d[4];
+    for (int i = 0; i < 4; i++) d[i] = a.ptr(i);
+    g4_lora l;
+    const g4_lora* lora = lora_arg(a, 4, &l);
+    void* ids = a.ptr(5);
+    void* out = a.ptr(6);
+    g4_linear_e4m3_params p;
+    a.params(7, &p);
+    void* ws = a.ptr(8);
+    const double ws_bytes = a.f64(9);
+    void* s = a.ptr(10);
+    if (!a.ok) return nullptr;
+    CALL(env, g4_linear_e4m3((const uint8_t*)d[0], (const float*)d[1], (const uint8_t*)d[2], (const float*)d[3], lora,
+                             (const int32_t*)ids, out, &p, ws, (size_t)ws_bytes, s));
+    return undefined(env);
+}
+
+napi_value LoraWorkspaceSize(napi_env env, napi_callback_info info) {
+    Args a(env, info, 2);  // lora, nTokens
+    g4_lora l;
+    a.params(0, &l);
+    const uint32_t n = a.u32(1);
+    if (!a.ok) return nullptr;
+    size_t bytes = 0;
+    CALL(env, g4_lora_workspace_size(&l, n, &bytes));
+    return number(env, (double)bytes);
+}
+
+// loraAdd(lora, adapterIds, x, xScales, base, out, params, workspace, workspaceBytes, stream)
+napi_value LoraAdd(napi_env env, napi_callback_info info) {
+    Args a(env, info, 10);
+    g4_lora l;
+    a.params(0, &l);
+    void* d[5];
+    for (int i = 0; i < 5; i++) d[i] = a.ptr(1 + i);
+    g4_lora_add_params p;
+    a.params(6, &p);
+    void* ws = a.ptr(7);
+    const double ws_bytes = a.f64(8);
+    void* s = a.ptr(9);
+    if (!a.ok) return nullptr;
+    CALL(env, g4_lora_add(&l, (const int32_t*)d[0], d[1], (const float*)d[2], d[3], d[4], &p, ws, (size_t)ws_bytes, s));
+    return undefined(env);
+}
+
 napi_value Init(napi_env env, napi_value exports) {
     struct {
         const char* name;
@@ -1531,6 +1628,12 @@ napi_value Init(napi_env env, napi_value exports) {
         {"pagedCommit", PagedCommit},
         {"tokenLogprobsWorkspaceSize", TokenLogprobsWorkspaceSize},
         {"tokenLogprobs", TokenLogprobs},
+        {"addRmsNorm", AddRmsNorm},
+        {"quantizeRows", QuantizeRows},
+        {"linearE4m3WorkspaceSize", LinearE4m3WorkspaceSize},
+        {"linearE4m3", LinearE4m3},
+        {"loraWorkspaceSize", LoraWorkspaceSize},
+        {"loraAdd", LoraAdd},
     };
     for (auto& f : fns) {
         napi_value fn;
@@ -1557,6 +1660,11 @@ napi_value Init(napi_env env, napi_value exports) {
         {"sizeofPagedAppendParams", sizeof(g4_paged_append_params)},
         {"sizeofPagedAttnParams", sizeof(g4_paged_attn_params)},
         {"sizeofTokenLogprobsParams", sizeof(g4_token_logprobs_params)},
+        {"sizeofAddRmsNormParams", sizeof(g4_add_rms_norm_params)},
+        {"sizeofQuantizeRowsParams", sizeof(g4_quantize_rows_params)},
+        {"sizeofLora", sizeof(g4_lora)},
+        {"sizeofLinearE4m3Params", sizeof(g4_linear_e4m3_params)},
+        {"sizeofLoraAddParams", sizeof(g4_lora_add_params)},
     };
     for (auto& s : sizes) NAPI_OK(env, napi_set_named_property(env, exports, s.name, number(env, (double)s.size)));
     return exports;

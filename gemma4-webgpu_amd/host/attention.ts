@@ -33,7 +33,7 @@ export type QuantKernelName = 'matmulQ8' | 'matmulQ4K';
 export type KernelName = AttnKernelName | SampleKernelName | QuantKernelName;
 
 export type FusedKernelName = 'attnStep' | 'attnPrefill' | 'attnPromptPrep' | 'lmHeadArgmax' | 'linearQkvPrep'
-  | 'pagedAppend' | 'pagedAttn' | 'pagedCommit' | 'tokenLogprobs';
+  | 'pagedAppend' | 'pagedAttn' | 'pagedCommit' | 'tokenLogprobs' | 'addRmsNorm' | 'quantizeRows' | 'linearE4m3' | 'loraAdd';
 
 export type UniformValue = { u: number } | { f: number };
 
@@ -92,6 +92,10 @@ export const PASS_LABELS: Record<string, string> = {
   pagedAttn: 'attn.paged',
   pagedCommit: 'attn.pagedCommit',
   tokenLogprobs: 'sample.tokenLogprobs',
+  addRmsNorm: 'norm.addRmsNorm',
+  quantizeRows: 'norm.quantizeRows',
+  linearE4m3: 'linear.e4m3',
+  loraAdd: 'linear.lora',
 };
 
 // The profiler's report types (src/types.ts:490-515).
@@ -340,6 +344,88 @@ export interface TokenLogprobs {
   temperature?: number;
 }
 
+export type RowDtype = 'f32' | 'f16' | 'bf16' | 'e4m3';
+
+// The residual's addition and the norms of a batch's rows; strides are elements from row to row, 0 for contiguous rows.
+export interface AddRmsNorm {
+  x: DeviceBuffer;            // [rows][n] of xDtype
+  residual?: DeviceBuffer;    // [rows][n] of residualDtype
+  residualOut?: DeviceBuffer; // of residualDtype; may be residual
+  postWeight?: DeviceBuffer;  // [n] of weightDtype: the branch's own norm, before the addition
+  weight?: DeviceBuffer;      // [n] of weightDtype (default: a norm without)
+  out?: DeviceBuffer;         // [rows][n] of outDtype (default: only the addition)
+  scales?: DeviceBuffer;      // f32 [rows], with an e4m3 out
+  rows: number;
+  n: number;
+  xDtype?: RowDtype;
+  residualDtype?: RowDtype;
+  weightDtype?: RowDtype;     // default f16
+  outDtype?: RowDtype;
+  eps?: number;
+  xStride?: number;
+  residualStride?: number;
+  residualOutStride?: number;
+  outStride?: number;
+}
+
+export interface QuantizeRows {
+  x: DeviceBuffer;            // [rows][n] of xDtype
+  out: DeviceBuffer;          // e4m3 [rows][n]
+  scales: DeviceBuffer;       // f32 [rows]
+  rows: number;
+  n: number;
+  xDtype?: RowDtype;
+  xStride?: number;
+  outStride?: number;
+}
+
+// The low-rank adapters of a projection: all of one rank, a segment of outputs for each part of a fused projection.
+export interface Lora {
+  a: DeviceBuffer;            // [nAdapters][widths.length * rank][n] of dtype
+  b: DeviceBuffer;            // [nAdapters][sum of widths][rank]
+  scales?: DeviceBuffer;      // f32 [nAdapters] (default: 1 each)
+  nAdapters: number;
+  rank: number;
+  n: number;
+  widths: number[];
+  dtype?: 'f16' | 'bf16';
+}
+
+// A projection of 8-bit rows, with its requests' adapters where lora and adapterIds are given.
+export interface LinearE4m3 {
+  x: DeviceBuffer;            // e4m3 [nTokens][n], scales f32 [nTokens]
+  xScales: DeviceBuffer;
+  weight: DeviceBuffer;       // e4m3 [rows][n], scales f32 [rows]
+  weightScales: DeviceBuffer;
+  out: DeviceBuffer;          // [nTokens][rows] of outDtype
+  nTokens: number;
+  rows: number;
+  n: number;
+  outDtype?: RowDtype;
+  xStride?: number;
+  outStride?: number;
+  lora?: Lora;
+  adapterIds?: DeviceBuffer;  // i32 [nTokens]; outside the adapters: none
+}
+
+// out = base + the adapters' part, beside a projection made elsewhere.
+export interface LoraAdd {
+  lora: Lora;
+  adapterIds: DeviceBuffer;   // i32 [nTokens]
+  x: DeviceBuffer;            // [nTokens][n] of xDtype, xScales f32 [nTokens] with e4m3
+  xScales?: DeviceBuffer;
+  base: DeviceBuffer;         // [nTokens][outputs] of outDtype; may be out
+  out: DeviceBuffer;
+  nTokens: number;
+  xDtype?: RowDtype;
+  outDtype?: RowDtype;
+  xStride?: number;
+  baseStride?: number;
+  outStride?: number;
+}
+
+const ROW_DTYPES: Record<string, number> = { f32: 0, f16: 1, bf16: 2, e4m3: 3 };
+const ROW_BYTES: Record<string, number> = { f32: 4, f16: 2, bf16: 2, e4m3: 1 };
 const KV_DTYPES: Record<string, number> = { f16: 0, e4m3: 1 };
 const LOGIT_DTYPES: Record<string, number> = { f32: 0, f16: 1, bf16: 2 };
 const LOGIT_BYTES: Record<string, number> = { f32: 4, f16: 2, bf16: 2 };
@@ -431,6 +517,15 @@ export interface Addon {
   tokenLogprobsWorkspaceSize(p: Uint8Array): number;
   tokenLogprobs(logits: bigint, tokens: bigint | null, logprobs: bigint | null, entropy: bigint | null,
     topIds: bigint | null, topLogprobs: bigint | null, p: Uint8Array, ws: bigint, wsBytes: number, s: bigint): void;
+  addRmsNorm(x: bigint, residual: bigint | null, post: bigint | null, weight: bigint | null, residualOut: bigint | null,
+    out: bigint | null, scales: bigint | null, p: Uint8Array, s: bigint): void;
+  quantizeRows(x: bigint, out: bigint, scales: bigint, p: Uint8Array, s: bigint): void;
+  linearE4m3WorkspaceSize(p: Uint8Array, lora: Uint8Array | null): number;
+  linearE4m3(x: bigint, xScales: bigint, weight: bigint, weightScales: bigint, lora: Uint8Array | null, ids: bigint | null,
+    out: bigint, p: Uint8Array, ws: bigint, wsBytes: number, s: bigint): void;
+  loraWorkspaceSize(lora: Uint8Array, nTokens: number): number;
+  loraAdd(lora: Uint8Array, ids: bigint, x: bigint, xScales: bigint | null, base: bigint, out: bigint, p: Uint8Array,
+    ws: bigint, wsBytes: number, s: bigint): void;
   [key: string]: any;
 }
 
@@ -988,6 +1083,137 @@ export class HipAttention {
     try {
       this.g4.tokenLogprobs(p.logits.ptr, ptr(p.tokens), ptr(p.logprobs), ptr(p.entropy), ptr(p.topIds), ptr(p.topLogprobs),
         params, workspace.ptr, workspace.size, this.stream);
+    } finally {
+      this.endPass(slot);
+    }
+  }
+
+  // Records of 4-byte fields, then 64-bit strides.
+  private static rowParams(fields: UniformValue[], strides: number[]): Uint8Array {
+    const bytes = new Uint8Array(4 * fields.length + 8 * strides.length);
+    const dv = new DataView(bytes.buffer);
+    fields.forEach(function (x, j) {
+      if ('f' in x) dv.setFloat32(4 * j, x.f, true);
+      else dv.setUint32(4 * j, x.u, true);
+    });
+    strides.forEach(function (x, j) { dv.setBigUint64(4 * fields.length + 8 * j, BigInt(x), true); });
+    return bytes;
+  }
+
+  // Throws where a buffer of rows (stride elements apart) is too small.
+  private static checkRows(what: string, name: string, b: DeviceBuffer | undefined, rows: number, n: number,
+    stride: number | undefined, dtype: string): void {
+    if (b && rows > 0 && b.size < ((rows - 1) * (stride || n) + n) * ROW_BYTES[dtype]) {
+      throw new RangeError(what + ': ' + name + ' too small');
+    }
+  }
+
+  // The residual's addition and the norm(s) of a batch's rows in one pass; e4m3 rows with a scale each for linearE4m3.
+  addRmsNorm(p: AddRmsNorm): void {
+    const what = 'addRmsNorm';
+    const x = p.xDtype || 'f32', r = p.residualDtype || x, w = p.weightDtype || 'f16', o = p.outDtype || 'f32';
+    const codes = [x, r, w, o].map(function (d) { return dtypeCode(ROW_DTYPES, d, what); });
+    HipAttention.checkRows(what, 'x', p.x, p.rows, p.n, p.xStride, x);
+    HipAttention.checkRows(what, 'residual', p.residual, p.rows, p.n, p.residualStride, r);
+    HipAttention.checkRows(what, 'residualOut', p.residualOut, p.rows, p.n, p.residualOutStride, r);
+    HipAttention.checkRows(what, 'out', p.out, p.rows, p.n, p.outStride, o);
+    HipAttention.checkRows(what, 'scales', p.scales, p.rows, 1, 1, 'f32');
+    HipAttention.checkRows(what, 'weight', p.weight, 1, p.n, 0, w);
+    HipAttention.checkRows(what, 'postWeight', p.postWeight, 1, p.n, 0, w);
+    const params = HipAttention.rowParams([{ u: p.rows }, { u: p.n }, { u: codes[0] }, { u: codes[1] }, { u: codes[2] },
+      { u: codes[3] }, { f: p.eps === undefined ? 1e-6 : p.eps }, { u: 0 }],
+      [p.xStride || 0, p.residualStride || 0, p.residualOutStride || 0, p.outStride || 0]);
+    function ptr(b: DeviceBuffer | undefined): bigint | null { return b ? b.ptr : null; }
+    const slot = this.beginPass(PASS_LABELS.addRmsNorm);
+    try {
+      this.g4.addRmsNorm(p.x.ptr, ptr(p.residual), ptr(p.postWeight), ptr(p.weight), ptr(p.residualOut), ptr(p.out),
+        ptr(p.scales), params, this.stream);
+    } finally {
+      this.endPass(slot);
+    }
+  }
+
+  // Rows in 8 bits with a scale each: activations before linearE4m3, its weights once.
+  quantizeRows(p: QuantizeRows): void {
+    const what = 'quantizeRows';
+    const x = p.xDtype || 'f32';
+    const code = dtypeCode(ROW_DTYPES, x, what);
+    HipAttention.checkRows(what, 'x', p.x, p.rows, p.n, p.xStride, x);
+    HipAttention.checkRows(what, 'out', p.out, p.rows, p.n, p.outStride, 'e4m3');
+    HipAttention.checkRows(what, 'scales', p.scales, p.rows, 1, 1, 'f32');
+    const params = HipAttention.rowParams([{ u: p.rows }, { u: p.n }, { u: code }, { u: 0 }], [p.xStride || 0, p.outStride || 0]);
+    const slot = this.beginPass(PASS_LABELS.quantizeRows);
+    try {
+      this.g4.quantizeRows(p.x.ptr, p.out.ptr, p.scales.ptr, params, this.stream);
+    } finally {
+      this.endPass(slot);
+    }
+  }
+
+  // g4_lora: three pointers, then ten 4-byte fields.
+  static loraBytes(l: Lora): Uint8Array {
+    const rows = l.widths.reduce(function (x, y) { return x + y; }, 0);
+    if (l.widths.length < 1 || l.widths.length > 4) throw new RangeError('lora: 1 to 4 segments');
+    if (l.a.size < l.nAdapters * l.widths.length * l.rank * l.n * 2) throw new RangeError('lora: a too small');
+    if (l.b.size < l.nAdapters * rows * l.rank * 2) throw new RangeError('lora: b too small');
+    if (l.scales && l.scales.size < l.nAdapters * 4) throw new RangeError('lora: scales too small');
+    const bytes = new Uint8Array(64);
+    const dv = new DataView(bytes.buffer);
+    [l.a, l.b, l.scales].forEach(function (x, j) { dv.setBigUint64(8 * j, x ? x.ptr : BigInt(0), true); });
+    [l.nAdapters, l.rank, l.n, l.widths.length].forEach(function (x, j) { dv.setUint32(24 + 4 * j, x, true); });
+    l.widths.forEach(function (x, j) { dv.setUint32(40 + 4 * j, x, true); });
+    dv.setUint32(56, dtypeCode(ROW_DTYPES, l.dtype || 'f16', 'lora'), true);
+    return bytes;
+  }
+
+  private static linearE4m3Params(p: LinearE4m3): Uint8Array {
+    return HipAttention.rowParams([{ u: p.nTokens }, { u: p.rows }, { u: p.n },
+      { u: dtypeCode(ROW_DTYPES, p.outDtype || 'f32', 'linearE4m3') }], [p.xStride || 0, p.outStride || 0]);
+  }
+
+  linearE4m3WorkspaceSize(p: LinearE4m3): number {
+    return this.g4.linearE4m3WorkspaceSize(HipAttention.linearE4m3Params(p), p.lora ? HipAttention.loraBytes(p.lora) : null);
+  }
+
+  linearE4m3(p: LinearE4m3, workspace: DeviceBuffer): void {
+    const what = 'linearE4m3';
+    const params = HipAttention.linearE4m3Params(p);
+    HipAttention.checkRows(what, 'x', p.x, p.nTokens, p.n, p.xStride, 'e4m3');
+    HipAttention.checkRows(what, 'xScales', p.xScales, p.nTokens, 1, 1, 'f32');
+    HipAttention.checkRows(what, 'weight', p.weight, p.rows, p.n, 0, 'e4m3');
+    HipAttention.checkRows(what, 'weightScales', p.weightScales, p.rows, 1, 1, 'f32');
+    HipAttention.checkRows(what, 'out', p.out, p.nTokens, p.rows, p.outStride, p.outDtype || 'f32');
+    HipAttention.checkRows(what, 'adapterIds', p.adapterIds, p.nTokens, 1, 1, 'f32');
+    const lora = p.lora ? HipAttention.loraBytes(p.lora) : null;
+    const slot = this.beginPass(PASS_LABELS.linearE4m3);
+    try {
+      this.g4.linearE4m3(p.x.ptr, p.xScales.ptr, p.weight.ptr, p.weightScales.ptr, lora,
+        p.adapterIds ? p.adapterIds.ptr : null, p.out.ptr, params, workspace.ptr, workspace.size, this.stream);
+    } finally {
+      this.endPass(slot);
+    }
+  }
+
+  loraWorkspaceSize(lora: Lora, nTokens: number): number {
+    return this.g4.loraWorkspaceSize(HipAttention.loraBytes(lora), nTokens);
+  }
+
+  loraAdd(p: LoraAdd, workspace: DeviceBuffer): void {
+    const what = 'loraAdd';
+    const rows = p.lora.widths.reduce(function (x, y) { return x + y; }, 0);
+    const x = p.xDtype || 'f32', o = p.outDtype || 'f32';
+    const params = HipAttention.rowParams([{ u: p.nTokens }, { u: dtypeCode(ROW_DTYPES, x, what) },
+      { u: dtypeCode(ROW_DTYPES, o, what) }, { u: 0 }], [p.xStride || 0, p.baseStride || 0, p.outStride || 0]);
+    HipAttention.checkRows(what, 'adapterIds', p.adapterIds, p.nTokens, 1, 1, 'f32');
+    HipAttention.checkRows(what, 'x', p.x, p.nTokens, p.lora.n, p.xStride, x);
+    HipAttention.checkRows(what, 'xScales', p.xScales, p.nTokens, 1, 1, 'f32');
+    HipAttention.checkRows(what, 'base', p.base, p.nTokens, rows, p.baseStride, o);
+    HipAttention.checkRows(what, 'out', p.out, p.nTokens, rows, p.outStride, o);
+    const lora = HipAttention.loraBytes(p.lora);
+    const slot = this.beginPass(PASS_LABELS.loraAdd);
+    try {
+      this.g4.loraAdd(lora, p.adapterIds.ptr, p.x.ptr, p.xScales ? p.xScales.ptr : null, p.base.ptr, p.out.ptr, params,
+        workspace.ptr, workspace.size, this.stream);
     } finally {
       this.endPass(slot);
     }

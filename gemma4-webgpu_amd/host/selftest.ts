@@ -122,6 +122,30 @@ function pagedChecks(g4: any): void {
     'temperature 0');
 }
 
+// The records of the operators between two blocks, and the refusals that need no GPU.
+function blockChecks(g4: any): void {
+  const sizes: [string, number][] = [['sizeofAddRmsNormParams', 64], ['sizeofQuantizeRowsParams', 32], ['sizeofLora', 64],
+    ['sizeofLinearE4m3Params', 32], ['sizeofLoraAddParams', 40]];
+  for (const s of sizes) if (g4[s[0]] !== s[1]) fail(`${s[0]}: ${g4[s[0]]} B, the host writes ${s[1]}`);
+  function buf(ptr: number, size: number): DeviceBuffer { return { ptr: BigInt(ptr), size: size }; }
+  const lora = { a: buf(0x1000, 2 * 16 * 64 * 2), b: buf(0x9000, 2 * 50 * 8 * 2), nAdapters: 2, rank: 8, n: 64, widths: [30, 20] };
+  const bytes = HipAttention.loraBytes(lora);
+  const dv = new DataView(bytes.buffer);
+  if (dv.getBigUint64(8, true) !== BigInt(0x9000) || dv.getUint32(44, true) !== 20 || dv.getUint32(56, true) !== 1) fail('lora record');
+  throws(() => HipAttention.loraBytes(Object.assign({}, lora, { nAdapters: 3 })), 'a too small');
+  throws(() => HipAttention.loraBytes(Object.assign({}, lora, { widths: [] })), 'no segment');
+  if (!(g4.loraWorkspaceSize(bytes, 5) >= 5 * 16 * 4)) fail('loraWorkspaceSize');
+  const short = new Uint8Array(bytes);
+  new DataView(short.buffer).setUint32(28, 12, true);
+  throws(() => g4.loraWorkspaceSize(short, 5), 'rank 12');
+  throws(() => g4.loraWorkspaceSize(bytes.subarray(0, 32), 5), 'short lora record');
+  const linear = new Uint8Array(32);
+  [5, 50, 64, 0].forEach(function (x, j) { new DataView(linear.buffer).setUint32(4 * j, x, true); });
+  if (!(g4.linearE4m3WorkspaceSize(linear, null) > 0)) fail('linearE4m3WorkspaceSize');
+  if (!(g4.linearE4m3WorkspaceSize(linear, bytes) > g4.linearE4m3WorkspaceSize(linear, null))) fail('linearE4m3WorkspaceSize with lora');
+  throws(() => g4.quantizeRows(BigInt(0), BigInt(16), BigInt(16), new Uint8Array(32), BigInt(0)), 'no rows, n 0');
+}
+
 export function cpuChecks(): string[] {
   const done: string[] = [];
   const g4 = loadAddon();
@@ -163,6 +187,7 @@ export function cpuChecks(): string[] {
   throws(() => g4.attnPromptPrepMany(new Uint8Array(100), 1, BigInt(0)), 'attnPromptPrepMany: short record');
   done.push('prompt prep records');
   pagedChecks(g4);
+  blockChecks(g4);
   done.push('paged records');
   return done;
 }
@@ -402,6 +427,80 @@ function paged(dir: string): string[] {
   for (const b of bufs) att.destroyBuffer(b);
   att.dispose();
   return ['paged: append, attention, log probabilities, commit', 'results written'];
+}
+
+interface BlockSpec {
+  nqh: number; hd: number; hidden: number; pages: number; pageSize: number; nSeqs: number; tableStride: number; nTokens: number;
+  maxTokens: number; rank: number; adapters: number; arrays: Record<string, number[]>;
+}
+
+// A block of a batch through the host: norm, fused projection with adapters, append, attention, 8-bit rows, output
+// projection, adapters beside it, residual and norm. out.bin = qkv, attention, sum, codes, scales, K pool, V pool.
+function block(dir: string): string[] {
+  const spec = JSON.parse(fs.readFileSync(path.join(dir, 'case.json'), 'utf8')) as BlockSpec;
+  const bin: Uint8Array = fs.readFileSync(path.join(dir, 'case.bin'));
+  const att = new HipAttention(loadAddon(), 0);
+  const bufs: DeviceBuffer[] = [];
+  function alloc(bytes: number): DeviceBuffer {
+    const b = att.createBuffer(bytes);
+    bufs.push(b);
+    return b;
+  }
+  function upload(name: string): DeviceBuffer {
+    const r = spec.arrays[name];
+    const b = alloc(r[1]);
+    att.writeBuffer(b, 0, bin.subarray(r[0], r[0] + r[1]));
+    return b;
+  }
+  const n = spec.nTokens, h = spec.hidden, hd = spec.hd, nqh = spec.nqh, width = (nqh + 2) * hd;
+  const cache = { kPool: upload('kPool'), vPool: upload('vPool'), numPages: spec.pages, pageSize: spec.pageSize, numKvHeads: 1,
+    headDim: hd };
+  const batch = { blockTable: upload('table'), tokenStart: upload('start'), ctxLens: upload('ctx'), nSeqs: spec.nSeqs,
+    tableStride: spec.tableStride, nTokens: n, maxTokens: spec.maxTokens };
+  const ids = upload('ids');
+  const rows8 = alloc(n * h), scales = alloc(n * 4), residual = upload('residual');
+  att.addRmsNorm({ x: upload('branch'), residual: residual, residualOut: residual, postWeight: upload('post'), weight: upload('pre'),
+    out: rows8, scales: scales, rows: n, n: h, outDtype: 'e4m3' });
+  const w8 = alloc(width * h), ws8 = alloc(width * 4);
+  att.quantizeRows({ x: upload('wqkv'), out: w8, scales: ws8, rows: width, n: h });
+  const lora1 = { a: upload('a1'), b: upload('b1'), nAdapters: spec.adapters, rank: spec.rank, n: h, widths: [nqh * hd, hd, hd] };
+  const qkv = alloc(n * width * 4);
+  const lin = { x: rows8, xScales: scales, weight: w8, weightScales: ws8, out: qkv, nTokens: n, rows: width, n: h, lora: lora1,
+    adapterIds: ids };
+  att.linearE4m3(lin, alloc(att.linearE4m3WorkspaceSize(lin)));
+  const qOut = alloc(n * nqh * hd * 2), out = alloc(n * nqh * hd * 4);
+  function part(first: number): DeviceBuffer {
+    return { ptr: qkv.ptr + BigInt(first * hd * 4), size: qkv.size - first * hd * 4 };
+  }
+  att.pagedAppend(cache, batch, { q: part(0), k: part(nqh), v: part(nqh + 1), qWeight: upload('qw'), kWeight: upload('kw'),
+    ropeInvFreq: upload('inv'), qOut: qOut, numQHeads: nqh, qStride: width, kStride: width, vStride: width });
+  att.pagedAttn(cache, batch, { q: qOut, out: out, numQHeads: nqh }, alloc(att.pagedAttnWorkspaceSize(cache, batch, nqh)));
+  const o8 = alloc(n * nqh * hd), os8 = alloc(n * 4), wo8 = alloc(h * nqh * hd), wos8 = alloc(h * 4), y = alloc(n * h * 4);
+  att.quantizeRows({ x: out, out: o8, scales: os8, rows: n, n: nqh * hd });
+  att.quantizeRows({ x: upload('wo'), out: wo8, scales: wos8, rows: h, n: nqh * hd });
+  const proj = { x: o8, xScales: os8, weight: wo8, weightScales: wos8, out: y, nTokens: n, rows: h, n: nqh * hd };
+  att.linearE4m3(proj, alloc(att.linearE4m3WorkspaceSize(proj)));
+  const lora2 = { a: upload('a2'), b: upload('b2'), scales: upload('alpha'), nAdapters: spec.adapters, rank: spec.rank, n: nqh * hd,
+    widths: [h] };
+  att.loraAdd({ lora: lora2, adapterIds: ids, x: o8, xScales: os8, base: y, out: y, nTokens: n, xDtype: 'e4m3' },
+    alloc(att.loraWorkspaceSize(lora2, n)));
+  att.addRmsNorm({ x: y, residual: residual, residualOut: residual, weight: upload('next'), out: rows8, scales: scales, rows: n, n: h,
+    outDtype: 'e4m3' });
+  throws(function () { att.quantizeRows({ x: out, out: os8, scales: os8, rows: n, n: nqh * hd }); }, 'quantizeRows: out too small');
+  throws(function () { att.linearE4m3(lin, os8); }, 'short workspace');
+  const outs = [qkv, out, residual, rows8, scales, cache.kPool, cache.vPool];
+  let total = 0;
+  for (const o of outs) total += o.size;
+  const res = new Uint8Array(total);
+  let off = 0;
+  for (const o of outs) {
+    att.readBuffer(o, 0, res.subarray(off, off + o.size));
+    off += o.size;
+  }
+  fs.writeFileSync(path.join(dir, 'out.bin'), res);
+  for (const b of bufs) att.destroyBuffer(b);
+  att.dispose();
+  return ['block: norm, projection with adapters, append, attention, 8-bit rows, projection, adapters, norm', 'results written'];
 }
 
 interface PromptPrepSpec {
@@ -923,8 +1022,9 @@ export function main(argv: string[]): void {
   else if (mode === 'prefill') done = prefill(argv[1]);
   else if (mode === 'promptprep') done = promptPrep(argv[1]);
   else if (mode === 'paged') done = paged(argv[1]);
+  else if (mode === 'block') done = block(argv[1]);
   else if (mode === 'linear') done = linear(argv[1]);
   else if (mode === 'qkvprep') done = qkvPrep(argv[1]);
-  else fail(`usage: run.js cpu | layer <dir> | prefill <dir> | promptprep <dir> | paged <dir> | head <dir> | linear <dir> | qkvprep <dir> | capture <dir> | batch <dir> | readback <dir> | profile`);
+  else fail(`usage: run.js cpu | layer <dir> | prefill <dir> | promptprep <dir> | paged <dir> | block <dir> | head <dir> | linear <dir> | qkvprep <dir> | capture <dir> | batch <dir> | readback <dir> | profile`);
   process.stdout.write(JSON.stringify({ ok: true, checks: done }) + '\n');
 }
