@@ -1,5 +1,10 @@
 // Low-rank adapters of many requests beside a projection made elsewhere
 // (g4_lora_add), and the down product that linear8.hip shares.
+//
+// Bound by latency for few tokens (one token's q, k, v of rank 16: 2.9 us down, 3.8 up, two launches that each wait for
+// ids, rows and sums in turn; 64 requests of 40 adapters beside their projection: 3.4 us down, 8.0 for the projection with
+// the up product in it), by the adapters' way through the caches for many: a tile of 16 tokens reads all of
+// its adapter (4003 tokens, n 2048, rank 64: 10.4 us for 64 MB of them).
 #include <type_traits>
 
 #include "lora.h"
@@ -333,8 +338,9 @@ LoraDev lora_dev(const g4_lora* l, uint32_t n_tokens) {
 
 size_t lora_bytes(const g4_lora* l, uint32_t n_tokens) { return (size_t)n_tokens * l->n_segs * l->rank * 4 + 16; }
 
-// Few tokens: a wave a token and four rows reads its rows and no others' (64 requests of 40 adapters, n 1536); from
-// some hundred tokens on, the matrix units' tiles read an adapter once for 32 of them.
+// Few tokens: a wave a token and four rows, no adapter waiting for another (64 requests of 40 adapters, n 1536: 3.4 us,
+// 5.0 by tiles and a split of k). Every token reads its adapter for itself, so from some hundred tokens on the matrix
+// units' tiles take their place, which read it once for 16 or 32 of them.
 constexpr uint32_t kLoraFewTokens = 128;
 
 template <int MODE>

@@ -85,18 +85,20 @@ static __device__ __attribute__((aligned(16))) const uint32_t kZeros[4] = {0, 0,
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"  // M0 is a reserved register: clobbering it is what is meant
 // 16 bytes a lane from base + its offset, or from its address, to LDS lds + at + 16 lane. No memory clobber: it writes a
-// stage that nothing reads before the barrier that waits for it, and reads of other stages may pass it.
+// stage that nothing reads before the barrier that waits for it, and reads of other stages may pass it. Wait states that
+// the compiler does not put into assembly: one between a scalar write of M0 and the DMA, five between a vector instruction
+// that leaves the base in scalar registers and the DMA.
 template <unsigned AT>
 __device__ __forceinline__ void stage_dma(const void* base, uint32_t off, uint32_t lds) {
-    asm volatile("s_add_u32 m0, %2, %3\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds), "n"(AT) : "m0", "scc");
+    asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds), "n"(AT) : "m0", "scc");
 }
 template <unsigned AT>
 __device__ __forceinline__ void stage_dma(const void* from, uint32_t lds) {
-    asm volatile("s_add_u32 m0, %1, %2\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(lds), "n"(AT) : "m0", "scc");
+    asm volatile("s_add_u32 m0, %1, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(lds), "n"(AT) : "m0", "scc");
 }
 // Four bytes a lane to LDS lds + 4 lane.
 __device__ __forceinline__ void scale_dma(const void* from, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(lds) : "m0");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(lds) : "m0");
 }
 #pragma clang diagnostic pop
 

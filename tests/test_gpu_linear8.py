@@ -86,6 +86,19 @@ def test_strided_rows(dev, tokens, kind, offset, stride):
     assert (flat == 7.0).all()
 
 
+@pytest.mark.parametrize("tokens,rows,stride", [(300, 4096, (1 << 24) - 16), (270, 40, 1 << 24), (20, 24, 1 << 28)])
+def test_offsets_past_32_bits(dev, tokens, rows, stride):
+    """Tokens that lie far apart: by tiles, and where a tile's offsets would not fit."""
+    announce(f"linearE4m3 tokens {stride} bytes apart")
+    x, xs, w, ws = make(dev, 13, tokens, rows, 64)
+    flat = torch.empty((tokens - 1) * stride + 64, dtype=torch.uint8, device=dev)
+    far = flat.as_strided((tokens, 64), (stride, 1))
+    far.copy_(x.view(torch.uint8))
+    got = call(far.view(TYPES["e4m3"]), xs, w, ws, "f16")
+    want, tol = linear(*(t.cpu().float() for t in (x, xs, w, ws)), "f16")
+    within(got.cpu(), want, tol + rounding(want, "f16"), "out")
+
+
 @pytest.mark.parametrize("tokens", [3, 50, 300])
 def test_rows_that_are_not_finite_stay_alone(dev, tokens):
     """A token of NaN codes or scale, and an output's weights: its row, its column, and nothing else. NaN behind a row's

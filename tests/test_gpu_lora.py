@@ -150,6 +150,23 @@ def test_sizes_of_the_inner_sums(dev, kind):
 
 
 @pytest.mark.parametrize("tokens", [6, 300])
+def test_adapters_past_32_bits(dev, tokens):
+    """The last of 1100 adapters begins 4.6e9 elements after the first."""
+    L, n, widths = 1100, 8192, (16, 8, 24, 16)
+    announce(f"lora adapters past 32 bits, tokens={tokens}")
+    small = adapters(dev, 39, 2, 128, widths, n)
+    a = torch.empty(L, 512, n, dtype=torch.float16, device=dev)
+    b = torch.empty(L, 64, 128, dtype=torch.float16, device=dev)
+    a[0], a[L - 1], b[0], b[L - 1] = small.a[0], small.a[1], small.b[0], small.b[1]
+    low = ops.LoraAdapters(a, b, None, widths)
+    same = ops.LoraAdapters(small.a, small.b, None, widths)
+    ids = (torch.arange(tokens, dtype=torch.int32, device=dev) % 3 - 1)
+    x = torch.randn(tokens, n, generator=torch.Generator().manual_seed(4)).half().to(dev)
+    base = torch.zeros(tokens, 64, device=dev)
+    assert torch.equal(add(low, torch.where(ids == 1, L - 1, ids).int(), x, base), add(same, ids, x, base))
+
+
+@pytest.mark.parametrize("tokens", [6, 300])
 def test_ids_out_of_range_and_other_adapters_do_not_matter(dev, tokens):
     announce(f"lora ids {tokens}")
     low = adapters(dev, 31, 4, 16, (90,), 192)
