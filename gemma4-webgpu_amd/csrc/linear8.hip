@@ -472,9 +472,10 @@ void launch_few(const Linear8Args& a, hipStream_t st) {
 }
 
 // The largest tile that there are about enough of for the compute units, as long as there are; else tiles of 16 or 32
-// whose waves share k (us, n 1536; tiles of 256 / 128 / 64 / few): 1024 tokens by 12288 outputs 29.4 / 33.6 / 40.5 / -,
-// 256 by 12288 22.5 / 12.7 / 14.7 / 36.6, 1024 by 2560 (f32) 43 / 22.9 / 17.8 / 30.7, 64 by 12288 19.2 / 11.1 / 7.1 / 12.2,
-// 256 by 2560 - / 21.8 / 11.0 / 11.4, 128 by 2560 - / 21.2 / 10.6 / 7.6, 64 by 2560 - / 20.3 / 10.6 / 5.8.
+// whose waves share k (us, n 1536; tiles of 256 / 128 / 64 / few): 1024 tokens by 12288 outputs 28.9 / 33.4 / 44.2 / 133, 256 by
+// 12288 22.2 / 12.4 / 15.4 / 35.7, 64 by 12288 19.4 / 11.1 / 7.5 / 11.6; f32 outputs: 1024 by 2560 43.1 / 23.4 / 18.0 / 31.1, 256 by
+// 2560 42.0 / 21.7 / 10.9 / 11.3, 64 by 2560 35.6 / 20.2 / 10.4 / 5.4. Few tokens: 16 outputs by 16 tokens (one token by 2560
+// 3.5 us, 32 outputs 4.3), 32 by 32 up to 96 tokens (64 by 2560 5.7, 32 by 64 7.2), above 32 by 64 (128 by 2560 7.6, 8.5).
 void launch_linear8(const Linear8Args& a, hipStream_t st) {
     auto tiles = [&](uint32_t side) { return (uint64_t)((a.rows + side - 1) / side) * ((a.n_tokens + side - 1) / side); };
     const uint64_t cus = device_cus();

@@ -338,10 +338,11 @@ LoraDev lora_dev(const g4_lora* l, uint32_t n_tokens) {
 
 size_t lora_bytes(const g4_lora* l, uint32_t n_tokens) { return (size_t)n_tokens * l->n_segs * l->rank * 4 + 16; }
 
-// Few tokens: a wave a token and four rows, no adapter waiting for another (64 requests of 40 adapters, n 1536: 3.4 us,
-// 5.0 by tiles and a split of k). Every token reads its adapter for itself, so from some hundred tokens on the matrix
-// units' tiles take their place, which read it once for 16 or 32 of them.
-constexpr uint32_t kLoraFewTokens = 128;
+// A wave a token and four rows where that reads at most 64 MB of adapters, no adapter waiting for another; beyond, the
+// matrix units' tiles, which read an adapter once for 16 or 32 tokens (us of lora_add, 2560 outputs, waves / tiles; four
+// runs of tokens: 256 tokens, rank 64, n 1536 9.5 / 10.0; 1024, 16, 1536 13.6 / 13.7; 256, 64, 4096 14.0 / 13.8; 512, 64, 1536
+// 14.9 / 12.3; 1024, 64, 1536 25.3 / 17.5; every token another of 40 adapters, rank 16: 64 tokens 6.7 / 58, 1024 22.7 / 73.5).
+static bool lora_by_waves(const LoraDev& d) { return (uint64_t)d.n_tokens * d.down * d.n <= 1u << 25; }
 
 template <int MODE>
 static void launch_down(const DownArgs& a, hipStream_t st) {
@@ -360,7 +361,7 @@ static void launch_down_few(const DownArgs& a, hipStream_t st) {
 void lora_launch_down(const LoraDev& d, uint32_t lora_type, const void* x, uint32_t x_type, uint64_t x_stride,
                       const float* x_scales, hipStream_t st) {
     const DownArgs a = {d, x, x_scales, x_stride, x_type, lora_type};
-    if (d.n_tokens <= kLoraFewTokens) {
+    if (lora_by_waves(d)) {
         if (x_type == G4_F32) launch_down_few<G4_F32>(a, st);
         else if (x_type == G4_F16) launch_down_few<G4_F16>(a, st);
         else if (x_type == G4_BF16) launch_down_few<G4_BF16>(a, st);
@@ -434,7 +435,9 @@ int g4_lora_add(const g4_lora* lora, const int32_t* adapter_ids, const void* x, 
         if (lora->type == G4_F16) G4_LAUNCH((k_lora_up<TILES, false>), grid, block, 0, as_stream(stream), a);
         else G4_LAUNCH((k_lora_up<TILES, true>), grid, block, 0, as_stream(stream), a);
     };
-    if (p->n_tokens <= kLoraFewTokens) launch(std::integral_constant<int, 1>{});  // more waves, each waiting for less
+    // Few tokens: more waves, each waiting for less; many: a token's sums serve four tiles (us, 2560 outputs, rank 16, one
+    // tile a wave / four: 64 tokens 6.8 / 10.6, 256 7.0 / 7.4, 512 9.0 / 8.7, 4096 34.5 / 28.5).
+    if (p->n_tokens <= 256) launch(std::integral_constant<int, 1>{});
     else launch(std::integral_constant<int, 4>{});
     G4_CHECK_LAUNCH("k_lora_up");
     return G4_OK;

@@ -112,6 +112,18 @@ def test_types(dev, x_kind, kind, out_kind):
     check_add(dev, 9, 330, 336, low, x_kind, out_kind, runs=5)
 
 
+@pytest.mark.parametrize("x_kind,kind", [("f16", "f16"), ("bf16", "bf16"), ("e4m3", "f16"), ("e4m3", "bf16"), ("f32", "f16"),
+                                         ("bf16", "f16"), ("f16", "bf16")])
+@pytest.mark.parametrize("tokens,rank,widths,n", [(530, 16, (40,), 4112), (1100, 128, (9, 20, 8, 3), 64), (2050, 24, (30, 30), 400)])
+@pytest.mark.parametrize("runs", [5, 5000])
+def test_down_products_by_tiles(dev, x_kind, kind, tokens, rank, widths, n, runs):
+    """More than 2^25 products' worth of adapters: runs of tokens, and tiles whose every token has another adapter."""
+    announce(f"lora tiles x={x_kind} adapters={kind} tokens={tokens} runs={runs}")
+    low = adapters(dev, tokens, 7, rank, widths, n, kind)
+    assert tokens * low.a.shape[1] * n > 1 << 25
+    check_add(dev, runs, tokens, n, low, x_kind, "f32", min(runs, tokens))
+
+
 @pytest.mark.parametrize("n", [16, 32, 48, 64, 80, 128, 1008, 1536, 2064, 8192])
 @pytest.mark.parametrize("tokens", [1, 20, 260])
 def test_inputs(dev, n, tokens):
