@@ -13,7 +13,7 @@
 // are under way (types told apart at run time: 87 us below).
 //
 // Measured (a copy reaches 5.0 TB/s here): 8191 rows of 5376, 16 bits in, sum out, e4m3 out, 61 us, 5.1 TB/s;
-// 4096 rows of 1536, f32 in, both norms, 15.2 us, 5.4 TB/s; 4000 attention outputs of 2048 in 8 bits 8.2 us; one row
+// 4096 rows of 1536, f32 in, both norms, 15.2 us; 4000 attention outputs of 2048 in 8 bits 8.2 us; one row
 // 2.9 us, the launch and two chains of loads and sums.
 #include <type_traits>
 
@@ -285,11 +285,12 @@ void launch_norm_rows(const NormRowsArgs& a, hipStream_t st) {
         G4_LAUNCH((k_norm_rows<TPR, NV, VEC, XW, RW, WW>), grid, block, 0, st, a);
     };
 #define G4_NORM(TPR, NV) launch(std::integral_constant<int, TPR>{}, std::integral_constant<int, NV>{})
-    // A wave a row where the rows fill the chip with waves; else four waves a row.
-    const bool many = a.rows >= 8 * device_cus();
+    // A wave a row where rows are short and many, else four waves a row (us, f32 with both norms into e4m3, a wave / four: rows
+    // of 512: 512 of them 3.6 / 3.8, 1024 4.3 / 5.3, 16384 22.6 / 37.1; 2048 of 1024 9.1 / 10.0; of 1536: 64 4.3 / 3.5, 2048 11.4 /
+    // 10.9, 16384 59.8 / 58.9).
+    const bool many = a.rows >= 2 * device_cus();
     if (many && a.n <= 512) G4_NORM(64, 1);
     else if (many && a.n <= 1024) G4_NORM(64, 2);
-    else if (many && a.n <= 1536) G4_NORM(64, 3);
     else if (a.n <= 2048) G4_NORM(256, 1);
     else if (a.n <= 4096) G4_NORM(256, 2);
     else if (a.n <= 6144) G4_NORM(256, 3);
