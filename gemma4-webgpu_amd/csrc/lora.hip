@@ -11,9 +11,9 @@
 
 namespace g4 {
 
-// How x and the adapters' rows meet. 16-bit products are exact in f32, and so is an e4m3 element as f16 or bf16; other
-// pairs are widened to f32.
-enum { kDownF16, kDownBf16, kDownE4m3F16, kDownE4m3Bf16, kDownF32 };
+// How x and the adapters' rows meet. 16-bit products are exact in f32, and so is an e4m3 element as f16 or bf16; f32 rows,
+// and 16-bit ones of the adapters' other type (mixed), meet them as f32.
+enum { kDownF16, kDownBf16, kDownE4m3F16, kDownE4m3Bf16, kDownF32, kDownMixed };
 
 struct DownArgs {
     LoraDev l;
@@ -42,21 +42,12 @@ __device__ __forceinline__ u32x4 e4m3_wide(u32x2 q) {
     return r;
 }
 
-// Sixteen elements of a row as f32.
-__device__ __forceinline__ void wide16(f32x4 (&v)[4], const void* row, uint32_t type, unsigned k, bool in) {
-    const bool full = type == G4_F32;
-    const char* p = static_cast<const char*>(row) + (full ? 4 * k : 2 * k);
-    u32x4 r[4];
+// 8 elements of a 16-bit type as f32.
+__device__ __forceinline__ void wide8(float (&v)[8], u32x4 q, uint32_t type) {
 #pragma unroll
-    for (int q = 0; q < 4; q++) {
-        r[q] = u32x4{0, 0, 0, 0};
-        if (in && (full || q < 2)) r[q] = ldg<u32x4>(p + 16 * q);
-    }
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
-        const uint32_t w = r[i / 8][i % 8 / 2];
-        const float h = h2f((uint16_t)(w >> (16 * (i & 1)))), b = __uint_as_float((i & 1) ? w & 0xFFFF0000u : w << 16);
-        v[i / 4][i % 4] = full ? __uint_as_float(r[i / 4][i % 4]) : type == G4_F16 ? h : b;
+    for (int i = 0; i < 8; i++) {
+        const float h = h2f((uint16_t)(q[i / 2] >> (16 * (i & 1)))), b = __uint_as_float((i & 1) ? q[i / 2] & 0xFFFF0000u : q[i / 2] << 16);
+        v[i] = type == G4_F16 ? h : b;
     }
 }
 
@@ -118,7 +109,10 @@ __global__ __launch_bounds__(kFewWaves * 64) void k_lora_down_few(const DownArgs
 //
 // Each wave takes every Wth 64 k and brings both operands of it to LDS by DMA, one chunk ahead: loaded straight into the matrix
 // unit's layout, in which neighbouring lanes lie in different rows, every lane's 16 bytes are an access of their own (4003
-// tokens, n 2048, rank 64: 21 us). Piece c (16 bytes) of row r lies at c ^ r % 8 of its 128 bytes, c ^ r / 2 % 4 of its 64.
+// tokens, n 2048, rank 64: 21 us). Piece c (16 bytes) of row r lies at
+// c ^ r / 2 % 4 of its 64 bytes, c ^ r % 8 of its 128, c ^ r % 16 of its 256.
+// Products in f32 (f32 rows, mixed types) run at a sixteenth of the 16-bit rate and fill that time with the widening: 4003 tokens,
+// n 2048, rank 64 and the up product to 2560 take 65 us, with equal 16-bit types 43.
 constexpr int kDownWaves = 4, kDownRows = 4;  // 16-wide tiles
 template <int N>
 __device__ __forceinline__ void down_wait() {  // all but the N newest requests of the wave
@@ -128,10 +122,12 @@ template <int MODE, int CT>
 __global__ __launch_bounds__(kDownWaves * 64) void k_lora_down(const DownArgs a) {
     constexpr int RT = kDownRows;
     constexpr bool BF = MODE == kDownBf16 || MODE == kDownE4m3Bf16, E4M3 = MODE == kDownE4m3F16 || MODE == kDownE4m3Bf16;
-    constexpr unsigned XROW = E4M3 ? 64 : 128, WBYTES = RT * 16 * 128, CHUNK = WBYTES + CT * 16 * XROW;
+    constexpr bool FULL = MODE == kDownF32 || MODE == kDownMixed;  // f32 products
+    constexpr unsigned XB = E4M3 ? 1 : MODE == kDownF32 ? 4 : 2, XROW = 64 * XB, XPER = 1024 / XROW, XP = XROW / 16;
+    constexpr unsigned WBYTES = RT * 16 * 128, CHUNK = WBYTES + CT * 16 * XROW;
     constexpr int DMAS = CHUNK / 1024;
     constexpr unsigned SUMS = RT * CT * 1024;
-    constexpr unsigned AREA = MODE == kDownF32 ? SUMS : 2 * CHUNK;  // a wave's: two chunks, then its sums
+    constexpr unsigned AREA = 2 * CHUNK;  // a wave's: two chunks, then its sums
     static_assert(AREA >= SUMS, "the sums take the chunks' place");
     __shared__ __attribute__((aligned(16))) uint8_t s_mem[kDownWaves * AREA];
     __shared__ int s_id[64];
@@ -154,66 +150,67 @@ __global__ __launch_bounds__(kDownWaves * 64) void k_lora_down(const DownArgs a)
         for (int rt = 0; rt < RT; rt++)
 #pragma unroll
             for (int ct = 0; ct < CT; ct++) acc[rt][ct] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        if constexpr (MODE == kDownF32) {
-            for (unsigned c = wave; c < chunks; c += kDownWaves) {
-                const unsigned k = c * 64 + g * 16;  // the lane's 16 elements
-                const bool in = k < l.n;
-                f32x4 x[CT][4];
+        const uint32_t lds = __builtin_amdgcn_readfirstlane(
+            (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)mine));
+        const char* from[DMAS];  // at k = 0
+        unsigned at[DMAS];       // the lane's first element of a chunk
 #pragma unroll
-                for (int ct = 0; ct < CT; ct++) {
-                    const unsigned t = min(t0 + 16 * ct + col, l.n_tokens - 1);
-                    wide16(x[ct], static_cast<const char*>(a.x) + t * a.x_stride * (a.x_type == G4_F32 ? 4 : 2), a.x_type, k, in);
-                }
-#pragma unroll
-                for (int rt = 0; rt < RT; rt++) {
-                    const unsigned row = min(r0 + 16 * rt + col, l.down - 1);
-                    f32x4 w[4];
-                    wide16(w, static_cast<const uint16_t*>(l.a) + ((uint64_t)ad * l.down + row) * l.n, a.a_type, k, in);
-#pragma unroll
-                    for (int e = 0; e < 16; e++)
-#pragma unroll
-                        for (int ct = 0; ct < CT; ct++)
-                            acc[rt][ct] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[e / 4][e % 4], x[ct][e / 4][e % 4], acc[rt][ct], 0, 0, 0);
-                }
+        for (int j = 0; j < DMAS; j++) {
+            if (j < RT * 2) {  // eight rows of 128 bytes
+                const unsigned r = 8 * j + (lane >> 3), piece = (lane & 7) ^ (r & 7);
+                at[j] = piece * 8;
+                from[j] = reinterpret_cast<const char*>(static_cast<const uint16_t*>(l.a) +
+                                                        ((uint64_t)ad * l.down + min(r0 + r, l.down - 1)) * l.n + at[j]);
+            } else {  // XPER rows of XROW bytes
+                const unsigned r = XPER * (j - RT * 2) + lane / XP, turn = E4M3 ? (r >> 1) & 3 : r & (XP - 1), piece = (lane % XP) ^ turn;
+                at[j] = piece * (16 / XB);
+                from[j] = static_cast<const char*>(a.x) + XB * (min(t0 + r, l.n_tokens - 1) * a.x_stride + at[j]);
             }
-        } else {
-            const uint32_t lds = __builtin_amdgcn_readfirstlane(
-                (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)mine));
-            const char* from[DMAS];  // at k = 0
-            unsigned at[DMAS];       // the lane's first element of a chunk
+        }
+        // A chunk into half `half` of the wave's; past the end, and lanes past n, zeros.
+        auto request = [&](unsigned c, unsigned half) __attribute__((always_inline)) {
 #pragma unroll
             for (int j = 0; j < DMAS; j++) {
-                if (j < RT * 2) {  // eight rows of 128 bytes
-                    const unsigned r = 8 * j + (lane >> 3), piece = (lane & 7) ^ (r & 7);
-                    at[j] = piece * 8;
-                    from[j] = reinterpret_cast<const char*>(static_cast<const uint16_t*>(l.a) +
-                                                            ((uint64_t)ad * l.down + min(r0 + r, l.down - 1)) * l.n + at[j]);
-                } else if (E4M3) {  // sixteen rows of 64
-                    const unsigned r = 16 * (j - RT * 2) + (lane >> 2), piece = (lane & 3) ^ ((r >> 1) & 3);
-                    at[j] = piece * 16;
-                    from[j] = static_cast<const char*>(a.x) + min(t0 + r, l.n_tokens - 1) * a.x_stride + at[j];
-                } else {
-                    const unsigned r = 8 * (j - RT * 2) + (lane >> 3), piece = (lane & 7) ^ (r & 7);
-                    at[j] = piece * 8;
-                    from[j] = static_cast<const char*>(a.x) + 2 * (min(t0 + r, l.n_tokens - 1) * a.x_stride + at[j]);
-                }
+                const char* p = from[j] + (uint64_t)c * (j < RT * 2 ? 128 : XROW);
+                if (c * 64 + at[j] >= l.n) p = reinterpret_cast<const char*>(kZeros);
+                stage_dma<0>(p, lds + half * CHUNK + j * 1024);
             }
-            // A chunk into half `half` of the wave's; past the end, and lanes past n, zeros.
-            auto request = [&](unsigned c, unsigned half) __attribute__((always_inline)) {
+        };
+        unsigned half = 0;
+        request(wave, 0);
+        for (unsigned c = wave; c < chunks; c += kDownWaves, half ^= 1) {
+            request(c + kDownWaves, half ^ 1);
+            down_wait<DMAS>();
+            const uint8_t* w = mine + half * CHUNK;
+            const uint8_t* x = w + WBYTES;
+            if constexpr (FULL) {
 #pragma unroll
-                for (int j = 0; j < DMAS; j++) {
-                    const char* p = from[j] + (uint64_t)c * ((j < RT * 2 || !E4M3) ? 128 : 64);
-                    if (c * 64 + at[j] >= l.n) p = reinterpret_cast<const char*>(kZeros);
-                    stage_dma<0>(p, lds + half * CHUNK + j * 1024);
+                for (int h = 0; h < 2; h++) {
+                    float xf[CT][8], wf[RT][8];
+#pragma unroll
+                    for (int ct = 0; ct < CT; ct++) {
+                        const uint8_t* row = x + (16 * ct + col) * XROW;
+                        if constexpr (MODE == kDownF32) {
+                            const f32x4 lo = *reinterpret_cast<const f32x4*>(row + ((8 * h + 2 * g) ^ col) * 16);
+                            const f32x4 hi = *reinterpret_cast<const f32x4*>(row + ((8 * h + 2 * g + 1) ^ col) * 16);
+#pragma unroll
+                            for (int e = 0; e < 8; e++) xf[ct][e] = e < 4 ? lo[e] : hi[e - 4];
+                        } else {
+                            wide8(xf[ct], *reinterpret_cast<const u32x4*>(row + ((4 * h + g) ^ (col & 7)) * 16), a.x_type);
+                        }
+                    }
+#pragma unroll
+                    for (int rt = 0; rt < RT; rt++)
+                        wide8(wf[rt], *reinterpret_cast<const u32x4*>(w + (16 * rt + col) * 128 + ((4 * h + g) ^ (col & 7)) * 16), a.a_type);
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+#pragma unroll
+                        for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                            for (int ct = 0; ct < CT; ct++)
+                                acc[rt][ct] = __builtin_amdgcn_mfma_f32_16x16x4f32(wf[rt][e], xf[ct][e], acc[rt][ct], 0, 0, 0);
                 }
-            };
-            unsigned half = 0;
-            request(wave, 0);
-            for (unsigned c = wave; c < chunks; c += kDownWaves, half ^= 1) {
-                request(c + kDownWaves, half ^ 1);
-                down_wait<DMAS>();
-                const uint8_t* w = mine + half * CHUNK;
-                const uint8_t* x = w + WBYTES;
+            } else {
                 u32x4 wv[RT][2], xv[CT][2];
 #pragma unroll
                 for (int h = 0; h < 2; h++) {  // k 32 h + 8 g of the chunk
@@ -243,10 +240,10 @@ __global__ __launch_bounds__(kDownWaves * 64) void k_lora_down(const DownArgs a)
                                 acc[rt][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
                                     __builtin_bit_cast(f16x8, wv[rt][h]), __builtin_bit_cast(f16x8, xv[ct][h]), acc[rt][ct], 0, 0, 0);
                         }
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read: the next request but one goes here
             }
-            down_wait<0>();  // the last, of zeros, has come too: its place is the sums'
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read: the next request but one goes here
         }
+        down_wait<0>();  // the last, of zeros, has come too: its place is the sums'
         f32x4* sums = reinterpret_cast<f32x4*>(mine);
 #pragma unroll
         for (int rt = 0; rt < RT; rt++)
@@ -372,8 +369,10 @@ void lora_launch_down(const LoraDev& d, uint32_t lora_type, const void* x, uint3
     } else if (x_type == lora_type) {
         if (lora_type == G4_F16) launch_down<kDownF16>(a, st);
         else launch_down<kDownBf16>(a, st);
-    } else {
+    } else if (x_type == G4_F32) {
         launch_down<kDownF32>(a, st);
+    } else {
+        launch_down<kDownMixed>(a, st);
     }
 }
 
