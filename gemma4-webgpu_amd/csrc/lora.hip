@@ -409,6 +409,7 @@ int g4_lora_add(const g4_lora* lora, const int32_t* adapter_ids, const void* x, 
                    os = p->out_stride ? p->out_stride : d.rows;
     if (xs < d.n || bs < d.rows || os < d.rows) return fail(G4_EINVAL, "%s: a stride is below its row", what);
     if (xs > (1ull << 40) || bs > (1ull << 40) || os > (1ull << 40)) return fail(G4_EINVAL, "%s: a stride is too long", what);
+    if (base == out && bs != os && p->n_tokens > 1) return fail(G4_EINVAL, "%s: base may be out with one stride only", what);
     if (!aligned(x, 16) || xs * type_bytes(p->x_type) % 16) return fail(G4_EINVAL, "%s: x's rows must be 16-byte aligned", what);
     const uint32_t width = type_bytes(p->out_type);
     if (!aligned(base, width) || !aligned(out, width) || !aligned(adapter_ids, 4) || !aligned(x_scales, 4))

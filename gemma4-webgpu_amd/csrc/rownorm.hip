@@ -329,6 +329,13 @@ int pointer_check(const char* what, const char* name, const void* p, uint32_t ty
     if (!aligned(p, type_bytes(type))) return fail(G4_EINVAL, "%s: misaligned %s", what, name);
     return G4_OK;
 }
+// A row is stored when another may not have been read: what shares memory has to share its rows.
+int shared_check(const char* what, const char* names, const void* p, uint32_t p_type, uint64_t p_stride, const void* q,
+                 uint32_t q_type, uint64_t q_stride, uint32_t rows) {
+    if (p && p == q && (p_type != q_type || (rows > 1 && p_stride != q_stride)))
+        return fail(G4_EINVAL, "%s: %s may share memory with one type and stride only", what, names);
+    return G4_OK;
+}
 // Whether rows can be read eight elements at a time.
 bool wide_rows(const void* p, uint32_t type, uint64_t stride) {
     const uint64_t to = type == G4_E4M3 ? 8 : 16;
@@ -370,6 +377,13 @@ int g4_add_rms_norm(const void* x, const void* residual, const void* post_weight
         (rc = pointer_check(what, "weight", weight, p->weight_type)) || (rc = pointer_check(what, "out", out, p->out_type)) ||
         (rc = pointer_check(what, "scales", scales, G4_F32)))
         return rc;
+    if (out && out == residual_out) return fail(G4_EINVAL, "%s: out is residual_out", what);
+    const uint64_t xs = a.x_stride, rs = a.residual_stride, ts = a.residual_out_stride, os = a.out_stride;
+    if ((rc = shared_check(what, "out and x", out, p->out_type, os, x, p->x_type, xs, p->rows)) ||
+        (rc = shared_check(what, "out and residual", out, p->out_type, os, residual, p->residual_type, rs, p->rows)) ||
+        (rc = shared_check(what, "residual_out and x", residual_out, p->residual_type, ts, x, p->x_type, xs, p->rows)) ||
+        (rc = shared_check(what, "residual_out and residual", residual_out, p->residual_type, ts, residual, p->residual_type, rs, p->rows)))
+        return rc;
     if (p->rows == 0) return G4_OK;
     a.x = x;
     a.residual = residual;
@@ -408,6 +422,7 @@ int g4_quantize_rows(const void* x, uint8_t* out, float* scales, const g4_quanti
     a.out_stride = p->out_stride;
     if ((rc = stride_check(what, "x", a.x_stride, p->n)) || (rc = stride_check(what, "out", a.out_stride, p->n))) return rc;
     if ((rc = pointer_check(what, "x", x, p->x_type)) || (rc = pointer_check(what, "scales", scales, G4_F32))) return rc;
+    if (out == x) return fail(G4_EINVAL, "%s: out is x", what);
     if (p->rows == 0) return G4_OK;
     a.x = x;
     a.out = out;

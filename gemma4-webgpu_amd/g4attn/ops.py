@@ -984,7 +984,7 @@ def add_rms_norm(x, weight, out, scales=None, residual=None, residual_out=None, 
     """The residual's addition and the norm of a batch's rows (g4_add_rms_norm). x: [rows, n], f32, f16 or bf16;
     residual and residual_out: one type of those three; post_weight: of the branch's own norm, before the addition; weight
     (None: a norm without) and out, any of those types or float8_e4m3fn with scales f32 [rows]; out None: only the
-    addition. Rows may lie apart; residual_out may be residual."""
+    addition. Rows may lie apart; residual_out and out may each be x or residual of the same type and strides."""
     dev = _device_of(x, "x")
     xp, xt, xs = _rows_of(x, "x", _WIDE_TYPES, dev)
     rows, n = x.shape

@@ -887,7 +887,7 @@ int g4_token_logprobs(const void* logits, const int32_t* tokens, float* logprobs
  * (or b), rounded to residual_type and written to residual_out; out = weight *
  * r / sqrt(mean r^2 + eps). post_weight, residual and residual_out may be NULL;
  * weight NULL: a norm without weights; out NULL (with weight NULL): only the
- * addition. residual_out may be residual, and out may be x where they have one
+ * addition. residual_out and out may each be x or residual where the two have one
  * type and stride. Sums in f32 (elements up to 1e16 in magnitude).
  * out_type G4_E4M3: scales[row] = max |out| / 448, codes of out / scale to nearest
  * even; rows all below 2^-100 are scaled as rows of that size; a row with an Inf

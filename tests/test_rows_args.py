@@ -172,6 +172,22 @@ def test_a_workspace_serves_every_smaller_call(rank, n, rows):
         last = sizes
 
 
+@pytest.mark.parametrize("args,want", [
+    (dict(out=256), "out and x"), (dict(out=256, out_type=0, scales=None, out_stride=80), "out and x"), (dict(out=2048), "out is"),
+    (dict(out=512), "out and residual"), (dict(total=256, residual_type=1), "residual_out and x"),
+    (dict(total=512, residual_stride=72), "residual_out and residual"), (dict(total=256, x_stride=72), "residual_out and x"),
+])
+def test_add_rms_norm_refuses_to_share_memory_with_other_rows(args, want):
+    refused(norm(**args), want)
+
+
+def test_quantize_rows_and_lora_add_refuse_to_share_memory_with_other_rows():
+    lib = abi.load()
+    refused(lib.g4_quantize_rows(256, 256, 1024, abi.QuantizeRowsParams(4, 64, 0, 0, 0, 0), None), "out is x")
+    refused(lib.g4_lora_add(lora(), 256, 4096, None, 512, 512, abi.LoraAddParams(4, 0, 0, 0, 0, 0, 80), 4096, 1 << 20, None),
+            "base may be out")
+
+
 def test_python_wrappers_refuse_tensors_of_the_cpu():
     x, w = torch.zeros(2, 64), torch.zeros(64, dtype=torch.float16)
     with pytest.raises(ValueError, match="GPU"):
