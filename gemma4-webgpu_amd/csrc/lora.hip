@@ -4,7 +4,7 @@
 // Bound by latency for few tokens (one token's q, k, v of rank 16: 2.9 us down, 3.8 up, two launches that each wait for
 // ids, rows and sums in turn; 64 requests of 40 adapters beside their projection: 3.4 us down, 8.0 for the projection with
 // the up product in it), by the adapters' way through the caches for many: a tile of 16 tokens reads all of
-// its adapter (4003 tokens, n 2048, rank 64: 10.4 us for 64 MB of them).
+// its adapter (4003 tokens, n 2048, rank 64: 9.5 us for 64 MB of them).
 #include <type_traits>
 
 #include "lora.h"
@@ -105,22 +105,21 @@ __global__ __launch_bounds__(kFewWaves * 64) void k_lora_down_few(const DownArgs
     }
 }
 
-// Many tokens: 16 CT tokens by 64 down rows a workgroup; the tile's adapters one after the other.
+// Many tokens: 16 CT tokens by 16 RT down rows a workgroup; the tile's adapters one after the other.
 //
 // Each wave takes every Wth 64 k and brings both operands of it to LDS by DMA, one chunk ahead: loaded straight into the matrix
 // unit's layout, in which neighbouring lanes lie in different rows, every lane's 16 bytes are an access of their own (4003
-// tokens, n 2048, rank 64: 21 us). Piece c (16 bytes) of row r lies at
-// c ^ r / 2 % 4 of its 64 bytes, c ^ r % 8 of its 128, c ^ r % 16 of its 256.
-// Products in f32 (f32 rows, mixed types) run at a sixteenth of the 16-bit rate and fill that time with the widening: 4003 tokens,
-// n 2048, rank 64 and the up product to 2560 take 65 us, with equal 16-bit types 43.
-constexpr int kDownWaves = 4, kDownRows = 4;  // 16-wide tiles
+// tokens, n 2048, rank 64: 21 us). Piece c (16 bytes) of row r lies at c ^ r / 2 % 4 of its 64 bytes, c ^ r % 8 of its 128,
+// c ^ r % 16 of its 256. Products in f32 (f32 rows, mixed types) run at a sixteenth of the 16-bit rate and fill that time with the widening: 4003 tokens,
+// n 2048, rank 64 and the up product to 2560 take 58 us, with equal 16-bit types 44.
+constexpr int kDownWaves = 4;
 template <int N>
 __device__ __forceinline__ void down_wait() {  // all but the N newest requests of the wave
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
-template <int MODE, int CT>
+template <int MODE, int RT>  // RT tiles of 16 rows
 __global__ __launch_bounds__(kDownWaves * 64) void k_lora_down(const DownArgs a) {
-    constexpr int RT = kDownRows;
+    constexpr int CT = 1;  // tiles of 16 tokens
     constexpr bool BF = MODE == kDownBf16 || MODE == kDownE4m3Bf16, E4M3 = MODE == kDownE4m3F16 || MODE == kDownE4m3Bf16;
     constexpr bool FULL = MODE == kDownF32 || MODE == kDownMixed;  // f32 products
     constexpr unsigned XB = E4M3 ? 1 : MODE == kDownF32 ? 4 : 2, XROW = 64 * XB, XPER = 1024 / XROW, XP = XROW / 16;
@@ -336,17 +335,23 @@ LoraDev lora_dev(const g4_lora* l, uint32_t n_tokens) {
 size_t lora_bytes(const g4_lora* l, uint32_t n_tokens) { return (size_t)n_tokens * l->n_segs * l->rank * 4 + 16; }
 
 // A wave a token and four rows where that reads at most 64 MB of adapters, no adapter waiting for another; beyond, the
-// matrix units' tiles, which read an adapter once for 16 or 32 tokens (us of lora_add, 2560 outputs, waves / tiles; four
+// matrix units' tiles, which read an adapter once for 16 tokens (us of lora_add, 2560 outputs, waves / tiles; four
 // runs of tokens: 256 tokens, rank 64, n 1536 9.5 / 10.0; 1024, 16, 1536 13.6 / 13.7; 256, 64, 4096 14.0 / 13.8; 512, 64, 1536
 // 14.9 / 12.3; 1024, 64, 1536 25.3 / 17.5; every token another of 40 adapters, rank 16: 64 tokens 6.7 / 58, 1024 22.7 / 73.5).
 static bool lora_by_waves(const LoraDev& d) { return (uint64_t)d.n_tokens * d.down * d.n <= 1u << 25; }
 
 template <int MODE>
 static void launch_down(const DownArgs& a, hipStream_t st) {
-    const uint32_t groups = (a.l.down + 16 * kDownRows - 1) / (16 * kDownRows), pairs = (a.l.n_tokens + 31) / 32;
-    // Tiles of 32 tokens read an adapter half as often; of 16 where those would leave compute units idle.
-    if (pairs * groups >= device_cus()) G4_LAUNCH((k_lora_down<MODE, 2>), dim3(pairs, groups), dim3(kDownWaves * 64), 0, st, a);
-    else G4_LAUNCH((k_lora_down<MODE, 1>), dim3((a.l.n_tokens + 15) / 16, groups), dim3(kDownWaves * 64), 0, st, a);
+    // A tile by 16 rows where three rounds of the chip's compute units hold those, for the wait of each chunk is what counts then;
+    // by 32 beyond, for half the reads of x (us of lora_add, 16 rows / 32 / 64; tokens, rank, n, outputs: f32 1691, 72, 1664, 1328
+    // 27.3 / 34.5 / 40.8, 8192, 16, 4096, 2048 63 / 70 / 100, 4003, 64, 2048, 2560 59.2 / 58.2 / 64.9, 4003, 128, 2048, 512 61 / 54 /
+    // 64; f16 700, 32, 1536, 2048 12.7 / 13.6 / 15.2, 4003, 64, 2048, 2560 47.6 / 43.8 / 43.3). 32 tokens a tile took 0 to 40 %
+    // longer in nearly all of them, at most 2 % less.
+    const uint32_t tokens = (a.l.n_tokens + 15) / 16, rows = (a.l.down + 15) / 16;
+    if ((uint64_t)tokens * rows <= 3 * device_cus())
+        G4_LAUNCH((k_lora_down<MODE, 1>), dim3(tokens, rows), dim3(kDownWaves * 64), 0, st, a);
+    else
+        G4_LAUNCH((k_lora_down<MODE, 2>), dim3(tokens, (rows + 1) / 2), dim3(kDownWaves * 64), 0, st, a);
 }
 template <uint32_t XT>
 static void launch_down_few(const DownArgs& a, hipStream_t st) {
