@@ -335,9 +335,10 @@ LoraDev lora_dev(const g4_lora* l, uint32_t n_tokens) {
 size_t lora_bytes(const g4_lora* l, uint32_t n_tokens) { return (size_t)n_tokens * l->n_segs * l->rank * 4 + 16; }
 
 // A wave a token and four rows where that reads at most 64 MB of adapters, no adapter waiting for another; beyond, the
-// matrix units' tiles, which read an adapter once for 16 tokens (us of lora_add, 2560 outputs, waves / tiles; four
-// runs of tokens: 256 tokens, rank 64, n 1536 9.5 / 10.0; 1024, 16, 1536 13.6 / 13.7; 256, 64, 4096 14.0 / 13.8; 512, 64, 1536
-// 14.9 / 12.3; 1024, 64, 1536 25.3 / 17.5; every token another of 40 adapters, rank 16: 64 tokens 6.7 / 58, 1024 22.7 / 73.5).
+// matrix units' tiles, which read an adapter once for 16 tokens (us of lora_add, 2560 outputs, waves / tiles, f16 and then f32
+// rows; four runs of tokens: 256 tokens, rank 64, n 1536 9.6 / 8.3, 9.8 / 10.7; 1024, 16, 1536 13.4 / 12.3, 14.1 / 14.7; 512, 64, 1536
+// 13.4 / 10.4, 14.1 / 13.0; 1024, 64, 1536 22.7 / 15.7, 24.4 / 18.1; every token another of 40 adapters, rank 16: 64 tokens 6.6 /
+// 26, 6.7 / 66; 1024 27 / 49, 28 / 86). Ids are the device's: what runs of tokens lose here is what mixed ones would lose many times.
 static bool lora_by_waves(const LoraDev& d) { return (uint64_t)d.n_tokens * d.down * d.n <= 1u << 25; }
 
 template <int MODE>
