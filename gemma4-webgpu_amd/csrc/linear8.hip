@@ -26,7 +26,7 @@ struct Linear8Args {
     void* __restrict__ out;
     uint64_t x_stride, out_stride;
     uint32_t n_tokens, rows, n;
-    uint32_t out_type, wide, low;  // low: 0 no adapters, else their type
+    uint32_t out_type, low;  // low: 0 no adapters, else their type
     LoraDev l;
 };
 
@@ -85,7 +85,7 @@ __device__ __forceinline__ void finish(const Linear8Args& a, f32x4 sum, const Ti
         if (a.low == G4_F16) lora_up<16, 1, false>(a.l, o0, t, id, add);
         else lora_up<16, 1, true>(a.l, o0, t, id, add);
     }
-    if (valid && o < a.rows) store4(a.out, a.out_type, t * a.out_stride + o, y, a.wide, a.rows - o);
+    if (valid && o < a.rows) store4(a.out, a.out_type, t * a.out_stride + o, y, a.rows - o);
 }
 
 // Few tokens: 16 RT outputs by 16 CT tokens a workgroup, its waves take every Wth 128 of k.
@@ -349,7 +349,7 @@ __global__ __launch_bounds__(64 * WO * WT, RT * CT >= 16 ? 1 : 2) void k_linear8
         const unsigned col = el & 31, g = el >> 5;
         const float* scales = reinterpret_cast<const float*>(s_mem + SCALES) + slot * (BO + BT);
         slot = (slot + 1) % SLOTS;
-        stored = a.wide && o0 + 32 * RT <= a.rows && t0 + 32 * CT <= a.n_tokens;  // uniform: every lane stores whole pieces
+        stored = o0 + 32 * RT <= a.rows && t0 + 32 * CT <= a.n_tokens;  // uniform: every lane stores whole pieces
         each_of<CT>([&](auto ct) __attribute__((always_inline)) {
             const unsigned t = t0 + 32 * ct + col;
             const float xs = scales[BO + wt + 32 * ct + col];
@@ -377,12 +377,12 @@ __global__ __launch_bounds__(64 * WO * WT, RT * CT >= 16 ? 1 : 2) void k_linear8
                     for (int q = 0; q < 4; q++) {
                         const unsigned oq = o + 8 * q + 4 * g;
                         if (t < a.n_tokens && oq < a.rows)
-                            store4(a.out, OT, t * a.out_stride + oq, yr[q], a.wide, a.rows - oq);
+                            store4(a.out, OT, t * a.out_stride + oq, yr[q], a.rows - oq);
                     }
                 } else if constexpr (WIDE) {
                     float* out = static_cast<float*>(a.out) + t * a.out_stride + o + 4 * g;
 #pragma unroll
-                    for (int q = 0; q < 4; q++) stg<f32x4>(out + 8 * q, yr[q]);
+                    for (int q = 0; q < 4; q++) *(__attribute__((address_space(1))) f32x4_any*)(out + 8 * q) = yr[q];
                 } else {
                     // Lane halves exchange, so that a lane has eight outputs one after the other: the lower half's of every
                     // even eight, the upper's of the odd.
@@ -401,7 +401,7 @@ __global__ __launch_bounds__(64 * WO * WT, RT * CT >= 16 ? 1 : 2) void k_linear8
                             v[e] = sw[0];
                             v[2 + e] = sw[1];
                         }
-                        stg<u32x4>(out + 8 * q, v);
+                        *(__attribute__((address_space(1))) u32x4_any*)(out + 8 * q) = v;
                     }
                 }
                 __builtin_amdgcn_sched_barrier(0);  // tile by tile: the registers hold no more
@@ -530,7 +530,6 @@ int g4_linear_e4m3(const uint8_t* x, const float* x_scales, const uint8_t* weigh
     a.rows = p->rows;
     a.n = p->n;
     a.out_type = p->out_type;
-    a.wide = aligned(out, 4 * width) && os % 4 == 0;
     const hipStream_t st = as_stream(stream);
     if (lora) {
         a.low = lora->type;

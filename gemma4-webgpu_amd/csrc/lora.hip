@@ -110,8 +110,8 @@ __global__ __launch_bounds__(kFewWaves * 64) void k_lora_down_few(const DownArgs
 // Each wave takes every Wth 64 k and brings both operands of it to LDS by DMA, one chunk ahead: loaded straight into the matrix
 // unit's layout, in which neighbouring lanes lie in different rows, every lane's 16 bytes are an access of their own (4003
 // tokens, n 2048, rank 64: 21 us). Piece c (16 bytes) of row r lies at c ^ r / 2 % 4 of its 64 bytes, c ^ r % 8 of its 128,
-// c ^ r % 16 of its 256. Products in f32 (f32 rows, mixed types) run at a sixteenth of the 16-bit rate and fill that time with the widening: 4003 tokens,
-// n 2048, rank 64 and the up product to 2560 take 58 us, with equal 16-bit types 44.
+// c ^ r % 16 of its 256. Products in f32 (f32 rows, mixed types) run at a sixteenth of the 16-bit rate, after the widening: 4003
+// tokens, n 2048, rank 64 and the up product to 2560 take 58 us, with equal 16-bit types 44.
 constexpr int kDownWaves = 4;
 template <int N>
 __device__ __forceinline__ void down_wait() {  // all but the N newest requests of the wave
@@ -270,7 +270,7 @@ struct UpArgs {
     const void* base;  // may be out
     void* out;
     uint64_t base_stride, out_stride;
-    uint32_t type, wide;
+    uint32_t type;
 };
 template <int TILES, bool BF>
 __global__ __launch_bounds__(kUpWaves * 64) void k_lora_up(const UpArgs a) {
@@ -284,13 +284,13 @@ __global__ __launch_bounds__(kUpWaves * 64) void k_lora_up(const UpArgs a) {
 #pragma unroll
     for (int rt = 0; rt < TILES; rt++) {
         const unsigned o = o0 + 16 * rt + 4 * g;
-        acc[rt] = valid && o < l.rows ? load4(a.base, a.type, t * a.base_stride + o, a.wide, l.rows - o) : f32x4{0, 0, 0, 0};
+        acc[rt] = valid && o < l.rows ? load4(a.base, a.type, t * a.base_stride + o, l.rows - o) : f32x4{0, 0, 0, 0};
     }
     lora_up<16, TILES, BF>(l, o0, t, id, [&](int rt, int i, float v) __attribute__((always_inline)) { acc[rt][i] += v; });
 #pragma unroll
     for (int rt = 0; rt < TILES; rt++) {
         const unsigned o = o0 + 16 * rt + 4 * g;
-        if (valid && o < l.rows) store4(a.out, a.type, t * a.out_stride + o, acc[rt], a.wide, l.rows - o);
+        if (valid && o < l.rows) store4(a.out, a.type, t * a.out_stride + o, acc[rt], l.rows - o);
     }
 }
 
@@ -434,7 +434,6 @@ int g4_lora_add(const g4_lora* lora, const int32_t* adapter_ids, const void* x, 
     a.base_stride = bs;
     a.out_stride = os;
     a.type = p->out_type;
-    a.wide = aligned(base, 4 * width) && aligned(out, 4 * width) && bs % 4 == 0 && os % 4 == 0;
     auto launch = [&](auto tiles) {
         constexpr int TILES = decltype(tiles)::value, per = 16 * TILES * kUpWaves;
         const dim3 grid((p->n_tokens + 15) / 16, (d.rows + per - 1) / per), block(kUpWaves * 64);
