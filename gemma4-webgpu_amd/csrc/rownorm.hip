@@ -258,12 +258,18 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_rows(const NormR
         const bool fine = __uint_as_float(top) * inv < INFINITY;  // and no NaN
         if (t == 0) a.scales[row] = fine ? most / 448.0f : __uint_as_float(0x7FC00000u);
         const float to = 448.0f / most;
-        inv = inv * to;
         if (!fine) {  // every code NaN
             uint8_t* o = static_cast<uint8_t*>(a.out) + row * a.out_stride;
             for (unsigned i = t; i < n; i += TPR) stg<uint8_t>(o + i, (uint8_t)0x7F);
             return;
         }
+        // Both factors as one, but where their product passes f32: rows whose eps is below 3e-12, of values that small.
+        if (!(inv * to < INFINITY)) {
+#pragma unroll
+            for (int i = 0; i < E; i++) v[i] *= inv;
+            inv = 1.0f;
+        }
+        inv = inv * to;
     }
 #pragma unroll
     for (int i = 0; i < E; i++) v[i] *= inv;
