@@ -236,11 +236,22 @@ __device__ __forceinline__ void lora_up(const LoraDev& l, unsigned o0, unsigned 
                     }
                 }
                 const float f = down * alpha;
+                if (o0 >= first && o0 + M * NRT <= end) {
 #pragma unroll
-                for (int rt = 0; rt < NRT; rt++) {
+                    for (int rt = 0; rt < NRT; rt++) {
 #pragma unroll
-                    for (int i = 0; i < N; i++)
-                        if (mine) add(rt, i, d[rt][i] * f);
+                        for (int i = 0; i < N; i++)
+                            if (mine) add(rt, i, d[rt][i] * f);
+                    }
+                } else {
+                    // Outputs of the tile's other segments: sums of zero weights, which an Inf or NaN among u makes NaN.
+                    const unsigned before = first - (o0 + 4 * g), width = mine ? end - first : 0;
+#pragma unroll
+                    for (int rt = 0; rt < NRT; rt++) {
+#pragma unroll
+                        for (int i = 0; i < N; i++)
+                            if (M * rt + 8 * (i / 4) + i % 4 - before < width) add(rt, i, d[rt][i] * f);
+                    }
                 }
             }
             first = end;

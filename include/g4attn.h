@@ -932,7 +932,7 @@ int g4_quantize_rows(const void* x, uint8_t* out, float* scales, const g4_quanti
  *   scales[a] * sum_j (sum_k x[t][k] a[a][s * rank + j][k]) * b[a][o][j]
  * (sums in f32; the inner sums enter the second product off by 2^-23 of themselves
  * or 2^-39 of the token's largest). An Inf or NaN among a token's inner sums
- * makes outputs of that token Inf or NaN. */
+ * makes that segment's outputs of that token Inf or NaN, and no others. */
 typedef struct g4_lora {
     const void* a;          /* [n_adapters][n_segs * rank][n], 16-byte aligned */
     const void* b;          /* [n_adapters][sum of widths][rank], 16-byte aligned */

@@ -33,3 +33,39 @@ def test_zero_rows_of_a_small_eps(dev, n, eps):
     ops.add_rms_norm(x, nothing, out, scales=scales, eps=eps)
     torch.cuda.synchronize()
     assert (out.float() == 0).all()
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("tokens,runs", [(1, 1), (20, 1), (20, 20), (300, 2), (300, 300)])
+@pytest.mark.parametrize("bad", ["inf", "nan"])
+def test_an_inner_sum_that_is_not_finite_stays_in_its_segment(dev, kind, tokens, runs, bad):
+    """Down rows of one segment that are not finite: its outputs are not, those of the segments beside it, in the same tile too,
+    are what they were, whether a tile's tokens share an adapter or have one each."""
+    announce(f"lora {bad} in a segment {kind} tokens={tokens} runs={runs}")
+    widths, rank, n = (10, 21, 9, 60), 16, 64
+    g = torch.Generator().manual_seed(tokens)
+    a = (torch.randn(5, 4 * rank, n, generator=g) * 0.1).to(TYPES[kind]).to(dev)
+    b = (torch.randn(5, sum(widths), rank, generator=g) + 3).to(TYPES[kind]).to(dev)
+    x, base = torch.randn(tokens, n, generator=g).half().to(dev), torch.randn(tokens, sum(widths), generator=g).to(dev)
+    ids = ((torch.arange(tokens) * runs // tokens) % 5).int().to(dev)
+    x8, xs = x.float().to(TYPES["e4m3"]), torch.ones(tokens, device=dev)
+    w, ws = torch.zeros(sum(widths), n, device=dev).to(TYPES["e4m3"]), torch.ones(sum(widths), device=dev)
+
+    def both(a):
+        low = ops.LoraAdapters(a, b, None, widths)
+        out, out8 = torch.empty_like(base), torch.empty_like(base)
+        ops.lora_add(low, ids, x, base, out, torch.empty(ops.lora_workspace_bytes(low, tokens), dtype=torch.uint8, device=dev))
+        ops.linear_e4m3(x8, xs, w, ws, out8, torch.empty(ops.linear_e4m3_workspace_bytes(tokens, sum(widths), n, low), dtype=torch.uint8,
+                                                          device=dev), lora=low, adapter_ids=ids)
+        torch.cuda.synchronize()
+        return out, out8
+
+    want = both(a)
+    for s in range(4):
+        odd = a.clone()
+        odd[:, s * rank + 3, 5] = float(bad)
+        first = sum(widths[:s])
+        others = [o for o in range(sum(widths)) if not first <= o < first + widths[s]]
+        for got, was in zip(both(odd), want):
+            assert not got[:, first:first + widths[s]].isfinite().any()
+            assert torch.equal(got[:, others], was[:, others])
