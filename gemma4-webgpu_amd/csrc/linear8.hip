@@ -531,11 +531,21 @@ int g4_linear_e4m3(const uint8_t* x, const float* x_scales, const uint8_t* weigh
     a.n = p->n;
     a.out_type = p->out_type;
     const hipStream_t st = as_stream(stream);
+    const Operand o_x = rows_operand("x", x, G4_E4M3, p->n, xs, p->n_tokens), o_xs = {"x_scales", one_range(x_scales, 4ull * p->n_tokens)},
+                  o_w = {"weight", one_range(weight, (uint64_t)p->rows * p->n)},
+                  o_ws = {"weight_scales", one_range(weight_scales, 4ull * p->rows)},
+                  o_out = rows_operand("out", out, p->out_type, p->rows, os, p->n_tokens);
+    int meet = apart_check(what, o_out, {o_x, o_xs, o_w, o_ws});
+    if (meet) return meet;
     if (lora) {
         a.low = lora->type;
         a.l = lora_dev(lora, p->n_tokens);
         a.l.ids = adapter_ids;
         a.l.u = static_cast<float*>(workspace);
+        const LoraOperands l = lora_operands(a.l);  // a, the down rows, are read before out is written
+        meet = apart_check(what, l.u, {o_x, o_xs, o_w, o_ws, l.a, l.b, l.scales, l.ids, o_out});
+        if (!meet) meet = apart_check(what, o_out, {l.b, l.scales, l.ids});
+        if (meet) return meet;
         lora_launch_down(a.l, lora->type, x, G4_E4M3, xs, x_scales, st);
         G4_CHECK_LAUNCH("k_lora_down");
     }

@@ -259,6 +259,19 @@ __device__ __forceinline__ void lora_up(const LoraDev& l, unsigned o0, unsigned 
     }
 }
 
+// What the up product reads beside its base, and what the down product does beside x and its scales.
+struct LoraOperands {
+    Operand a, b, scales, ids, u;
+};
+inline LoraOperands lora_operands(const LoraDev& d) {
+    const uint64_t L = d.n_adapters;
+    return {{"the adapters' down rows", one_range(d.a, L * d.down * d.n * 2)},
+            {"the adapters' up rows", one_range(d.b, L * d.rows * d.rank * 2)},
+            {"the adapters' scales", one_range(d.scales, L * 4)},
+            {"adapter_ids", one_range(d.ids, (uint64_t)d.n_tokens * 4)},
+            {"workspace", one_range(d.u, (uint64_t)d.n_tokens * d.down * 4)}};
+}
+
 // The description checked and brought into the kernels' form; `what` names the call.
 int lora_check(const char* what, const g4_lora* l);
 LoraDev lora_dev(const g4_lora* l, uint32_t n_tokens);

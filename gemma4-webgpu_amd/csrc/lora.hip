@@ -425,6 +425,15 @@ int g4_lora_add(const g4_lora* lora, const int32_t* adapter_ids, const void* x, 
     if (p->n_tokens == 0) return G4_OK;
     d.ids = adapter_ids;
     d.u = static_cast<float*>(workspace);
+    // The down product is done with x before out is written.
+    const LoraOperands l = lora_operands(d);
+    const Operand o_x = rows_operand("x", x, p->x_type, d.n, xs, p->n_tokens),
+                  o_xs = {"x_scales", one_range(x_scales, 4ull * p->n_tokens)},
+                  o_base = rows_operand("base", base, p->out_type, d.rows, bs, p->n_tokens),
+                  o_out = rows_operand("out", out, p->out_type, d.rows, os, p->n_tokens);
+    int meet = apart_check(what, l.u, {o_x, o_xs, l.a, l.b, l.scales, l.ids, o_base, o_out});
+    if (!meet) meet = apart_check(what, o_out, {out == base ? Operand{} : o_base, l.b, l.scales, l.ids});
+    if (meet) return meet;
     lora_launch_down(d, lora->type, x, p->x_type, xs, x_scales, as_stream(stream));
     G4_CHECK_LAUNCH("k_lora_down");
     UpArgs a = {};

@@ -335,7 +335,7 @@ int pointer_check(const char* what, const char* name, const void* p, uint32_t ty
     if (!aligned(p, type_bytes(type))) return fail(G4_EINVAL, "%s: misaligned %s", what, name);
     return G4_OK;
 }
-// A row is stored when another may not have been read: what shares memory has to share its rows.
+// A row is stored when another may not have been read: what shares memory has to share its rows (other overlaps: apart_check).
 int shared_check(const char* what, const char* names, const void* p, uint32_t p_type, uint64_t p_stride, const void* q,
                  uint32_t q_type, uint64_t q_stride, uint32_t rows) {
     if (p && p == q && (p_type != q_type || (rows > 1 && p_stride != q_stride)))
@@ -391,6 +391,19 @@ int g4_add_rms_norm(const void* x, const void* residual, const void* post_weight
         (rc = shared_check(what, "residual_out and residual", residual_out, p->residual_type, ts, residual, p->residual_type, rs, p->rows)))
         return rc;
     if (p->rows == 0) return G4_OK;
+    const uint64_t n = p->n, rows = p->rows;
+    const Operand o_out = rows_operand("out", out, p->out_type, n, os, rows),
+                  o_sum = rows_operand("residual_out", residual_out, p->residual_type, n, ts, rows),
+                  o_scales = {"scales", one_range(scales, 4 * rows)};
+    const Operand o_x = rows_operand("x", x, p->x_type, n, xs, rows),
+                  o_res = rows_operand("residual", residual, p->residual_type, n, rs, rows),
+                  o_post = rows_operand("post_weight", post_weight, p->weight_type, n, n, 1),
+                  o_weight = rows_operand("weight", weight, p->weight_type, n, n, 1);
+    const Operand none = {};
+    if ((rc = apart_check(what, o_out, {out == x ? none : o_x, out == residual ? none : o_res, o_post, o_weight, o_sum, o_scales})) ||
+        (rc = apart_check(what, o_sum, {residual_out == x ? none : o_x, residual_out == residual ? none : o_res, o_post, o_weight, o_scales})) ||
+        (rc = apart_check(what, o_scales, {o_x, o_res, o_post, o_weight})))
+        return rc;
     a.x = x;
     a.residual = residual;
     a.post = post_weight;
@@ -430,6 +443,10 @@ int g4_quantize_rows(const void* x, uint8_t* out, float* scales, const g4_quanti
     if ((rc = pointer_check(what, "x", x, p->x_type)) || (rc = pointer_check(what, "scales", scales, G4_F32))) return rc;
     if (out == x) return fail(G4_EINVAL, "%s: out is x", what);
     if (p->rows == 0) return G4_OK;
+    const Operand o_x = rows_operand("x", x, p->x_type, p->n, a.x_stride, p->rows),
+                  o_out = rows_operand("out", out, G4_E4M3, p->n, a.out_stride, p->rows),
+                  o_scales = {"scales", one_range(scales, 4ull * p->rows)};
+    if ((rc = apart_check(what, o_out, {o_x, o_scales})) || (rc = apart_check(what, o_scales, {o_x}))) return rc;
     a.x = x;
     a.out = out;
     a.scales = scales;

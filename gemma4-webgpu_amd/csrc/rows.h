@@ -2,7 +2,10 @@
 // checks that their entry points share.
 #pragma once
 
+#include <initializer_list>
+
 #include "common.h"
+#include "row_ranges.h"
 
 namespace g4 {
 
@@ -17,6 +20,21 @@ constexpr uint32_t kMaxRows = 1u << 22;  // tokens of a batch's buffers
 
 inline uint32_t type_bytes(uint32_t type) { return type == G4_F32 ? 4 : type == G4_E4M3 ? 1 : 2; }
 inline bool aligned(const void* p, uint64_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+
+// An operand by its name, for the checks below.
+struct Operand {
+    const char* name;
+    RowRange at;
+};
+inline Operand rows_operand(const char* name, const void* p, uint32_t type, uint64_t n, uint64_t stride, uint64_t rows) {
+    return {name, {p, n * type_bytes(type), stride * type_bytes(type), rows}};
+}
+// What a call writes shares no memory with what other workgroups of it may still read, or write.
+inline int apart_check(const char* what, const Operand& written, std::initializer_list<Operand> others) {
+    for (const Operand& o : others)
+        if (rows_meet(written.at, o.at)) return fail(G4_EINVAL, "%s: %s lies over %s", what, written.name, o.name);
+    return G4_OK;
+}
 
 __device__ __forceinline__ uint16_t f2bf(float x) { return __builtin_bit_cast(uint16_t, static_cast<__bf16>(x)); }
 __device__ __forceinline__ float bf2f(uint16_t x) { return __uint_as_float((uint32_t)x << 16); }

@@ -877,6 +877,10 @@ int g4_token_logprobs(const void* logits, const int32_t* tokens, float* logprobs
  * have no counterpart there. g4_paged_append takes such a projection's q, k and
  * v, g4_quantize_rows g4_paged_attn's outputs for the next.
  *
+ * Rows may lie apart, between others of the same buffer. What a call writes (its
+ * workspace too) shares no memory with what it reads, unless said below; a call
+ * whose pointers, sizes and strides say that it would is refused.
+ *
  * Element types: */
 #define G4_F32 0
 #define G4_F16 1
