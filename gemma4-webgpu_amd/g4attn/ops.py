@@ -1009,7 +1009,7 @@ def add_rms_norm(x, weight, out, scales=None, residual=None, residual_out=None, 
     if rows == 0:
         return
     abi.call("g4_add_rms_norm", xp, rp, pp, wp, sp, op, cp,
-             _norm_params(rows, n, xt, xt if rt is None else rt, wt or 0, ot, eps, 0, xs, rs, ss, os_), _stream(stream))
+             _norm_params(rows, n, xt, xt if rt is None else rt, wt or 0, ot, float(eps), 0, xs, rs, ss, os_), _stream(stream))
 
 
 def quantize_rows(x, out, scales, stream=None):

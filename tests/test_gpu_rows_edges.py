@@ -69,3 +69,16 @@ def test_an_inner_sum_that_is_not_finite_stays_in_its_segment(dev, kind, tokens,
         for got, was in zip(both(odd), want):
             assert not got[:, first:first + widths[s]].isfinite().any()
             assert torch.equal(got[:, others], was[:, others])
+
+
+def test_an_eps_that_changes_in_place(dev):
+    """eps as a tensor of one element: its value at the call counts, as with any number."""
+    announce("addRmsNorm eps in a tensor")
+    x = torch.randn(3, 64, generator=torch.Generator().manual_seed(1)).to(dev)
+    eps = torch.tensor(1e-6)
+    for value in (1e-6, 0.5, 1e-6):
+        eps.fill_(value)
+        got, want = torch.empty_like(x), torch.empty_like(x)
+        ops.add_rms_norm(x, None, got, eps=eps)
+        ops.add_rms_norm(x, None, want, eps=float(eps))
+        assert torch.equal(got, want)
