@@ -56,4 +56,8 @@ inline bool attn_output_chain(uint64_t workgroups, uint32_t seq_len, uint32_t cu
 // logits 2.7 / 2.2, 768 logits 2.7 / 2.3).
 inline bool argmax_small(uint32_t size) { return size <= 768; }
 
+// Workgroups along x of a launch of `rows` workgroups of 1024 threads; what is left of the rows goes along y. A launch takes
+// fewer than 2^32 threads along x, and 2^22 rows have as many.
+inline uint32_t long_row_columns(uint32_t rows) { return rows < (1u << 21) ? rows : 1u << 21; }
+
 }  // namespace g4

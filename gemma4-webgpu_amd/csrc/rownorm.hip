@@ -18,6 +18,7 @@
 #include <type_traits>
 
 #include "decode_core.h"
+#include "launch_rules.h"
 #include "rows.h"
 
 namespace g4 {
@@ -199,7 +200,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_rows(const NormR
     constexpr bool LATE = TPR == 1024;  // 128 registers a wave: each operand only when the one before is done with
     __shared__ float s_sum[2][W];
     __shared__ uint32_t s_top[2][W];
-    const unsigned row = TPR < 256 ? blockIdx.x * (256 / TPR) + threadIdx.x / TPR : blockIdx.x;
+    const unsigned group = TPR == 1024 ? blockIdx.y * gridDim.x + blockIdx.x : blockIdx.x;
+    const unsigned row = TPR < 256 ? group * (256 / TPR) + threadIdx.x / TPR : group;
     const unsigned t = TPR < 256 ? threadIdx.x % TPR : threadIdx.x;
     if (row >= a.rows) return;  // whole waves, of a kernel without barriers
     const unsigned n = a.n;
@@ -280,7 +282,8 @@ constexpr uint32_t kNormMaxN = 32768;
 
 // Eight elements a load would not fit the registers.
 void launch_longest(const NormRowsArgs& a, hipStream_t st) {
-    G4_LAUNCH((k_norm_rows<1024, 4, false, 0, 0, 0>), dim3(a.rows), dim3(1024), 0, st, a);
+    const uint32_t columns = long_row_columns(a.rows);
+    G4_LAUNCH((k_norm_rows<1024, 4, false, 0, 0, 0>), dim3(columns, (a.rows + columns - 1) / columns), dim3(1024), 0, st, a);
 }
 template <bool VEC, int XW, int RW, int WW>
 void launch_norm_rows(const NormRowsArgs& a, hipStream_t st) {

@@ -82,3 +82,22 @@ def test_an_eps_that_changes_in_place(dev):
         ops.add_rms_norm(x, None, got, eps=eps)
         ops.add_rms_norm(x, None, want, eps=float(eps))
         assert torch.equal(got, want)
+
+
+def test_the_most_rows_of_the_longest_kind(dev):
+    """2^22 rows of more than 16384 elements: as many threads as a launch cannot take along one side."""
+    rows, n = 2 ** 22, 16385
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < rows * n * 2 + (16 << 30):
+        pytest.skip("needs 144 GB of free memory")
+    announce("addRmsNorm 2^22 rows of 16385")
+    x = torch.empty(rows, n, dtype=torch.float16, device=dev)
+    part = rows // 16
+    for i in range(16):
+        x[i * part:(i + 1) * part] = 2.0 - 4.0 * (i % 2)
+    ops.add_rms_norm(x, None, x)
+    torch.cuda.synchronize()
+    for i in range(16):  # 2 / sqrt(4 + 1e-6) is 1 in f16
+        assert (x[i * part:(i + 1) * part] == 1.0 - 2.0 * (i % 2)).all()
+    del x
+    torch.cuda.empty_cache()
