@@ -60,4 +60,17 @@ inline bool argmax_small(uint32_t size) { return size <= 768; }
 // fewer than 2^32 threads along x, and 2^22 rows have as many.
 inline uint32_t long_row_columns(uint32_t rows) { return rows < (1u << 21) ? rows : 1u << 21; }
 
+// The side of linear_e4m3's tiles for many tokens, or 0: tiles of 16 or 32 whose waves share k. The largest tile that there are
+// about enough of for the compute units, as long as there are; a tile's offsets fit 32 bits. Measured (us, n 1536; tiles of 256 /
+// 128 / 64 / few): 1024 tokens by 12288 outputs 28.9 / 33.4 / 44.2 / 133, 256 by 12288 22.2 / 12.4 / 15.4 / 35.7, 64 by 12288 19.4 /
+// 11.1 / 7.5 / 11.6; f32 outputs: 1024 by 2560 43.1 / 23.4 / 18.0 / 31.1, 256 by 2560 42.0 / 21.7 / 10.9 / 11.3, 64 by 2560 35.6 /
+// 20.2 / 10.4 / 5.4.
+inline uint32_t linear8_tile(uint32_t tokens, uint32_t rows, uint64_t x_stride, uint32_t cus) {
+    if (x_stride >= 1u << 24) return 0;
+    const auto tiles = [&](uint32_t side) { return (uint64_t)((rows + side - 1) / side) * ((tokens + side - 1) / side); };
+    if (tiles(256) >= (uint64_t)cus * 3 / 4) return 256;
+    if (tiles(128) >= (uint64_t)cus * 3 / 4) return 128;
+    return tiles(64) >= (uint64_t)cus * 5 / 8 ? 64 : 0;
+}
+
 }  // namespace g4

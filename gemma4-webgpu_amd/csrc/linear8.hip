@@ -14,6 +14,7 @@
 // outputs of 1536 3.6.
 #include <utility>
 
+#include "launch_rules.h"
 #include "lora.h"
 
 namespace g4 {
@@ -471,18 +472,13 @@ void launch_few(const Linear8Args& a, hipStream_t st) {
     G4_LAUNCH((k_linear8_few<RT, CT, W>), dim3(o_tiles * t_tiles), dim3(W * 64), 0, st, a);
 }
 
-// The largest tile that there are about enough of for the compute units, as long as there are; else tiles of 16 or 32
-// whose waves share k (us, n 1536; tiles of 256 / 128 / 64 / few): 1024 tokens by 12288 outputs 28.9 / 33.4 / 44.2 / 133, 256 by
-// 12288 22.2 / 12.4 / 15.4 / 35.7, 64 by 12288 19.4 / 11.1 / 7.5 / 11.6; f32 outputs: 1024 by 2560 43.1 / 23.4 / 18.0 / 31.1, 256 by
-// 2560 42.0 / 21.7 / 10.9 / 11.3, 64 by 2560 35.6 / 20.2 / 10.4 / 5.4. Few tokens: 16 outputs by 16 tokens (one token by 2560
-// 3.5 us, 32 outputs 4.3), 32 by 32 up to 96 tokens (64 by 2560 5.7, 32 by 64 7.2), above 32 by 64 (128 by 2560 7.6, 8.5).
+// Tiles by the rule; else tiles of 16 or 32 whose waves share k: 16 outputs by 16 tokens (us, n 1536: one token by 2560 3.5, 32
+// outputs 4.3), 32 by 32 up to 96 tokens (64 by 2560 5.7, 32 by 64 7.2), above 32 by 64 (128 by 2560 7.6, 8.5).
 void launch_linear8(const Linear8Args& a, hipStream_t st) {
-    auto tiles = [&](uint32_t side) { return (uint64_t)((a.rows + side - 1) / side) * ((a.n_tokens + side - 1) / side); };
-    const uint64_t cus = device_cus();
-    const bool staged = a.x_stride < (1u << 24);  // a tile's offsets fit 32 bits
-    if (staged && tiles(256) >= cus * 3 / 4) launch_tiles<2, 4, 4, 2, 4>(a, st);
-    else if (staged && tiles(128) >= cus * 3 / 4) launch_tiles<2, 2, 2, 2, 4>(a, st);
-    else if (staged && tiles(64) >= cus * 5 / 8) launch_tiles<2, 2, 1, 1, 4>(a, st);
+    const uint32_t side = linear8_tile(a.n_tokens, a.rows, a.x_stride, device_cus());
+    if (side == 256) launch_tiles<2, 4, 4, 2, 4>(a, st);
+    else if (side == 128) launch_tiles<2, 2, 2, 2, 4>(a, st);
+    else if (side == 64) launch_tiles<2, 2, 1, 1, 4>(a, st);
     else if (a.n_tokens <= 16) launch_few<1, 1, 8>(a, st);
     else if (a.n_tokens <= 96) launch_few<2, 2, 8>(a, st);
     else launch_few<2, 4, 8>(a, st);

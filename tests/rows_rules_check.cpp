@@ -10,9 +10,12 @@
 int main() {
     std::string rule;
     while (std::cin >> rule) {
-        uint32_t a = 0;
+        uint32_t a = 0, b = 0, d = 0;
+        uint64_t c = 0;
         if (rule == "long_row_columns" && std::cin >> a)
             printf("%u\n", g4::long_row_columns(a));
+        else if (rule == "linear8_tile" && std::cin >> a >> b >> c >> d)
+            printf("%u\n", g4::linear8_tile(a, b, c, d));
         else
             return fprintf(stderr, "unknown rule %s\n", rule.c_str()), 1;
     }
