@@ -172,6 +172,7 @@ class TokenLogprobsParams(C.Structure):
 
 
 G4_F32, G4_F16, G4_BF16, G4_E4M3 = 0, 1, 2, 3
+G4_F32_SUMS = 0x100
 
 
 class AddRmsNormParams(C.Structure):

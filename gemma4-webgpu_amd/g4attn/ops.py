@@ -1059,11 +1059,12 @@ def linear_e4m3_workspace_bytes(n_tokens, rows, n, lora=None) -> int:
     return size.value
 
 
-def linear_e4m3(x, x_scales, weight, weight_scales, out, workspace, lora=None, adapter_ids=None, stream=None):
+def linear_e4m3(x, x_scales, weight, weight_scales, out, workspace, lora=None, adapter_ids=None, stream=None, f32_sums=False):
     """Projection of 8-bit rows (g4_linear_e4m3). x: float8_e4m3fn [n_tokens, n] with f32 scales [n_tokens], tokens may lie
     apart; weight: float8_e4m3fn [rows, n] with f32 scales [rows]; out: [n_tokens, rows], f32, f16 or bf16, tokens may lie
     apart. lora: a LoraAdapters of n inputs and rows outputs, with adapter_ids int32 [n_tokens] (outside the adapters: none).
-    workspace: uint8, linear_e4m3_workspace_bytes."""
+    workspace: uint8, linear_e4m3_workspace_bytes. f16 and bf16 outputs of larger calls have sums of the 8-bit matrix unit, whose
+    products lose what lies below 2^-13 of the largest of their eight; f32_sums: sums in f32 there too, at half the rate."""
     dev = _device_of(x, "x")
     e4m3, f32 = torch.float8_e4m3fn, torch.float32
     xp, _, xs = _rows_of(x, "x", _E4M3, dev)
@@ -1081,7 +1082,7 @@ def linear_e4m3(x, x_scales, weight, weight_scales, out, workspace, lora=None, a
     abi.call("g4_linear_e4m3", xp, _at(x_scales, "x_scales", f32, tokens, dev), _at(weight, "weight", e4m3, rows * n, dev),
              _at(weight_scales, "weight_scales", f32, rows, dev), None if lora is None else lora.c,
              None if lora is None else _at(adapter_ids, "adapter_ids", torch.int32, tokens, dev), op,
-             _linear_params(tokens, rows, n, ot, xs, os_), _at(workspace, "workspace", torch.uint8, 0, dev),
+             _linear_params(tokens, rows, n, ot | abi.G4_F32_SUMS if f32_sums else ot, xs, os_), _at(workspace, "workspace", torch.uint8, 0, dev),
              workspace.numel(), _stream(stream))
 
 

@@ -402,6 +402,7 @@ export interface LinearE4m3 {
   rows: number;
   n: number;
   outDtype?: RowDtype;
+  f32Sums?: boolean;          // f16 and bf16 outputs: sums in f32 in large calls too, at half the rate
   xStride?: number;
   outStride?: number;
   lora?: Lora;
@@ -426,6 +427,7 @@ export interface LoraAdd {
 
 const ROW_DTYPES: Record<string, number> = { f32: 0, f16: 1, bf16: 2, e4m3: 3 };
 const ROW_BYTES: Record<string, number> = { f32: 4, f16: 2, bf16: 2, e4m3: 1 };
+const F32_SUMS = 0x100;
 const KV_DTYPES: Record<string, number> = { f16: 0, e4m3: 1 };
 const LOGIT_DTYPES: Record<string, number> = { f32: 0, f16: 1, bf16: 2 };
 const LOGIT_BYTES: Record<string, number> = { f32: 4, f16: 2, bf16: 2 };
@@ -1168,7 +1170,7 @@ export class HipAttention {
 
   private static linearE4m3Params(p: LinearE4m3): Uint8Array {
     return HipAttention.rowParams([{ u: p.nTokens }, { u: p.rows }, { u: p.n },
-      { u: dtypeCode(ROW_DTYPES, p.outDtype || 'f32', 'linearE4m3') }], [p.xStride || 0, p.outStride || 0]);
+      { u: dtypeCode(ROW_DTYPES, p.outDtype || 'f32', 'linearE4m3') + (p.f32Sums ? F32_SUMS : 0) }], [p.xStride || 0, p.outStride || 0]);
   }
 
   linearE4m3WorkspaceSize(p: LinearE4m3): number {

@@ -143,6 +143,8 @@ function blockChecks(g4: any): void {
   [5, 50, 64, 0].forEach(function (x, j) { new DataView(linear.buffer).setUint32(4 * j, x, true); });
   if (!(g4.linearE4m3WorkspaceSize(linear, null) > 0)) fail('linearE4m3WorkspaceSize');
   if (!(g4.linearE4m3WorkspaceSize(linear, bytes) > g4.linearE4m3WorkspaceSize(linear, null))) fail('linearE4m3WorkspaceSize with lora');
+  const sums = (HipAttention as any).linearE4m3Params({ nTokens: 5, rows: 50, n: 64, outDtype: 'bf16', f32Sums: true });
+  if (new DataView(sums.buffer).getUint32(12, true) !== 0x102 || !(g4.linearE4m3WorkspaceSize(sums, null) > 0)) fail('linearE4m3 record');
   throws(() => g4.quantizeRows(BigInt(0), BigInt(16), BigInt(16), new Uint8Array(32), BigInt(0)), 'no rows, n 0');
 }
 

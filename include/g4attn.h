@@ -951,17 +951,27 @@ typedef struct g4_lora {
 } g4_lora;
 
 /* out[t][o] = x_scales[t] * weight_scales[o] * sum_k x[t][k] weight[o][k] of e4m3
- * rows (sums in f32), with the adapters' part added before the rounding where
- * lora is given. x: [n_tokens][n], as g4_add_rms_norm or g4_quantize_rows leave
- * it; weight: [rows][n], its scales one a row. Rows 16-byte aligned. The workspace
- * holds partial results within a call; calls that overlap need one each, and a
- * size (g4_linear_e4m3_workspace_size) serves every call of no more tokens with
- * the same projection and adapters. The same call gives the same bits. */
+ * rows, with the adapters' part added before the rounding where lora is given. x:
+ * [n_tokens][n], as g4_add_rms_norm or g4_quantize_rows leave it (rows of more than
+ * their 32768 elements are the caller's); weight: [rows][n], its scales one a row.
+ * Rows 16-byte aligned. The workspace holds partial results within a call; calls
+ * that overlap need one each, and a size (g4_linear_e4m3_workspace_size) serves every
+ * call of no more tokens with the same projection and adapters. The same call gives
+ * the same bits.
+ * Sums: in f32 for f32 outputs and, in calls of few tokens and outputs, for all. With
+ * f16 and bf16 outputs larger calls multiply on the 8-bit matrix unit, which adds
+ * products eight at a time (k 8 i .. 8 i + 7), each cut off below 2^-13 of the largest
+ * of its eight, and those sums in f32: a sum is off by less than 7 * 2^-13 of the
+ * largest product of each eight. That is 0.08 of f16's own rounding (root mean square)
+ * for normal rows, 0.3 with channels 100 times the others; where large products
+ * cancel, the rest keeps their error, and a token's bits depend on the size of its
+ * batch. out_type | G4_F32_SUMS: sums in f32 in every call, at half the products' rate. */
+#define G4_F32_SUMS 0x100
 typedef struct g4_linear_e4m3_params {
     uint32_t n_tokens;   /* at most 2^22 */
     uint32_t rows;       /* outputs, at most 2^20 */
     uint32_t n;          /* inputs: a multiple of 16, at most 65536 */
-    uint32_t out_type;   /* G4_F32, G4_F16 or G4_BF16 */
+    uint32_t out_type;   /* G4_F32, G4_F16 or G4_BF16; may have G4_F32_SUMS */
     uint64_t x_stride;   /* elements from token to token; 0: n */
     uint64_t out_stride; /* 0: rows */
 } g4_linear_e4m3_params;

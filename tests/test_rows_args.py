@@ -200,3 +200,13 @@ def test_python_wrappers_refuse_tensors_of_the_cpu():
         ops.linear_e4m3(x, w, x, w, x, w)
     with pytest.raises(ValueError, match="GPU"):
         ops.LoraAdapters(torch.zeros(2, 8, 64, dtype=torch.float16), torch.zeros(2, 64, 8, dtype=torch.float16))
+
+
+@pytest.mark.parametrize("kind", [abi.G4_F32, abi.G4_F16, abi.G4_BF16])
+def test_sums_in_f32_go_with_every_output_type_and_nothing_else_does(kind):
+    assert linear(out_type=kind | abi.G4_F32_SUMS, n_tokens=0) == abi.G4_OK
+    refused(linear(out_type=abi.G4_E4M3 | abi.G4_F32_SUMS), "out_type")
+    for other in (kind | 0x200, kind | 0x80, kind | 0x80000000, kind | abi.G4_F32_SUMS | 0x10):
+        refused(linear(out_type=other), "out_type")
+    header = HEADER.read_text()
+    assert f"#define G4_F32_SUMS {abi.G4_F32_SUMS:#x}" in header
