@@ -64,7 +64,12 @@ inline uint32_t long_row_columns(uint32_t rows) { return rows < (1u << 21) ? row
 // about enough of for the compute units, as long as there are; a tile's offsets fit 32 bits. Measured (us, n 1536; tiles of 256 /
 // 128 / 64 / few): 1024 tokens by 12288 outputs 28.9 / 33.4 / 44.2 / 133, 256 by 12288 22.2 / 12.4 / 15.4 / 35.7, 64 by 12288 19.4 /
 // 11.1 / 7.5 / 11.6; f32 outputs: 1024 by 2560 43.1 / 23.4 / 18.0 / 31.1, 256 by 2560 42.0 / 21.7 / 10.9 / 11.3, 64 by 2560 35.6 /
-// 20.2 / 10.4 / 5.4.
+// 20.2 / 10.4 / 5.4. At n 512: 256 by 2560 f32 21.8 / 11.1 / 6.5 / 6.1, 1024 by 12288 f16 16.2 / 16.1 / 20.3 / 49.3; at n 8192, f16: 64
+// by 2560 71 / 38 / 25.2 / 17.2, 64 by 12288 88 / 47 / 33.6 / 48.3, 1024 by 12288 107 / 133 / 231 / 512.
+// The rule counts tiles: it sees neither how few tokens fill one nor n. What it then gives away: one token by 12288 outputs f32 36 /
+// 21 / 11.3 / 6.6 (takes 64), by 24576 37 / 21.3 / 13.8 / 12.4 (128), by 65536 44 / 30 / 26.5 / 28 (256), by 262144 159 / 103 / 91 / 102
+// (256; f16 98 / 82 / 86 / 103); 64 by 8192 of n 8192 f16 87 / 46 / 32.4 / 33.8 (few); 1024 by 2560 f16 of n 1536 21.5 / 12.2 / 14.2 /
+// 24.5, of n 8192 77 / 41 / 49 / 108 (64); 60000 tokens by 24 f32 43 / 25 / 20 / 19 (256).
 inline uint32_t linear8_tile(uint32_t tokens, uint32_t rows, uint64_t x_stride, uint32_t cus) {
     if (x_stride >= 1u << 24) return 0;
     const auto tiles = [&](uint32_t side) { return (uint64_t)((rows + side - 1) / side) * ((tokens + side - 1) / side); };

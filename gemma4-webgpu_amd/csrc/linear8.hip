@@ -13,8 +13,8 @@
 // outputs of one token.
 //
 // Measured (us; the library's 8-bit product of the same shape beside): 8192 by 8192 by 8192 440, 2.5 PFLOP/s (408); 4096 tokens
-// by 12288 outputs of 1536 90 (74); 64 tokens by the same 7.4 (the weights' bytes at a copy's rate: 4); one token by 2560
-// outputs of 1536 3.6.
+// by 12288 outputs of 1536 92 (74); 64 tokens by the same 7.6 (the weights' bytes at a copy's rate: 4); one token by 2560
+// outputs of 1536 3.5. Sums in f32 for 16-bit outputs, without and with: 426 / 792, 85 / 135 and 7.8 / 10.9.
 #include <utility>
 
 #include "launch_rules.h"
@@ -159,7 +159,7 @@ __global__ __launch_bounds__(W * 64) void k_linear8_few(const Linear8Args a) {
 // while it multiplies this one's, so LDS, the DMA and the matrix unit work at once, with one barrier a stage. The
 // workgroup goes on to its next tile without a pause: the DMA runs up to four stages ahead, across the tiles' ends.
 //
-// What bounds it: at 8192 cubed the matrix unit is busy 0.72 of the cycles, and the chip runs them at 1.6 GHz: with
+// What bounds it: at 8192 cubed the matrix unit is busy 0.73 of the cycles, and the chip runs them at 1.6 GHz: with
 // neither DMA nor LDS reads the same products take 0.61 of the time, at 2.2 GHz. Four waves of 128 by 128 (a third fewer LDS
 // reads, one wave a SIMD) took 5 % longer: nothing covers a wave's own requests. Tiles of 256 by 128, two workgroups a
 // CU, 24 % longer. A tile's stores go on under the next tile's first stages; through LDS, as whole lines, they took longer

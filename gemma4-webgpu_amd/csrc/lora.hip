@@ -111,7 +111,7 @@ __global__ __launch_bounds__(kFewWaves * 64) void k_lora_down_few(const DownArgs
 // unit's layout, in which neighbouring lanes lie in different rows, every lane's 16 bytes are an access of their own (4003
 // tokens, n 2048, rank 64: 21 us). Piece c (16 bytes) of row r lies at c ^ r / 2 % 4 of its 64 bytes, c ^ r % 8 of its 128,
 // c ^ r % 16 of its 256. Products in f32 (f32 rows, mixed types) run at a sixteenth of the 16-bit rate, after the widening: 4003
-// tokens, n 2048, rank 64 and the up product to 2560 take 58 us, with equal 16-bit types 44.
+// tokens, n 2048, rank 64 and the up product to 2560 take 60 us, with equal 16-bit types 45.
 constexpr int kDownWaves = 4;
 template <int N>
 __device__ __forceinline__ void down_wait() {  // all but the N newest requests of the wave
