@@ -962,7 +962,7 @@ typedef struct g4_lora {
  * f16 and bf16 outputs larger calls multiply on the 8-bit matrix unit, which adds
  * products eight at a time (k 8 i .. 8 i + 7), each cut off below 2^-13 of the largest
  * of its eight, and those sums in f32: a sum is off by less than 7 * 2^-13 of the
- * largest product of each eight. That is 0.08 of f16's own rounding (root mean square)
+ * largest product of each eight (codes below 2^-6 but 0 counted as 2^-6). That is 0.08 of f16's own rounding (root mean square)
  * for normal rows, 0.3 with channels 100 times the others; where large products
  * cancel, the rest keeps their error, and a token's bits depend on the size of its
  * batch. out_type | G4_F32_SUMS: sums in f32 in every call, at half the products' rate. */
